@@ -73,6 +73,21 @@ class ALIFLayout(ctypes.Structure):
         "LIST1", "total")]
 
 
+class LinAttn(ctypes.Structure):
+    _fields_ = [(n, c_i) for n in ("dtype", "Dk", "Dv", "q_heads", "k_heads", "v_heads")] + \
+        [(n, c_i64) for n in ("T", "B", "H")] + [(n, c_p) for n in ("q", "k", "v")] + \
+        [(n, c_i64) for n in ("q_st", "q_sb", "q_sh", "k_st", "k_sb", "k_sh", "v_st", "v_sb", "v_sh")] + \
+        [(n, c_p) for n in ("beta", "s0", "o", "s_end")] + [("scale", c_f)]
+
+
+class BlockNorm(ctypes.Structure):
+    _fields_ = [(n, c_i) for n in ("x_dtype", "dtype", "act", "D")] + [("rows", c_i64)] + \
+        [(n, c_p) for n in ("x", "y", "gate", "w_post", "w_pre", "scale")] + [("scale1", c_f), ("eps", c_f)]
+
+
+# element types of the language-model operators
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
 # name -> (restype, argtypes); mirrors include/lifscan_hip.h
 SIGNATURES = {
     "lsh_abi_version": (c_i, []),
@@ -167,6 +182,17 @@ SIGNATURES = {
     "lsh_lif_scan_bwd_workspace": (c_sz, [c_i64, c_i64, c_i]),
     "lsh_lif_scan_bwd": (c_i, [c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_i64, c_i64, c_f, c_f, c_f, c_f,
                                c_i, c_i, c_p, c_sz, c_p]),
+    "lsh_linattn_fwd": (c_i, [c_p, c_p]),
+    "lsh_linattn_bwd_workspace": (c_sz, [c_p]),
+    "lsh_linattn_bwd": (c_i, [c_p, c_p, c_i64, c_i64, c_i64, c_p, c_p, c_p, c_p, c_p, c_p, c_sz, c_p]),
+    "lsh_linattn_step": (c_i, [c_p, c_p, c_p]),
+    "lsh_block_norm_fwd": (c_i, [c_p, c_p, c_p, c_p]),
+    "lsh_block_norm_bwd_workspace": (c_sz, [c_p]),
+    "lsh_block_norm_bwd": (c_i, [c_p] * 10 + [c_sz, c_p]),
+    "lsh_embed_fwd": (c_i, [c_i, c_p, c_p, c_p, c_i64, c_i64, c_i64, c_i64, c_f, c_p]),
+    "lsh_embed_bwd": (c_i, [c_i, c_p, c_p, c_p, c_i64, c_i64, c_i64, c_i64, c_f, c_p]),
+    "lsh_distill_fwd": (c_i, [c_i, c_p, c_i64, c_i, c_p, c_p, c_p, c_p, c_i64, c_i64, c_i, c_f, c_p]),
+    "lsh_distill_bwd": (c_i, [c_i, c_p, c_i64, c_i, c_p, c_p, c_p, c_p, c_i64, c_p, c_i64, c_i64, c_i, c_f, c_p]),
 }
 
 

@@ -509,6 +509,95 @@ int lsh_alif_bwd_recompute(const float* I, const float* U, const float* W, const
                            float rho, float q, float theta0, float u_r, float alpha, int mode,
                            int C, void* ws, size_t ws_bytes, void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Operators of a spiking language model around the neuron scans.  No counterpart in the reference.
+ * Tensors are of one element type (a dtype code), sums, states and statistics fp32; results are
+ * rounded to the tensor's type once, to nearest even.  Row, batch and head strides are in elements;
+ * the last axis is contiguous. */
+#define LSH_F32 0
+#define LSH_BF16 1
+#define LSH_F16 2
+
+/* Linear attention with a decay for each head, over time-major [T, B, heads, D]:
+ *   S_t = beta[h]*S_{t-1} + k_t v_t^T,  o_t = scale * q_t^T S_t,  S a [Dk, Dv] matrix per (b, h).
+ * H query/state heads; q_heads, k_heads and v_heads divide H, head h reads head h/(H/heads).
+ * beta: [H] fp32 on the device, 0 <= beta.  s0: [B, H, Dk, Dv] fp32 or NULL (zeros).
+ * o: contiguous [T, B, H, Dv].  s_end: the state after the last row, [B, H, Dk, Dv], or NULL;
+ * 1 <= Dk, Dv <= LSH_LINATTN_MAX_D; T = 0 is allowed (s_end = s0). */
+#define LSH_LINATTN_MAX_D 256
+typedef struct lsh_linattn {
+  int dtype, Dk, Dv, q_heads, k_heads, v_heads;
+  int64_t T, B, H;
+  const void *q, *k, *v;
+  int64_t q_st, q_sb, q_sh, k_st, k_sb, k_sh, v_st, v_sb, v_sh;
+  const float* beta;
+  const float* s0;
+  void* o;
+  float* s_end;
+  float scale;
+} lsh_linattn;
+int lsh_linattn_fwd(const lsh_linattn* a, void* stream);
+/* Its gradients: reads q, k, v, s0 of *a (not o, s_end), d_o [T, B, H, Dv] with the given strides
+ * and ds_end = dL/ds_end (fp32, or NULL); writes contiguous dq, dk, dv with the heads of q, k, v
+ * (sums over the heads that share one, in fp32 and head order) and ds0 (fp32, or NULL). */
+size_t lsh_linattn_bwd_workspace(const lsh_linattn* a);
+int lsh_linattn_bwd(const lsh_linattn* a, const void* d_o, int64_t do_st, int64_t do_sb, int64_t do_sh,
+                    const float* ds_end, void* dq, void* dk, void* dv, float* ds0, void* ws,
+                    size_t ws_bytes, void* stream);
+/* One token (T = 1; the row strides are not read): `state` [B, H, Dk, Dv] is updated in place, o is
+ * [B, H, Dv].  s0 and s_end are not read. */
+int lsh_linattn_step(const lsh_linattn* a, float* state, void* stream);
+
+/* The norm after a block with its gate and residual scale, and the norm before the next block, over
+ * [rows, D]:
+ *   n = y / sqrt(mean(y^2) + eps) * w_post,  x_new = x + scale * act(gate) * n,
+ *   z = x_new / sqrt(mean(x_new^2) + eps) * w_pre
+ * x, x_new and their gradients have x_dtype (LSH_F32, or dtype); y, gate, z and theirs dtype.
+ * w_post, w_pre: [D] fp32.  scale: [D] fp32, or NULL for the number scale1.  act: LSH_GATE_*; gate is
+ * not read with LSH_GATE_NONE.  All rows are contiguous. */
+#define LSH_GATE_NONE 0
+#define LSH_GATE_SILU 1
+#define LSH_GATE_SIGMOID 2
+#define LSH_BLOCK_NORM_MAX_D 16384
+typedef struct lsh_block_norm {
+  int x_dtype, dtype, act, D;
+  int64_t rows;
+  const void *x, *y, *gate;
+  const float *w_post, *w_pre, *scale;
+  float scale1, eps;
+} lsh_block_norm;
+int lsh_block_norm_fwd(const lsh_block_norm* a, void* x_new, void* z, void* stream);
+/* Its gradients from gx = dL/dx_new and gz = dL/dz (either may be NULL: zeros): dx, dy, dgate (or
+ * NULL), and the sums over the rows dw_post, dw_pre, dscale ([D] fp32, each may be NULL), in a fixed
+ * order. */
+size_t lsh_block_norm_bwd_workspace(const lsh_block_norm* a);
+int lsh_block_norm_bwd(const lsh_block_norm* a, const void* gx, const void* gz, void* dx, void* dy,
+                       void* dgate, float* dw_post, float* dw_pre, float* dscale, void* ws,
+                       size_t ws_bytes, void* stream);
+
+/* Embedding lookup: out[i] = scale * weight[tokens[i]] ([n, D] from [V, D]); rows of `padding` (-1: no
+ * padding id) and of ids outside 0..V-1 are zero.  The gradient dweight [V, D] = scale * the sum of
+ * dout over each token's positions, in fp32 and position order (every row is written). */
+int lsh_embed_fwd(int dtype, const int64_t* tokens, const void* weight, void* out, int64_t n, int64_t V,
+                  int64_t D, int64_t padding, float scale, void* stream);
+int lsh_embed_bwd(int dtype, const int64_t* tokens, const void* dout, void* dweight, int64_t n, int64_t V,
+                  int64_t D, int64_t padding, float scale, void* stream);
+
+/* Distillation from a teacher's top K logits: values (of v_dtype: LSH_F32, or dtype) and index, both
+ * [rows, K] and contiguous; an index outside 0..V-1 is no
+ * entry; logits [rows, V] with a row stride in elements.  With p the softmax of values/tau over
+ * the entries and q that of logits/tau over the vocabulary,
+ *   loss = tau^2 * sum_k p_k (log p_k - log q_{index_k}),
+ * 0 for a row without entries.  lse: [rows], log(sum exp(logits/tau)), which the gradient reads.
+ *   dlogits = g * tau * (q - p at its ids), contiguous [rows, V]; g: [rows] with an element stride. */
+#define LSH_DISTILL_MAX_K 4096
+int lsh_distill_fwd(int dtype, const void* logits, int64_t stride, int v_dtype, const void* values,
+                    const int64_t* index, float* loss, float* lse, int64_t rows, int64_t V, int K,
+                    float tau, void* stream);
+int lsh_distill_bwd(int dtype, const void* logits, int64_t stride, int v_dtype, const void* values,
+                    const int64_t* index, const float* lse, const float* g, int64_t g_stride,
+                    void* dlogits, int64_t rows, int64_t V, int K, float tau, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,373 @@
+"""GPU: linear attention with a decay for each head (lifscan.hip_linattn) against the recurrence
+S_t = beta*S_{t-1} + k_t v_t^T, o_t = scale * q_t^T S_t token by token in 64 bits, and its gradients
+against the adjoint recurrence in 64 bits and against differences.
+
+Tolerances.  Every result is a sum of products whose absolute values sum to M (the same recurrence
+over absolute values).  With unit roundoff u of the type (2^-8, 2^-11, 2^-24), a 16-bit type rounds a
+score or a state to its type once on the way of each product and the result once: 2u*M + u*|o|, plus
+fp32 sums, below (T + D + 64)*2^-24*M for any order.  In the norm the roundings are independent and
+average to less than u/sqrt(3) each, so ||error|| <= u*||result|| for 16 bits (two roundings and the
+fp32 part); fp32 is held to 4e-6 (some 64 roundings of independent sign).  States are fp32 in every
+type."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+NORM = {torch.float32: 4e-6, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+
+
+def _inputs(dtype, T, B, heads, H, Dk, Dv, dev, seed=0, s0=True):
+    g = torch.Generator().manual_seed(seed + T)
+    hq, hk, hv = heads
+    mk = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    q, k, v = (mk(T, B, h, d).to(dtype) for h, d in ((hq, Dk), (hk, Dk), (hv, Dv)))
+    beta = 1 - torch.exp2(-torch.linspace(2, 9, H)) * (0.9 + 0.1 * torch.rand(H, generator=g))
+    S = 2 * mk(B, H, Dk, Dv) if s0 else None
+    do, ds = mk(T, B, H, Dv).to(dtype), 0.5 * mk(B, H, Dk, Dv)
+    return [t.to(dev) if t is not None else None for t in (q, k, v, beta, S, do, ds)]
+
+
+def reference(q, k, v, beta, s0, scale, do=None, ds=None):
+    """The definitions in 64 bits on the CPU -> (o, s_end[, dq, dk, dv, ds0])."""
+    q, k, v, beta = (t.detach().double().cpu() for t in (q, k, v, beta))
+    H = beta.numel()
+    share = [H // t.shape[2] for t in (q, k, v)]
+    q, k, v = (t.repeat_interleave(r, 2) for t, r in zip((q, k, v), share))
+    T, B, _, Dk = q.shape
+    Dv = v.shape[-1]
+    b = beta[:, None, None]
+    S = torch.zeros(B, H, Dk, Dv, dtype=torch.float64) if s0 is None else s0.detach().double().cpu()
+    o = torch.zeros(T, B, H, Dv, dtype=torch.float64)
+    back = do is not None or ds is not None
+    if back:
+        do = torch.zeros_like(o) if do is None else do.double().cpu()
+        E = torch.zeros_like(S) if ds is None else ds.double().cpu()
+        dq, dk, dv = torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v)
+    for t in range(T):
+        S = b * S + k[t][..., :, None] * v[t][..., None, :]
+        o[t] = scale * (q[t][..., None, :] @ S)[..., 0, :]
+        if back:
+            dq[t] = scale * (S @ do[t][..., :, None])[..., 0]
+    if not back:
+        return o, S
+    for t in range(T - 1, -1, -1):
+        G = E + scale * q[t][..., :, None] * do[t][..., None, :]
+        dk[t] = (G @ v[t][..., :, None])[..., 0]
+        dv[t] = (k[t][..., None, :] @ G)[..., 0, :]
+        E = b * G
+    dq, dk, dv = (d.unflatten(2, (-1, r)).sum(3) for d, r in zip((dq, dk, dv), share))
+    return o, S, dq, dk, dv, E
+
+
+def check(got, want, most, dtype, T, D):
+    """got against want; most: the sum of the absolute values of want's products."""
+    u = U[got.dtype]
+    assert got.dtype in (dtype, torch.float32) and tuple(got.shape) == tuple(want.shape)
+    err = (got.detach().double().cpu() - want).abs()
+    bound = u * want.abs() + ((2 * u if u > 1e-6 else 0.0) + (T + D + 64) * 2.0 ** -24) * most
+    assert bool((err <= bound).all()), float((err / bound.clamp(min=1e-300)).max())
+    if want.numel() > 2000:
+        assert float(err.norm()) <= NORM[got.dtype] * float(want.norm())
+
+
+def _absolute(q, k, v, beta, s0, scale, *grads):
+    return reference(q.abs(), k.abs(), v.abs(), beta, None if s0 is None else s0.abs(), abs(scale),
+                     *(None if t is None else t.abs() for t in grads))
+
+
+def run_all(q, k, v, beta, s0, scale, do, ds):
+    from lifscan import hip_linattn as LA
+    ins = [t.detach().requires_grad_(True) if t is not None else None for t in (q, k, v, s0)]
+    o, s_end = LA.lin_attn(*ins[:3], beta, s0=ins[3], scale=scale)
+    outs = [(t, g) for t, g in ((o, do), (s_end, ds)) if g is not None]
+    grads = torch.autograd.grad([t for t, _ in outs], [t for t in ins if t is not None], [g for _, g in outs])
+    return (o, s_end, *grads)
+
+
+SHAPES = [  # T, B, (Hq, Hk, Hv), H, Dk, Dv
+    (1, 1, (1, 1, 1), 1, 1, 1),
+    (1, 3, (4, 4, 4), 4, 64, 64),
+    (2, 2, (4, 2, 2), 4, 128, 128),
+    (31, 2, (2, 2, 2), 2, 64, 128),
+    (32, 1, (4, 1, 1), 4, 32, 64),
+    (33, 1, (1, 1, 4), 4, 17, 40),
+    (63, 2, (2, 1, 2), 2, 48, 80),
+    (64, 1, (3, 3, 3), 3, 128, 64),
+    (65, 2, (4, 4, 2), 4, 100, 7),
+    (129, 1, (2, 2, 2), 2, 128, 128),
+    (200, 1, (2, 2, 2), 2, 256, 48),
+    (191, 2, (1, 1, 1), 1, 40, 256),
+    (515, 1, (2, 1, 1), 2, 256, 256),
+    (130, 9, (16, 16, 16), 16, 24, 16),
+]
+
+
+@pytest.mark.parametrize("dtype", list(U), ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: f"T{s[0]}-{s[4]}x{s[5]}")
+def test_forward_and_gradients(dev, dtype, shape):
+    T, B, heads, H, Dk, Dv = shape
+    print(f"linattn {dtype} {shape}", flush=True)
+    args = _inputs(dtype, T, B, heads, H, Dk, Dv, dev)
+    scale = Dk ** -0.5
+    q, k, v, beta, s0, do, ds = args
+    got = run_all(q, k, v, beta, s0, scale, do, ds)
+    want = reference(q, k, v, beta, s0, scale, do, ds)
+    most = _absolute(q, k, v, beta, s0, scale, do, ds)
+    for g, w, m in zip(got, want, most):
+        check(g, w, m, dtype, T, max(Dk, Dv))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("T,B,H,Dk,Dv", [(5000, 1, 1, 64, 64), (2300, 1, 2, 128, 128), (1801, 2, 2, 32, 200)])
+def test_long_sequences_of_few_heads(dev, dtype, T, B, H, Dk, Dv):
+    """The time axis split over workgroups and joined."""
+    print(f"linattn long {dtype} {T} {B} {H} {Dk} {Dv}", flush=True)
+    q, k, v, beta, s0, do, ds = _inputs(dtype, T, B, (H,) * 3, H, Dk, Dv, dev, seed=3)
+    got = run_all(q, k, v, beta, s0, 0.1, do, ds)
+    want = reference(q, k, v, beta, s0, 0.1, do, ds)
+    most = _absolute(q, k, v, beta, s0, 0.1, do, ds)
+    for g, w, m in zip(got, want, most):
+        check(g, w, m, dtype, T, max(Dk, Dv))
+
+
+@pytest.mark.parametrize("which", ["no_s0", "only_o", "only_state"])
+def test_parts_of_the_gradient(dev, which):
+    dtype, T = torch.float32, 70
+    q, k, v, beta, s0, do, ds = _inputs(dtype, T, 2, (2, 2, 2), 2, 32, 48, dev, seed=5)
+    if which == "no_s0":
+        s0 = None
+    elif which == "only_o":
+        ds = None
+    else:
+        do = None
+    got = run_all(q, k, v, beta, s0, 0.2, do, ds)
+    want = reference(q, k, v, beta, s0, 0.2, do, ds)
+    most = _absolute(q, k, v, beta, s0, 0.2, do, ds)
+    for g, w, m in zip(got, want, most):
+        check(g, w, m, dtype, T, 48)
+
+
+@pytest.mark.parametrize("beta", [0.0, 1.0, 1e-30, 0.5])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_decays_at_the_ends(dev, beta, dtype):
+    """A decay of 0 keeps the newest token only, 1 forgets nothing, a tiny one underflows; also as one
+    number for all heads."""
+    from lifscan import hip_linattn as LA
+    T, H = 100, 2
+    q, k, v, _, s0, do, ds = _inputs(dtype, T, 1, (H,) * 3, H, 64, 64, dev, seed=9)
+    b = torch.full((H,), beta, device=dev)
+    got = run_all(q, k, v, b, s0, 0.3, do, ds)
+    want = reference(q, k, v, b, s0, 0.3, do, ds)
+    most = _absolute(q, k, v, b, s0, 0.3, do, ds)
+    for g, w, m in zip(got, want, most):
+        check(g, w, m, dtype, T, 64)
+    o, s_end = LA.lin_attn(q, k, v, beta, s0=s0, scale=0.3)
+    assert torch.equal(o, got[0].detach()) and torch.equal(s_end, got[1].detach())
+
+
+@pytest.mark.parametrize("dtype", list(U), ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("layout", ["batch_major", "one_projection", "shared_by_stride", "odd_offset", "last_axis"])
+def test_layouts(dev, dtype, layout):
+    """Strides other than the contiguous ones give the contiguous operands' bits."""
+    from lifscan import hip_linattn as LA
+    T, B, H, D = 77, 2, 2, 64
+    q, k, v, beta, s0, do, ds = _inputs(dtype, T, B, (H,) * 3, H, D, D, dev, seed=11)
+    if layout == "shared_by_stride":
+        q, k, v = (t[:, :, :1].contiguous().expand(T, B, H, D) for t in (q, k, v))
+    plain = [t.contiguous() for t in (q, k, v)]
+    if layout == "batch_major":
+        q, k, v = (t.transpose(0, 1).contiguous().transpose(0, 1) for t in plain)
+    elif layout == "one_projection":
+        q, k, v = torch.stack(plain, 2).unbind(2)
+    elif layout == "odd_offset":
+        q, k, v = (torch.cat([t.flatten()[:3], t.flatten()])[3:].view(t.shape) for t in plain)
+    elif layout == "last_axis":
+        q, k, v = (t.transpose(2, 3).contiguous().transpose(2, 3) for t in plain)
+    got = run_all(q, k, v, beta, s0, 0.125, do, ds)
+    want = run_all(*plain, beta, s0, 0.125, do, ds)
+    # operands that are read element by element take the same sums: the same bits
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    o, s_end = LA.lin_attn(q, k, v, beta, s0=s0, scale=0.125)
+    assert torch.equal(o, want[0]) and torch.equal(s_end, want[1])
+
+
+def test_offsets_beyond_32_bits(dev):
+    """Rows more than 2^31 elements apart."""
+    from lifscan import hip_linattn as LA
+    T, H, D = 3, 1, 64
+    q, k, v, beta, s0, _, _ = _inputs(torch.bfloat16, T, 1, (1, 1, 1), H, D, D, dev, seed=13)
+    step = 2 ** 31 - 64  # row 2 starts past 2^32 - 128
+    far = torch.empty(2 * step + D, dtype=torch.bfloat16, device=dev)
+    wide = far.as_strided((T, 1, H, D), (step, D, D, 1))
+    wide.copy_(v)
+    o, s = LA.lin_attn(q, k, wide, beta, s0=s0)
+    o2, s2 = LA.lin_attn(q, k, v, beta, s0=s0)
+    assert torch.equal(o, o2) and torch.equal(s, s2)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_gradients_against_differences(dev, dtype):
+    """The loss <o, do> + <s_end, ds> is linear in each operand, so a whole step along one operand
+    changes it by <gradient, step> exactly; in fp32 (64-bit sums of the outputs) up to the outputs'
+    own rounding, in bf16 up to the outputs' and the gradient's roundings, of independent signs."""
+    from lifscan import hip_linattn as LA
+    T, H, D = 90, 2, 64
+    q, k, v, beta, s0, do, ds = _inputs(dtype, T, 2, (H,) * 3, H, D, D, dev, seed=17)
+    grads = run_all(q, k, v, beta, s0, 0.125, do, ds)[2:]
+    ops = [q, k, v, s0]
+
+    def loss(ops):
+        o, s = LA.lin_attn(*ops[:3], beta, s0=ops[3], scale=0.125)
+        return o, s, (o.double() * do.double()).sum() + (s.double() * ds.double()).sum()
+
+    o, s, base = loss(ops)
+    for i, gr in enumerate(grads):
+        d = torch.randn(ops[i].shape, generator=torch.Generator().manual_seed(i)).to(dev, ops[i].dtype)
+        moved = list(ops)
+        moved[i] = (ops[i].double() + d.double()).to(ops[i].dtype)
+        d = moved[i].double() - ops[i].double()
+        o2, s2, after = loss(moved)
+        # independent roundings: sqrt of the sum of squares, eight standard deviations
+        u = {torch.float32: 2.0 ** -20, torch.bfloat16: 2.0 ** -8}[dtype]
+        tol = 8 * u * (sum(float((a.double() * do.double()).norm()) ** 2 for a in (o, o2)) +
+                       float((gr.double() * d).norm()) ** 2) ** 0.5
+        tol += 8 * 2.0 ** -20 * sum(float((a.double() * ds.double()).norm()) for a in (s, s2))
+        assert abs(float(after - base) - float((gr.double() * d).sum())) <= tol
+
+
+@pytest.mark.parametrize("dtype", list(U), ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("B,heads,H,Dk,Dv", [(1, (8, 8, 8), 8, 64, 64), (3, (4, 2, 1), 4, 128, 128),
+                                             (2, (1, 1, 1), 1, 1, 1), (5, (2, 2, 2), 2, 33, 70),
+                                             (2, (3, 3, 3), 3, 256, 256), (1, (2, 1, 2), 2, 15, 130)])
+def test_single_tokens_follow_the_recurrence(dev, dtype, B, heads, H, Dk, Dv):
+    from lifscan import hip_linattn as LA
+    T = 4
+    q, k, v, beta, s0, _, _ = _inputs(dtype, T, B, heads, H, Dk, Dv, dev, seed=19)
+    want, s_want = reference(q, k, v, beta, s0, 0.2)
+    most, s_most = _absolute(q, k, v, beta, s0, 0.2)
+    state = s0.clone()
+    o = torch.stack([LA.lin_attn_step(q[t], k[t], v[t], beta, state, scale=0.2) for t in range(T)])
+    check(o, want, most, dtype, T, max(Dk, Dv))
+    check(state, s_want, s_most, dtype, T, max(Dk, Dv))
+
+
+def test_prompt_then_tokens(dev):
+    """A prompt in one call and its continuation token by token: the states of the whole sequence."""
+    from lifscan import hip_linattn as LA
+    q, k, v, beta, _, _, _ = _inputs(torch.float32, 100, 2, (2, 2, 2), 2, 64, 96, dev, seed=23)
+    o, s = LA.lin_attn(q, k, v, beta, scale=0.1)
+    a, state = LA.lin_attn(q[:97], k[:97], v[:97], beta, scale=0.1)
+    b = [LA.lin_attn_step(q[t], k[t], v[t], beta, state, scale=0.1) for t in range(97, 100)]
+    most, s_most = _absolute(q, k, v, beta, None, 0.1)
+    tol = 2 * (100 + 96 + 64) * 2.0 ** -24
+    assert bool(((torch.cat([a, torch.stack(b)]) - o).abs().cpu().double() <= tol * most).all())
+    assert bool(((state - s).abs().cpu().double() <= tol * s_most).all())
+
+
+def test_no_tokens_and_no_batch(dev):
+    from lifscan import hip_linattn as LA
+    q, k, v, beta, s0, _, _ = _inputs(torch.float32, 0, 2, (2, 2, 2), 2, 8, 8, dev)
+    o, s = LA.lin_attn(q, k, v, beta, s0=s0)
+    assert o.shape == (0, 2, 2, 8) and torch.equal(s, s0)
+    o, s = LA.lin_attn(q, k, v, beta)
+    assert bool((s == 0).all())
+    got = run_all(q, k, v, beta, s0, 1.0, o, torch.ones_like(s0))
+    assert bool((got[5] == 1).all()) and got[2].shape == q.shape
+    o, s = LA.lin_attn(q.new_zeros(3, 0, 2, 8), k.new_zeros(3, 0, 2, 8), v.new_zeros(3, 0, 2, 8), beta)
+    assert o.shape == (3, 0, 2, 8) and s.shape == (0, 2, 8, 8)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_same_bits_on_every_run_and_stream(dev, dtype):
+    q, k, v, beta, s0, do, ds = _inputs(dtype, 700, 1, (4, 2, 2), 4, 64, 64, dev, seed=29)
+    first = run_all(q, k, v, beta, s0, 0.1, do, ds)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        again = run_all(q, k, v, beta, s0, 0.1, do, ds)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    for a, b in zip(first, again):
+        assert torch.equal(a, b)
+
+
+def test_graph_replays(dev):
+    """A prompt and a token captured in a HIP graph, replayed three times with eager work between."""
+    from lifscan import hip_linattn as LA
+    q, k, v, beta, s0, _, _ = _inputs(torch.bfloat16, 1000, 1, (2, 2, 2), 2, 64, 64, dev, seed=31)
+    state = s0.clone()
+
+    def work():
+        o, s = LA.lin_attn(q, k, v, beta, s0=state, scale=0.1)
+        state.copy_(s)
+        return o, LA.lin_attn_step(q[0], k[0], v[0], beta, state, scale=0.1)
+
+    want = []
+    for _ in range(4):
+        want.append([t.clone() for t in work()] + [state.clone()])
+    state.copy_(s0)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        work()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = work()
+    for r in range(1, 4):
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip([*outs, state], want[r]):
+            assert torch.equal(a, b), r
+        LA.lin_attn(q, k, v, beta)  # eager work between the replays
+        torch.cuda.synchronize()
+
+
+def test_values_that_are_not_finite_stay_in_their_rows(dev):
+    """An infinite q row is its own row's matter; a NaN value reaches the rows after it, not those
+    before it."""
+    from lifscan import hip_linattn as LA
+    for dtype in U:
+        q, k, v, beta, _, _, _ = _inputs(dtype, 100, 1, (1, 1, 1), 1, 64, 64, dev, seed=37)
+        q[10, 0, 0, 3] = float("inf")
+        v[70, 0, 0, 5] = float("nan")
+        o, s = LA.lin_attn(q, k, v, beta, scale=0.1)
+        bad = ~torch.isfinite(o[:, 0, 0])
+        assert bool(bad[10].all()) and not bool(bad[:10].any()) and not bool(bad[11:70].any())
+        assert bool(bad[70:, 5].all()) and int(bad[70:].sum()) == 30
+        assert int((~torch.isfinite(s)).sum()) == 64
+
+
+def test_refusals(dev):
+    from lifscan import hip_linattn as LA
+    q = torch.randn(4, 2, 2, 8, device=dev)
+    b = torch.full((2,), 0.9, device=dev)
+    s = torch.zeros(2, 2, 8, 8, device=dev)
+    bad = [
+        lambda: LA.lin_attn(q.cpu(), q.cpu(), q.cpu(), b),
+        lambda: LA.lin_attn(q.double(), q.double(), q.double(), b),
+        lambda: LA.lin_attn(q, q.half(), q, b),
+        lambda: LA.lin_attn(q[0], q[0], q[0], b),
+        lambda: LA.lin_attn(q, q[:3], q, b),
+        lambda: LA.lin_attn(q, q[..., :4], q, b),
+        lambda: LA.lin_attn(q, q, q, torch.full((3,), 0.9, device=dev)),
+        lambda: LA.lin_attn(q, q, q, b.cpu()),
+        lambda: LA.lin_attn(q, q, q, -0.5),
+        lambda: LA.lin_attn(q, q, q, float("nan")),
+        lambda: LA.lin_attn(q, q, q, b.clone().requires_grad_(True)),
+        lambda: LA.lin_attn(q, q, q, b, s0=s[:1]),
+        lambda: LA.lin_attn(q, q, q, b, s0=s.half()),
+        lambda: LA.lin_attn(torch.randn(4, 2, 2, 257, device=dev), torch.randn(4, 2, 2, 257, device=dev), q, b),
+        lambda: LA.lin_attn_step(q, q, q, b, s),
+        lambda: LA.lin_attn_step(q[0], q[0], q[0], b, s.transpose(2, 3)),
+        lambda: LA.lin_attn_step(q[0], q[0], q[0], b, s.half()),
+        lambda: LA.lin_attn_step(q[0].clone().requires_grad_(True), q[0], q[0], b, s),
+    ]
+    for i, f in enumerate(bad):
+        with pytest.raises(ValueError):
+            f()
+            print("not refused:", i)
