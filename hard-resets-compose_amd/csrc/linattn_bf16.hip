@@ -1,0 +1,6 @@
+// The chunked walk of linear attention for one operand type (linattn_walk.h).
+#include "linattn_walk.h"
+
+namespace lsh {
+int la_launch_bf16(const LaWalk& a, bool sums, hipStream_t st) { return la_launch<bf16_t, bf16_t>(a, sums, st); }
+}  // namespace lsh

@@ -1,0 +1,6 @@
+// The chunked walk of linear attention for one operand type (linattn_walk.h).
+#include "linattn_walk.h"
+
+namespace lsh {
+int la_launch_f16(const LaWalk& a, bool sums, hipStream_t st) { return la_launch<f16_t, float>(a, sums, st); }
+}  // namespace lsh

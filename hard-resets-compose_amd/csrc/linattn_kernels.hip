@@ -9,84 +9,28 @@
 //   G_t  = E_{t+1} + scale * q_t do_t^T,    dk_t = G_t v_t,    dv_t = G_t^T k_t
 // so dq is the forward walk with (do, v, k) in the place of (q, k, v) and the state transposed, and
 // dk and dv are walks from the last row to the first with (v, do, q) and (k, q, do), which decay
-// after the sum instead of before it.  One walk kernel therefore serves the forward and the
+// after the sum instead of before it.  One walk (linattn_walk.h) therefore serves the forward and the
 // backward: LaWalk names the operands by their place in the walk.
 #include <algorithm>
 #include <utility>
 
-#include "lsh_lm.h"
+#include "linattn_walk.h"
 
 namespace lsh {
 
-// A [T, B, heads, D] operand: element strides of its rows, batches and heads (the last axis is
-// contiguous), and how many of the walk's heads share one of its heads.
-struct LaIn {
-  const void* p;
-  int64_t st, sb, sh;
-  int share;
-};
-
-// One walk: out_r = so * Q_r^T S_r over the rows in walking order.
-struct LaWalk {
-  LaIn q, k, v;
-  void* out;            // [T, B, H, DV], contiguous
-  const float* s_in;    // [B*H] states of sk*DK or sv*DV elements, or NULL (zeros)
-  float* s_out;         // the state after the last row, or NULL
-  const float* beta;    // [H]
-  int64_t T, B, H;
-  int DK, DV;
-  int sk, sv;           // element strides of a state along DK and DV
-  int rev;              // rows from the last to the first
-  int late;             // decay after the sum (gradient walks): S = beta*(S + K V^T)
-  float so, su;         // out's scale, and the sum's
-};
-
-template <class T>
-__device__ __forceinline__ const T* la_row(const LaIn& x, int64_t b, int64_t h) {
-  return (const T*)x.p + b * x.sb + (h / x.share) * x.sh;
-}
-
-// One wave per state column: lane l holds rows l, l + 64, ... of column dv.
-template <class T, class TO>
-__global__ __launch_bounds__(256) void k_la_recur(LaWalk a) {
-  const int lane = threadIdx.x & 63;
-  const int dv = blockIdx.y * 4 + (threadIdx.x >> 6);
-  if (dv >= a.DV) return;
-  const int64_t bh = blockIdx.x, b = bh / a.H, h = bh % a.H;
-  const T* q = la_row<T>(a.q, b, h);
-  const T* k = la_row<T>(a.k, b, h);
-  const T* v = la_row<T>(a.v, b, h);
-  TO* out = (TO*)a.out + (b * a.H + h) * a.DV + dv;
-  const float beta = a.beta[h];
-  const size_t state = (size_t)bh * a.DK * a.DV + (size_t)dv * a.sv;
-  float S[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int dk = lane + 64 * i;
-    S[i] = a.s_in && dk < a.DK ? a.s_in[state + (size_t)dk * a.sk] : 0.0f;
-  }
-  for (int64_t r = 0; r < a.T; ++r) {
-    const int64_t t = a.rev ? a.T - 1 - r : r;
-    const float vt = a.su * to_f(v[t * a.v.st + dv]);
-    float o = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int dk = lane + 64 * i;
-      if (dk < a.DK) {
-        const float s = __builtin_fmaf(to_f(k[t * a.k.st + dk]), vt, a.late ? S[i] : beta * S[i]);
-        o = __builtin_fmaf(to_f(q[t * a.q.st + dk]), s, o);
-        S[i] = a.late ? beta * s : s;
-      }
-    }
-    o = wave_sum_f(o);
-    if (lane == 0) out[t * a.B * a.H * a.DV] = from_f<TO>(a.so * o);
-  }
-  if (a.s_out) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int dk = lane + 64 * i;
-      if (dk < a.DK) a.s_out[state + (size_t)dk * a.sk] = S[i];
-    }
+// The states before the segments from the segments' sums: starts[0] = s0 (or zeros), starts[s] =
+// beta^L starts[s-1] + sum of segment s-1, in place.  One thread an element.
+__global__ __launch_bounds__(256) void k_la_join(float* __restrict__ starts, const float* __restrict__ s0,
+                                                 const float* __restrict__ beta, int64_t n, int64_t size,
+                                                 int64_t H, int segs, int64_t L) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  const float f = __builtin_amdgcn_exp2f(la_log2(beta[i / size % H]) * (float)L);
+  float s = s0 ? s0[i] : 0.0f;
+  starts[i] = s;
+  for (int j = 1; j < segs; ++j) {
+    s = __builtin_fmaf(f, s, starts[(size_t)j * n + i]);
+    starts[(size_t)j * n + i] = s;
   }
 }
 
@@ -103,16 +47,39 @@ __global__ __launch_bounds__(256) void k_la_share(const float* __restrict__ x, T
   y[i] = from_f<T>(s);
 }
 
-static int la_walk(const LaWalk& a, int dtype, bool out_f32, hipStream_t st) {
-  if (a.B * a.H == 0) return LSH_OK;
-  const dim3 grid((unsigned)(a.B * a.H), (a.DV + 3) / 4);
-  with_dtype(dtype, [&](auto t) {
-    using T = decltype(t);
-    if (out_f32)
-      k_la_recur<T, float><<<grid, 256, 0, st>>>(a);
-    else
-      k_la_recur<T, T><<<grid, 256, 0, st>>>(a);
-  });
+static int la_go(const LaWalk& a, int dtype, bool sums, hipStream_t st) {
+  return dtype == LSH_F32    ? la_launch_f32(a, sums, st)
+         : dtype == LSH_BF16 ? la_launch_bf16(a, sums, st)
+                             : la_launch_f16(a, sums, st);
+}
+
+// How the rows are split: every segment but the last has L rows.  The walk alone has a workgroup for
+// each (batch, head) and block of columns; where these are too few for the chip the rows are split,
+// at the price of a pass over K and V for the segments' sums and of their states.
+struct LaSplit {
+  int segs;
+  int64_t L;
+};
+static LaSplit la_split(int dtype, int64_t T, int64_t BH, int DK, int DV) {
+  const int64_t C = la_chunk(dtype), chunks = (T + C - 1) / C;
+  const int block = la_block(DK, DV);
+  const int64_t groups = BH * ((DV + block - 1) / block);
+  int64_t segs = std::min<int64_t>((512 + groups - 1) / std::max<int64_t>(groups, 1), chunks / 4);
+  if (segs < 2) return {1, std::max<int64_t>(T, 1)};
+  const int64_t per = (chunks + segs - 1) / segs;
+  return {(int)((chunks + per - 1) / per), per * C};
+}
+
+static void la_set_split(LaWalk& a, LaSplit s) { a.segs = s.segs, a.L = s.L; }
+
+// The states before the segments (s.segs > 1), into `starts`.
+static int la_starts(LaWalk a, int dtype, LaSplit s, const float* s0, float* starts, hipStream_t st) {
+  la_set_split(a, s);
+  a.s_in = nullptr;
+  a.s_out = starts;
+  if (int rc = la_go(a, dtype, true, st)) return rc;
+  const int64_t size = (int64_t)a.DK * a.DV, n = a.B * a.H * size;
+  k_la_join<<<dim3((unsigned)((n + 255) / 256)), 256, 0, st>>>(starts, s0, a.beta, n, size, a.H, s.segs, s.L);
   LSH_CHECK_LAUNCH();
   return LSH_OK;
 }
@@ -191,30 +158,58 @@ static int la_check(const lsh_linattn* a) {
   return LSH_OK;
 }
 
-static LaIn la_in(const void* p, int64_t st, int64_t sb, int64_t sh, int64_t H, int heads) {
-  return LaIn{p, st, sb, sh, (int)(H / heads)};
+static LaIn la_in(const void* p, int64_t st, int64_t sb, int64_t sh, int64_t H, int heads, int dtype, int D) {
+  const int w = 16 / lm_dtype_size(dtype);
+  const bool wide = (uintptr_t)p % 16 == 0 && st % w == 0 && sb % w == 0 && sh % w == 0 && D % w == 0;
+  return LaIn{p, st, sb, sh, (int)(H / heads), wide};
+}
+static LaIn la_q(const lsh_linattn* a) {
+  return la_in(a->q, a->q_st, a->q_sb, a->q_sh, a->H, a->q_heads, a->dtype, a->Dk);
+}
+static LaIn la_k(const lsh_linattn* a) {
+  return la_in(a->k, a->k_st, a->k_sb, a->k_sh, a->H, a->k_heads, a->dtype, a->Dk);
+}
+static LaIn la_v(const lsh_linattn* a) {
+  return la_in(a->v, a->v_st, a->v_sb, a->v_sh, a->H, a->v_heads, a->dtype, a->Dv);
+}
+
+// The split of the forward, and of its gradients' walks over the same rows.
+static LaSplit la_split_of(const lsh_linattn* a) {
+  return la_split(a->dtype, a->T, a->B * a->H, a->Dk, a->Dv);
+}
+static size_t la_starts_bytes(const lsh_linattn* a) {
+  const LaSplit s = la_split_of(a);
+  return s.segs > 1 ? (size_t)s.segs * a->B * a->H * a->Dk * a->Dv * sizeof(float) : 0;
 }
 
 }  // namespace lsh
 
 using namespace lsh;
 
-extern "C" int lsh_linattn_fwd(const lsh_linattn* a, void* stream) {
+extern "C" size_t lsh_linattn_workspace(const lsh_linattn* a) {
+  return la_check(a) || a->H == 0 ? 0 : la_starts_bytes(a);
+}
+
+extern "C" int lsh_linattn_fwd(const lsh_linattn* a, void* ws, size_t ws_bytes, void* stream) {
   if (int rc = la_check(a)) return rc;
   if (a->B == 0 || a->H == 0) return LSH_OK;
   if (a->T > 0 && bad_ptr(a->o)) return LSH_ERR_ARG;
+  const LaSplit split = la_split_of(a);
+  if (split.segs > 1 && (bad_ptr(ws) || ws_bytes < la_starts_bytes(a))) return LSH_ERR_WORKSPACE;
   LaWalk w = {};
-  w.q = la_in(a->q, a->q_st, a->q_sb, a->q_sh, a->H, a->q_heads);
-  w.k = la_in(a->k, a->k_st, a->k_sb, a->k_sh, a->H, a->k_heads);
-  w.v = la_in(a->v, a->v_st, a->v_sb, a->v_sh, a->H, a->v_heads);
-  w.out = a->o;
-  w.s_in = a->s0;
-  w.s_out = a->s_end;
+  w.q = la_q(a), w.k = la_k(a), w.v = la_v(a);
+  w.out = a->o, w.out_f32 = a->dtype == LSH_F32;
   w.beta = a->beta;
   w.T = a->T, w.B = a->B, w.H = a->H, w.DK = a->Dk, w.DV = a->Dv;
   w.sk = a->Dv, w.sv = 1;
   w.so = a->scale, w.su = 1.0f;
-  return la_walk(w, a->dtype, false, (hipStream_t)stream);
+  hipStream_t st = (hipStream_t)stream;
+  if (split.segs > 1)
+    if (int rc = la_starts(w, a->dtype, split, a->s0, (float*)ws, st)) return rc;
+  la_set_split(w, split);
+  w.s_in = split.segs > 1 ? (const float*)ws : a->s0;
+  w.s_out = a->s_end;
+  return la_go(w, a->dtype, false, st);
 }
 
 extern "C" size_t lsh_linattn_bwd_workspace(const lsh_linattn* a) {
@@ -222,35 +217,39 @@ extern "C" size_t lsh_linattn_bwd_workspace(const lsh_linattn* a) {
   size_t n = 0;
   for (auto [heads, D] : {std::pair<int, int>{a->q_heads, a->Dk}, {a->k_heads, a->Dk}, {a->v_heads, a->Dv}})
     if (heads != a->H) n = std::max(n, (size_t)a->T * a->B * a->H * D * 4);
-  return n;
+  return align_up(la_starts_bytes(a), 256) + n;
 }
 
-extern "C" int lsh_linattn_bwd(const lsh_linattn* a, const void* d_o, int64_t do_st, int64_t do_sb,
-                               int64_t do_sh, const float* ds_end, void* dq, void* dk, void* dv,
-                               float* ds0, void* ws, size_t ws_bytes, void* stream) {
+extern "C" int lsh_linattn_bwd(const lsh_linattn* a, const void* starts, const void* d_o, int64_t do_st,
+                               int64_t do_sb, int64_t do_sh, const float* ds_end, void* dq, void* dk,
+                               void* dv, float* ds0, void* ws, size_t ws_bytes, void* stream) {
   if (int rc = la_check(a)) return rc;
   if (a->B == 0 || a->H == 0) return LSH_OK;
   if (a->T > 0 && (bad_ptr(d_o) || bad_ptr(dq) || bad_ptr(dk) || bad_ptr(dv))) return LSH_ERR_ARG;
+  const LaSplit split = la_split_of(a);
   const size_t need = lsh_linattn_bwd_workspace(a);
-  if (need && (bad_ptr(ws) || ws_bytes < need)) return LSH_ERR_WORKSPACE;
+  if ((need && (bad_ptr(ws) || ws_bytes < need)) || (split.segs > 1 && bad_ptr(starts)))
+    return LSH_ERR_WORKSPACE;
   hipStream_t st = (hipStream_t)stream;
-  const LaIn q = la_in(a->q, a->q_st, a->q_sb, a->q_sh, a->H, a->q_heads);
-  const LaIn k = la_in(a->k, a->k_st, a->k_sb, a->k_sh, a->H, a->k_heads);
-  const LaIn v = la_in(a->v, a->v_st, a->v_sb, a->v_sh, a->H, a->v_heads);
-  const LaIn d = la_in(d_o, do_st, do_sb, do_sh, a->H, (int)a->H);
+  float* e_starts = (float*)ws;
+  float* heads_f32 = (float*)((char*)ws + align_up(la_starts_bytes(a), 256));
+  const LaIn q = la_q(a), k = la_k(a), v = la_v(a);
+  const LaIn d = la_in(d_o, do_st, do_sb, do_sh, a->H, (int)a->H, a->dtype, a->Dv);
   LaWalk w = {};
   w.beta = a->beta;
   w.T = a->T, w.B = a->B, w.H = a->H;
+  la_set_split(w, split);
   auto run = [&](void* out, int heads) -> int {
     const bool shared = heads != a->H;
-    w.out = shared ? ws : out;
-    if (int rc = la_walk(w, a->dtype, shared, st)) return rc;
+    w.out = shared ? heads_f32 : out;
+    w.out_f32 = shared || a->dtype == LSH_F32;
+    if (int rc = la_go(w, a->dtype, false, st)) return rc;
     if (shared && a->T > 0) {
       const int64_t n = a->T * a->B * heads * w.DV;
       with_dtype(a->dtype, [&](auto t) {
         using T = decltype(t);
-        k_la_share<T><<<dim3((unsigned)((n + 255) / 256)), 256, 0, st>>>((const float*)ws, (T*)out, n,
-                                                                        w.DV, (int)(a->H / heads));
+        k_la_share<T><<<dim3((unsigned)((n + 255) / 256)), 256, 0, st>>>(heads_f32, (T*)out, n, w.DV,
+                                                                        (int)(a->H / heads));
       });
       LSH_CHECK_LAUNCH();
     }
@@ -259,16 +258,22 @@ extern "C" int lsh_linattn_bwd(const lsh_linattn* a, const void* d_o, int64_t do
   // dq: the forward walk with the state transposed
   w.q = d, w.k = v, w.v = k;
   w.DK = a->Dv, w.DV = a->Dk, w.sk = 1, w.sv = a->Dv;
-  w.s_in = a->s0, w.so = a->scale, w.su = 1.0f;
+  w.s_in = split.segs > 1 ? (const float*)starts : a->s0;
+  w.so = a->scale, w.su = 1.0f;
   if (int rc = run(dq, a->q_heads)) return rc;
-  // dk, from the last row
-  w.q = v, w.k = d, w.v = q;
-  w.rev = 1, w.late = 1, w.s_in = ds_end, w.so = 1.0f, w.su = a->scale;
-  if (int rc = run(dk, a->k_heads)) return rc;
-  // dv, and the gradient that leaves the first row
+  // dv from the last row, and the gradient that leaves the first
   w.q = k, w.k = q, w.v = d;
-  w.DK = a->Dk, w.DV = a->Dv, w.sk = a->Dv, w.sv = 1, w.s_out = ds0;
-  return run(dv, a->v_heads);
+  w.DK = a->Dk, w.DV = a->Dv, w.sk = a->Dv, w.sv = 1;
+  w.rev = 1, w.late = 1, w.so = 1.0f, w.su = a->scale;
+  if (split.segs > 1)
+    if (int rc = la_starts(w, a->dtype, split, ds_end, e_starts, st)) return rc;
+  w.s_in = split.segs > 1 ? e_starts : ds_end;
+  w.s_out = ds0;
+  if (int rc = run(dv, a->v_heads)) return rc;
+  // dk, likewise with the state transposed
+  w.q = v, w.k = d, w.v = q;
+  w.DK = a->Dv, w.DV = a->Dk, w.sk = 1, w.sv = a->Dv, w.s_out = nullptr;
+  return run(dk, a->k_heads);
 }
 
 extern "C" int lsh_linattn_step(const lsh_linattn* a, float* state, void* stream) {
@@ -276,9 +281,7 @@ extern "C" int lsh_linattn_step(const lsh_linattn* a, float* state, void* stream
   if (a->T != 1) return LSH_ERR_SHAPE;
   if (a->B == 0 || a->H == 0) return LSH_OK;
   if (bad_ptr(a->o) || bad_ptr(state)) return LSH_ERR_ARG;
-  const LaIn q = la_in(a->q, 0, a->q_sb, a->q_sh, a->H, a->q_heads);
-  const LaIn k = la_in(a->k, 0, a->k_sb, a->k_sh, a->H, a->k_heads);
-  const LaIn v = la_in(a->v, 0, a->v_sb, a->v_sh, a->H, a->v_heads);
+  const LaIn q = la_q(a), k = la_k(a), v = la_v(a);
   const dim3 grid((unsigned)(a->B * a->H), (a->Dv + 63) / 64);
   const bool wide = a->Dv % 4 == 0 && (uintptr_t)state % 16 == 0;
   with_dtype(a->dtype, [&](auto t) {

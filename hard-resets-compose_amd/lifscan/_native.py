@@ -182,9 +182,10 @@ SIGNATURES = {
     "lsh_lif_scan_bwd_workspace": (c_sz, [c_i64, c_i64, c_i]),
     "lsh_lif_scan_bwd": (c_i, [c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_i64, c_i64, c_f, c_f, c_f, c_f,
                                c_i, c_i, c_p, c_sz, c_p]),
-    "lsh_linattn_fwd": (c_i, [c_p, c_p]),
+    "lsh_linattn_workspace": (c_sz, [c_p]),
+    "lsh_linattn_fwd": (c_i, [c_p, c_p, c_sz, c_p]),
     "lsh_linattn_bwd_workspace": (c_sz, [c_p]),
-    "lsh_linattn_bwd": (c_i, [c_p, c_p, c_i64, c_i64, c_i64, c_p, c_p, c_p, c_p, c_p, c_p, c_sz, c_p]),
+    "lsh_linattn_bwd": (c_i, [c_p, c_p, c_p, c_i64, c_i64, c_i64, c_p, c_p, c_p, c_p, c_p, c_p, c_sz, c_p]),
     "lsh_linattn_step": (c_i, [c_p, c_p, c_p]),
     "lsh_block_norm_fwd": (c_i, [c_p, c_p, c_p, c_p]),
     "lsh_block_norm_bwd_workspace": (c_sz, [c_p]),

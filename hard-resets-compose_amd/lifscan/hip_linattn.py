@@ -95,12 +95,15 @@ def _forward(q, k, v, beta, s0, scale):
     o = torch.empty(a.T, a.B, a.H, a.Dv, dtype=q.dtype, device=q.device)
     s_end = torch.empty(shape, dtype=torch.float32, device=q.device)
     a.o, a.s_end = o.data_ptr(), s_end.data_ptr()
+    lib = _n.lib()
+    nbytes = lib.lsh_linattn_workspace(ctypes.byref(a))
+    ws = _n.workspace(nbytes, q.device) if nbytes else None
     with _n.on_device(q):
-        _n.check(_n.lib().lsh_linattn_fwd(ctypes.byref(a), _n.stream_of(q)), "lsh_linattn_fwd")
-    return o, s_end, (q, k, v, beta, s0)
+        _n.check(lib.lsh_linattn_fwd(ctypes.byref(a), _n.ptr(ws), nbytes, _n.stream_of(q)), "lsh_linattn_fwd")
+    return o, s_end, (q, k, v, beta, s0, ws)
 
 
-def _backward(q, k, v, beta, s0, scale, do, ds_end, want_ds0):
+def _backward(q, k, v, beta, s0, starts, scale, do, ds_end, want_ds0):
     a, q, k, v, beta = _args(q, k, v, beta, scale, 4)
     a.s0 = _n.ptr(s0)
     dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
@@ -116,7 +119,7 @@ def _backward(q, k, v, beta, s0, scale, do, ds_end, want_ds0):
     ws = _n.workspace(nbytes, q.device) if nbytes else None
     with _n.on_device(q):
         _n.check(lib.lsh_linattn_bwd(
-            ctypes.byref(a), _n.ptr(do), do.stride(0), do.stride(1), do.stride(2), _n.ptr(ds_end),
+            ctypes.byref(a), _n.ptr(starts), _n.ptr(do), do.stride(0), do.stride(1), do.stride(2), _n.ptr(ds_end),
             _n.ptr(dq), _n.ptr(dk), _n.ptr(dv), _n.ptr(ds0), _n.ptr(ws), nbytes, _n.stream_of(q)),
             "lsh_linattn_bwd")
     return dq, dk, dv, ds0
@@ -137,8 +140,8 @@ class LinAttnFn(torch.autograd.Function):
     def backward(ctx, do, ds_end):
         if do is None and ds_end is None:
             return None, None, None, None, None, None
-        q, k, v, beta, s0 = ctx.saved_tensors
-        dq, dk, dv, ds0 = _backward(q, k, v, beta, s0, ctx.scale, do, ds_end, ctx.needs_input_grad[4])
+        q, k, v, beta, s0, starts = ctx.saved_tensors  # starts: the states before the row segments
+        dq, dk, dv, ds0 = _backward(q, k, v, beta, s0, starts, ctx.scale, do, ds_end, ctx.needs_input_grad[4])
         return dq, dk, dv, None, ds0, None
 
 

@@ -536,14 +536,16 @@ typedef struct lsh_linattn {
   float* s_end;
   float scale;
 } lsh_linattn;
-int lsh_linattn_fwd(const lsh_linattn* a, void* stream);
-/* Its gradients: reads q, k, v, s0 of *a (not o, s_end), d_o [T, B, H, Dv] with the given strides
+size_t lsh_linattn_workspace(const lsh_linattn* a); /* 0: ws may be NULL */
+int lsh_linattn_fwd(const lsh_linattn* a, void* ws, size_t ws_bytes, void* stream);
+/* Its gradients: reads q, k, v, s0 of *a (not o, s_end), `starts` as the forward of the same *a left its
+ * workspace (NULL where that has no bytes), d_o [T, B, H, Dv] with the given strides
  * and ds_end = dL/ds_end (fp32, or NULL); writes contiguous dq, dk, dv with the heads of q, k, v
  * (sums over the heads that share one, in fp32 and head order) and ds0 (fp32, or NULL). */
 size_t lsh_linattn_bwd_workspace(const lsh_linattn* a);
-int lsh_linattn_bwd(const lsh_linattn* a, const void* d_o, int64_t do_st, int64_t do_sb, int64_t do_sh,
-                    const float* ds_end, void* dq, void* dk, void* dv, float* ds0, void* ws,
-                    size_t ws_bytes, void* stream);
+int lsh_linattn_bwd(const lsh_linattn* a, const void* starts, const void* d_o, int64_t do_st,
+                    int64_t do_sb, int64_t do_sh, const float* ds_end, void* dq, void* dk, void* dv,
+                    float* ds0, void* ws, size_t ws_bytes, void* stream);
 /* One token (T = 1; the row strides are not read): `state` [B, H, Dk, Dv] is updated in place, o is
  * [B, H, Dv].  s0 and s_end are not read. */
 int lsh_linattn_step(const lsh_linattn* a, float* state, void* stream);
