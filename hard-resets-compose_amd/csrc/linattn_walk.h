@@ -55,7 +55,7 @@ struct La;
 
 template <>
 struct La<bf16_t> {
-  static constexpr int KB = 32, C = 64, TILES = 2;
+    static constexpr int KB = 32, C = 32, TILES = 2;
   // a decayed value is taken in three bf16 parts, which hold its 24 bits: the state is kept to fp32
   static constexpr int PARTS = 3;
   using Frag = bf16x8;
@@ -64,10 +64,14 @@ struct La<bf16_t> {
   static __device__ __forceinline__ f32x4 mma(Frag a, Frag b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
   }
+  // a row's 32 values from their natural order, and from the order of packed()
   static __device__ __forceinline__ Frag row(const bf16_t* p, int g) {
     const bf16x4 a = *(const bf16x4*)(p + 4 * g), b = *(const bf16x4*)(p + 16 + 4 * g);
     return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
   }
+  static __device__ __forceinline__ Frag packed_row(const bf16_t* p, int g) { return *(const Frag*)(p + 8 * g); }
+  // where four values from c on lie when a fragment's eight are to be neighbours
+  static __device__ __forceinline__ int packed(int c) { return (c & ~31) + (c & 12) * 2 + (c & 16) / 4; }
   // column l%16 of 32 rows: the LDS read that transposes blocks of 4 rows by 16 lanes
   static __device__ __forceinline__ Frag col(const bf16_t* p, int pitch, int g, int m) {
     using Lds = __attribute__((address_space(3))) s16x4*;
@@ -98,6 +102,8 @@ struct La<float> {
     return c;
   }
   static __device__ __forceinline__ Frag row(const float* p, int g) { return *(const f32x4*)(p + 4 * g); }
+  static __device__ __forceinline__ Frag packed_row(const float* p, int g) { return row(p, g); }
+  static __device__ __forceinline__ int packed(int c) { return c; }
   static __device__ __forceinline__ Frag col(const float* p, int pitch, int g, int m) {
     Frag f;
 #pragma unroll
@@ -117,288 +123,361 @@ __device__ __forceinline__ const T* la_row(const LaIn& x, int64_t b, int64_t h) 
 __device__ __forceinline__ float la_pow(float l2, int n) { return __builtin_amdgcn_exp2f(l2 * (float)n); }
 __device__ __forceinline__ float la_log2(float beta) { return fmaxf(log2f(beta), -1e4f); }
 
-// A chunk of one operand on its way to LDS: C rows of DP columns (zeros beyond n rows and D columns),
-// 16 bytes a piece, held in registers while the chunk before is worked on.
-template <class T, class L, int C, int DP>
+using u32x2 = unsigned __attribute__((ext_vector_type(2)));
+using u32x4 = unsigned __attribute__((ext_vector_type(4)));
+
+// Rows from a wave-uniform address on, by byte offsets below 2^31; kLaNowhere reads as zeros and is not
+// written.
+constexpr unsigned kLaNowhere = 0x80000000u;
+struct LaRows {
+  __amdgpu_buffer_rsrc_t r;
+  __device__ __forceinline__ explicit LaRows(const void* base)
+      : r(__builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, (int)kLaNowhere, 0x00020000)) {}
+};
+
+// A chunk of one operand on its way to LDS: C rows of DP columns, 16 bytes a piece, held in registers
+// while the chunk before is worked on.  Row i of the n rows of a short chunk comes to row C - n + i, and
+// the rows before it and the columns from D on are zeros: the distance to a chunk's end is the same in
+// every chunk.  The loads have no branches around them (those cost the wait for all of them at the next
+// loop head).  PACKED: in the order of La::packed.
+template <class T, class L, int C, int DP, int THREADS, bool PACKED>
 struct LaStage {
-  static constexpr int W = kWide<T>, PER_ROW = DP / W, N = C * PER_ROW / 256;
-  static_assert(C * PER_ROW % 256 == 0, "whole pieces for 256 threads");
-  Vec<T, W> x[N];
-  __device__ __forceinline__ void load(const T* base, int64_t st, bool wide, int D, int64_t t0, int rev,
-                                       int n) {
+  static constexpr int W = kWide<T>, PER_ROW = DP / W, ROWS = THREADS / PER_ROW;  // rows a piece of all threads
+  static constexpr int N = C > ROWS ? C / ROWS : 1;
+  static_assert(THREADS % PER_ROW == 0 && (C % ROWS == 0 || ROWS % C == 0), "whole rows");
+  u32x4 x[N];
+  unsigned at;  // this thread's first piece, in bytes from the chunk's lowest row
+  int r0;
+  // step: bytes from a row to the next in memory
+  __device__ __forceinline__ void init(unsigned step, int rev, int D) {
+    r0 = threadIdx.x / PER_ROW;
+    const int c = threadIdx.x % PER_ROW * W;
+    at = (rev ? C - 1 - r0 : r0) * step + c * (unsigned)sizeof(T);
+    if (c >= D || r0 >= C) at = kLaNowhere;
+  }
+  // the chunk's last n rows; low: the lowest address of a whole chunk
+  __device__ __forceinline__ void load(const T* low, unsigned step, int rev, int n) {
+    const LaRows rows(low);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int u = threadIdx.x + 256 * i, r = u / PER_ROW, c = u % PER_ROW * W;
-      const T* p = base + (rev ? t0 - r : t0 + r) * st + c;
-      if (wide) {
-        if (r < n && c < D) {
-          x[i] = *(const Vec<T, W>*)p;
-        } else {
-#pragma unroll
-          for (int j = 0; j < W; ++j) x[i].v[j] = (T)0.0f;
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < W; ++j) x[i].v[j] = r < n && c + j < D ? p[j] : (T)0.0f;
-      }
+      const unsigned o = at == kLaNowhere || r0 + i * ROWS < C - n ? kLaNowhere
+                         : rev                                     ? at - i * ROWS * step
+                                                                   : at + i * ROWS * step;
+      x[i] = __builtin_amdgcn_raw_buffer_load_b128(rows.r, o, 0, 0);
     }
   }
   __device__ __forceinline__ void put(L* lds, int pitch) const {
+    const int c = threadIdx.x % PER_ROW * W;
+    if (ROWS > C && r0 >= C) return;
+    constexpr int Q = PACKED ? 4 : kWide<L>;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int u = threadIdx.x + 256 * i, r = u / PER_ROW, c = u % PER_ROW * W;
+      const Vec<T, W> z = __builtin_bit_cast(Vec<T, W>, x[i]);
       Vec<L, W> y;
 #pragma unroll
-      for (int j = 0; j < W; ++j) y.v[j] = (L)x[i].v[j];
-      constexpr int Q = kWide<L>;
+      for (int j = 0; j < W; ++j) y.v[j] = (L)z.v[j];
 #pragma unroll
-      for (int j = 0; j < W; j += Q) *(Vec<L, Q>*)&lds[r * pitch + c + j] = *(Vec<L, Q>*)&y.v[j];
+      for (int j = 0; j < W; j += Q)
+        *(Vec<L, Q>*)&lds[(r0 + i * ROWS) * pitch + (PACKED ? La<L>::packed(c + j) : c + j)] = *(Vec<L, Q>*)&y.v[j];
+    }
+  }
+  // operands whose rows cannot be read 16 bytes at a time come straight from memory, element by element
+  static __device__ __forceinline__ void copy(L* lds, int pitch, const T* p, int64_t step, int D, int n) {
+#pragma unroll 1
+    for (int u = threadIdx.x; u < C * DP; u += THREADS) {
+      const int r = u / DP, c = u % DP;
+      lds[r * pitch + (PACKED ? La<L>::packed(c & ~3) + (c & 3) : c)] =
+          r >= C - n && c < D ? (L)p[r * step + c] : (L)0.0f;
     }
   }
 };
 
 __device__ __forceinline__ bool la_odd(float x) { return !(fabsf(x) < INFINITY); }
 
+// Four columns of the chunk's rows i*16 + m to the output, o[i] to byte at + i*16*step (or -) from low.
+template <class TO, int CT>
+__device__ __forceinline__ void la_store(TO* low, unsigned at, unsigned step, int rev, const f32x4 (&o)[CT],
+                                         int first) {
+  const LaRows rows(low);
+#pragma unroll
+  for (int i = 0; i < CT; ++i) {
+    Vec<TO, 4> y;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y.v[e] = from_f<TO>(o[i][e]);
+    const unsigned b = at == kLaNowhere || i * 16 < first ? kLaNowhere
+                       : rev                              ? at - i * 16 * step
+                                                          : at + i * 16 * step;
+    if constexpr (sizeof(TO) == 4)
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, y), rows.r, b, 0, 0);
+    else
+      __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, y), rows.r, b, 0, 0);
+  }
+}
+// The same element by element: p is row m's first column, left of them are there.
+template <class TO, int CT>
+__device__ __forceinline__ void la_store_some(TO* p, int64_t step, const f32x4 (&o)[CT], int first, int left) {
+#pragma unroll
+  for (int i = 0; i < CT; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (i * 16 >= first && e < left) p[i * 16 * step + e] = from_f<TO>(o[i][e]);
+}
+
+// Whether any of a fragment's values is not finite.
+__device__ __forceinline__ bool la_odd(bf16x8 x) {
+  // the exponent's bits, plus one in its last place: all ones carry into the bit above
+  const u32x4 b = __builtin_bit_cast(u32x4, x);
+  unsigned any = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) any |= (b[i] & 0x7f807f80u) + 0x00800080u;
+  return (any & 0x80008000u) != 0;
+}
+__device__ __forceinline__ bool la_odd(f32x4 x) {
+  bool any = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) any |= la_odd(x[i]);
+  return any;
+}
+
 // The walk.  SUMS: only the segments' sums (the state after each segment from a zero state before
 // it), written to s_out [segments, B*H] one place further on (segment s to s + 1), for every segment
-// but the last.
+// but the last.  WIDE: every row is read and written in whole pieces (la_wide).
 //
-// Four waves; a wave owns NT*16 state columns and all DKP rows of them (the accumulators S), the four
-// together a block of NT*64 columns.  Scores are computed once, their 16x16 tiles dealt to the waves,
-// and shared through LDS.  All products are taken transposed (columns of the state by rows of the
-// chunk), so scores, states and decayed values go from accumulator to operand in registers.
+// W waves; a wave owns 16 state columns and all DKP rows of them (the accumulators S).  Scores are
+// computed once, their 16x16 tiles dealt to the waves, and shared through LDS.  All products are taken
+// transposed (columns of the state by rows of the chunk), so scores, states and decayed values go from
+// accumulator to operand in registers.
 //
-// LDS rows are padded: by 4 dwords modulo 64 where rows are read (16 rows of 8 or 16 bytes meet
-// different banks), by 8 where the transposing read takes 8 rows of 32 bytes at once.
-template <class T, class L, int DKP, int NT, bool SUMS>
-__global__ __launch_bounds__(256, DKP <= 128 ? 2 : 1) void k_la_walk(LaWalk a) {
+// LDS rows are padded: by 4 dwords modulo 64 where rows are read (16 rows of 16 bytes meet different
+// banks), by 8 where the transposing read takes 8 rows of 32 bytes at once.
+template <class T, class L, int DKP, int W, bool SUMS, bool WIDE>
+__global__ __launch_bounds__(W * 64, DKP > 128 ? W / 4 : 2) void k_la_walk(LaWalk a) {
   using X = La<L>;
   using Frag = typename X::Frag;
-  constexpr int C = X::C, KB = X::KB, DVB = NT * 64, KT = DKP / 16, CT = C / 16, KS = DKP / KB, CS = C / KB;
+  constexpr int C = X::C, KB = X::KB, DVB = W * 16, KT = DKP / 16, CT = C / 16, KS = DKP / KB, CS = C / KB;
+  static_assert(CT * (CT + 1) / 2 <= W, "a wave has one tile of the scores at most");
   constexpr int PQ = DKP + X::kPadRow, PK = DKP + X::kPadCol, PV = DVB + X::kPadCol, PP = C + X::kPadRow;
-  __shared__ alignas(16) L s_q[SUMS ? 1 : C * PQ], s_k[C * PK], s_v[C * PV], s_p[SUMS ? 1 : C * PP];
+  constexpr int HALVES = WIDE ? 2 : 1;  // of LDS: one is filled while the other is read
+  __shared__ alignas(16) L s_q[SUMS ? 8 : HALVES * C * PQ], s_k[HALVES * C * PK], s_v[HALVES * C * PV];
+  __shared__ alignas(16) L s_p[SUMS ? 8 : C * PP];
 
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, m = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t BH = a.B * a.H;
-  const int64_t seg = blockIdx.x / BH, bh = blockIdx.x % BH, b = bh / a.H, h = bh % a.H;
-  const int dv0 = blockIdx.y * DVB, wc = w * NT * 16;  // the block's first column, the wave's within it
+  const int blocks = (a.DV + DVB - 1) / DVB;
+  const int64_t job = xcd_neuron(blockIdx.x, gridDim.x), pair = job / blocks;
+  const int64_t seg = pair / BH, bh = pair % BH, b = bh / a.H, h = bh % a.H;
+  const int dv0 = (int)(job % blocks) * DVB, wc = w * 16;  // the block's first column, the wave's within it
   const int64_t r0 = seg * a.L, r1 = min(a.T, r0 + a.L);
-  const float l2 = la_log2(a.beta[h]);
-
   const T* q = la_row<T>(a.q, b, h);
   const T* k = la_row<T>(a.k, b, h);
   const T* v = la_row<T>(a.v, b, h) + dv0;
 
+  // state element (i*16 + 4g + e, m) of the wave's columns is at i*16*sk + e*sk from here
   const size_t size = (size_t)a.DK * a.DV;
-  f32x4 S[KT][NT];
+  int at0 = 4 * g * a.sk + (dv0 + wc + m) * a.sv;
+  const bool col = dv0 + wc + m < a.DV;
+  f32x4 S[KT];
+  {
+    const float* from = a.s_in + (size_t)(seg * BH + bh) * size;
 #pragma unroll
-  for (int i = 0; i < KT; ++i)
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
+    for (int i = 0; i < KT; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int dk = i * 16 + 4 * g + e, dv = dv0 + wc + t * 16 + m;
-        S[i][t][e] = 0.0f;
-        if (!SUMS && a.s_in && dk < a.DK && dv < a.DV)
-          S[i][t][e] = a.s_in[(size_t)(seg * BH + bh) * size + (size_t)dk * a.sk + (size_t)dv * a.sv];
+        S[i][e] = 0.0f;
+        if (!SUMS && a.s_in && col && i * 16 + 4 * g + e < a.DK) S[i][e] = from[at0 + (i * 16 + e) * a.sk];
       }
+  }
   if (!SUMS) {
-    for (int i = threadIdx.x; i < C * PP; i += 256) s_p[i] = (L)0.0f;  // tiles above the diagonal stay so
+    for (int i = threadIdx.x; i < C * PP; i += W * 64) s_p[i] = (L)0.0f;  // tiles above the diagonal stay so
   }
 
-  LaStage<T, L, C, DKP> xq, xk;
-  LaStage<T, L, C, DVB> xv;
-  auto fetch = [&](int64_t r) {
-    const int n = (int)min((int64_t)C, r1 - r);
-    const int64_t t0 = a.rev ? a.T - 1 - r : r;
-    if (!SUMS) xq.load(q, a.q.st, a.q.wide, a.DK, t0, a.rev, n);
-    xk.load(k, a.k.st, a.k.wide, a.DK, t0, a.rev, n);
-    xv.load(v, a.v.st, a.v.wide, a.DV - dv0, t0, a.rev, n);
-  };
-  if (r0 < r1) fetch(r0);
-  for (int64_t r = r0; r < r1; r += C) {
-    const int n = (int)min((int64_t)C, r1 - r);
-    __syncthreads();  // everyone has read the chunk before
-    if (!SUMS) xq.put(s_q, PQ);
-    xk.put(s_k, PK);
-    xv.put(s_v, PV);
-    __syncthreads();
-    if (r + C < r1) fetch(r + C);
 
-    f32x4 o[NT][CT];
+  // row r of the walk is row (rev ? T - 1 - r : r); the first chunk is the short one
+  int n = r0 < r1 ? (int)((r1 - r0 - 1) % C) + 1 : 0;
+  int64_t r = r0 + n - C;  // where the chunk's row 0 would be
+  const float l2 = la_log2(a.beta[h]);
+  float decay[CS][KB / 4];  // of the rows to the chunk's end
+#pragma unroll
+  for (int s = 0; s < CS; ++s)
+#pragma unroll
+    for (int e = 0; e < KB / 4; ++e)
+      decay[s][e] = a.su * la_pow(l2, C - 1 - (s * KB + X::at(e) + 4 * g) + a.late);
+  // this wave's tile of the scores: rows 16*ti + m against rows 16*tj + 4g + e
+  const int ti = w == 0 ? 0 : w < 3 ? 1 : w < 6 ? 2 : 3, tj = w - ti * (ti + 1) / 2;
+  float fall[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) fall[e] = a.so * a.su * la_pow(l2, max((ti - tj) * 16 + m - 4 * g - e, 0));
+
+  LaStage<T, L, C, DKP, W * 64, true> xq;
+  LaStage<T, L, C, DKP, W * 64, false> xk;
+  LaStage<T, L, C, DVB, W * 64, false> xv;
+  // the row of lowest address of the chunk whose row 0 is at r
+  auto low = [&](int64_t r) { return a.rev ? a.T - r - C : r; };
+  const unsigned bq = (unsigned)a.q.st * sizeof(T), bk = (unsigned)a.k.st * sizeof(T), bv = (unsigned)a.v.st * sizeof(T);
+  auto fetch = [&](int64_t r, int n) {
+    if (!SUMS) xq.load(q + low(r) * a.q.st, bq, a.rev, n);
+    xk.load(k + low(r) * a.k.st, bk, a.rev, n);
+    xv.load(v + low(r) * a.v.st, bv, a.rev, n);
+  };
+  auto put = [&](int half) {
+    if (!SUMS) xq.put(s_q + half * (C * PQ), PQ);
+    xk.put(s_k + half * (C * PK), PK);
+    xv.put(s_v + half * (C * PV), PV);
+  };
+  auto copy = [&](int64_t r, int n) {  // not WIDE
+    const int64_t t0 = a.rev ? a.T - 1 - r : r, sign = a.rev ? -1 : 1;
+    if (!SUMS) xq.copy(s_q, PQ, q + t0 * a.q.st, sign * a.q.st, a.DK, n);
+    xk.copy(s_k, PK, k + t0 * a.k.st, sign * a.k.st, a.DK, n);
+    xv.copy(s_v, PV, v + t0 * a.v.st, sign * a.v.st, a.DV - dv0, n);
+  };
+  const int64_t so = BH * a.DV;  // elements from a row of the output to the next
+  const int dv = dv0 + wc + 4 * g;
+  const unsigned eo = a.out_f32 ? 4 : sizeof(T), bo = (unsigned)so * eo;
+  const unsigned at_o = dv < a.DV ? (a.rev ? C - 1 - m : m) * bo + (wc + 4 * g) * eo : kLaNowhere;
+  if (WIDE) {
+    xq.init(bq, a.rev, a.DK), xk.init(bk, a.rev, a.DK), xv.init(bv, a.rev, a.DV - dv0);
+    if (n) {
+      fetch(r, n);
+      put(0);
+      fetch(r + C, r + 2 * C <= r1 ? C : 0);
+    }
+    __syncthreads();
+  }
+  int half = 0;
+  for (; n && r + C <= r1; r += C, n = C) {
+    if (!WIDE) {
+      __syncthreads();  // everyone has read the chunk before
+      copy(r, n);
+      __syncthreads();
+    }
+    const L *cq = s_q + half * (C * PQ), *ck = s_k + half * (C * PK), *cv = s_v + half * (C * PV);
     if (!SUMS) {
-      // scores of rows 16i.. against rows 16j.., j <= i, with their decays
-      int tile = 0;
+      // scores with their decays
+      if (w < CT * (CT + 1) / 2) {
+        f32x4 p = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int i = 0; i < CT; ++i)
+        for (int s = 0; s < KS; ++s)
+          p = X::mma(X::row(&ck[(tj * 16 + m) * PK + s * KB], g), X::packed_row(&cq[(ti * 16 + m) * PQ + s * KB], g), p);
+        typename X::Quad y;
 #pragma unroll
-        for (int j = 0; j <= i; ++j, ++tile) {
-          if ((tile & 3) != w) continue;
-          f32x4 p = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-          for (int s = 0; s < KS; ++s)
-            p = X::mma(X::row(&s_k[(j * 16 + m) * PK + s * KB], g), X::row(&s_q[(i * 16 + m) * PQ + s * KB], g), p);
-          typename X::Quad y;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int far = (i - j) * 16 + m - 4 * g - e;
-            y[e] = (L)(far >= 0 ? p[e] * (a.so * a.su) * la_pow(l2, far) : 0.0f);
-          }
-          *(typename X::Quad*)&s_p[(i * 16 + m) * PP + j * 16 + 4 * g] = y;
-        }
+        for (int e = 0; e < 4; ++e)
+          y[e] = (L)((ti - tj) * 16 + m - 4 * g - e >= 0 ? p[e] * fall[e] : 0.0f);
+        *(typename X::Quad*)&s_p[(ti * 16 + m) * PP + X::packed(tj * 16 + 4 * g)] = y;
+      }
       // what the state before the chunk gives
+      f32x4 o[CT];
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int i = 0; i < CT; ++i) o[t][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int i = 0; i < CT; ++i) o[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
-        Frag st[NT];
+        const Frag st = X::of(&S[s * X::TILES]);
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          f32x4 x[X::TILES];
-#pragma unroll
-          for (int e = 0; e < X::TILES; ++e) x[e] = S[s * X::TILES + e][t];
-          st[t] = X::of(x);
-        }
-#pragma unroll
-        for (int i = 0; i < CT; ++i) {
-          const Frag x = X::row(&s_q[(i * 16 + m) * PQ + s * KB], g);
-#pragma unroll
-          for (int t = 0; t < NT; ++t) o[t][i] = X::mma(st[t], x, o[t][i]);
-        }
+        for (int i = 0; i < CT; ++i) o[i] = X::mma(st, X::packed_row(&cq[(i * 16 + m) * PQ + s * KB], g), o[i]);
       }
+      const int first = C - n - m;  // a lane's rows of the chunk are those with 16i >= first
 #pragma unroll
-      for (int i = 0; i < CT; ++i) {
-        const float f = a.so * la_pow(l2, i * 16 + m + 1 - a.late);
-#pragma unroll
-        for (int t = 0; t < NT; ++t) o[t][i] *= f;
-      }
+      for (int i = 0; i < CT; ++i) o[i] *= a.so * la_pow(l2, max(i * 16 - first, 0) + 1 - a.late);
       __syncthreads();  // the scores are there
+
+      // what the chunk's own rows give
+      Frag x[CS];
+      bool odd = false;
+#pragma unroll
+      for (int s = 0; s < CS; ++s) {
+        x[s] = X::col(&cv[s * KB * PV + wc], PV, g, m);
+        odd |= la_odd(x[s]);
+      }
+      if (wave_ballot(odd)) {
+        // values that are not finite must not meet the zero scores of the rows before them
+#pragma unroll 1
+        for (int j = C - n; j < C; ++j) {
+          const typename X::Quad y = *(const typename X::Quad*)&cv[j * PV + wc + 4 * g];
+#pragma unroll
+          for (int i = 0; i < CT; ++i) {
+            const float p = (float)s_p[(i * 16 + m) * PP + X::packed(j & ~3) + (j & 3)];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[i][e] += i * 16 + m >= j ? p * (float)y[e] : 0.0f;
+          }
+        }
+      } else {
+#pragma unroll
+        for (int s = 0; s < CS; ++s)
+#pragma unroll
+          for (int i = 0; i < CT; ++i)
+            if (s * X::TILES <= i) o[i] = X::mma(x[s], X::packed_row(&s_p[(i * 16 + m) * PP + s * KB], g), o[i]);
+      }
+      if (WIDE) {
+        const int64_t to = (low(r) * BH + bh) * a.DV + dv0;
+        if (a.out_f32)
+          la_store<float, CT>((float*)a.out + to, at_o, bo, a.rev, o, first);
+        else
+          la_store<T, CT>((T*)a.out + to, at_o, bo, a.rev, o, first);
+      } else {
+        const int64_t to = ((a.rev ? a.T - 1 - r - m : r + m) * BH + bh) * a.DV + dv;
+        if (a.out_f32)
+          la_store_some<float, CT>((float*)a.out + to, a.rev ? -so : so, o, first, a.DV - dv);
+        else
+          la_store_some<T, CT>((T*)a.out + to, a.rev ? -so : so, o, first, a.DV - dv);
+      }
     }
 
     const float whole = la_pow(l2, n);
 #pragma unroll
-    for (int i = 0; i < KT; ++i)
-#pragma unroll
-      for (int t = 0; t < NT; ++t) S[i][t] *= whole;
-    bool odd = false;
+    for (int i = 0; i < KT; ++i) S[i] *= whole;
 #pragma unroll
     for (int s = 0; s < CS; ++s) {
-      Frag x[NT], part[NT][X::PARTS];
-      float decay[KB / 4];
+      const Frag x = X::col(&cv[s * KB * PV + wc], PV, g, m);
+      Frag part[X::PARTS];
 #pragma unroll
       for (int e = 0; e < KB / 4; ++e) {
-        const int left = n - 1 - (s * KB + X::at(e) + 4 * g);
-        decay[e] = left >= 0 ? a.su * la_pow(l2, left + a.late) : 0.0f;
-      }
+        float rest = (float)x[e] * decay[s][e];
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        x[t] = X::col(&s_v[s * KB * PV + wc + t * 16], PV, g, m);
-#pragma unroll
-        for (int e = 0; e < KB / 4; ++e) {
-          const float y = (float)x[t][e];
-          const bool bad = la_odd(y);
-          odd |= bad;
-          float rest = y * decay[e];
-#pragma unroll
-          for (int c = 0; c < X::PARTS; ++c) {
-            const L top = (L)rest;
-            part[t][c][e] = top;
-            rest = bad ? 0.0f : rest - (float)top;
-          }
-          // a value that is not finite must not meet the zero scores of the rows before it
-          if (bad) x[t][e] = (L)0.0f;
-        }
-      }
-      if (!SUMS) {
-#pragma unroll
-        for (int i = 0; i < CT; ++i) {
-          if (s * X::TILES > i) continue;
-          const Frag p = X::row(&s_p[(i * 16 + m) * PP + s * KB], g);
-#pragma unroll
-          for (int t = 0; t < NT; ++t) o[t][i] = X::mma(x[t], p, o[t][i]);
+        for (int c = 0; c < X::PARTS; ++c) {
+          const L top = (L)rest;
+          part[c][e] = top;
+          rest -= (float)top;
         }
       }
 #pragma unroll
       for (int i = 0; i < KT; ++i) {
-        const Frag y = X::col(&s_k[s * KB * PK + i * 16], PK, g, m);
+        const Frag y = X::col(&ck[s * KB * PK + i * 16], PK, g, m);
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int c = 0; c < X::PARTS; ++c) S[i][t] = X::mma(y, part[t][c], S[i][t]);
+        for (int c = 0; c < X::PARTS; ++c) S[i] = X::mma(y, part[c], S[i]);
       }
     }
-
-    if (!SUMS) {
-      if (wave_ballot(odd)) {
-        // the values left out above, row by row for the rows from theirs on
-        for (int j = 0; j < n; ++j)
-#pragma unroll
-          for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float y = (float)s_v[j * PV + wc + t * 16 + 4 * g + e];
-              if (la_odd(y))
-#pragma unroll
-                for (int i = 0; i < CT; ++i)
-                  if (i * 16 + m >= j) o[t][i][e] += y * (float)s_p[(i * 16 + m) * PP + j];
-            }
-      }
-#pragma unroll
-      for (int i = 0; i < CT; ++i) {
-        if (i * 16 + m >= n) continue;
-        const int64_t row = a.rev ? a.T - 1 - (r + i * 16 + m) : r + i * 16 + m;
-        const size_t at = (size_t)(row * BH + bh) * a.DV;
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          const int dv = dv0 + wc + t * 16 + 4 * g;
-          if (dv >= a.DV) continue;
-          const bool four = a.DV % 4 == 0;
-          if (a.out_f32) {
-            float* p = (float*)a.out + at + dv;
-            if (four) {
-              *(f32x4*)p = o[t][i];
-            } else {
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (dv + e < a.DV) p[e] = o[t][i][e];
-            }
-          } else {
-            T* p = (T*)a.out + at + dv;
-            Vec<T, 4> y;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) y.v[e] = from_f<T>(o[t][i][e]);
-            if (four) {
-              *(Vec<T, 4>*)p = y;
-            } else {
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (dv + e < a.DV) p[e] = y.v[e];
-            }
-          }
-        }
-      }
+    if (WIDE) {
+      half ^= 1;
+      put(half);  // zeros after the last chunk
+      fetch(r + 2 * C, r + 3 * C <= r1 ? C : 0);
+      __syncthreads();  // the next chunk is there, and the scores have been read
     }
   }
 
   if (SUMS || (a.s_out && seg == a.segs - 1)) {
     float* to = a.s_out + (size_t)(SUMS ? (seg + 1) * BH + bh : bh) * size;
+    asm volatile("" : "+v"(at0));  // or the first loads' addresses are held in registers up to here
 #pragma unroll
     for (int i = 0; i < KT; ++i)
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int dk = i * 16 + 4 * g + e, dv = dv0 + wc + t * 16 + m;
-          if (dk < a.DK && dv < a.DV) to[(size_t)dk * a.sk + (size_t)dv * a.sv] = S[i][t][e];
-        }
+      for (int e = 0; e < 4; ++e)
+        if (col && i * 16 + 4 * g + e < a.DK) to[at0 + (i * 16 + e) * a.sk] = S[i][e];
   }
 }
 
 // Rows of a chunk for a dtype code, and columns of a workgroup's block for widths DK, DV.
 inline int la_chunk(int dtype) { return dtype == LSH_BF16 ? La<bf16_t>::C : La<float>::C; }
+// 128 columns read Q and K and form the scores once where two blocks of 64 do it twice (4096 x 4 x 16 x
+// 128, forward and backward: 425 us, with blocks of 64 461); 256 rows of a state leave LDS for 64 only.
 inline int la_block(int DK, int DV) { return DK <= 128 && DV > 64 ? 128 : 64; }
+
+// Whether the walk's rows can be read and written in whole pieces: a chunk's byte offsets stay below
+// 2^30 and the output's columns come in fours.
+inline bool la_wide(const LaWalk& a, int chunk) {
+  const int64_t most = ((int64_t)1 << 30) / 4 / chunk;
+  auto near = [&](const LaIn& x) { return x.wide && x.st >= 0 && x.st < most; };
+  return near(a.q) && near(a.k) && near(a.v) && a.DV % 4 == 0 && a.B * a.H * a.DV < most;
+}
 
 // Launches the walk (its sums: SUMS) for operands of T computed in L.
 template <class T, class L>
@@ -406,26 +485,31 @@ inline int la_launch(const LaWalk& a, bool sums, hipStream_t st) {
   const int64_t n = a.B * a.H * (sums ? a.segs - 1 : a.segs);
   if (n == 0) return LSH_OK;
   const int block = la_block(a.DK, a.DV);
-  const dim3 grid((unsigned)n, (a.DV + block - 1) / block);
-  auto go = [&](auto dkp, auto nt) {
-    constexpr int DKP = decltype(dkp)::value, NT = decltype(nt)::value;
-    if (sums)
-      k_la_walk<T, L, DKP, NT, true><<<grid, 256, 0, st>>>(a);
+  const dim3 grid((unsigned)(n * ((a.DV + block - 1) / block)));
+  const bool wide = la_wide(a, La<L>::C);
+  auto go = [&](auto dkp, auto waves) {
+    constexpr int DKP = decltype(dkp)::value, W = decltype(waves)::value;
+    if (sums && wide)
+      k_la_walk<T, L, DKP, W, true, true><<<grid, W * 64, 0, st>>>(a);
+    else if (sums)
+      k_la_walk<T, L, DKP, W, true, false><<<grid, W * 64, 0, st>>>(a);
+    else if (wide)
+      k_la_walk<T, L, DKP, W, false, true><<<grid, W * 64, 0, st>>>(a);
     else
-      k_la_walk<T, L, DKP, NT, false><<<grid, 256, 0, st>>>(a);
+      k_la_walk<T, L, DKP, W, false, false><<<grid, W * 64, 0, st>>>(a);
   };
   auto with = [&](auto dkp) {
     if (block == 128)
-      go(dkp, std::integral_constant<int, 2>{});
+      go(dkp, std::integral_constant<int, 8>{});
     else
-      go(dkp, std::integral_constant<int, 1>{});
+      go(dkp, std::integral_constant<int, 4>{});
   };
   if (a.DK <= 64)
     with(std::integral_constant<int, 64>{});
   else if (a.DK <= 128)
     with(std::integral_constant<int, 128>{});
   else
-    go(std::integral_constant<int, 256>{}, std::integral_constant<int, 1>{});
+    go(std::integral_constant<int, 256>{}, std::integral_constant<int, 4>{});
   LSH_CHECK_LAUNCH();
   return LSH_OK;
 }
