@@ -251,7 +251,7 @@ __device__ __forceinline__ bool la_odd(f32x4 x) {
 // LDS rows are padded: by 4 dwords modulo 64 where rows are read (16 rows of 16 bytes meet different
 // banks), by 8 where the transposing read takes 8 rows of 32 bytes at once.
 template <class T, class L, int DKP, int W, bool SUMS, bool WIDE>
-__global__ __launch_bounds__(W * 64, DKP > 128 ? W / 4 : 2) void k_la_walk(LaWalk a) {
+__global__ __launch_bounds__(W * 64, DKP > 128 ? W / 4 : W == 8 && sizeof(L) == 2 ? 4 : 2) void k_la_walk(LaWalk a) {
   using X = La<L>;
   using Frag = typename X::Frag;
   constexpr int C = X::C, KB = X::KB, DVB = W * 16, KT = DKP / 16, CT = C / 16, KS = DKP / KB, CS = C / KB;
