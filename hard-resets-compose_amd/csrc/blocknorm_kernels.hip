@@ -12,39 +12,11 @@
 //   m = dn*w_post,   dy = ry*(m - y*ry^2*<m*y>)
 //   dw_pre = sum gz*x_new*rx,  dw_post = sum dn*y*ry,  da = sum dx*h      over the rows
 // Bound by the rows' bytes; x_new is computed again instead of being kept.
+#include <type_traits>
+
 #include "lsh_lm.h"
 
 namespace lsh {
-
-constexpr int kBnThreads = 256;
-
-template <int N>
-__device__ __forceinline__ void block_sums(float (&v)[N], float* s) {
-#pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = wave_sum_f(v[i]);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0)
-#pragma unroll
-    for (int i = 0; i < N; ++i) s[(threadIdx.x >> 6) * N + i] = v[i];
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    v[i] = 0.0f;
-    for (int w = 0; w < kBnThreads / 64; ++w) v[i] += s[w * N + i];
-  }
-}
-
-// act(g) and its derivative
-__device__ __forceinline__ float bn_act(int act, float g, float& d) {
-  if (act == LSH_GATE_NONE) {
-    d = 0.0f;
-    return 1.0f;
-  }
-  const float sg = 1.0f / (1.0f + expf(-g));
-  const float ds = sg * (1.0f - sg);
-  d = act == LSH_GATE_SILU ? __builtin_fmaf(g, ds, sg) : ds;
-  return act == LSH_GATE_SILU ? g * sg : sg;
-}
 
 struct BnArgs {
   const void *x, *y, *gate;
@@ -59,114 +31,250 @@ struct BnArgs {
   float* part;  // [grid, 3, D]: this workgroup's sums of dw_post, dw_pre and da
 };
 
-template <class TX, class TY>
-__global__ __launch_bounds__(kBnThreads) void k_block_norm(BnArgs a) {
-  __shared__ float s_red[kBnThreads / 64];
-  const size_t o = (size_t)blockIdx.x * a.D;
-  const TX* x = (const TX*)a.x + o;
-  const TY* y = (const TY*)a.y + o;
-  const TY* gate = (const TY*)a.gate + o;
-  float r[1] = {0.0f};
-  for (int d = threadIdx.x; d < a.D; d += kBnThreads) {
-    const float v = to_f(y[d]);
-    r[0] = __builtin_fmaf(v, v, r[0]);
-  }
-  block_sums(r, s_red);
-  const float ry = 1.0f / sqrtf(r[0] / a.D + a.eps);
-  auto next = [&](int d) {
-    float unused;
-    const float act = a.act == LSH_GATE_NONE ? 1.0f : bn_act(a.act, to_f(gate[d]), unused);
-    const float n = to_f(y[d]) * ry * a.w_post[d];
-    return __builtin_fmaf(a.scale ? a.scale[d] : a.scale1, act * n, to_f(x[d]));
-  };
-  r[0] = 0.0f;
-  for (int d = threadIdx.x; d < a.D; d += kBnThreads) {
-    const float v = next(d);
-    r[0] = __builtin_fmaf(v, v, r[0]);
-  }
-  block_sums(r, s_red);
-  const float rx = 1.0f / sqrtf(r[0] / a.D + a.eps);
-  for (int d = threadIdx.x; d < a.D; d += kBnThreads) {
-    const float v = next(d);
-    ((TX*)a.x_new)[o + d] = from_f<TX>(v);
-    ((TY*)a.z)[o + d] = from_f<TY>(v * rx * a.w_pre[d]);
+// Sums over the lanes that share a row: one wave, or all W of the workgroup (through s, in wave order).
+template <int W, int N>
+__device__ __forceinline__ void row_sums(float (&v)[N], float* s) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = wave_sum_f(v[i]);
+  if constexpr (W > 1) {
+    const int w = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 0)
+#pragma unroll
+      for (int i = 0; i < N; ++i) s[w * N + i] = v[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      v[i] = s[i];
+#pragma unroll
+      for (int j = 1; j < W; ++j) v[i] += s[j * N + i];
+    }
+    __syncthreads();
   }
 }
 
-template <class TX, class TY>
-__global__ __launch_bounds__(kBnThreads) void k_block_norm_bwd(BnArgs a) {
-  __shared__ float s_red[kBnThreads / 64 * 2];
-  float* part = a.part + (size_t)blockIdx.x * 3 * a.D;
-  for (int d = threadIdx.x; d < 3 * a.D; d += kBnThreads) part[d] = 0.0f;
-  __syncthreads();
+// act(g) and its derivative
+__device__ __forceinline__ float bn_act(int act, float g, float& d) {
+  if (act == LSH_GATE_NONE) {
+    d = 0.0f;
+    return 1.0f;
+  }
+  const float sg = sigmoid_neg(g);
+  const float ds = sg * (1.0f - sg);
+  d = act == LSH_GATE_SILU ? __builtin_fmaf(g, ds, sg) : ds;
+  return act == LSH_GATE_SILU ? g * sg : sg;
+}
+
+// V values of a row from column d on, as fp32: WIDE in one access, otherwise one by one (zeros beyond D).
+template <int V, bool WIDE, class T>
+__device__ __forceinline__ void ld_vals(float (&f)[V], const T* p, int d, int D) {
+  if constexpr (WIDE) {
+    if (d < D) {
+      constexpr int P = V * sizeof(T) > 16 ? 16 / sizeof(T) : V;
+#pragma unroll
+      for (int i = 0; i < V; i += P) {
+        const Vec<T, P> x = *(const Vec<T, P>*)(p + d + i);
+#pragma unroll
+        for (int j = 0; j < P; ++j) f[i + j] = to_f(x.v[j]);
+      }
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) f[j] = 0.0f;
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) f[j] = d + j < D ? to_f(p[d + j]) : 0.0f;
+  }
+}
+template <int V, bool WIDE, class T>
+__device__ __forceinline__ void st_vals(const float (&f)[V], T* p, int d, int D) {
+  if constexpr (WIDE) {
+    if (d < D) {
+      constexpr int P = V * sizeof(T) > 16 ? 16 / sizeof(T) : V;
+#pragma unroll
+      for (int i = 0; i < V; i += P) {
+        Vec<T, P> x;
+#pragma unroll
+        for (int j = 0; j < P; ++j) x.v[j] = from_f<T>(f[i + j]);
+        *(Vec<T, P>*)(p + d + i) = x;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (d + j < D) p[d + j] = from_f<T>(f[j]);
+  }
+}
+
+// A row is held in registers by W waves, E groups of V = 8 columns a lane: columns (e*64*W + lane)*8.
+template <class TX, class TY, int W, int E, bool WIDE>
+__global__ __launch_bounds__(W == 1 ? 256 : W * 64) void k_block_norm(BnArgs a) {
+  constexpr int V = 8;
+  __shared__ float s_red[W];
+  const int lane = W == 1 ? threadIdx.x & 63 : threadIdx.x;
+  const int64_t row = W == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+  if (row >= a.rows) return;
+  const size_t o = (size_t)row * a.D;
+  float xn[E][V], y[E][V], g[E][V];
+  float r[1] = {0.0f};
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int d = (e * 64 * W + lane) * V;
+    ld_vals<V, WIDE>(y[e], (const TY*)a.y + o, d, a.D);
+    ld_vals<V, WIDE>(xn[e], (const TX*)a.x + o, d, a.D);
+    if (a.act != LSH_GATE_NONE) ld_vals<V, WIDE>(g[e], (const TY*)a.gate + o, d, a.D);
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+#pragma unroll
+    for (int j = 0; j < V; ++j) r[0] = __builtin_fmaf(y[e][j], y[e][j], r[0]);
+  row_sums<W>(r, s_red);
+  const float ry = 1.0f / sqrtf(r[0] / a.D + a.eps);
+  r[0] = 0.0f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int d = (e * 64 * W + lane) * V;
+    float w[V], s[V];
+    ld_vals<V, WIDE>(w, a.w_post, d, a.D);
+    if (a.scale) ld_vals<V, WIDE>(s, a.scale, d, a.D);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      float unused;
+      const float act = a.act == LSH_GATE_NONE ? 1.0f : bn_act(a.act, g[e][j], unused);
+      xn[e][j] = __builtin_fmaf(a.scale ? s[j] : a.scale1, act * (y[e][j] * ry * w[j]), xn[e][j]);
+      r[0] = __builtin_fmaf(xn[e][j], xn[e][j], r[0]);
+    }
+    st_vals<V, WIDE>(xn[e], (TX*)a.x_new + o, d, a.D);
+  }
+  row_sums<W>(r, s_red);
+  const float rx = 1.0f / sqrtf(r[0] / a.D + a.eps);
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int d = (e * 64 * W + lane) * V;
+    float w[V];
+    ld_vals<V, WIDE>(w, a.w_pre, d, a.D);
+#pragma unroll
+    for (int j = 0; j < V; ++j) w[j] *= xn[e][j] * rx;
+    st_vals<V, WIDE>(w, (TY*)a.z + o, d, a.D);
+  }
+}
+
+// The gradients.  A workgroup takes rows blockIdx.x, + gridDim.x, ...; its sums of the parameters'
+// gradients stay in registers until the last row and go to its place of `part`.
+template <class TX, class TY, int W, int E, bool WIDE>
+__global__ __launch_bounds__(W * 64) void k_block_norm_bwd(BnArgs a) {
+  constexpr int V = 8;
+  __shared__ float s_red[W * 2];
+  float sum[3][E][V] = {};
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const size_t o = (size_t)row * a.D;
-    const TX* x = (const TX*)a.x + o;
-    const TY* y = (const TY*)a.y + o;
-    const TY* gate = (const TY*)a.gate + o;
-    const TX* gx = (const TX*)a.gx + o;
-    const TY* gz = (const TY*)a.gz + o;
+    float x[E][V], y[E][V], g[E][V], gz[E][V], gx[E][V];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int d = (e * 64 * W + threadIdx.x) * V;
+      ld_vals<V, WIDE>(y[e], (const TY*)a.y + o, d, a.D);
+      ld_vals<V, WIDE>(x[e], (const TX*)a.x + o, d, a.D);
+      if (a.act != LSH_GATE_NONE) ld_vals<V, WIDE>(g[e], (const TY*)a.gate + o, d, a.D);
+      if (a.gz) ld_vals<V, WIDE>(gz[e], (const TY*)a.gz + o, d, a.D);
+      if (a.gx) ld_vals<V, WIDE>(gx[e], (const TX*)a.gx + o, d, a.D);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        if (!a.gz) gz[e][j] = 0.0f;
+        if (!a.gx) gx[e][j] = 0.0f;
+        if (a.act == LSH_GATE_NONE) g[e][j] = 0.0f;
+      }
+    }
     float r[1] = {0.0f};
-    for (int d = threadIdx.x; d < a.D; d += kBnThreads) {
-      const float v = to_f(y[d]);
-      r[0] = __builtin_fmaf(v, v, r[0]);
-    }
-    block_sums(r, s_red);
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+#pragma unroll
+      for (int j = 0; j < V; ++j) r[0] = __builtin_fmaf(y[e][j], y[e][j], r[0]);
+    row_sums<W>(r, s_red);
     const float ry = 1.0f / sqrtf(r[0] / a.D + a.eps);
-    struct Row {
-      float n, act, dact, s, xn, u;
-    };
-    auto at = [&](int d) {
-      Row e;
-      e.act = bn_act(a.act, a.act == LSH_GATE_NONE ? 0.0f : to_f(gate[d]), e.dact);
-      e.n = to_f(y[d]) * ry * a.w_post[d];
-      e.s = a.scale ? a.scale[d] : a.scale1;
-      e.xn = __builtin_fmaf(e.s, e.act * e.n, to_f(x[d]));
-      e.u = a.gz ? to_f(gz[d]) * a.w_pre[d] : 0.0f;
-      return e;
-    };
+    // x becomes x_new
     float t[2] = {0.0f, 0.0f};
-    for (int d = threadIdx.x; d < a.D; d += kBnThreads) {
-      const Row e = at(d);
-      t[0] = __builtin_fmaf(e.xn, e.xn, t[0]);
-      t[1] = __builtin_fmaf(e.u, e.xn, t[1]);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int d = (e * 64 * W + threadIdx.x) * V;
+      float wp[V], wq[V], s[V];
+      ld_vals<V, WIDE>(wp, a.w_post, d, a.D);
+      ld_vals<V, WIDE>(wq, a.w_pre, d, a.D);
+      if (a.scale) ld_vals<V, WIDE>(s, a.scale, d, a.D);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        float unused;
+        const float act = bn_act(a.act, g[e][j], unused);
+        x[e][j] = __builtin_fmaf(a.scale ? s[j] : a.scale1, act * (y[e][j] * ry * wp[j]), x[e][j]);
+        t[0] = __builtin_fmaf(x[e][j], x[e][j], t[0]);
+        t[1] = __builtin_fmaf(gz[e][j] * wq[j], x[e][j], t[1]);
+      }
     }
-    block_sums(t, s_red);
+    row_sums<W>(t, s_red);
     const float rx = 1.0f / sqrtf(t[0] / a.D + a.eps);
     const float cx = rx * rx * (t[1] / a.D);
+    // gx becomes dx, gz becomes dn
     r[0] = 0.0f;
-    auto grad_x = [&](const Row& e, int d) {
-      return (a.gx ? to_f(gx[d]) : 0.0f) + rx * (e.u - e.xn * cx);
-    };
-    for (int d = threadIdx.x; d < a.D; d += kBnThreads) {
-      const Row e = at(d);
-      const float m = e.s * grad_x(e, d) * e.act * a.w_post[d];
-      r[0] = __builtin_fmaf(m, to_f(y[d]), r[0]);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int d = (e * 64 * W + threadIdx.x) * V;
+      float wp[V], wq[V], s[V];
+      ld_vals<V, WIDE>(wp, a.w_post, d, a.D);
+      ld_vals<V, WIDE>(wq, a.w_pre, d, a.D);
+      if (a.scale) ld_vals<V, WIDE>(s, a.scale, d, a.D);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float dx = gx[e][j] + rx * (gz[e][j] * wq[j] - x[e][j] * cx);
+        float dact;
+        const float act = bn_act(a.act, g[e][j], dact);
+        const float n = y[e][j] * ry * wp[j], dh = (a.scale ? s[j] : a.scale1) * dx;
+        sum[1][e][j] = __builtin_fmaf(gz[e][j] * x[e][j], rx, sum[1][e][j]);
+        sum[2][e][j] = __builtin_fmaf(dx * act, n, sum[2][e][j]);
+        gx[e][j] = dx;
+        gz[e][j] = dh * act;
+        g[e][j] = dh * n * dact;
+        sum[0][e][j] = __builtin_fmaf(gz[e][j] * y[e][j], ry, sum[0][e][j]);
+        r[0] = __builtin_fmaf(gz[e][j] * wp[j], y[e][j], r[0]);
+      }
+      st_vals<V, WIDE>(gx[e], (TX*)a.dx + o, d, a.D);
+      if (a.dgate) st_vals<V, WIDE>(g[e], (TY*)a.dgate + o, d, a.D);
     }
-    block_sums(r, s_red);
+    row_sums<W>(r, s_red);
     const float cy = ry * ry * (r[0] / a.D);
-    for (int d = threadIdx.x; d < a.D; d += kBnThreads) {
-      const Row e = at(d);
-      const float yd = to_f(y[d]), dx = grad_x(e, d), dh = e.s * dx, dn = dh * e.act;
-      ((TX*)a.dx)[o + d] = from_f<TX>(dx);
-      ((TY*)a.dy)[o + d] = from_f<TY>(ry * (dn * a.w_post[d] - yd * cy));
-      if (a.dgate) ((TY*)a.dgate)[o + d] = from_f<TY>(dh * e.n * e.dact);
-      part[d] += dn * yd * ry;
-      if (a.gz) part[a.D + d] += to_f(gz[d]) * e.xn * rx;
-      part[2 * a.D + d] += dx * e.act * e.n;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int d = (e * 64 * W + threadIdx.x) * V;
+      float wp[V];
+      ld_vals<V, WIDE>(wp, a.w_post, d, a.D);
+#pragma unroll
+      for (int j = 0; j < V; ++j) wp[j] = ry * (gz[e][j] * wp[j] - y[e][j] * cy);
+      st_vals<V, WIDE>(wp, (TY*)a.dy + o, d, a.D);
     }
   }
+  float* part = a.part + (size_t)blockIdx.x * 3 * a.D;
+#pragma unroll
+  for (int i = 0; i < 3; ++i)
+#pragma unroll
+    for (int e = 0; e < E; ++e) st_vals<V, WIDE>(sum[i][e], part + (size_t)i * a.D, (e * 64 * W + threadIdx.x) * V, a.D);
 }
 
-// dw_post, dw_pre and da: the workgroups' sums in workgroup order.
+// dw_post, dw_pre and da: the workgroups' sums, 16 runs of workgroups at once and then in run order.
 __global__ __launch_bounds__(256) void k_block_norm_sums(const float* __restrict__ part, int P, int D,
                                                          float* dw_post, float* dw_pre, float* da) {
-  const int i = blockIdx.x * 256 + threadIdx.x;
-  if (i >= 3 * D) return;
+  __shared__ float s_run[16][16];
+  const int c = threadIdx.x & 15, run = threadIdx.x >> 4;
+  const int i = blockIdx.x * 16 + c;
+  const int per = (P + 15) / 16, p1 = min(P, (run + 1) * per);
+  float s = 0.0f;
+  if (i < 3 * D)
+#pragma unroll 8
+    for (int p = run * per; p < p1; ++p) s += part[(size_t)p * 3 * D + i];
+  s_run[run][c] = s;
+  __syncthreads();
+  if (run != 0 || i >= 3 * D) return;
   float* out = i < D ? dw_post : i < 2 * D ? dw_pre : da;
   if (!out) return;
-  float s = 0.0f;
-  for (int p = 0; p < P; ++p) s += part[(size_t)p * 3 * D + i];
+  s = 0.0f;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) s += s_run[r][c];
   out[i % D] = s;
 }
 
@@ -179,6 +287,28 @@ static void with_types(int tx, int ty, F&& f) {
     else
       f(y, y);
   });
+}
+
+// Calls f with the waves and column groups that hold D channels of a row.  The gradients hold eight
+// values a channel: 16 waves' share of the registers is too small for them up to 8192 channels.
+template <class F>
+static void with_row(int D, bool grads, F&& f) {
+  auto go = [&](auto w, auto e) { f(w, e); };
+  using std::integral_constant;
+  if (D <= 512)
+    go(integral_constant<int, 1>{}, integral_constant<int, 1>{});
+  else if (D <= 1024)
+    go(integral_constant<int, 2>{}, integral_constant<int, 1>{});
+  else if (D <= 2048)
+    go(integral_constant<int, 4>{}, integral_constant<int, 1>{});
+  else if (D <= 4096)
+    go(integral_constant<int, 8>{}, integral_constant<int, 1>{});
+  else if (D <= 8192 && grads)
+    go(integral_constant<int, 8>{}, integral_constant<int, 2>{});
+  else if (D <= 8192)
+    go(integral_constant<int, 16>{}, integral_constant<int, 1>{});
+  else
+    go(integral_constant<int, 16>{}, integral_constant<int, 2>{});
 }
 
 static int bn_check(const lsh_block_norm* a) {
@@ -200,7 +330,21 @@ static BnArgs bn_args(const lsh_block_norm* p) {
   return a;
 }
 
-static int64_t bn_grid(int64_t rows) { return rows < 512 ? rows : 512; }
+// Whether every row of every tensor begins at a multiple of 16 bytes.
+static bool bn_wide(const BnArgs& a) {
+  if (a.D % 8) return false;
+  for (const void* p : {a.x, a.y, a.gate, (const void*)a.w_post, (const void*)a.w_pre, (const void*)a.scale,
+                        (const void*)a.x_new, (const void*)a.z, a.gx, a.gz, (const void*)a.dx,
+                        (const void*)a.dy, (const void*)a.dgate, (const void*)a.part})
+    if ((uintptr_t)p % 16) return false;
+  return true;
+}
+
+// Workgroups of the gradients: each writes 3*D sums of its own, so no more than keep the chip busy.
+static int64_t bn_grid(int64_t rows, int D) {
+  const int64_t most = D <= 1024 ? 2048 : D <= 2048 ? 1024 : 512;
+  return rows < most ? rows : most;
+}
 
 }  // namespace lsh
 
@@ -212,16 +356,26 @@ extern "C" int lsh_block_norm_fwd(const lsh_block_norm* p, void* x_new, void* z,
   if (bad_ptr(x_new) || bad_ptr(z)) return LSH_ERR_ARG;
   BnArgs a = bn_args(p);
   a.x_new = x_new, a.z = z;
+  const bool wide = bn_wide(a);
   with_types(p->x_dtype, p->dtype, [&](auto tx, auto ty) {
-    k_block_norm<decltype(tx), decltype(ty)>
-        <<<dim3((unsigned)p->rows), kBnThreads, 0, (hipStream_t)stream>>>(a);
+    with_row(p->D, false, [&](auto w, auto e) {
+      using TX = decltype(tx);
+      using TY = decltype(ty);
+      constexpr int W = decltype(w)::value, E = decltype(e)::value;
+      const dim3 grid((unsigned)(W == 1 ? (p->rows + 3) / 4 : p->rows));
+      const int threads = W == 1 ? 256 : W * 64;
+      if (wide)
+        k_block_norm<TX, TY, W, E, true><<<grid, threads, 0, (hipStream_t)stream>>>(a);
+      else
+        k_block_norm<TX, TY, W, E, false><<<grid, threads, 0, (hipStream_t)stream>>>(a);
+    });
   });
   LSH_CHECK_LAUNCH();
   return LSH_OK;
 }
 
 extern "C" size_t lsh_block_norm_bwd_workspace(const lsh_block_norm* p) {
-  return bn_check(p) ? 0 : (size_t)bn_grid(p->rows) * 3 * p->D * sizeof(float);
+  return bn_check(p) ? 0 : (size_t)bn_grid(p->rows, p->D) * 3 * p->D * sizeof(float);
 }
 
 extern "C" int lsh_block_norm_bwd(const lsh_block_norm* p, const void* gx, const void* gz, void* dx,
@@ -230,19 +384,28 @@ extern "C" int lsh_block_norm_bwd(const lsh_block_norm* p, const void* gx, const
   if (int rc = bn_check(p)) return rc;
   hipStream_t st = (hipStream_t)stream;
   const size_t need = lsh_block_norm_bwd_workspace(p);
+  const int64_t grid = bn_grid(p->rows, p->D);
   if (p->rows > 0) {
     if (bad_ptr(dx) || bad_ptr(dy)) return LSH_ERR_ARG;
     if (bad_ptr(ws) || ws_bytes < need) return LSH_ERR_WORKSPACE;
     BnArgs a = bn_args(p);
     a.gx = gx, a.gz = gz, a.dx = dx, a.dy = dy, a.dgate = dgate, a.part = (float*)ws;
+    const bool wide = bn_wide(a);
     with_types(p->x_dtype, p->dtype, [&](auto tx, auto ty) {
-      k_block_norm_bwd<decltype(tx), decltype(ty)>
-          <<<dim3((unsigned)bn_grid(p->rows)), kBnThreads, 0, st>>>(a);
+      with_row(p->D, true, [&](auto w, auto e) {
+        using TX = decltype(tx);
+        using TY = decltype(ty);
+        constexpr int W = decltype(w)::value, E = decltype(e)::value;
+        if (wide)
+          k_block_norm_bwd<TX, TY, W, E, true><<<dim3((unsigned)grid), W * 64, 0, st>>>(a);
+        else
+          k_block_norm_bwd<TX, TY, W, E, false><<<dim3((unsigned)grid), W * 64, 0, st>>>(a);
+      });
     });
     LSH_CHECK_LAUNCH();
   }
-  k_block_norm_sums<<<dim3((3 * p->D + 255) / 256), 256, 0, st>>>((const float*)ws, (int)bn_grid(p->rows),
-                                                                p->D, dw_post, dw_pre, dscale);
+  k_block_norm_sums<<<dim3((3 * p->D + 15) / 16), 256, 0, st>>>((const float*)ws, (int)grid, p->D, dw_post,
+                                                              dw_pre, dscale);
   LSH_CHECK_LAUNCH();
   return LSH_OK;
 }
