@@ -64,47 +64,6 @@ __device__ __forceinline__ float bn_act(int act, float g, float& d) {
   return act == LSH_GATE_SILU ? g * sg : sg;
 }
 
-// V values of a row from column d on, as fp32: WIDE in one access, otherwise one by one (zeros beyond D).
-template <int V, bool WIDE, class T>
-__device__ __forceinline__ void ld_vals(float (&f)[V], const T* p, int d, int D) {
-  if constexpr (WIDE) {
-    if (d < D) {
-      constexpr int P = V * sizeof(T) > 16 ? 16 / sizeof(T) : V;
-#pragma unroll
-      for (int i = 0; i < V; i += P) {
-        const Vec<T, P> x = *(const Vec<T, P>*)(p + d + i);
-#pragma unroll
-        for (int j = 0; j < P; ++j) f[i + j] = to_f(x.v[j]);
-      }
-      return;
-    }
-#pragma unroll
-    for (int j = 0; j < V; ++j) f[j] = 0.0f;
-  } else {
-#pragma unroll
-    for (int j = 0; j < V; ++j) f[j] = d + j < D ? to_f(p[d + j]) : 0.0f;
-  }
-}
-template <int V, bool WIDE, class T>
-__device__ __forceinline__ void st_vals(const float (&f)[V], T* p, int d, int D) {
-  if constexpr (WIDE) {
-    if (d < D) {
-      constexpr int P = V * sizeof(T) > 16 ? 16 / sizeof(T) : V;
-#pragma unroll
-      for (int i = 0; i < V; i += P) {
-        Vec<T, P> x;
-#pragma unroll
-        for (int j = 0; j < P; ++j) x.v[j] = from_f<T>(f[i + j]);
-        *(Vec<T, P>*)(p + d + i) = x;
-      }
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < V; ++j)
-      if (d + j < D) p[d + j] = from_f<T>(f[j]);
-  }
-}
-
 // A row is held in registers by W waves, E groups of V = 8 columns a lane: columns (e*64*W + lane)*8.
 template <class TX, class TY, int W, int E, bool WIDE>
 __global__ __launch_bounds__(W == 1 ? 256 : W * 64) void k_block_norm(BnArgs a) {
@@ -116,12 +75,22 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * 64) void k_block_norm(BnArgs a) 
   const size_t o = (size_t)row * a.D;
   float xn[E][V], y[E][V], g[E][V];
   float r[1] = {0.0f};
+  {
+    Raw<V, WIDE, TX> rx[E];
+    Raw<V, WIDE, TY> ry[E], rg[E];
+    const TY* gate = a.act != LSH_GATE_NONE ? (const TY*)a.gate : (const TY*)a.y;
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const int d = (e * 64 * W + lane) * V;
-    ld_vals<V, WIDE>(y[e], (const TY*)a.y + o, d, a.D);
-    ld_vals<V, WIDE>(xn[e], (const TX*)a.x + o, d, a.D);
-    if (a.act != LSH_GATE_NONE) ld_vals<V, WIDE>(g[e], (const TY*)a.gate + o, d, a.D);
+    for (int e = 0; e < E; ++e) {
+      const int d = (e * 64 * W + lane) * V;
+      ry[e].load((const TY*)a.y + o, d, a.D);
+      rx[e].load((const TX*)a.x + o, d, a.D);
+      rg[e].load(gate + o, d, a.D);
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int d = (e * 64 * W + lane) * V;
+      ry[e].get(y[e], d, a.D), rx[e].get(xn[e], d, a.D), rg[e].get(g[e], d, a.D);
+    }
   }
 #pragma unroll
   for (int e = 0; e < E; ++e)
@@ -168,19 +137,27 @@ __global__ __launch_bounds__(W * 64) void k_block_norm_bwd(BnArgs a) {
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const size_t o = (size_t)row * a.D;
     float x[E][V], y[E][V], g[E][V], gz[E][V], gx[E][V];
+    {
+      Raw<V, WIDE, TX> qx[E], qgx[E];
+      Raw<V, WIDE, TY> qy[E], qg[E], qgz[E];
+      // what is not there is read from what is, and not used
+      const TY* gate = a.act != LSH_GATE_NONE ? (const TY*)a.gate : (const TY*)a.y;
+      const TY* gzp = a.gz ? (const TY*)a.gz : (const TY*)a.y;
+      const TX* gxp = a.gx ? (const TX*)a.gx : (const TX*)a.x;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int d = (e * 64 * W + threadIdx.x) * V;
-      ld_vals<V, WIDE>(y[e], (const TY*)a.y + o, d, a.D);
-      ld_vals<V, WIDE>(x[e], (const TX*)a.x + o, d, a.D);
-      if (a.act != LSH_GATE_NONE) ld_vals<V, WIDE>(g[e], (const TY*)a.gate + o, d, a.D);
-      if (a.gz) ld_vals<V, WIDE>(gz[e], (const TY*)a.gz + o, d, a.D);
-      if (a.gx) ld_vals<V, WIDE>(gx[e], (const TX*)a.gx + o, d, a.D);
+      for (int e = 0; e < E; ++e) {
+        const int d = (e * 64 * W + threadIdx.x) * V;
+        qy[e].load((const TY*)a.y + o, d, a.D);
+        qx[e].load((const TX*)a.x + o, d, a.D);
+        qg[e].load(gate + o, d, a.D);
+        qgz[e].load(gzp + o, d, a.D);
+        qgx[e].load(gxp + o, d, a.D);
+      }
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        if (!a.gz) gz[e][j] = 0.0f;
-        if (!a.gx) gx[e][j] = 0.0f;
-        if (a.act == LSH_GATE_NONE) g[e][j] = 0.0f;
+      for (int e = 0; e < E; ++e) {
+        const int d = (e * 64 * W + threadIdx.x) * V;
+        qy[e].get(y[e], d, a.D), qx[e].get(x[e], d, a.D), qg[e].get(g[e], d, a.D, a.act != LSH_GATE_NONE);
+        qgz[e].get(gz[e], d, a.D, a.gz != nullptr), qgx[e].get(gx[e], d, a.D, a.gx != nullptr);
       }
     }
     float r[1] = {0.0f};
@@ -291,8 +268,8 @@ static void with_types(int tx, int ty, F&& f) {
 
 // Calls f with the waves and column groups that hold D channels of a row.  The gradients hold eight
 // values a channel: 16 waves' share of the registers is too small for them up to 8192 channels.
-template <class F>
-static void with_row(int D, bool grads, F&& f) {
+template <bool GRADS, class F>
+static void with_row(int D, F&& f) {
   auto go = [&](auto w, auto e) { f(w, e); };
   using std::integral_constant;
   if (D <= 512)
@@ -303,10 +280,8 @@ static void with_row(int D, bool grads, F&& f) {
     go(integral_constant<int, 4>{}, integral_constant<int, 1>{});
   else if (D <= 4096)
     go(integral_constant<int, 8>{}, integral_constant<int, 1>{});
-  else if (D <= 8192 && grads)
-    go(integral_constant<int, 8>{}, integral_constant<int, 2>{});
   else if (D <= 8192)
-    go(integral_constant<int, 16>{}, integral_constant<int, 1>{});
+    go(integral_constant<int, GRADS ? 8 : 16>{}, integral_constant<int, GRADS ? 2 : 1>{});
   else
     go(integral_constant<int, 16>{}, integral_constant<int, 2>{});
 }
@@ -358,7 +333,7 @@ extern "C" int lsh_block_norm_fwd(const lsh_block_norm* p, void* x_new, void* z,
   a.x_new = x_new, a.z = z;
   const bool wide = bn_wide(a);
   with_types(p->x_dtype, p->dtype, [&](auto tx, auto ty) {
-    with_row(p->D, false, [&](auto w, auto e) {
+    with_row<false>(p->D, [&](auto w, auto e) {
       using TX = decltype(tx);
       using TY = decltype(ty);
       constexpr int W = decltype(w)::value, E = decltype(e)::value;
@@ -392,7 +367,7 @@ extern "C" int lsh_block_norm_bwd(const lsh_block_norm* p, const void* gx, const
     a.gx = gx, a.gz = gz, a.dx = dx, a.dy = dy, a.dgate = dgate, a.part = (float*)ws;
     const bool wide = bn_wide(a);
     with_types(p->x_dtype, p->dtype, [&](auto tx, auto ty) {
-      with_row(p->D, true, [&](auto w, auto e) {
+      with_row<true>(p->D, [&](auto w, auto e) {
         using TX = decltype(tx);
         using TY = decltype(ty);
         constexpr int W = decltype(w)::value, E = decltype(e)::value;

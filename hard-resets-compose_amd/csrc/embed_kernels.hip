@@ -2,51 +2,352 @@
 //
 //   out[i] = scale * W[tok_i]          dW[v] = scale * sum_{i: tok_i = v} dout[i]
 //
-// Ids outside the table and the padding id read as zero rows and leave no gradient.  The gradient
-// sums the rows of a token in the order of their positions, in fp32, with no atomics: the same bits
-// on every run.
+// Ids outside the table and the padding id read as zero rows and leave no gradient.  For the gradient
+// the positions are sorted by token (stable, so in position order within a token) and every table row
+// sums its own, in fp32 with no atomics: the same bits on every run, and every row is written once.
+#include <algorithm>
+
 #include "lsh_lm.h"
 
 namespace lsh {
 
-template <class T>
+// One thread a piece of V columns.
+template <class T, bool WIDE>
 __global__ __launch_bounds__(256) void k_embed(const int64_t* __restrict__ tok, const T* __restrict__ W,
-                                               T* __restrict__ out, int64_t V, int D, int64_t pad,
-                                               float scale) {
-  const int64_t i = blockIdx.x, v = tok[i];
-  const bool there = v >= 0 && v < V && v != pad;
-  for (int d = threadIdx.x; d < D; d += 256)
-    out[(size_t)i * D + d] = there ? from_f<T>(scale * to_f(W[(size_t)v * D + d])) : from_f<T>(0.0f);
+                                               T* __restrict__ out, int64_t n, int64_t V, int D, int64_t pad,
+                                               float scale, int pieces) {
+  constexpr int P = kWide<T>;
+  const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t i = u / pieces;
+  if (i >= n) return;
+  const int d = (int)(u - i * pieces) * P;
+  const int64_t v = tok[i];
+  float f[P] = {};
+  if (v >= 0 && v < V && v != pad) {
+    ld_vals<P, WIDE>(f, W + (size_t)v * D, d, D);
+#pragma unroll
+    for (int j = 0; j < P; ++j) f[j] *= scale;
+  }
+  st_vals<P, WIDE>(f, out + (size_t)i * D, d, D);
 }
 
-template <class T>
-__global__ __launch_bounds__(256) void k_embed_bwd(const int64_t* __restrict__ tok,
-                                                   const T* __restrict__ dout, T* __restrict__ dW,
-                                                   int64_t n, int64_t V, int D, int64_t pad, float scale) {
-  const int64_t v = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63;
-  if (v >= V) return;
-  for (int d0 = 0; d0 < D; d0 += 64) {
-    const int d = d0 + lane;
-    float s = 0.0f;
-    if (v != pad) {
-      for (int64_t i0 = 0; i0 < n; i0 += 64) {
-        unsigned long long hit = wave_ballot(i0 + lane < n && tok[i0 + lane] == v);
-        while (hit) {
-          const int64_t i = i0 + __builtin_ctzll(hit);
-          hit &= hit - 1;
-          if (d < D) s += to_f(dout[(size_t)i * D + d]);
+// ---- positions by token
+// The table's rows are dealt to `parts` workgroups (a power of two, row v to workgroup v % parts, so
+// that frequent neighbours go to different ones).  Each reads all tokens twice: it counts its rows'
+// tokens and those of the workgroups before it, which gives every row's place in the list, and then
+// puts its positions there in order.  The second reading needs no memory up to kEsTile tokens.
+// Bound by the reading, n * parts * 8 bytes from L2 (16384 tokens, 256 workgroups: 33 MB).
+constexpr int kEsThreads = 1024, kEsPer = 16, kEsTile = kEsThreads * kEsPer;
+constexpr int kEsRuns = kEsTile / 64;
+constexpr int kEsRows = 8192;  // table rows of a workgroup at most
+constexpr int kEsList = 4096;  // positions on their way to the list
+
+inline int es_parts(int64_t V) {
+  int64_t p = 256;
+  while ((V + p - 1) / p > kEsRows) p *= 2;
+  return (int)p;
+}
+
+__global__ __launch_bounds__(kEsThreads) void k_embed_sort(const int64_t* __restrict__ tok, int n, int V,
+                                                           int64_t pad, int parts, int* __restrict__ start,
+                                                           int* __restrict__ count, int* __restrict__ list) {
+  __shared__ int s_row[kEsRows];   // a row's tokens, then where its next position goes
+  __shared__ int s_at[kEsList];    // positions found, in order, with
+  __shared__ short s_of[kEsList];  // the row of each
+  __shared__ int s_wave[kEsThreads / 64], s_sum[kEsThreads / 64];
+  __shared__ int s_runs[kEsRuns + 1];  // runs of 64 tokens of a tile: how many are found before each, and in all
+  const int p = blockIdx.x, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int rows = (V - p + parts - 1) / parts, shift = __builtin_ctz(parts);
+  const unsigned long long lower = (1ull << lane) - 1;
+  // a token's row v, or -1; thread t has tokens t, t + 1024, ... of a tile
+  int v[kEsPer];
+  auto read = [&](int t0) {
+#pragma unroll
+    for (int j = 0; j < kEsPer; ++j) {
+      const int i = t0 + j * kEsThreads + threadIdx.x;
+      const int64_t x = i < n ? tok[i] : -1;
+      v[j] = (uint64_t)x < (uint64_t)V && (int)x != (int)pad ? (int)x : -1;
+    }
+  };
+  for (int i = threadIdx.x; i < rows; i += kEsThreads) s_row[i] = 0;
+  __syncthreads();
+  int before = 0;
+  for (int t0 = 0; t0 < n; t0 += kEsTile) {
+    read(t0);
+#pragma unroll
+    for (int j = 0; j < kEsPer; ++j) {
+      const int part = v[j] & (parts - 1);
+      before += v[j] >= 0 && part < p;
+      if (v[j] >= 0 && part == p) atomicAdd(&s_row[v[j] >> shift], 1);
+    }
+  }
+  before = wave_sum_i(before);
+  if (lane == 0) s_wave[w] = before;
+  __syncthreads();
+  before = 0;
+  for (int i = 0; i < kEsThreads / 64; ++i) before += s_wave[i];
+  __syncthreads();
+  // each row's place: an exclusive sum over the rows, 1024 at a time
+  for (int i0 = 0; i0 < rows; i0 += kEsThreads) {
+    const int i = i0 + threadIdx.x, c = i < rows ? s_row[i] : 0;
+    int incl = c;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int x = __shfl_up(incl, o, 64);
+      if (lane >= o) incl += x;
+    }
+    if (lane == 63) s_sum[w] = incl;
+    __syncthreads();
+    int at = before + incl - c;
+    for (int j = 0; j < kEsThreads / 64; ++j) {
+      if (j < w) at += s_sum[j];
+      before += s_sum[j];
+    }
+    if (i < rows) {
+      s_row[i] = at;
+      start[(size_t)i * parts + p] = at;
+      count[(size_t)i * parts + p] = c;
+    }
+    __syncthreads();
+  }
+  int found = 0;
+  // the positions found so far to their places, by one wave, 64 at a time
+  auto flush = [&]() {
+    __syncthreads();
+    if (w == 0) {
+      for (int i0 = 0; i0 < found; i0 += 64) {
+        const bool there = i0 + lane < found;
+        const int row = there ? s_of[i0 + lane] : -1;
+        const int at = there ? s_at[i0 + lane] : 0;
+        // the lanes with this lane's row
+        unsigned long long same = wave_ballot(there);
+        if (wave_ballot(row == __shfl(row, 0, 64)) != ~0ull) {
+#pragma unroll
+          for (int b = 0; b < 13; ++b) {
+            const unsigned long long m = wave_ballot((row >> b) & 1);
+            same &= (row >> b) & 1 ? m : ~m;
+          }
+        }
+        if (there) {
+          const int to = s_row[row];
+          list[to + __popcll(same & lower)] = at;
+          if (!(same >> lane >> 1)) s_row[row] = to + __popcll(same);
         }
       }
     }
-    if (d < D) dW[(size_t)v * D + d] = from_f<T>(scale * s);
+    __syncthreads();
+    found = 0;
+  };
+  for (int t0 = 0; t0 < n; t0 += kEsTile) {
+    if (n > kEsTile) read(t0);
+    // where each position found goes: those of earlier runs of 64 tokens, then of earlier lanes
+    unsigned long long hit[kEsPer];
+#pragma unroll
+    for (int j = 0; j < kEsPer; ++j) {
+      hit[j] = wave_ballot(v[j] >= 0 && (v[j] & (parts - 1)) == p);
+      if (lane == 0) s_runs[j * (kEsThreads / 64) + w] = __popcll(hit[j]);
+    }
+    __syncthreads();
+    if (w == 0) {
+      constexpr int E = kEsRuns / 64;
+      int c[E], sum = 0;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        c[e] = s_runs[lane * E + e];
+        sum += c[e];
+      }
+      int incl = sum;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int x = __shfl_up(incl, o, 64);
+        if (lane >= o) incl += x;
+      }
+      if (lane == 63) s_runs[kEsRuns] = incl;
+      int at = incl - sum;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        s_runs[lane * E + e] = at;
+        at += c[e];
+      }
+    }
+    __syncthreads();
+    const int total = s_runs[kEsRuns];
+    // the tile's positions pass through the list in windows of its size
+    for (int win = 0; win < total; win += kEsList) {
+#pragma unroll
+      for (int j = 0; j < kEsPer; ++j) {
+        const int at = s_runs[j * (kEsThreads / 64) + w] + __popcll(hit[j] & lower) - win;
+        if ((hit[j] >> lane & 1) && at >= 0 && at < kEsList) {
+          s_at[at] = t0 + j * kEsThreads + threadIdx.x;
+          s_of[at] = (short)(v[j] >> shift);
+        }
+      }
+      found = min(total - win, kEsList);
+      flush();
+    }
+    __syncthreads();  // s_runs has been read
+  }
+}
+
+// ---- the sums
+// A workgroup takes a block of kEbLanes*16 bytes of columns; a table row is taken by `lanes` lanes of a
+// wave, 16 bytes a lane, so a wave takes 4 rows or more at once.  Up to kEbFew positions are summed by the
+// row's own lanes; longer rows are dealt to the workgroup's waves, up to kEbHot positions to one (its lane
+// groups take positions in turn), more to all, always joined in a fixed order.  Neighbouring rows, which
+// are often frequent together, go to different workgroups.
+// Bound by the rows read and written (16384 tokens, 32000 x 1024 bf16: 97 MB); what a Zipf text costs beyond
+// that is the chain of dependent loads of its longest rows.
+constexpr int kEbThreads = 1024, kEbLanes = 16, kEbFew = 4, kEbHot = 256, kEbGroups = 64;
+
+// The sum of dout's rows at list[begin .. begin + n) in columns d.., dealt to `groups` lane groups, this
+// lane's the group-th, Q positions at once.
+template <class T, bool WIDE, int Q, class At>
+__device__ __forceinline__ void eb_sum(float (&t)[kWide<T>], At&& at, int n, int group, int groups,
+                                       const T* __restrict__ dout, int d, int D) {
+  constexpr int P = kWide<T>;
+  for (int i = group; i < n; i += Q * groups) {
+    Raw<P, WIDE, T> x[Q];
+#pragma unroll
+    for (int q = 0; q < Q; ++q) x[q].load(dout + (size_t)at(min(i + q * groups, n - 1)) * D, d, D);
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      float f[P];
+      x[q].get(f, d, D, i + q * groups < n);
+#pragma unroll
+      for (int j = 0; j < P; ++j) t[j] += f[j];
+    }
+  }
+}
+
+template <class T, bool WIDE>
+__global__ __launch_bounds__(kEbThreads) void k_embed_bwd(const int* __restrict__ start,
+                                                          const int* __restrict__ count,
+                                                          const int* __restrict__ list,
+                                                          const T* __restrict__ dout, T* __restrict__ dW, int n,
+                                                          int V, int D, float scale, int lanes) {
+  constexpr int P = kWide<T>, WAVES = kEbThreads / 64, EACH = kEbGroups / WAVES;
+  // longer rows with their places and lengths, from the front; the longest from the back
+  __shared__ int s_row[kEbGroups * 64], s_begin[kEbGroups * 64], s_count[kEbGroups * 64], s_n[2];
+  __shared__ int s_list[WAVES][kEbHot];
+  __shared__ float s_sum[WAVES][kEbLanes * P];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int per = 64 / lanes, sub = lane / lanes, l = lane % lanes;  // rows of a wave, this lane's, its place
+  const int d0 = blockIdx.y * kEbLanes * P, d = d0 + l * P;
+  if (threadIdx.x < 2) s_n[threadIdx.x] = 0;
+  __syncthreads();
+  int c[EACH], at[EACH][kEbFew];
+  int64_t row[EACH];
+#pragma unroll
+  for (int k = 0; k < EACH; ++k) {
+    // short rows stay with their neighbours, so that a wave writes whole lines
+    const int g = k * WAVES + w;
+    row[k] = lanes == kEbLanes ? (int64_t)(g * per + sub) * gridDim.x + blockIdx.x
+                               : ((int64_t)g * gridDim.x + blockIdx.x) * per + sub;
+    c[k] = row[k] < V ? count[row[k]] : -1;
+    at[k][0] = row[k] < V ? start[row[k]] : 0;
+  }
+#pragma unroll
+  for (int k = 0; k < EACH; ++k) {
+    if (c[k] > kEbFew) {
+      if (l == 0) {
+        const bool hot = c[k] > kEbHot;
+        const int i = atomicAdd(&s_n[hot], 1), to = hot ? kEbGroups * 64 - 1 - i : i;
+        s_row[to] = (int)row[k], s_begin[to] = at[k][0], s_count[to] = c[k];
+      }
+      c[k] = -1;
+    }
+#pragma unroll
+    for (int q = kEbFew - 1; q >= 0; --q) at[k][q] = n > 0 ? list[min(at[k][0] + q, n - 1)] : 0;
+  }
+  if (n > 0) {
+    Raw<P, WIDE, T> x[EACH];
+#pragma unroll
+    for (int k = 0; k < EACH; ++k) x[k].load(dout + (size_t)(c[k] > 0 ? at[k][0] : 0) * D, d, D);
+#pragma unroll
+    for (int k = 0; k < EACH; ++k) {
+      float s[P];
+      x[k].get(s, d, D, c[k] > 0);
+      if (wave_ballot(c[k] > 1)) {
+        Raw<P, WIDE, T> y[kEbFew - 1];
+#pragma unroll
+        for (int q = 1; q < kEbFew; ++q) y[q - 1].load(dout + (size_t)(q < c[k] ? at[k][q] : 0) * D, d, D);
+#pragma unroll
+        for (int q = 1; q < kEbFew; ++q) {
+          float f[P];
+          y[q - 1].get(f, d, D, q < c[k]);
+#pragma unroll
+          for (int j = 0; j < P; ++j) s[j] += f[j];
+        }
+      }
+      if (c[k] < 0) continue;
+#pragma unroll
+      for (int j = 0; j < P; ++j) s[j] *= scale;
+      st_vals<P, WIDE>(s, dW + (size_t)row[k] * D, d, D);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < EACH; ++k) {
+      const float s[P] = {};
+      if (c[k] == 0) st_vals<P, WIDE>(s, dW + (size_t)row[k] * D, d, D);
+    }
+  }
+  __syncthreads();
+  for (int h = w; h < s_n[0]; h += WAVES) {
+    const int v = s_row[h], n = s_count[h], begin = s_begin[h];
+    for (int i = lane; i < n; i += 64) s_list[w][i] = list[begin + i];
+    __builtin_amdgcn_wave_barrier();
+    float t[P] = {};
+    eb_sum<T, WIDE, 8>(t, [&](int i) { return s_list[w][i]; }, n, sub, per, dout, d, D);
+    for (int o = lanes; o < 64; o *= 2)
+#pragma unroll
+      for (int j = 0; j < P; ++j) t[j] += __shfl_xor(t[j], o, 64);
+    if (sub == 0) {
+#pragma unroll
+      for (int j = 0; j < P; ++j) t[j] *= scale;
+      st_vals<P, WIDE>(t, dW + (size_t)v * D, d, D);
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+  for (int h = kEbGroups * 64 - s_n[1]; h < kEbGroups * 64; ++h) {
+    const int v = s_row[h], n = s_count[h], begin = s_begin[h];
+    float t[P] = {};
+    for (int i0 = 0; i0 < n; i0 += WAVES * kEbHot) {
+      const int m = min(n - i0, WAVES * kEbHot);
+      __syncthreads();  // s_list and s_sum have been read
+      for (int i = threadIdx.x; i < m; i += kEbThreads) s_list[0][i] = list[begin + i0 + i];
+      __syncthreads();
+      eb_sum<T, WIDE, 8>(t, [&](int i) { return s_list[0][i]; }, m, w * per + sub, per * WAVES, dout, d, D);
+    }
+    for (int o = lanes; o < 64; o *= 2)
+#pragma unroll
+      for (int j = 0; j < P; ++j) t[j] += __shfl_xor(t[j], o, 64);
+    if (sub == 0)
+#pragma unroll
+      for (int j = 0; j < P; ++j) s_sum[w][l * P + j] = t[j];
+    __syncthreads();
+    if ((int)threadIdx.x < lanes) {
+#pragma unroll
+      for (int j = 0; j < P; ++j) t[j] = 0.0f;
+      for (int k = 0; k < WAVES; ++k)
+#pragma unroll
+        for (int j = 0; j < P; ++j) t[j] += s_sum[k][threadIdx.x * P + j];
+#pragma unroll
+      for (int j = 0; j < P; ++j) t[j] *= scale;
+      st_vals<P, WIDE>(t, dW + (size_t)v * D, d, D);
+    }
   }
 }
 
 static int embed_check(int dtype, int64_t n, int64_t V, int64_t D) {
   if (!lm_dtype_ok(dtype)) return LSH_ERR_ARG;
-  if (n < 0 || n > 0x7fffffff || V < 0 || V > 0x7fffffff || D < 1 || D > 0x7fffffff / 4) return LSH_ERR_SHAPE;
+  if (n < 0 || n > 0x7fffffff - kEsTile || V < 0 || V > 0x7fffffff / 2 || D < 1 || D > (1 << 18))
+    return LSH_ERR_SHAPE;
   return LSH_OK;
+}
+
+// Whether rows of D elements of a type begin at multiples of 16 bytes in both arrays.
+static bool embed_wide(int dtype, int64_t D, const void* a, const void* b) {
+  return D * lm_dtype_size(dtype) % 16 == 0 && (uintptr_t)a % 16 == 0 && (uintptr_t)b % 16 == 0;
 }
 
 }  // namespace lsh
@@ -58,24 +359,61 @@ extern "C" int lsh_embed_fwd(int dtype, const int64_t* tokens, const void* weigh
   if (int rc = embed_check(dtype, n, V, D)) return rc;
   if (n == 0) return LSH_OK;
   if (bad_ptr(tokens) || (V > 0 && bad_ptr(weight)) || bad_ptr(out)) return LSH_ERR_ARG;
+  const int per = 16 / lm_dtype_size(dtype), pieces = (int)((D + per - 1) / per);
+  const int64_t blocks = (n * pieces + 255) / 256;
+  if (blocks > 0x7fffffff) return LSH_ERR_SHAPE;
+  const bool wide = embed_wide(dtype, D, weight, out);
   with_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    k_embed<T><<<dim3((unsigned)n), 256, 0, (hipStream_t)stream>>>(tokens, (const T*)weight, (T*)out, V,
-                                                                  (int)D, padding, scale);
+    auto go = [&](auto kernel) {
+      kernel<<<dim3((unsigned)blocks), 256, 0, (hipStream_t)stream>>>(tokens, (const T*)weight, (T*)out, n, V,
+                                                                     (int)D, padding, scale, pieces);
+    };
+    if (wide)
+      go(k_embed<T, true>);
+    else
+      go(k_embed<T, false>);
   });
   LSH_CHECK_LAUNCH();
   return LSH_OK;
 }
 
+extern "C" size_t lsh_embed_bwd_workspace(int64_t n, int64_t V) {
+  if (embed_check(LSH_F32, n, V, 1)) return 0;
+  const size_t rows = align_up((size_t)V, es_parts(V));
+  return (2 * rows + (size_t)n) * sizeof(int);
+}
+
 extern "C" int lsh_embed_bwd(int dtype, const int64_t* tokens, const void* dout, void* dweight, int64_t n,
-                             int64_t V, int64_t D, int64_t padding, float scale, void* stream) {
+                             int64_t V, int64_t D, int64_t padding, float scale, void* ws, size_t ws_bytes,
+                             void* stream) {
   if (int rc = embed_check(dtype, n, V, D)) return rc;
   if (V == 0) return LSH_OK;
   if (bad_ptr(dweight) || (n > 0 && (bad_ptr(tokens) || bad_ptr(dout)))) return LSH_ERR_ARG;
+  if (bad_ptr(ws) || ws_bytes < lsh_embed_bwd_workspace(n, V)) return LSH_ERR_WORKSPACE;
+  hipStream_t st = (hipStream_t)stream;
+  const int parts = es_parts(V);
+  const size_t rows = align_up((size_t)V, parts);
+  int *start = (int*)ws, *count = start + rows, *list = count + rows;
+  k_embed_sort<<<dim3((unsigned)parts), kEsThreads, 0, st>>>(tokens, (int)n, (int)V, padding, parts, start,
+                                                            count, list);
+  LSH_CHECK_LAUNCH();
+  const int per = 16 / lm_dtype_size(dtype);
+  int lanes = 1;
+  while (lanes < kEbLanes && lanes * per < D) lanes *= 2;
+  const int64_t groups = (V + 64 / lanes - 1) / (64 / lanes);
+  const dim3 grid((unsigned)((groups + kEbGroups - 1) / kEbGroups), (unsigned)((D + kEbLanes * per - 1) / (kEbLanes * per)));
+  const bool wide = embed_wide(dtype, D, dout, dweight);
   with_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    k_embed_bwd<T><<<dim3((unsigned)((V + 3) / 4)), 256, 0, (hipStream_t)stream>>>(
-        tokens, (const T*)dout, (T*)dweight, n, V, (int)D, padding, scale);
+    auto go = [&](auto kernel) {
+      kernel<<<grid, kEbThreads, 0, st>>>(start, count, list, (const T*)dout, (T*)dweight, (int)n, (int)V, (int)D,
+                                          scale, lanes);
+    };
+    if (wide)
+      go(k_embed_bwd<T, true>);
+    else
+      go(k_embed_bwd<T, false>);
   });
   LSH_CHECK_LAUNCH();
   return LSH_OK;

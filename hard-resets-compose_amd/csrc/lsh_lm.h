@@ -50,4 +50,53 @@ __device__ __forceinline__ float wave_sum_f(float v) {
   return v;
 }
 
+// V values of a row from column d on, as read: WIDE in 16-byte accesses (D a multiple of V), otherwise one
+// by one.  Columns beyond D are read from the row's last ones, so that no branch stands around a wide
+// load: behind a branch the compiler waits for each load before it issues the next.
+template <int V, bool WIDE, class T>
+struct Raw {
+  static constexpr int P = V * sizeof(T) > 16 ? 16 / (int)sizeof(T) : V;
+  Vec<T, P> x[V / P];
+  __device__ __forceinline__ void load(const T* p, int d, int D) {
+    if constexpr (WIDE) {
+      const int at = min(d, D - V);
+#pragma unroll
+      for (int i = 0; i < V / P; ++i) x[i] = *(const Vec<T, P>*)(p + at + i * P);
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) x[j / P].v[j % P] = p[min(d + j, D - 1)];
+    }
+  }
+  // as fp32, zeros beyond D or where `there` is false
+  __device__ __forceinline__ void get(float (&f)[V], int d, int D, bool there = true) const {
+#pragma unroll
+    for (int j = 0; j < V; ++j) f[j] = there && d + (WIDE ? 0 : j) < D ? to_f(x[j / P].v[j % P]) : 0.0f;
+  }
+};
+template <int V, bool WIDE, class T>
+__device__ __forceinline__ void ld_vals(float (&f)[V], const T* p, int d, int D) {
+  Raw<V, WIDE, T> x;
+  x.load(p, d, D);
+  x.get(f, d, D);
+}
+template <int V, bool WIDE, class T>
+__device__ __forceinline__ void st_vals(const float (&f)[V], T* p, int d, int D) {
+  if constexpr (WIDE) {
+    if (d < D) {
+      constexpr int P = V * sizeof(T) > 16 ? 16 / sizeof(T) : V;
+#pragma unroll
+      for (int i = 0; i < V; i += P) {
+        Vec<T, P> x;
+#pragma unroll
+        for (int j = 0; j < P; ++j) x.v[j] = from_f<T>(f[i + j]);
+        *(Vec<T, P>*)(p + d + i) = x;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (d + j < D) p[d + j] = from_f<T>(f[j]);
+  }
+}
+
 }  // namespace lsh

@@ -157,10 +157,13 @@ class EmbedFn(torch.autograd.Function):
         (V, D), dtype, scale, pad = ctx.cfg
         dout = dout.contiguous()
         dw = torch.empty(V, D, dtype=dtype, device=dout.device)
+        lib = _n.lib()
+        nbytes = lib.lsh_embed_bwd_workspace(tokens.numel(), V)
+        ws = _n.workspace(nbytes, dout.device)
         with _n.on_device(dout):
-            _n.check(_n.lib().lsh_embed_bwd(
+            _n.check(lib.lsh_embed_bwd(
                 _n.DTYPES[dtype], _n.ptr(tokens), _n.ptr(dout), _n.ptr(dw), tokens.numel(), V, D, pad, scale,
-                _n.stream_of(dout)), "lsh_embed_bwd")
+                _n.ptr(ws), nbytes, _n.stream_of(dout)), "lsh_embed_bwd")
         return None, dw, None, None
 
 

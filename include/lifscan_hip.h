@@ -582,8 +582,9 @@ int lsh_block_norm_bwd(const lsh_block_norm* a, const void* gx, const void* gz, 
  * dout over each token's positions, in fp32 and position order (every row is written). */
 int lsh_embed_fwd(int dtype, const int64_t* tokens, const void* weight, void* out, int64_t n, int64_t V,
                   int64_t D, int64_t padding, float scale, void* stream);
+size_t lsh_embed_bwd_workspace(int64_t n, int64_t V);
 int lsh_embed_bwd(int dtype, const int64_t* tokens, const void* dout, void* dweight, int64_t n, int64_t V,
-                  int64_t D, int64_t padding, float scale, void* stream);
+                  int64_t D, int64_t padding, float scale, void* ws, size_t ws_bytes, void* stream);
 
 /* Distillation from a teacher's top K logits: values (of v_dtype: LSH_F32, or dtype) and index, both
  * [rows, K] and contiguous; an index outside 0..V-1 is no
