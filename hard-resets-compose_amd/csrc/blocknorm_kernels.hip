@@ -32,6 +32,7 @@ struct BnArgs {
 };
 
 // Sums over the lanes that share a row: one wave, or all W of the workgroup (through s, in wave order).
+// One barrier: s is written again only after a barrier behind the next call's, which has another s.
 template <int W, int N>
 __device__ __forceinline__ void row_sums(float (&v)[N], float* s) {
 #pragma unroll
@@ -48,7 +49,6 @@ __device__ __forceinline__ void row_sums(float (&v)[N], float* s) {
 #pragma unroll
       for (int j = 1; j < W; ++j) v[i] += s[j * N + i];
     }
-    __syncthreads();
   }
 }
 
@@ -68,7 +68,7 @@ __device__ __forceinline__ float bn_act(int act, float g, float& d) {
 template <class TX, class TY, int W, int E, bool WIDE>
 __global__ __launch_bounds__(W == 1 ? 256 : W * 64) void k_block_norm(BnArgs a) {
   constexpr int V = 8;
-  __shared__ float s_red[W];
+  __shared__ float s_red[2][W];
   const int lane = W == 1 ? threadIdx.x & 63 : threadIdx.x;
   const int64_t row = W == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
   if (row >= a.rows) return;
@@ -96,7 +96,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * 64) void k_block_norm(BnArgs a) 
   for (int e = 0; e < E; ++e)
 #pragma unroll
     for (int j = 0; j < V; ++j) r[0] = __builtin_fmaf(y[e][j], y[e][j], r[0]);
-  row_sums<W>(r, s_red);
+  row_sums<W>(r, s_red[0]);
   const float ry = 1.0f / sqrtf(r[0] / a.D + a.eps);
   r[0] = 0.0f;
 #pragma unroll
@@ -114,7 +114,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * 64) void k_block_norm(BnArgs a) 
     }
     st_vals<V, WIDE>(xn[e], (TX*)a.x_new + o, d, a.D);
   }
-  row_sums<W>(r, s_red);
+  row_sums<W>(r, s_red[1]);
   const float rx = 1.0f / sqrtf(r[0] / a.D + a.eps);
 #pragma unroll
   for (int e = 0; e < E; ++e) {
@@ -131,41 +131,44 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * 64) void k_block_norm(BnArgs a) 
 // gradients stay in registers until the last row and go to its place of `part`.
 template <class TX, class TY, int W, int E, bool WIDE>
 __global__ __launch_bounds__(W * 64) void k_block_norm_bwd(BnArgs a) {
-  constexpr int V = 8;
-  __shared__ float s_red[W * 2];
+  constexpr int V = 4;  // with 8 the eight values a column take 168 registers: 8192 x 2048 197 us, not NN
+  __shared__ float s_red[3][W * 2];
   float sum[3][E][V] = {};
+  Raw<V, WIDE, TX> qx[E], qgx[E];
+  Raw<V, WIDE, TY> qy[E], qg[E], qgz[E];
+  // what is not there is read from what is, and not used
+  const TY* gate = a.act != LSH_GATE_NONE ? (const TY*)a.gate : (const TY*)a.y;
+  const TY* gzp = a.gz ? (const TY*)a.gz : (const TY*)a.y;
+  const TX* gxp = a.gx ? (const TX*)a.gx : (const TX*)a.x;
+  auto fetch = [&](int64_t row) {
+    const size_t o = (size_t)row * a.D;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int d = (e * 64 * W + threadIdx.x) * V;
+      qy[e].load((const TY*)a.y + o, d, a.D);
+      qx[e].load((const TX*)a.x + o, d, a.D);
+      qg[e].load(gate + o, d, a.D);
+      qgz[e].load(gzp + o, d, a.D);
+      qgx[e].load(gxp + o, d, a.D);
+    }
+  };
+  fetch(blockIdx.x);
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const size_t o = (size_t)row * a.D;
     float x[E][V], y[E][V], g[E][V], gz[E][V], gx[E][V];
-    {
-      Raw<V, WIDE, TX> qx[E], qgx[E];
-      Raw<V, WIDE, TY> qy[E], qg[E], qgz[E];
-      // what is not there is read from what is, and not used
-      const TY* gate = a.act != LSH_GATE_NONE ? (const TY*)a.gate : (const TY*)a.y;
-      const TY* gzp = a.gz ? (const TY*)a.gz : (const TY*)a.y;
-      const TX* gxp = a.gx ? (const TX*)a.gx : (const TX*)a.x;
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const int d = (e * 64 * W + threadIdx.x) * V;
-        qy[e].load((const TY*)a.y + o, d, a.D);
-        qx[e].load((const TX*)a.x + o, d, a.D);
-        qg[e].load(gate + o, d, a.D);
-        qgz[e].load(gzp + o, d, a.D);
-        qgx[e].load(gxp + o, d, a.D);
-      }
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const int d = (e * 64 * W + threadIdx.x) * V;
-        qy[e].get(y[e], d, a.D), qx[e].get(x[e], d, a.D), qg[e].get(g[e], d, a.D, a.act != LSH_GATE_NONE);
-        qgz[e].get(gz[e], d, a.D, a.gz != nullptr), qgx[e].get(gx[e], d, a.D, a.gx != nullptr);
-      }
+    for (int e = 0; e < E; ++e) {
+      const int d = (e * 64 * W + threadIdx.x) * V;
+      qy[e].get(y[e], d, a.D), qx[e].get(x[e], d, a.D), qg[e].get(g[e], d, a.D, a.act != LSH_GATE_NONE);
+      qgz[e].get(gz[e], d, a.D, a.gz != nullptr), qgx[e].get(gx[e], d, a.D, a.gx != nullptr);
     }
+    fetch(min(row + gridDim.x, a.rows - 1));  // while this row is worked on
     float r[1] = {0.0f};
 #pragma unroll
     for (int e = 0; e < E; ++e)
 #pragma unroll
       for (int j = 0; j < V; ++j) r[0] = __builtin_fmaf(y[e][j], y[e][j], r[0]);
-    row_sums<W>(r, s_red);
+    row_sums<W>(r, s_red[0]);
     const float ry = 1.0f / sqrtf(r[0] / a.D + a.eps);
     // x becomes x_new
     float t[2] = {0.0f, 0.0f};
@@ -185,7 +188,7 @@ __global__ __launch_bounds__(W * 64) void k_block_norm_bwd(BnArgs a) {
         t[1] = __builtin_fmaf(gz[e][j] * wq[j], x[e][j], t[1]);
       }
     }
-    row_sums<W>(t, s_red);
+    row_sums<W>(t, s_red[1]);
     const float rx = 1.0f / sqrtf(t[0] / a.D + a.eps);
     const float cx = rx * rx * (t[1] / a.D);
     // gx becomes dx, gz becomes dn
@@ -214,7 +217,7 @@ __global__ __launch_bounds__(W * 64) void k_block_norm_bwd(BnArgs a) {
       st_vals<V, WIDE>(gx[e], (TX*)a.dx + o, d, a.D);
       if (a.dgate) st_vals<V, WIDE>(g[e], (TY*)a.dgate + o, d, a.D);
     }
-    row_sums<W>(r, s_red);
+    row_sums<W>(r, s_red[2]);
     const float cy = ry * ry * (r[0] / a.D);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
@@ -266,24 +269,25 @@ static void with_types(int tx, int ty, F&& f) {
   });
 }
 
-// Calls f with the waves and column groups that hold D channels of a row.  The gradients hold eight
-// values a channel: 16 waves' share of the registers is too small for them up to 8192 channels.
-template <bool GRADS, class F>
+// Calls f with the waves and the groups of PER columns a lane that hold D channels of a row.
+template <int PER, class F>
 static void with_row(int D, F&& f) {
-  auto go = [&](auto w, auto e) { f(w, e); };
   using std::integral_constant;
-  if (D <= 512)
-    go(integral_constant<int, 1>{}, integral_constant<int, 1>{});
-  else if (D <= 1024)
-    go(integral_constant<int, 2>{}, integral_constant<int, 1>{});
-  else if (D <= 2048)
-    go(integral_constant<int, 4>{}, integral_constant<int, 1>{});
-  else if (D <= 4096)
-    go(integral_constant<int, 8>{}, integral_constant<int, 1>{});
-  else if (D <= 8192)
-    go(integral_constant<int, GRADS ? 8 : 16>{}, integral_constant<int, GRADS ? 2 : 1>{});
-  else
-    go(integral_constant<int, 16>{}, integral_constant<int, 2>{});
+  const int lanes = (D + PER - 1) / PER;
+  if (lanes <= 64)
+    f(integral_constant<int, 1>{}, integral_constant<int, 1>{});
+  else if (lanes <= 128)
+    f(integral_constant<int, 2>{}, integral_constant<int, 1>{});
+  else if (lanes <= 256)
+    f(integral_constant<int, 4>{}, integral_constant<int, 1>{});
+  else if (lanes <= 512)
+    f(integral_constant<int, 8>{}, integral_constant<int, 1>{});
+  else if (lanes <= 1024)
+    f(integral_constant<int, 16>{}, integral_constant<int, 1>{});
+  else if (lanes <= 2048)
+    f(integral_constant<int, 16>{}, integral_constant<int, 2>{});
+  else if constexpr (PER == 4)
+    f(integral_constant<int, 16>{}, integral_constant<int, 4>{});
 }
 
 static int bn_check(const lsh_block_norm* a) {
@@ -315,9 +319,9 @@ static bool bn_wide(const BnArgs& a) {
   return true;
 }
 
-// Workgroups of the gradients: each writes 3*D sums of its own, so no more than keep the chip busy.
+// Workgroups of the gradients, each with 3*D sums of its own: 16 waves a CU.
 static int64_t bn_grid(int64_t rows, int D) {
-  const int64_t most = D <= 1024 ? 2048 : D <= 2048 ? 1024 : 512;
+  const int64_t most = D <= 256 ? 4096 : D <= 512 ? 2048 : D <= 1024 ? 1024 : D <= 2048 ? 512 : 256;
   return rows < most ? rows : most;
 }
 
@@ -333,7 +337,7 @@ extern "C" int lsh_block_norm_fwd(const lsh_block_norm* p, void* x_new, void* z,
   a.x_new = x_new, a.z = z;
   const bool wide = bn_wide(a);
   with_types(p->x_dtype, p->dtype, [&](auto tx, auto ty) {
-    with_row<false>(p->D, [&](auto w, auto e) {
+    with_row<8>(p->D, [&](auto w, auto e) {
       using TX = decltype(tx);
       using TY = decltype(ty);
       constexpr int W = decltype(w)::value, E = decltype(e)::value;
@@ -367,7 +371,7 @@ extern "C" int lsh_block_norm_bwd(const lsh_block_norm* p, const void* gx, const
     a.gx = gx, a.gz = gz, a.dx = dx, a.dy = dy, a.dgate = dgate, a.part = (float*)ws;
     const bool wide = bn_wide(a);
     with_types(p->x_dtype, p->dtype, [&](auto tx, auto ty) {
-      with_row<true>(p->D, [&](auto w, auto e) {
+      with_row<4>(p->D, [&](auto w, auto e) {
         using TX = decltype(tx);
         using TY = decltype(ty);
         constexpr int W = decltype(w)::value, E = decltype(e)::value;
