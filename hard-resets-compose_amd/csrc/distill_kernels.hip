@@ -5,164 +5,314 @@
 //   loss = tau^2 * sum_k p_k (log p_k - log q_{i_k})
 //   dz_v = g * tau * (q_v - sum_{k: i_k = v} p_k)
 //
-// A row without entries has loss 0 and gradient 0.  The forward reads the logits once (running
-// maximum and sum) and keeps log(sum exp(z/tau)); the backward reads them once more and writes dz.
+// A row without entries has loss 0 and gradient 0.  All exponents are in base 2: with c = log2(e)/tau,
+// q_v = 2^(c*z_v - l) where l = log2(sum 2^(c*z)), and c*z_v - l is one fused operation.  The forward
+// reads the logits once, with the running maximum and sum of the softmax, and keeps l and the teacher's
+// log2-sum; the backward reads them once more and writes dz.  Both are bound by the logits' bytes
+// (4096 x 32000 bf16: 262 MB forward, 524 MB backward).  A row is split over several workgroups where there
+// are too few rows for the chip, and the parts' maxima and sums are joined in order.
+#include <algorithm>
+
 #include "lsh_lm.h"
 
 namespace lsh {
 
 constexpr int kDsThreads = 256;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-// (maximum, sum of exp(x - maximum)) of two parts
-__device__ __forceinline__ void lse_join(float& m, float& s, float m2, float s2) {
-  const float top = fmaxf(m, m2);
-  const float a = m == top ? 1.0f : expf(m - top), b = m2 == top ? 1.0f : expf(m2 - top);
-  s = s * a + s2 * b;
+struct DsArgs {
+  const void* z;
+  int64_t stride;
+  const void* t;
+  bool t_f32;
+  const int64_t* id;
+  float* loss;
+  float* stats;  // [2, rows]: l, and the teacher's log2-sum (-inf: no entry)
+  float* part;   // [rows, splits, 2]: maximum and sum of each part
+  const float* g;
+  int64_t g_stride;
+  void* dz;
+  int64_t rows, V;
+  int K, splits;
+  int64_t len;  // logits of a part
+  float c, tau;
+};
+
+// (maximum, sum of 2^(c*(x - maximum))) of two parts; a part without values has maximum -inf, sum 0
+__device__ __forceinline__ void ds_join(float& m, float& s, float m2, float s2, float c) {
+  const float top = fmaxf(m, m2), at = top > -INFINITY ? top : 0.0f;
+  s = s * __builtin_amdgcn_exp2f((m - at) * c) + s2 * __builtin_amdgcn_exp2f((m2 - at) * c);
   m = top;
 }
 
-// Element i of an array of either type
+// Element i of the teacher's logits, of either type
 template <class T>
-__device__ __forceinline__ float ds_value(const void* p, int64_t i, bool f32) {
-  return f32 ? ((const float*)p)[i] : to_f(((const T*)p)[i]);
+__device__ __forceinline__ float ds_value(const DsArgs& a, int64_t i) {
+  return a.t_f32 ? ((const float*)a.t)[i] : to_f(((const T*)a.t)[i]);
 }
 
-// The teacher's distribution of a row, in LDS: p[k] and id[k] (-1: no entry).  Returns whether the
-// row has an entry of weight.
+// The part of a row from element v0 on, as pieces of 16 bytes at aligned addresses with single elements
+// before and behind them.
 template <class T>
-__device__ __forceinline__ bool ds_teacher(const void* t, bool t_f32, const int64_t* ids, int64_t row,
-                                           int K, int64_t V, float itau, float* p, int* id, float* red) {
-  const int lane = threadIdx.x & 63;
-  if (threadIdx.x < 64) {
-    float m = -INFINITY;
-    for (int k = lane; k < K; k += 64) {
-      const int64_t i = ids[row * K + k];
-      const bool there = i >= 0 && i < V;
-      id[k] = there ? (int)i : -1;
-      p[k] = there ? ds_value<T>(t, row * K + k, t_f32) * itau : -INFINITY;
-      m = fmaxf(m, p[k]);
-    }
-    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-    float s = 0.0f;
-    for (int k = lane; k < K; k += 64) {
-      p[k] = m > -INFINITY ? expf(p[k] - m) : 0.0f;
-      s += p[k];
-    }
-    s = wave_sum_f(s);
-    for (int k = lane; k < K; k += 64) p[k] = s != 0.0f ? p[k] / s : 0.0f;
-    if (lane == 0) red[0] = s;
+struct DsPart {
+  static constexpr int P = kWide<T>;
+  int lead, pieces, n;  // elements before the first piece, pieces, elements in all
+  __device__ __forceinline__ DsPart(const T* p, int64_t count) {
+    n = (int)count;
+    lead = min((int)((16 - ((uintptr_t)p & 15)) & 15) / (int)sizeof(T), n);
+    pieces = (n - lead) / P;
   }
-  __syncthreads();
-  return red[0] != 0.0f;
+  // this thread's single element, or -1
+  __device__ __forceinline__ int single() const {
+    const int i = threadIdx.x, tail = lead + pieces * P;
+    return i < lead ? i : i - lead < n - tail ? tail + i - lead : -1;
+  }
+};
+
+// The teacher's side of a row by one wave: log2-sum of its entries, and the loss given l.
+template <class T>
+__device__ __forceinline__ void ds_loss(const DsArgs& a, int64_t row, float l) {
+  const int lane = threadIdx.x & 63;
+  const T* z = (const T*)a.z + row * a.stride;
+  float m = -INFINITY, s = 0.0f;
+  for (int k = lane; k < a.K; k += 64) {
+    const int64_t i = a.id[row * a.K + k];
+    if (i >= 0 && i < a.V) ds_join(m, s, ds_value<T>(a, row * a.K + k), 1.0f, a.c);
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) ds_join(m, s, __shfl_xor(m, o, 64), __shfl_xor(s, o, 64), a.c);
+  const bool some = s != 0.0f && m != -INFINITY;  // a NaN counts
+  const float tl = some ? __builtin_fmaf(m, a.c, __builtin_amdgcn_logf(s)) : -INFINITY;
+  float sum = 0.0f;
+  for (int k = lane; k < a.K && some; k += 64) {
+    const int64_t i = a.id[row * a.K + k];
+    if (i < 0 || i >= a.V) continue;
+    const float lp = __builtin_fmaf(ds_value<T>(a, row * a.K + k), a.c, -tl);
+    const float p = __builtin_amdgcn_exp2f(lp);
+    if (p != 0.0f) sum += p * (lp - __builtin_fmaf(to_f(z[i]), a.c, -l));
+  }
+  sum = wave_sum_f(sum);
+  if (lane == 0) {
+    a.loss[row] = some ? a.tau * a.tau * kLn2 * sum : 0.0f;
+    a.stats[row] = l;
+    a.stats[a.rows + row] = tl;
+  }
 }
 
-template <class T>
-__global__ __launch_bounds__(kDsThreads) void k_distill(const T* __restrict__ z, int64_t stride,
-                                                        const void* __restrict__ tv, bool tv_f32,
-                                                        const int64_t* __restrict__ ti,
-                                                        float* __restrict__ loss, float* __restrict__ lse,
-                                                        int64_t V, int K, float tau) {
-  extern __shared__ float s_dyn[];
-  float* p = s_dyn;
-  int* id = (int*)(s_dyn + K);
-  __shared__ float s_m[kDsThreads / 64], s_s[kDsThreads / 64], red[1];
-  const int64_t row = blockIdx.x;
-  z += row * stride;
-  const float itau = 1.0f / tau;
-  const bool some = ds_teacher<T>(tv, tv_f32, ti, row, K, V, itau, p, id, red);
+template <class T, bool SPLIT>
+__global__ __launch_bounds__(kDsThreads) void k_distill(DsArgs a) {
+  constexpr int P = kWide<T>, U = 4;
+  __shared__ float s_m[kDsThreads / 64], s_s[kDsThreads / 64];
+  const int64_t row = SPLIT ? blockIdx.x / a.splits : blockIdx.x, part = SPLIT ? blockIdx.x % a.splits : 0;
+  const int64_t v0 = part * a.len;
+  const T* z = (const T*)a.z + row * a.stride + v0;
+  const DsPart<T> x(z, min(a.len, a.V - v0));
   float m = -INFINITY, s = 0.0f;
-  for (int64_t v = threadIdx.x; v < V; v += kDsThreads) lse_join(m, s, to_f(z[v]) * itau, 1.0f);
-  for (int o = 32; o > 0; o >>= 1) lse_join(m, s, __shfl_xor(m, o, 64), __shfl_xor(s, o, 64));
+  auto take = [&](const float (&f)[P], int n) {
+    float top = m;
+#pragma unroll
+    for (int j = 0; j < P; ++j) top = fmaxf(top, j < n ? f[j] : -INFINITY);
+    const float at = top > -INFINITY ? top : 0.0f, off = -at * a.c;
+    s *= __builtin_amdgcn_exp2f((m - at) * a.c);
+#pragma unroll
+    for (int j = 0; j < P; ++j)
+      if (j < n) s += __builtin_amdgcn_exp2f(__builtin_fmaf(f[j], a.c, off));
+    m = top;
+  };
+  const Vec<T, P>* v = (const Vec<T, P>*)(z + x.lead);
+  int i = threadIdx.x;
+  for (; i + (U - 1) * kDsThreads < x.pieces; i += U * kDsThreads) {
+    Vec<T, P> y[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) y[u] = v[i + u * kDsThreads];
+    float f[U][P], top = m;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < P; ++j) {
+        f[u][j] = to_f(y[u].v[j]);
+        top = fmaxf(top, f[u][j]);
+      }
+    const float at = top > -INFINITY ? top : 0.0f, off = -at * a.c;
+    s *= __builtin_amdgcn_exp2f((m - at) * a.c);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < P; ++j) s += __builtin_amdgcn_exp2f(__builtin_fmaf(f[u][j], a.c, off));
+    m = top;
+  }
+  for (; i < x.pieces; i += kDsThreads) {
+    const Vec<T, P> y = v[i];
+    float f[P];
+#pragma unroll
+    for (int j = 0; j < P; ++j) f[j] = to_f(y.v[j]);
+    take(f, P);
+  }
+  if (const int e = x.single(); e >= 0) {
+    const float f[P] = {to_f(z[e])};
+    take(f, 1);
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) ds_join(m, s, __shfl_xor(m, o, 64), __shfl_xor(s, o, 64), a.c);
   if ((threadIdx.x & 63) == 0) s_m[threadIdx.x >> 6] = m, s_s[threadIdx.x >> 6] = s;
   __syncthreads();
-  if (threadIdx.x < 64) {
-    m = s_m[0], s = s_s[0];
-    for (int w = 1; w < kDsThreads / 64; ++w) lse_join(m, s, s_m[w], s_s[w]);
-    const float l = m + logf(s);
-    float sum = 0.0f;
-    for (int k = threadIdx.x; k < K; k += 64)
-      if (id[k] >= 0 && p[k] > 0.0f) sum += p[k] * (logf(p[k]) - (to_f(z[id[k]]) * itau - l));
-    sum = wave_sum_f(sum);
+  if (threadIdx.x >= 64) return;
+  m = s_m[0], s = s_s[0];
+#pragma unroll
+  for (int w = 1; w < kDsThreads / 64; ++w) ds_join(m, s, s_m[w], s_s[w], a.c);
+  if (SPLIT) {
     if (threadIdx.x == 0) {
-      loss[row] = some ? tau * tau * sum : 0.0f;
-      lse[row] = l;
+      float* to = a.part + (row * a.splits + part) * 2;
+      to[0] = m, to[1] = s;
     }
+  } else {
+    ds_loss<T>(a, row, (m > -INFINITY ? m * a.c : 0.0f) + __builtin_amdgcn_logf(s));
   }
 }
 
+// The parts of a row joined, one wave a row.
 template <class T>
-__global__ __launch_bounds__(kDsThreads) void k_distill_bwd(const T* __restrict__ z, int64_t stride,
-                                                            const void* __restrict__ tv, bool tv_f32,
-                                                            const int64_t* __restrict__ ti,
-                                                            const float* __restrict__ lse,
-                                                            const float* __restrict__ g, int64_t g_stride,
-                                                            T* __restrict__ dz, int64_t V, int K, float tau) {
-  extern __shared__ float s_dyn[];
-  float* p = s_dyn;
-  int* id = (int*)(s_dyn + K);
-  __shared__ float red[1];
+__global__ __launch_bounds__(64) void k_distill_join(DsArgs a) {
   const int64_t row = blockIdx.x;
-  z += row * stride;
-  dz += row * V;
-  const float itau = 1.0f / tau, l = lse[row];
-  const bool some = ds_teacher<T>(tv, tv_f32, ti, row, K, V, itau, p, id, red);
-  const float f = g[row * g_stride] * tau;
-  for (int64_t v = threadIdx.x; v < V; v += kDsThreads)
-    dz[v] = from_f<T>(some ? f * expf(to_f(z[v]) * itau - l) : 0.0f);
-  __syncthreads();  // the rows' entries are written again with the teacher's part
+  float m = -INFINITY, s = 0.0f;
+  for (int i = 0; i < a.splits; ++i) {
+    const float* p = a.part + (row * a.splits + i) * 2;
+    ds_join(m, s, p[0], p[1], a.c);
+  }
+  ds_loss<T>(a, row, (m > -INFINITY ? m * a.c : 0.0f) + __builtin_amdgcn_logf(s));
+}
+
+template <class T>
+__global__ __launch_bounds__(kDsThreads) void k_distill_bwd(DsArgs a) {
+  constexpr int P = kWide<T>, U = 4;
+  extern __shared__ int s_id[];  // the teacher's ids of this part, as places in it (-1: none), then their p
+  float* s_p = (float*)(s_id + a.K);
+  const int64_t row = blockIdx.x / a.splits, v0 = blockIdx.x % a.splits * a.len;
+  const T* z = (const T*)a.z + row * a.stride + v0;
+  T* dz = (T*)a.dz + row * a.V + v0;
+  const DsPart<T> x(z, min(a.len, a.V - v0));
+  const float l = a.stats[row], tl = a.stats[a.rows + row];
+  const bool some = tl != -INFINITY;
+  const float f = some ? a.g[row * a.g_stride] * a.tau : 0.0f;
+  auto grad = [&](float y) { return some ? f * __builtin_amdgcn_exp2f(__builtin_fmaf(y, a.c, -l)) : 0.0f; };
+  const Vec<T, P>* v = (const Vec<T, P>*)(z + x.lead);
+  const bool wide = ((uintptr_t)(dz + x.lead) & 15) == 0;
+  auto put = [&](const Vec<T, P>& y, int i) {
+    Vec<T, P> d;
+#pragma unroll
+    for (int j = 0; j < P; ++j) d.v[j] = from_f<T>(grad(to_f(y.v[j])));
+    if (wide) {
+      *(Vec<T, P>*)(dz + x.lead + (int64_t)i * P) = d;
+    } else {
+#pragma unroll
+      for (int j = 0; j < P; ++j) dz[x.lead + (int64_t)i * P + j] = d.v[j];
+    }
+  };
+  int i = threadIdx.x;
+  for (; i + (U - 1) * kDsThreads < x.pieces; i += U * kDsThreads) {
+    Vec<T, P> y[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) y[u] = v[i + u * kDsThreads];
+#pragma unroll
+    for (int u = 0; u < U; ++u) put(y[u], i + u * kDsThreads);
+  }
+  for (; i < x.pieces; i += kDsThreads) put(v[i], i);
+  if (const int e = x.single(); e >= 0) dz[e] = from_f<T>(grad(to_f(z[e])));
   if (!some) return;
-  for (int k = threadIdx.x; k < K; k += kDsThreads) {
-    const int v = id[k];
-    bool first = v >= 0;
-    float sum = 0.0f;
-    for (int j = 0; j < K && first; ++j)
-      if (id[j] == v) {
-        first = j >= k;
-        sum += p[j];
+  for (int k = threadIdx.x; k < a.K; k += kDsThreads) {
+    const int64_t id = a.id[row * a.K + k];
+    const bool here = id >= v0 && id < v0 + x.n;
+    s_id[k] = here ? (int)(id - v0) : -1;
+    s_p[k] = here ? __builtin_amdgcn_exp2f(__builtin_fmaf(ds_value<T>(a, row * a.K + k), a.c, -tl)) : 0.0f;
+  }
+  __syncthreads();  // also the part's stores: its entries are written again with the teacher's part
+  for (int k = threadIdx.x; k < a.K; k += kDsThreads) {
+    const int e = s_id[k];
+    if (e < 0) continue;
+    bool first = true;
+    float p = 0.0f;
+    for (int j = 0; j < a.K; ++j)
+      if (s_id[j] == e) {
+        first = first && j >= k;
+        p += s_p[j];
       }
-    if (first) dz[v] = from_f<T>(f * (expf(to_f(z[v]) * itau - l) - sum));
+    if (first) dz[e] = from_f<T>(f * (__builtin_amdgcn_exp2f(__builtin_fmaf(to_f(z[e]), a.c, -l)) - p));
   }
 }
 
 static int ds_check(int dtype, int v_dtype, int64_t rows, int64_t V, int K, float tau) {
-  if (!lm_dtype_ok(dtype) || (v_dtype != LSH_F32 && v_dtype != dtype) || !(tau > 0.0f) || !(tau < INFINITY)) return LSH_ERR_ARG;
-  if (rows < 0 || rows > 0x7fffffff || V < 1 || V > 0x7fffffff || K < 0 || K > LSH_DISTILL_MAX_K)
+  if (!lm_dtype_ok(dtype) || (v_dtype != LSH_F32 && v_dtype != dtype) || !(tau > 0.0f) || !(tau < INFINITY))
+    return LSH_ERR_ARG;
+  if (rows < 0 || rows > 0x7fffffff / 64 || V < 1 || V > 0x7fffffff / 2 || K < 0 || K > LSH_DISTILL_MAX_K)
     return LSH_ERR_SHAPE;
   return LSH_OK;
+}
+
+// Parts of a row: about 1024 workgroups, none of less than 4096 logits.
+static int ds_splits(int64_t rows, int64_t V) {
+  const int64_t most = std::min<int64_t>((V + 4095) / 4096, 64);
+  return (int)std::max<int64_t>(1, std::min(most, 1024 / std::max<int64_t>(rows, 1)));
+}
+
+static DsArgs ds_args(const void* logits, int64_t stride, int v_dtype, const void* values,
+                      const int64_t* index, int64_t rows, int64_t V, int K, float tau) {
+  DsArgs a = {};
+  a.z = logits, a.stride = stride, a.t = values, a.t_f32 = v_dtype == LSH_F32, a.id = index;
+  a.rows = rows, a.V = V, a.K = K;
+  a.splits = ds_splits(rows, V);
+  a.len = (V + a.splits - 1) / a.splits;
+  a.c = kLog2e / tau, a.tau = tau;
+  return a;
 }
 
 }  // namespace lsh
 
 using namespace lsh;
 
+extern "C" size_t lsh_distill_workspace(int64_t rows, int64_t V) {
+  if (ds_check(LSH_F32, LSH_F32, rows, V, 0, 1.0f)) return 0;
+  const int splits = ds_splits(rows, V);
+  return splits > 1 ? (size_t)rows * splits * 2 * sizeof(float) : 0;
+}
+
 extern "C" int lsh_distill_fwd(int dtype, const void* logits, int64_t stride, int v_dtype, const void* values,
-                               const int64_t* index, float* loss, float* lse, int64_t rows, int64_t V,
-                               int K, float tau, void* stream) {
+                               const int64_t* index, float* loss, float* stats, int64_t rows, int64_t V,
+                               int K, float tau, void* ws, size_t ws_bytes, void* stream) {
   if (int rc = ds_check(dtype, v_dtype, rows, V, K, tau)) return rc;
   if (rows == 0) return LSH_OK;
-  if (bad_ptr(logits) || (K > 0 && (bad_ptr(values) || bad_ptr(index))) || bad_ptr(loss) || bad_ptr(lse))
+  if (bad_ptr(logits) || (K > 0 && (bad_ptr(values) || bad_ptr(index))) || bad_ptr(loss) || bad_ptr(stats))
     return LSH_ERR_ARG;
+  const size_t need = lsh_distill_workspace(rows, V);
+  if (need && (bad_ptr(ws) || ws_bytes < need)) return LSH_ERR_WORKSPACE;
+  DsArgs a = ds_args(logits, stride, v_dtype, values, index, rows, V, K, tau);
+  a.loss = loss, a.stats = stats, a.part = (float*)ws;
+  hipStream_t st = (hipStream_t)stream;
   with_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    k_distill<T><<<dim3((unsigned)rows), kDsThreads, (size_t)K * 8, (hipStream_t)stream>>>(
-        (const T*)logits, stride, values, v_dtype == LSH_F32, index, loss, lse, V, K, tau);
+    if (a.splits > 1) {
+      k_distill<T, true><<<dim3((unsigned)(rows * a.splits)), kDsThreads, 0, st>>>(a);
+      k_distill_join<T><<<dim3((unsigned)rows), 64, 0, st>>>(a);
+    } else {
+      k_distill<T, false><<<dim3((unsigned)rows), kDsThreads, 0, st>>>(a);
+    }
   });
   LSH_CHECK_LAUNCH();
   return LSH_OK;
 }
 
 extern "C" int lsh_distill_bwd(int dtype, const void* logits, int64_t stride, int v_dtype, const void* values,
-                               const int64_t* index, const float* lse, const float* g, int64_t g_stride,
+                               const int64_t* index, const float* stats, const float* g, int64_t g_stride,
                                void* dlogits, int64_t rows, int64_t V, int K, float tau, void* stream) {
   if (int rc = ds_check(dtype, v_dtype, rows, V, K, tau)) return rc;
   if (rows == 0) return LSH_OK;
-  if (bad_ptr(logits) || (K > 0 && (bad_ptr(values) || bad_ptr(index))) || bad_ptr(lse) || bad_ptr(g) ||
+  if (bad_ptr(logits) || (K > 0 && (bad_ptr(values) || bad_ptr(index))) || bad_ptr(stats) || bad_ptr(g) ||
       bad_ptr(dlogits))
     return LSH_ERR_ARG;
+  DsArgs a = ds_args(logits, stride, v_dtype, values, index, rows, V, K, tau);
+  a.stats = (float*)stats, a.g = g, a.g_stride = g_stride, a.dz = dlogits;
   with_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    k_distill_bwd<T><<<dim3((unsigned)rows), kDsThreads, (size_t)K * 8, (hipStream_t)stream>>>(
-        (const T*)logits, stride, values, v_dtype == LSH_F32, index, lse, g, g_stride, (T*)dlogits, V, K, tau);
+    k_distill_bwd<T><<<dim3((unsigned)(rows * a.splits)), kDsThreads, (size_t)K * 8, (hipStream_t)stream>>>(a);
   });
   LSH_CHECK_LAUNCH();
   return LSH_OK;

@@ -193,7 +193,8 @@ SIGNATURES = {
     "lsh_embed_fwd": (c_i, [c_i, c_p, c_p, c_p, c_i64, c_i64, c_i64, c_i64, c_f, c_p]),
     "lsh_embed_bwd_workspace": (c_sz, [c_i64, c_i64]),
     "lsh_embed_bwd": (c_i, [c_i, c_p, c_p, c_p, c_i64, c_i64, c_i64, c_i64, c_f, c_p, c_sz, c_p]),
-    "lsh_distill_fwd": (c_i, [c_i, c_p, c_i64, c_i, c_p, c_p, c_p, c_p, c_i64, c_i64, c_i, c_f, c_p]),
+    "lsh_distill_workspace": (c_sz, [c_i64, c_i64]),
+    "lsh_distill_fwd": (c_i, [c_i, c_p, c_i64, c_i, c_p, c_p, c_p, c_p, c_i64, c_i64, c_i, c_f, c_p, c_sz, c_p]),
     "lsh_distill_bwd": (c_i, [c_i, c_p, c_i64, c_i, c_p, c_p, c_p, c_p, c_i64, c_p, c_i64, c_i64, c_i, c_f, c_p]),
 }
 

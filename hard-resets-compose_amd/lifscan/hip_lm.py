@@ -189,13 +189,17 @@ def embed(tokens, weight, scale=1.0, padding_idx=None):
 # ------------------------------------------------------------------------- distillation
 def _distill_forward(logits, values, index, tau):
     rows, V = logits.shape
-    loss, lse = torch.empty(2, rows, dtype=torch.float32, device=logits.device)
+    loss = torch.empty(rows, dtype=torch.float32, device=logits.device)
+    stats = torch.empty(2, rows, dtype=torch.float32, device=logits.device)
+    lib = _n.lib()
+    nbytes = lib.lsh_distill_workspace(rows, V)
+    ws = _n.workspace(nbytes, logits.device) if nbytes else None
     with _n.on_device(logits):
-        _n.check(_n.lib().lsh_distill_fwd(
-            _n.DTYPES[logits.dtype], _n.ptr(logits), logits.stride(0), _n.DTYPES[values.dtype], _n.ptr(values), _n.ptr(index),
-            _n.ptr(loss), _n.ptr(lse), rows, V, values.shape[1], tau, _n.stream_of(logits)),
-            "lsh_distill_fwd")
-    return loss, lse
+        _n.check(lib.lsh_distill_fwd(
+            _n.DTYPES[logits.dtype], _n.ptr(logits), logits.stride(0), _n.DTYPES[values.dtype], _n.ptr(values),
+            _n.ptr(index), _n.ptr(loss), _n.ptr(stats), rows, V, values.shape[1], tau, _n.ptr(ws), nbytes,
+            _n.stream_of(logits)), "lsh_distill_fwd")
+    return loss, stats
 
 
 class DistillFn(torch.autograd.Function):
@@ -203,20 +207,20 @@ class DistillFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, values, index, tau):
-        loss, lse = _distill_forward(logits, values, index, tau)
-        ctx.save_for_backward(logits, values, index, lse)
+        loss, stats = _distill_forward(logits, values, index, tau)
+        ctx.save_for_backward(logits, values, index, stats)
         ctx.tau = tau
         return loss
 
     @staticmethod
     def backward(ctx, g):
-        logits, values, index, lse = ctx.saved_tensors
+        logits, values, index, stats = ctx.saved_tensors
         rows, V = logits.shape
         dz = torch.empty(rows, V, dtype=logits.dtype, device=logits.device)
         with _n.on_device(logits):
             _n.check(_n.lib().lsh_distill_bwd(
                 _n.DTYPES[logits.dtype], _n.ptr(logits), logits.stride(0), _n.DTYPES[values.dtype], _n.ptr(values), _n.ptr(index),
-                _n.ptr(lse), _n.ptr(g), g.stride(0), _n.ptr(dz), rows, V, values.shape[1], ctx.tau,
+                _n.ptr(stats), _n.ptr(g), g.stride(0), _n.ptr(dz), rows, V, values.shape[1], ctx.tau,
                 _n.stream_of(logits)), "lsh_distill_bwd")
         return dz, None, None, None
 

@@ -591,14 +591,16 @@ int lsh_embed_bwd(int dtype, const int64_t* tokens, const void* dout, void* dwei
  * entry; logits [rows, V] with a row stride in elements.  With p the softmax of values/tau over
  * the entries and q that of logits/tau over the vocabulary,
  *   loss = tau^2 * sum_k p_k (log p_k - log q_{index_k}),
- * 0 for a row without entries.  lse: [rows], log(sum exp(logits/tau)), which the gradient reads.
+ * 0 for a row without entries.  stats: [2, rows], what the gradient reads: log2(sum exp(logits/tau)) and
+ * the teacher's log2(sum exp(values/tau)), -inf for a row without entries.
  *   dlogits = g * tau * (q - p at its ids), contiguous [rows, V]; g: [rows] with an element stride. */
 #define LSH_DISTILL_MAX_K 4096
+size_t lsh_distill_workspace(int64_t rows, int64_t V); /* 0: ws may be NULL */
 int lsh_distill_fwd(int dtype, const void* logits, int64_t stride, int v_dtype, const void* values,
-                    const int64_t* index, float* loss, float* lse, int64_t rows, int64_t V, int K,
-                    float tau, void* stream);
+                    const int64_t* index, float* loss, float* stats, int64_t rows, int64_t V, int K,
+                    float tau, void* ws, size_t ws_bytes, void* stream);
 int lsh_distill_bwd(int dtype, const void* logits, int64_t stride, int v_dtype, const void* values,
-                    const int64_t* index, const float* lse, const float* g, int64_t g_stride,
+                    const int64_t* index, const float* stats, const float* g, int64_t g_stride,
                     void* dlogits, int64_t rows, int64_t V, int K, float tau, void* stream);
 
 #ifdef __cplusplus
