@@ -85,9 +85,6 @@ class BlockNorm(ctypes.Structure):
         [(n, c_p) for n in ("x", "y", "gate", "w_post", "w_pre", "scale")] + [("scale1", c_f), ("eps", c_f)]
 
 
-# element types of the language-model operators
-DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-
 # name -> (restype, argtypes); mirrors include/lifscan_hip.h
 SIGNATURES = {
     "lsh_abi_version": (c_i, []),
@@ -243,10 +240,20 @@ def ops():
         mod = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(mod)
         L = lib()
-        mod.set_entry_points({name: ctypes.cast(getattr(L, name), ctypes.c_void_p).value
-                              for name in SIGNATURES})
+        addresses = {name: ctypes.cast(getattr(L, name), ctypes.c_void_p).value for name in SIGNATURES}
+        mod.set_entry_points(addresses)
+        mod.set_lm_entry_points(addresses)
         _OPS = mod
     return _OPS
+
+
+def lm_ops():
+    """The same module for the language-model operators, which have no other path."""
+    mod = _OPS or ops()
+    if mod is None:
+        raise RuntimeError(f"C++ operators not built ({_build.OPS_PATH} missing): run `python -c \"import "
+                           f"__graft_entry__ as g; g.build()\"`")
+    return mod
 
 
 def check(rc, what):

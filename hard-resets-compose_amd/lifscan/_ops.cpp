@@ -351,6 +351,8 @@ std::vector<double> read_scalars(const std::vector<Tensor>& ts) {
 
 }  // namespace
 
+void register_lm_ops(pybind11::module_& m);  // _ops_lm.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "C++ autograd functions of the lifscan layers over the lifscan C ABI";
   m.def("set_entry_points", &set_entry_points, "addresses of the C-ABI entry points, by name");
@@ -360,4 +362,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("last_lookback", &last_lookback, "workspace of the most recent look-back adjoint here, or None");
   m.def("lookback_runs", &lookback_runs, "look-back adjoints run here so far");
   m.def("read_scalars", &read_scalars, "values of one-element tensors in one copy");
+  register_lm_ops(m);
 }
