@@ -2,5 +2,5 @@
 #include "linattn_walk.h"
 
 namespace lsh {
-int la_launch_bf16(const LaWalk& a, bool sums, hipStream_t st) { return la_launch<bf16_t, bf16_t>(a, sums, st); }
+int la_launch_bf16(const LaWalks& all, bool sums, hipStream_t st) { return la_launch<bf16_t, bf16_t>(all, sums, st); }
 }  // namespace lsh

@@ -2,5 +2,5 @@
 #include "linattn_walk.h"
 
 namespace lsh {
-int la_launch_f32(const LaWalk& a, bool sums, hipStream_t st) { return la_launch<float, float>(a, sums, st); }
+int la_launch_f32(const LaWalks& all, bool sums, hipStream_t st) { return la_launch<float, float>(all, sums, st); }
 }  // namespace lsh

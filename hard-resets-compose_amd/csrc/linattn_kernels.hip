@@ -28,9 +28,15 @@ __global__ __launch_bounds__(256) void k_la_join(float* __restrict__ starts, con
   const float f = __builtin_amdgcn_exp2f(la_log2(beta[i / size % H]) * (float)L);
   float s = s0 ? s0[i] : 0.0f;
   starts[i] = s;
-  for (int j = 1; j < segs; ++j) {
-    s = __builtin_fmaf(f, s, starts[(size_t)j * n + i]);
-    starts[(size_t)j * n + i] = s;
+  for (int j0 = 1; j0 < segs; j0 += 16) {
+    float x[16];  // the loads first: one latency for sixteen segments
+#pragma unroll
+    for (int j = 0; j < 16; ++j) x[j] = starts[(size_t)min(j0 + j, segs - 1) * n + i];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      s = __builtin_fmaf(f, s, x[j]);
+      if (j0 + j < segs) starts[(size_t)(j0 + j) * n + i] = s;
+    }
   }
 }
 
@@ -47,10 +53,16 @@ __global__ __launch_bounds__(256) void k_la_share(const float* __restrict__ x, T
   y[i] = from_f<T>(s);
 }
 
+static int la_go(const LaWalks& all, int dtype, bool sums, hipStream_t st) {
+  return dtype == LSH_F32    ? la_launch_f32(all, sums, st)
+         : dtype == LSH_BF16 ? la_launch_bf16(all, sums, st)
+                             : la_launch_f16(all, sums, st);
+}
 static int la_go(const LaWalk& a, int dtype, bool sums, hipStream_t st) {
-  return dtype == LSH_F32    ? la_launch_f32(a, sums, st)
-         : dtype == LSH_BF16 ? la_launch_bf16(a, sums, st)
-                             : la_launch_f16(a, sums, st);
+  LaWalks all = {};
+  all.w[0] = a;
+  all.n = 1;
+  return la_go(all, dtype, sums, st);
 }
 
 // How the rows are split: every segment but the last has L rows.  The walk alone has a workgroup for
@@ -62,12 +74,12 @@ struct LaSplit {
 };
 static LaSplit la_split(int dtype, int64_t T, int64_t BH, int DK, int DV) {
   const int64_t C = la_chunk(dtype), chunks = (T + C - 1) / C;
-  const int block = la_block(DK, DV);
+  const int block = la_block(dtype, DK, DV);
   const int64_t groups = BH * ((DV + block - 1) / block);
   // LDS holds two workgroups a CU in bf16, one in fp32 from 65 state rows on.  Measured with 256 and 512
   // workgroups: bf16 4096 x 4 x 16 x 128 forward 137 and 127 us, fp32 2048 x 4 x 16 x 128 168 and 183 us.
   const int64_t fill = dtype == LSH_BF16 || std::max(DK, DV) <= 64 ? 512 : 256;
-  int64_t segs = std::min<int64_t>((fill + groups - 1) / std::max<int64_t>(groups, 1), chunks / 4);
+  int64_t segs = std::min<int64_t>((fill + groups - 1) / std::max<int64_t>(groups, 1), chunks / 2);
   if (segs < 2) return {1, std::max<int64_t>(T, 1)};
   const int64_t per = (chunks + segs - 1) / segs;
   return {(int)((chunks + per - 1) / per), per * C};
@@ -219,7 +231,7 @@ extern "C" size_t lsh_linattn_bwd_workspace(const lsh_linattn* a) {
   if (la_check(a) || a->H == 0) return 0;
   size_t n = 0;
   for (auto [heads, D] : {std::pair<int, int>{a->q_heads, a->Dk}, {a->k_heads, a->Dk}, {a->v_heads, a->Dv}})
-    if (heads != a->H) n = std::max(n, (size_t)a->T * a->B * a->H * D * 4);
+    if (heads != a->H) n += (size_t)a->T * a->B * a->H * D * 4;
   return align_up(la_starts_bytes(a), 256) + n;
 }
 
@@ -242,28 +254,20 @@ extern "C" int lsh_linattn_bwd(const lsh_linattn* a, const void* starts, const v
   w.beta = a->beta;
   w.T = a->T, w.B = a->B, w.H = a->H;
   la_set_split(w, split);
-  auto run = [&](void* out, int heads) -> int {
-    const bool shared = heads != a->H;
-    w.out = shared ? heads_f32 : out;
-    w.out_f32 = shared || a->dtype == LSH_F32;
-    if (int rc = la_go(w, a->dtype, false, st)) return rc;
-    if (shared && a->T > 0) {
-      const int64_t n = a->T * a->B * heads * w.DV;
-      with_dtype(a->dtype, [&](auto t) {
-        using T = decltype(t);
-        k_la_share<T><<<dim3((unsigned)((n + 255) / 256)), 256, 0, st>>>(heads_f32, (T*)out, n, w.DV,
-                                                                        (int)(a->H / heads));
-      });
-      LSH_CHECK_LAUNCH();
-    }
-    return LSH_OK;
+  // a shared head's gradient is formed for every head that shares it, in fp32, and then summed
+  struct Out {
+    void* to;
+    int heads;
+    int D;
+    float* f32;
   };
-  // dq: the forward walk with the state transposed
-  w.q = d, w.k = v, w.v = k;
-  w.DK = a->Dv, w.DV = a->Dk, w.sk = 1, w.sv = a->Dv;
-  w.s_in = split.segs > 1 ? (const float*)starts : a->s0;
-  w.so = a->scale, w.su = 1.0f;
-  if (int rc = run(dq, a->q_heads)) return rc;
+  auto out = [&](LaWalk& x, void* to, int heads) {
+    const Out o = {to, heads, x.DV, heads != a->H ? heads_f32 : nullptr};
+    x.out = o.f32 ? o.f32 : to;
+    x.out_f32 = o.f32 || a->dtype == LSH_F32;
+    if (o.f32) heads_f32 += (size_t)a->T * a->B * a->H * x.DV;
+    return o;
+  };
   // dv from the last row, and the gradient that leaves the first
   w.q = k, w.k = q, w.v = d;
   w.DK = a->Dk, w.DV = a->Dv, w.sk = a->Dv, w.sv = 1;
@@ -271,12 +275,35 @@ extern "C" int lsh_linattn_bwd(const lsh_linattn* a, const void* starts, const v
   if (split.segs > 1)
     if (int rc = la_starts(w, a->dtype, split, ds_end, e_starts, st)) return rc;
   w.s_in = split.segs > 1 ? e_starts : ds_end;
-  w.s_out = ds0;
-  if (int rc = run(dv, a->v_heads)) return rc;
+  LaWalk w_v = w, w_k = w, w_q = w;
+  w_v.s_out = ds0;
   // dk, likewise with the state transposed
-  w.q = v, w.k = d, w.v = q;
-  w.DK = a->Dv, w.DV = a->Dk, w.sk = 1, w.sv = a->Dv, w.s_out = nullptr;
-  return run(dk, a->k_heads);
+  w_k.q = v, w_k.k = d, w_k.v = q;
+  w_k.DK = a->Dv, w_k.DV = a->Dk, w_k.sk = 1, w_k.sv = a->Dv;
+  // dq: the forward walk with the state transposed
+  w_q.q = d, w_q.k = v, w_q.v = k;
+  w_q.DK = a->Dv, w_q.DV = a->Dk, w_q.sk = 1, w_q.sv = a->Dv;
+  w_q.rev = w_q.late = 0, w_q.so = a->scale, w_q.su = 1.0f;
+  w_q.s_in = split.segs > 1 ? (const float*)starts : a->s0;
+  const Out outs[3] = {out(w_q, dq, a->q_heads), out(w_k, dk, a->k_heads), out(w_v, dv, a->v_heads)};
+  LaWalks all = {};
+  all.w[0] = w_q, all.w[1] = w_k, all.w[2] = w_v;
+  const bool alike = la_rows(w_v.DK) == la_rows(w_q.DK) && la_block(a->dtype, w_v.DK, w_v.DV) == la_block(a->dtype, w_q.DK, w_q.DV);
+  all.n = alike ? 3 : 2;
+  if (int rc = la_go(all, a->dtype, false, st)) return rc;
+  if (!alike)
+    if (int rc = la_go(w_v, a->dtype, false, st)) return rc;
+  for (const Out& o : outs) {
+    if (!o.f32 || a->T == 0) continue;
+    const int64_t n = a->T * a->B * o.heads * o.D;
+    with_dtype(a->dtype, [&](auto t) {
+      using T = decltype(t);
+      k_la_share<T><<<dim3((unsigned)((n + 255) / 256)), 256, 0, st>>>(o.f32, (T*)o.to, n, o.D,
+                                                                      (int)(a->H / o.heads));
+    });
+    LSH_CHECK_LAUNCH();
+  }
+  return LSH_OK;
 }
 
 extern "C" int lsh_linattn_step(const lsh_linattn* a, float* state, void* stream) {

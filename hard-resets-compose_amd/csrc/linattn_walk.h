@@ -39,6 +39,12 @@ struct LaWalk {
   float so, su;         // out's scale, and the sum's
 };
 
+// Walks of one size class that do not wait for each other: workgroups (., i) take walk i.
+struct LaWalks {
+  LaWalk w[3];
+  int n;
+};
+
 using f32x4 = float __attribute__((ext_vector_type(4)));
 using bf16x4 = __bf16 __attribute__((ext_vector_type(4)));
 using bf16x8 = __bf16 __attribute__((ext_vector_type(8)));
@@ -239,6 +245,11 @@ __device__ __forceinline__ bool la_odd(f32x4 x) {
   return any;
 }
 
+// Waves a SIMD that LDS has room for.
+constexpr int la_waves(int size, int DKP, int W) {
+  return DKP > 128 ? W / 4 : size == 4 ? DKP > 64 ? W / 4 : 2 : W == 8 ? 4 : 2;
+}
+
 // The walk.  SUMS: only the segments' sums (the state after each segment from a zero state before
 // it), written to s_out [segments, B*H] one place further on (segment s to s + 1), for every segment
 // but the last.  WIDE: every row is read and written in whole pieces (la_wide).
@@ -251,7 +262,8 @@ __device__ __forceinline__ bool la_odd(f32x4 x) {
 // LDS rows are padded: by 4 dwords modulo 64 where rows are read (16 rows of 16 bytes meet different
 // banks), by 8 where the transposing read takes 8 rows of 32 bytes at once.
 template <class T, class L, int DKP, int W, bool SUMS, bool WIDE>
-__global__ __launch_bounds__(W * 64, DKP > 128 ? W / 4 : W == 8 && sizeof(L) == 2 ? 4 : 2) void k_la_walk(LaWalk a) {
+__global__ __launch_bounds__(W * 64, la_waves(sizeof(L), DKP, W)) void k_la_walk(LaWalks all) {
+  const LaWalk& a = all.w[blockIdx.y];
   using X = La<L>;
   using Frag = typename X::Frag;
   constexpr int C = X::C, KB = X::KB, DVB = W * 16, KT = DKP / 16, CT = C / 16, KS = DKP / KB, CS = C / KB;
@@ -267,6 +279,7 @@ __global__ __launch_bounds__(W * 64, DKP > 128 ? W / 4 : W == 8 && sizeof(L) == 
   const int blocks = (a.DV + DVB - 1) / DVB;
   const int64_t job = xcd_neuron(blockIdx.x, gridDim.x), pair = job / blocks;
   const int64_t seg = pair / BH, bh = pair % BH, b = bh / a.H, h = bh % a.H;
+  if (seg >= a.segs - SUMS) return;  // another walk of the launch has more blocks
   const int dv0 = (int)(job % blocks) * DVB, wc = w * 16;  // the block's first column, the wave's within it
   const int64_t r0 = seg * a.L, r1 = min(a.T, r0 + a.L);
   const T* q = la_row<T>(a.q, b, h);
@@ -467,9 +480,12 @@ __global__ __launch_bounds__(W * 64, DKP > 128 ? W / 4 : W == 8 && sizeof(L) == 
 
 // Rows of a chunk for a dtype code, and columns of a workgroup's block for widths DK, DV.
 inline int la_chunk(int dtype) { return dtype == LSH_BF16 ? La<bf16_t>::C : La<float>::C; }
-// 128 columns read Q and K and form the scores once where two blocks of 64 do it twice (4096 x 4 x 16 x
-// 128, forward and backward: 425 us, with blocks of 64 461); 256 rows of a state leave LDS for 64 only.
-inline int la_block(int DK, int DV) { return DK <= 128 && DV > 64 ? 128 : 64; }
+// 128 columns read Q and K and form the scores once where two blocks of 64 do it twice (bf16 4096 x 4 x 16
+// x 128, forward and backward: 425 us, with blocks of 64 461; 4096 x 16 x 256 x 256: 282 us backward, with
+// blocks of 64 383); 256 rows of a state in fp32 leave LDS for 64 only.
+inline int la_block(int dtype, int DK, int DV) {
+  return DV > 64 && (dtype == LSH_BF16 || DK <= 128) ? 128 : 64;
+}
 
 // Whether the walk's rows can be read and written in whole pieces: a chunk's byte offsets stay below
 // 2^30 and the output's columns come in fours.
@@ -479,24 +495,34 @@ inline bool la_wide(const LaWalk& a, int chunk) {
   return near(a.q) && near(a.k) && near(a.v) && a.DV % 4 == 0 && a.B * a.H * a.DV < most;
 }
 
-// Launches the walk (its sums: SUMS) for operands of T computed in L.
+// State rows that a kernel is built for, by the walk's DK.
+inline int la_rows(int DK) { return DK <= 64 ? 64 : DK <= 128 ? 128 : 256; }
+
+// Launches walks of one la_rows and la_block (their sums: SUMS) for operands of T computed in L.
 template <class T, class L>
-inline int la_launch(const LaWalk& a, bool sums, hipStream_t st) {
+inline int la_launch(const LaWalks& all, bool sums, hipStream_t st) {
+  const LaWalk& a = all.w[0];
   const int64_t n = a.B * a.H * (sums ? a.segs - 1 : a.segs);
-  if (n == 0) return LSH_OK;
-  const int block = la_block(a.DK, a.DV);
-  const dim3 grid((unsigned)(n * ((a.DV + block - 1) / block)));
-  const bool wide = la_wide(a, La<L>::C);
+  if (n == 0 || all.n == 0) return LSH_OK;
+  constexpr int dtype = sizeof(L) == 2 ? LSH_BF16 : LSH_F32;
+  const int block = la_block(dtype, a.DK, a.DV);
+  bool wide = true;
+  int blocks = 0;
+  for (int i = 0; i < all.n; ++i) {
+    wide = wide && la_wide(all.w[i], La<L>::C);
+    blocks = blocks > (all.w[i].DV + block - 1) / block ? blocks : (all.w[i].DV + block - 1) / block;
+  }
+  const dim3 grid((unsigned)(n * blocks), (unsigned)all.n);
   auto go = [&](auto dkp, auto waves) {
     constexpr int DKP = decltype(dkp)::value, W = decltype(waves)::value;
     if (sums && wide)
-      k_la_walk<T, L, DKP, W, true, true><<<grid, W * 64, 0, st>>>(a);
+      k_la_walk<T, L, DKP, W, true, true><<<grid, W * 64, 0, st>>>(all);
     else if (sums)
-      k_la_walk<T, L, DKP, W, true, false><<<grid, W * 64, 0, st>>>(a);
+      k_la_walk<T, L, DKP, W, true, false><<<grid, W * 64, 0, st>>>(all);
     else if (wide)
-      k_la_walk<T, L, DKP, W, false, true><<<grid, W * 64, 0, st>>>(a);
+      k_la_walk<T, L, DKP, W, false, true><<<grid, W * 64, 0, st>>>(all);
     else
-      k_la_walk<T, L, DKP, W, false, false><<<grid, W * 64, 0, st>>>(a);
+      k_la_walk<T, L, DKP, W, false, false><<<grid, W * 64, 0, st>>>(all);
   };
   auto with = [&](auto dkp) {
     if (block == 128)
@@ -504,18 +530,21 @@ inline int la_launch(const LaWalk& a, bool sums, hipStream_t st) {
     else
       go(dkp, std::integral_constant<int, 4>{});
   };
-  if (a.DK <= 64)
-    with(std::integral_constant<int, 64>{});
-  else if (a.DK <= 128)
-    with(std::integral_constant<int, 128>{});
-  else
-    go(std::integral_constant<int, 256>{}, std::integral_constant<int, 4>{});
+  switch (la_rows(a.DK)) {
+    case 64: with(std::integral_constant<int, 64>{}); break;
+    case 128: with(std::integral_constant<int, 128>{}); break;
+    default:
+      if constexpr (sizeof(L) == 2)
+        with(std::integral_constant<int, 256>{});
+      else
+        go(std::integral_constant<int, 256>{}, std::integral_constant<int, 4>{});
+  }
   LSH_CHECK_LAUNCH();
   return LSH_OK;
 }
 
-int la_launch_f32(const LaWalk& a, bool sums, hipStream_t st);
-int la_launch_bf16(const LaWalk& a, bool sums, hipStream_t st);
-int la_launch_f16(const LaWalk& a, bool sums, hipStream_t st);
+int la_launch_f32(const LaWalks& all, bool sums, hipStream_t st);
+int la_launch_bf16(const LaWalks& all, bool sums, hipStream_t st);
+int la_launch_f16(const LaWalks& all, bool sums, hipStream_t st);
 
 }  // namespace lsh
