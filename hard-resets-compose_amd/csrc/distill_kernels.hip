@@ -6,9 +6,10 @@
 //   dz_v = g * tau * (q_v - sum_{k: i_k = v} p_k)
 //
 // A row without entries has loss 0 and gradient 0.  All exponents are in base 2: with c = log2(e)/tau,
-// q_v = 2^(c*z_v - l) where l = log2(sum 2^(c*z)), and c*z_v - l is one fused operation.  The forward
-// reads the logits once, with the running maximum and sum of the softmax, and keeps l and the teacher's
-// log2-sum; the backward reads them once more and writes dz.  Both are bound by the logits' bytes
+// m the largest logit and l = log2(sum 2^(c*(z - m))), q_v = 2^(c*(z_v - m) - l).  (m stays apart from l:
+// their sum would round by a share of the logits' size where only their differences matter.)  The
+// forward reads the logits once, with the running maximum and sum of the softmax, and keeps m, l and the
+// teacher's two; the backward reads them once more and writes dz.  Both are bound by the logits' bytes
 // (4096 x 32000 bf16: 262 MB forward, 524 MB backward).  A row is split over several workgroups where there
 // are too few rows for the chip, and the parts' maxima and sums are joined in order.
 #include <algorithm>
@@ -27,7 +28,7 @@ struct DsArgs {
   bool t_f32;
   const int64_t* id;
   float* loss;
-  float* stats;  // [2, rows]: l, and the teacher's log2-sum (-inf: no entry)
+  float* stats;  // [4, rows]: m and l, and the teacher's (-inf: no entry)
   float* part;   // [rows, splits, 2]: maximum and sum of each part
   const float* g;
   int64_t g_stride;
@@ -51,27 +52,24 @@ __device__ __forceinline__ float ds_value(const DsArgs& a, int64_t i) {
   return a.t_f32 ? ((const float*)a.t)[i] : to_f(((const T*)a.t)[i]);
 }
 
-// The part of a row from element v0 on, as pieces of 16 bytes at aligned addresses with single elements
-// before and behind them.
+// 16 bytes at the address of any element: pieces lie at fixed places of a row, so that its sums do not
+// depend on where it begins.
 template <class T>
-struct DsPart {
-  static constexpr int P = kWide<T>;
-  int lead, pieces, n;  // elements before the first piece, pieces, elements in all
-  __device__ __forceinline__ DsPart(const T* p, int64_t count) {
-    n = (int)count;
-    lead = min((int)((16 - ((uintptr_t)p & 15)) & 15) / (int)sizeof(T), n);
-    pieces = (n - lead) / P;
-  }
-  // this thread's single element, or -1
-  __device__ __forceinline__ int single() const {
-    const int i = threadIdx.x, tail = lead + pieces * P;
-    return i < lead ? i : i - lead < n - tail ? tail + i - lead : -1;
-  }
-};
+using Piece = Vec<T, kWide<T>>;
+template <class T>
+__device__ __forceinline__ Piece<T> ld_piece(const T* p) {
+  Piece<T> x;
+  __builtin_memcpy(&x, p, 16);
+  return x;
+}
+template <class T>
+__device__ __forceinline__ void st_piece(T* p, const Piece<T>& x) {
+  __builtin_memcpy(p, &x, 16);
+}
 
-// The teacher's side of a row by one wave: log2-sum of its entries, and the loss given l.
+// The teacher's side of a row by one wave: its maximum and log2-sum, and the loss given the logits'.
 template <class T>
-__device__ __forceinline__ void ds_loss(const DsArgs& a, int64_t row, float l) {
+__device__ __forceinline__ void ds_loss(const DsArgs& a, int64_t row, float zm, float l) {
   const int lane = threadIdx.x & 63;
   const T* z = (const T*)a.z + row * a.stride;
   float m = -INFINITY, s = 0.0f;
@@ -82,20 +80,22 @@ __device__ __forceinline__ void ds_loss(const DsArgs& a, int64_t row, float l) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) ds_join(m, s, __shfl_xor(m, o, 64), __shfl_xor(s, o, 64), a.c);
   const bool some = s != 0.0f && m != -INFINITY;  // a NaN counts
-  const float tl = some ? __builtin_fmaf(m, a.c, __builtin_amdgcn_logf(s)) : -INFINITY;
+  const float tl = __builtin_amdgcn_logf(s);
   float sum = 0.0f;
   for (int k = lane; k < a.K && some; k += 64) {
     const int64_t i = a.id[row * a.K + k];
     if (i < 0 || i >= a.V) continue;
-    const float lp = __builtin_fmaf(ds_value<T>(a, row * a.K + k), a.c, -tl);
+    const float lp = __builtin_fmaf(ds_value<T>(a, row * a.K + k) - m, a.c, -tl);
     const float p = __builtin_amdgcn_exp2f(lp);
-    if (p != 0.0f) sum += p * (lp - __builtin_fmaf(to_f(z[i]), a.c, -l));
+    if (p != 0.0f) sum += p * (lp - __builtin_fmaf(to_f(z[i]) - zm, a.c, -l));
   }
   sum = wave_sum_f(sum);
   if (lane == 0) {
     a.loss[row] = some ? a.tau * a.tau * kLn2 * sum : 0.0f;
-    a.stats[row] = l;
-    a.stats[a.rows + row] = tl;
+    a.stats[row] = zm;
+    a.stats[a.rows + row] = l;
+    a.stats[2 * a.rows + row] = some ? m : -INFINITY;
+    a.stats[3 * a.rows + row] = tl;
   }
 }
 
@@ -106,25 +106,24 @@ __global__ __launch_bounds__(kDsThreads) void k_distill(DsArgs a) {
   const int64_t row = SPLIT ? blockIdx.x / a.splits : blockIdx.x, part = SPLIT ? blockIdx.x % a.splits : 0;
   const int64_t v0 = part * a.len;
   const T* z = (const T*)a.z + row * a.stride + v0;
-  const DsPart<T> x(z, min(a.len, a.V - v0));
+  const int n = (int)min(a.len, a.V - v0), pieces = n / P;
   float m = -INFINITY, s = 0.0f;
   auto take = [&](const float (&f)[P], int n) {
     float top = m;
 #pragma unroll
     for (int j = 0; j < P; ++j) top = fmaxf(top, j < n ? f[j] : -INFINITY);
-    const float at = top > -INFINITY ? top : 0.0f, off = -at * a.c;
+    const float at = top > -INFINITY ? top : 0.0f;
     s *= __builtin_amdgcn_exp2f((m - at) * a.c);
 #pragma unroll
     for (int j = 0; j < P; ++j)
-      if (j < n) s += __builtin_amdgcn_exp2f(__builtin_fmaf(f[j], a.c, off));
+      if (j < n) s += __builtin_amdgcn_exp2f((f[j] - at) * a.c);
     m = top;
   };
-  const Vec<T, P>* v = (const Vec<T, P>*)(z + x.lead);
   int i = threadIdx.x;
-  for (; i + (U - 1) * kDsThreads < x.pieces; i += U * kDsThreads) {
-    Vec<T, P> y[U];
+  for (; i + (U - 1) * kDsThreads < pieces; i += U * kDsThreads) {
+    Piece<T> y[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) y[u] = v[i + u * kDsThreads];
+    for (int u = 0; u < U; ++u) y[u] = ld_piece(z + (int64_t)(i + u * kDsThreads) * P);
     float f[U][P], top = m;
 #pragma unroll
     for (int u = 0; u < U; ++u)
@@ -133,22 +132,22 @@ __global__ __launch_bounds__(kDsThreads) void k_distill(DsArgs a) {
         f[u][j] = to_f(y[u].v[j]);
         top = fmaxf(top, f[u][j]);
       }
-    const float at = top > -INFINITY ? top : 0.0f, off = -at * a.c;
+    const float at = top > -INFINITY ? top : 0.0f;
     s *= __builtin_amdgcn_exp2f((m - at) * a.c);
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int j = 0; j < P; ++j) s += __builtin_amdgcn_exp2f(__builtin_fmaf(f[u][j], a.c, off));
+      for (int j = 0; j < P; ++j) s += __builtin_amdgcn_exp2f((f[u][j] - at) * a.c);
     m = top;
   }
-  for (; i < x.pieces; i += kDsThreads) {
-    const Vec<T, P> y = v[i];
+  for (; i < pieces; i += kDsThreads) {
+    const Piece<T> y = ld_piece(z + (int64_t)i * P);
     float f[P];
 #pragma unroll
     for (int j = 0; j < P; ++j) f[j] = to_f(y.v[j]);
     take(f, P);
   }
-  if (const int e = x.single(); e >= 0) {
+  if (const int e = pieces * P + threadIdx.x; e < n) {
     const float f[P] = {to_f(z[e])};
     take(f, 1);
   }
@@ -166,7 +165,7 @@ __global__ __launch_bounds__(kDsThreads) void k_distill(DsArgs a) {
       to[0] = m, to[1] = s;
     }
   } else {
-    ds_loss<T>(a, row, (m > -INFINITY ? m * a.c : 0.0f) + __builtin_amdgcn_logf(s));
+    ds_loss<T>(a, row, m, __builtin_amdgcn_logf(s));
   }
 }
 
@@ -179,7 +178,7 @@ __global__ __launch_bounds__(64) void k_distill_join(DsArgs a) {
     const float* p = a.part + (row * a.splits + i) * 2;
     ds_join(m, s, p[0], p[1], a.c);
   }
-  ds_loss<T>(a, row, (m > -INFINITY ? m * a.c : 0.0f) + __builtin_amdgcn_logf(s));
+  ds_loss<T>(a, row, m, __builtin_amdgcn_logf(s));
 }
 
 template <class T>
@@ -190,40 +189,34 @@ __global__ __launch_bounds__(kDsThreads) void k_distill_bwd(DsArgs a) {
   const int64_t row = blockIdx.x / a.splits, v0 = blockIdx.x % a.splits * a.len;
   const T* z = (const T*)a.z + row * a.stride + v0;
   T* dz = (T*)a.dz + row * a.V + v0;
-  const DsPart<T> x(z, min(a.len, a.V - v0));
-  const float l = a.stats[row], tl = a.stats[a.rows + row];
-  const bool some = tl != -INFINITY;
+  const int n = (int)min(a.len, a.V - v0), pieces = n / P;
+  const float zm = a.stats[row], l = a.stats[a.rows + row], tm = a.stats[2 * a.rows + row],
+              tl = a.stats[3 * a.rows + row];
+  const bool some = tm != -INFINITY;
   const float f = some ? a.g[row * a.g_stride] * a.tau : 0.0f;
-  auto grad = [&](float y) { return some ? f * __builtin_amdgcn_exp2f(__builtin_fmaf(y, a.c, -l)) : 0.0f; };
-  const Vec<T, P>* v = (const Vec<T, P>*)(z + x.lead);
-  const bool wide = ((uintptr_t)(dz + x.lead) & 15) == 0;
-  auto put = [&](const Vec<T, P>& y, int i) {
-    Vec<T, P> d;
+  auto grad = [&](float y) { return some ? f * __builtin_amdgcn_exp2f(__builtin_fmaf(y - zm, a.c, -l)) : 0.0f; };
+  auto put = [&](const Piece<T>& y, int i) {
+    Piece<T> d;
 #pragma unroll
     for (int j = 0; j < P; ++j) d.v[j] = from_f<T>(grad(to_f(y.v[j])));
-    if (wide) {
-      *(Vec<T, P>*)(dz + x.lead + (int64_t)i * P) = d;
-    } else {
-#pragma unroll
-      for (int j = 0; j < P; ++j) dz[x.lead + (int64_t)i * P + j] = d.v[j];
-    }
+    st_piece(dz + (int64_t)i * P, d);
   };
   int i = threadIdx.x;
-  for (; i + (U - 1) * kDsThreads < x.pieces; i += U * kDsThreads) {
-    Vec<T, P> y[U];
+  for (; i + (U - 1) * kDsThreads < pieces; i += U * kDsThreads) {
+    Piece<T> y[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) y[u] = v[i + u * kDsThreads];
+    for (int u = 0; u < U; ++u) y[u] = ld_piece(z + (int64_t)(i + u * kDsThreads) * P);
 #pragma unroll
     for (int u = 0; u < U; ++u) put(y[u], i + u * kDsThreads);
   }
-  for (; i < x.pieces; i += kDsThreads) put(v[i], i);
-  if (const int e = x.single(); e >= 0) dz[e] = from_f<T>(grad(to_f(z[e])));
+  for (; i < pieces; i += kDsThreads) put(ld_piece(z + (int64_t)i * P), i);
+  if (const int e = pieces * P + threadIdx.x; e < n) dz[e] = from_f<T>(grad(to_f(z[e])));
   if (!some) return;
   for (int k = threadIdx.x; k < a.K; k += kDsThreads) {
     const int64_t id = a.id[row * a.K + k];
-    const bool here = id >= v0 && id < v0 + x.n;
+    const bool here = id >= v0 && id < v0 + n;
     s_id[k] = here ? (int)(id - v0) : -1;
-    s_p[k] = here ? __builtin_amdgcn_exp2f(__builtin_fmaf(ds_value<T>(a, row * a.K + k), a.c, -tl)) : 0.0f;
+    s_p[k] = here ? __builtin_amdgcn_exp2f(__builtin_fmaf(ds_value<T>(a, row * a.K + k) - tm, a.c, -tl)) : 0.0f;
   }
   __syncthreads();  // also the part's stores: its entries are written again with the teacher's part
   for (int k = threadIdx.x; k < a.K; k += kDsThreads) {
@@ -236,7 +229,7 @@ __global__ __launch_bounds__(kDsThreads) void k_distill_bwd(DsArgs a) {
         first = first && j >= k;
         p += s_p[j];
       }
-    if (first) dz[e] = from_f<T>(f * (__builtin_amdgcn_exp2f(__builtin_fmaf(to_f(z[e]), a.c, -l)) - p));
+    if (first) dz[e] = from_f<T>(f * (__builtin_amdgcn_exp2f(__builtin_fmaf(to_f(z[e]) - zm, a.c, -l)) - p));
   }
 }
 
@@ -260,7 +253,7 @@ static DsArgs ds_args(const void* logits, int64_t stride, int v_dtype, const voi
   a.z = logits, a.stride = stride, a.t = values, a.t_f32 = v_dtype == LSH_F32, a.id = index;
   a.rows = rows, a.V = V, a.K = K;
   a.splits = ds_splits(rows, V);
-  a.len = (V + a.splits - 1) / a.splits;
+  a.len = align_up((size_t)((V + a.splits - 1) / a.splits), 8);
   a.c = kLog2e / tau, a.tau = tau;
   return a;
 }

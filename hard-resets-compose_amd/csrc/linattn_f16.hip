@@ -2,5 +2,5 @@
 #include "linattn_walk.h"
 
 namespace lsh {
-int la_launch_f16(const LaWalks& all, bool sums, hipStream_t st) { return la_launch<f16_t, float>(all, sums, st); }
+int la_launch_f16(const LaWalks& all, bool sums, hipStream_t st) { return la_launch<f16_t, f16_t>(all, sums, st); }
 }  // namespace lsh

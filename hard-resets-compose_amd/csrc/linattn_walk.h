@@ -48,57 +48,109 @@ struct LaWalks {
 using f32x4 = float __attribute__((ext_vector_type(4)));
 using bf16x4 = __bf16 __attribute__((ext_vector_type(4)));
 using bf16x8 = __bf16 __attribute__((ext_vector_type(8)));
+using f16x4 = _Float16 __attribute__((ext_vector_type(4)));
+using f16x8 = _Float16 __attribute__((ext_vector_type(8)));
 using s16x4 = short __attribute__((ext_vector_type(4)));
 
 // What the matrix instructions take.  A fragment holds KB values of the summed axis for one of 16
 // rows: lane l has row l%16 and, with g = l/16, the values 4g..4g+3 of each 16 (the order in which an
 // accumulator holds its rows, so that an accumulator turns into a fragment in registers).
 //
-// bf16: products of bf16, fp32 sums.  fp32: the fp32 matrix instruction, exact products.  fp16 operands
-// are computed in fp32: a state or a score can pass fp16's range where its result does not.
+// 16 bits: products of the type, fp32 sums.  A decayed value is taken in as many parts as hold the 24
+// bits of fp32 (bf16 three, fp16 two), so the state is kept to fp32; a score and the state that meets q
+// are rounded to the type once.  SCALED (fp16): what is rounded is first scaled by a power of two that
+// brings its largest value below 2^15, since scores, states and decayed values can leave fp16's range,
+// or sink below its normal numbers, where the results do not.
+// fp32: the fp32 matrix instruction, exact products.
 template <class L>
 struct La;
 
-template <>
-struct La<bf16_t> {
-    static constexpr int KB = 32, C = 32, TILES = 2;
-  // a decayed value is taken in three bf16 parts, which hold its 24 bits: the state is kept to fp32
-  static constexpr int PARTS = 3;
-  using Frag = bf16x8;
-  using Quad = bf16x4;
+template <class L, class F4, class F8>
+struct La16 {
+  static constexpr int KB = 32, C = 32, TILES = 2;
+  using Frag = F8;
+  using Quad = F4;
   static constexpr int kPadRow = 8, kPadCol = 16;  // elements; see the LDS layout at k_la_walk
-  static __device__ __forceinline__ f32x4 mma(Frag a, Frag b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
-  }
   // a row's 32 values from their natural order, and from the order of packed()
-  static __device__ __forceinline__ Frag row(const bf16_t* p, int g) {
-    const bf16x4 a = *(const bf16x4*)(p + 4 * g), b = *(const bf16x4*)(p + 16 + 4 * g);
+  static __device__ __forceinline__ Frag row(const L* p, int g) {
+    const F4 a = *(const F4*)(p + 4 * g), b = *(const F4*)(p + 16 + 4 * g);
     return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
   }
-  static __device__ __forceinline__ Frag packed_row(const bf16_t* p, int g) { return *(const Frag*)(p + 8 * g); }
+  static __device__ __forceinline__ Frag packed_row(const L* p, int g) { return *(const Frag*)(p + 8 * g); }
   // where four values from c on lie when a fragment's eight are to be neighbours
   static __device__ __forceinline__ int packed(int c) { return (c & ~31) + (c & 12) * 2 + (c & 16) / 4; }
   // column l%16 of 32 rows: the LDS read that transposes blocks of 4 rows by 16 lanes
-  static __device__ __forceinline__ Frag col(const bf16_t* p, int pitch, int g, int m) {
+  static __device__ __forceinline__ Frag col(const L* p, int pitch, int g, int m) {
     using Lds = __attribute__((address_space(3))) s16x4*;
-    const bf16_t* at = p + (4 * g + (m >> 2)) * pitch + (m & 3) * 4;
-    const bf16x4 a = __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)at));
-    const bf16x4 b =
-        __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(at + 16 * pitch)));
+    const L* at = p + (4 * g + (m >> 2)) * pitch + (m & 3) * 4;
+    const F4 a = __builtin_bit_cast(F4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)at));
+    const F4 b = __builtin_bit_cast(F4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(at + 16 * pitch)));
     return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
   }
-  static __device__ __forceinline__ Frag of(const f32x4* acc) {
+  static __device__ __forceinline__ Frag of(const f32x4* acc, float scale) {
     Frag f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = (bf16_t)acc[e >> 2][e & 3];
+    for (int e = 0; e < 8; ++e) f[e] = (L)(acc[e >> 2][e & 3] * scale);
     return f;
   }
   static __device__ __forceinline__ int at(int e) { return (e >> 2) * 16 + (e & 3); }  // + 4g
 };
 
 template <>
+struct La<bf16_t> : La16<bf16_t, bf16x4, bf16x8> {
+  static constexpr int PARTS = 3;
+  static constexpr bool SCALED = false;
+  static __device__ __forceinline__ f32x4 mma(Frag a, Frag b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+};
+
+template <>
+struct La<f16_t> : La16<f16_t, f16x4, f16x8> {
+  static constexpr int PARTS = 2;
+  static constexpr bool SCALED = true;
+  static __device__ __forceinline__ f32x4 mma(Frag a, Frag b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
+  // the same over half a fragment: rows 16*half.. of the 32
+  static __device__ __forceinline__ f32x4 mma_half(Frag a, Frag b, int half, f32x4 c) {
+    const f16x4 x = half ? __builtin_shufflevector(a, a, 4, 5, 6, 7) : __builtin_shufflevector(a, a, 0, 1, 2, 3);
+    const f16x4 y = half ? __builtin_shufflevector(b, b, 4, 5, 6, 7) : __builtin_shufflevector(b, b, 0, 1, 2, 3);
+    return __builtin_amdgcn_mfma_f32_16x16x16f16(x, y, c, 0, 0, 0);
+  }
+};
+
+// A power of two that scales a wave's values below 2^15, and its reciprocal.  Values that are not finite
+// are left out: t holds a lane's largest of la_bits.
+struct LaScale {
+  float to, from;
+};
+__device__ __forceinline__ unsigned la_bits(float x) {  // grows with a finite |x|; 2^24 above its exponent
+  return (__builtin_bit_cast(unsigned, x) << 1) + 0x01000000u;
+}
+__device__ __forceinline__ LaScale la_scale(unsigned t) {
+  auto ror = [&](auto n) {
+    const unsigned o = __builtin_amdgcn_update_dpp(t, t, 0x120 + decltype(n)::value, 0xf, 0xf, false);
+    t = t > o ? t : o;
+  };
+  ror(std::integral_constant<int, 8>{});
+  ror(std::integral_constant<int, 4>{});
+  ror(std::integral_constant<int, 2>{});
+  ror(std::integral_constant<int, 1>{});
+  unsigned top = 0;
+#pragma unroll
+  for (int i = 0; i < 64; i += 16) {
+    const unsigned o = __builtin_amdgcn_readlane(t, i);
+    top = top > o ? top : o;
+  }
+  const int e = min(max((int)(top >> 24) - 1, 15), 253);  // the exponent's bits
+  return {__builtin_bit_cast(float, (unsigned)(268 - e) << 23), __builtin_bit_cast(float, (unsigned)(e - 14) << 23)};
+}
+
+template <>
 struct La<float> {
   static constexpr int KB = 16, C = 32, TILES = 1, PARTS = 1;
+  static constexpr bool SCALED = false;
   using Frag = f32x4;
   using Quad = f32x4;
   static constexpr int kPadRow = 4, kPadCol = 4;
@@ -116,7 +168,7 @@ struct La<float> {
     for (int e = 0; e < 4; ++e) f[e] = p[(4 * g + e) * pitch + m];
     return f;
   }
-  static __device__ __forceinline__ Frag of(const f32x4* acc) { return acc[0]; }
+  static __device__ __forceinline__ Frag of(const f32x4* acc, float) { return acc[0]; }
   static __device__ __forceinline__ int at(int e) { return e; }
 };
 
@@ -229,14 +281,19 @@ __device__ __forceinline__ void la_store_some(TO* p, int64_t step, const f32x4 (
       if (i * 16 >= first && e < left) p[i * 16 * step + e] = from_f<TO>(o[i][e]);
 }
 
-// Whether any of a fragment's values is not finite.
-__device__ __forceinline__ bool la_odd(bf16x8 x) {
-  // the exponent's bits, plus one in its last place: all ones carry into the bit above
-  const u32x4 b = __builtin_bit_cast(u32x4, x);
+// Whether any of a fragment's values is not finite: the exponent's bits, plus one in their last place; all
+// ones carry into the bit above.
+__device__ __forceinline__ bool la_odd(u32x4 b, unsigned exponents, unsigned one) {
   unsigned any = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) any |= (b[i] & 0x7f807f80u) + 0x00800080u;
+  for (int i = 0; i < 4; ++i) any |= (b[i] & exponents) + one;
   return (any & 0x80008000u) != 0;
+}
+__device__ __forceinline__ bool la_odd(bf16x8 x) {
+  return la_odd(__builtin_bit_cast(u32x4, x), 0x7f807f80u, 0x00800080u);
+}
+__device__ __forceinline__ bool la_odd(f16x8 x) {
+  return la_odd(__builtin_bit_cast(u32x4, x), 0x7c007c00u, 0x04000400u);
 }
 __device__ __forceinline__ bool la_odd(f32x4 x) {
   bool any = false;
@@ -272,6 +329,7 @@ __global__ __launch_bounds__(W * 64, la_waves(sizeof(L), DKP, W)) void k_la_walk
   constexpr int HALVES = WIDE ? 2 : 1;  // of LDS: one is filled while the other is read
   __shared__ alignas(16) L s_q[SUMS ? 8 : HALVES * C * PQ], s_k[HALVES * C * PK], s_v[HALVES * C * PV];
   __shared__ alignas(16) L s_p[SUMS ? 8 : C * PP];
+  __shared__ float s_from[W];  // SCALED: what takes each tile of the scores back
 
   const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -373,24 +431,43 @@ __global__ __launch_bounds__(W * 64, la_waves(sizeof(L), DKP, W)) void k_la_walk
         for (int s = 0; s < KS; ++s)
           p = X::mma(X::row(&ck[(tj * 16 + m) * PK + s * KB], g), X::packed_row(&cq[(ti * 16 + m) * PQ + s * KB], g), p);
         typename X::Quad y;
+        unsigned big = 0;
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          y[e] = (L)((ti - tj) * 16 + m - 4 * g - e >= 0 ? p[e] * fall[e] : 0.0f);
+        for (int e = 0; e < 4; ++e) {
+          p[e] = (ti - tj) * 16 + m - 4 * g - e >= 0 ? p[e] * fall[e] : 0.0f;
+          big = max(big, la_bits(p[e]));
+        }
+        if constexpr (X::SCALED) {
+          const LaScale c = la_scale(big);
+          p *= c.to;
+          if (lane == 0) s_from[w] = c.from;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = (L)p[e];
         *(typename X::Quad*)&s_p[(ti * 16 + m) * PP + X::packed(tj * 16 + 4 * g)] = y;
       }
       // what the state before the chunk gives
       f32x4 o[CT];
 #pragma unroll
       for (int i = 0; i < CT; ++i) o[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      LaScale in = {1.0f, 1.0f};
+      if constexpr (X::SCALED) {
+        unsigned big = 0;
+#pragma unroll
+        for (int i = 0; i < KT; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) big = max(big, la_bits(S[i][e]));
+        in = la_scale(big);
+      }
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
-        const Frag st = X::of(&S[s * X::TILES]);
+        const Frag st = X::of(&S[s * X::TILES], in.to);
 #pragma unroll
         for (int i = 0; i < CT; ++i) o[i] = X::mma(st, X::packed_row(&cq[(i * 16 + m) * PQ + s * KB], g), o[i]);
       }
       const int first = C - n - m;  // a lane's rows of the chunk are those with 16i >= first
 #pragma unroll
-      for (int i = 0; i < CT; ++i) o[i] *= a.so * la_pow(l2, max(i * 16 - first, 0) + 1 - a.late);
+      for (int i = 0; i < CT; ++i) o[i] *= a.so * in.from * la_pow(l2, max(i * 16 - first, 0) + 1 - a.late);
       __syncthreads();  // the scores are there
 
       // what the chunk's own rows give
@@ -408,7 +485,8 @@ __global__ __launch_bounds__(W * 64, la_waves(sizeof(L), DKP, W)) void k_la_walk
           const typename X::Quad y = *(const typename X::Quad*)&cv[j * PV + wc + 4 * g];
 #pragma unroll
           for (int i = 0; i < CT; ++i) {
-            const float p = (float)s_p[(i * 16 + m) * PP + X::packed(j & ~3) + (j & 3)];
+            float p = (float)s_p[(i * 16 + m) * PP + X::packed(j & ~3) + (j & 3)];
+            if constexpr (X::SCALED) p *= s_from[i * (i + 1) / 2 + min(j / 16, i)];
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[i][e] += i * 16 + m >= j ? p * (float)y[e] : 0.0f;
           }
@@ -417,8 +495,18 @@ __global__ __launch_bounds__(W * 64, la_waves(sizeof(L), DKP, W)) void k_la_walk
 #pragma unroll
         for (int s = 0; s < CS; ++s)
 #pragma unroll
-          for (int i = 0; i < CT; ++i)
-            if (s * X::TILES <= i) o[i] = X::mma(x[s], X::packed_row(&s_p[(i * 16 + m) * PP + s * KB], g), o[i]);
+          for (int i = 0; i < CT; ++i) {
+            if (s * X::TILES > i) continue;
+            const Frag p = X::packed_row(&s_p[(i * 16 + m) * PP + s * KB], g);
+            if constexpr (X::SCALED) {  // each 16 rows' scores have a scale of their own
+#pragma unroll
+              for (int j = 0; j < 2; ++j)
+                if (s * 2 + j <= i)
+                  o[i] += X::mma_half(x[s], p, j, f32x4{0.0f, 0.0f, 0.0f, 0.0f}) * s_from[i * (i + 1) / 2 + s * 2 + j];
+            } else {
+              o[i] = X::mma(x[s], p, o[i]);
+            }
+          }
       }
       if (WIDE) {
         const int64_t to = (low(r) * BH + bh) * a.DV + dv0;
@@ -442,21 +530,37 @@ __global__ __launch_bounds__(W * 64, la_waves(sizeof(L), DKP, W)) void k_la_walk
     for (int s = 0; s < CS; ++s) {
       const Frag x = X::col(&cv[s * KB * PV + wc], PV, g, m);
       Frag part[X::PARTS];
+      float rest[KB / 4];
+      unsigned big = 0;
 #pragma unroll
       for (int e = 0; e < KB / 4; ++e) {
-        float rest = (float)x[e] * decay[s][e];
+        rest[e] = (float)x[e] * decay[s][e];
+        big = max(big, la_bits(rest[e]));
+      }
+      LaScale in = {1.0f, 1.0f};
+      if constexpr (X::SCALED) in = la_scale(big);
+#pragma unroll
+      for (int e = 0; e < KB / 4; ++e) {
+        if constexpr (X::SCALED) rest[e] *= in.to;
 #pragma unroll
         for (int c = 0; c < X::PARTS; ++c) {
-          const L top = (L)rest;
+          const L top = (L)rest[e];
           part[c][e] = top;
-          rest -= (float)top;
+          rest[e] -= (float)top;
         }
       }
 #pragma unroll
       for (int i = 0; i < KT; ++i) {
         const Frag y = X::col(&ck[s * KB * PK + i * 16], PK, g, m);
+        if constexpr (X::SCALED) {
+          f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int c = 0; c < X::PARTS; ++c) S[i] = X::mma(y, part[c], S[i]);
+          for (int c = 0; c < X::PARTS; ++c) sum = X::mma(y, part[c], sum);
+          S[i] += sum * in.from;
+        } else {
+#pragma unroll
+          for (int c = 0; c < X::PARTS; ++c) S[i] = X::mma(y, part[c], S[i]);
+        }
       }
     }
     if (WIDE) {
@@ -478,13 +582,13 @@ __global__ __launch_bounds__(W * 64, la_waves(sizeof(L), DKP, W)) void k_la_walk
   }
 }
 
-// Rows of a chunk for a dtype code, and columns of a workgroup's block for widths DK, DV.
-inline int la_chunk(int dtype) { return dtype == LSH_BF16 ? La<bf16_t>::C : La<float>::C; }
+// Rows of a chunk (of every type), and columns of a workgroup's block for widths DK, DV.
+inline int la_chunk() { return La<float>::C; }
 // 128 columns read Q and K and form the scores once where two blocks of 64 do it twice (bf16 4096 x 4 x 16
 // x 128, forward and backward: 425 us, with blocks of 64 461; 4096 x 16 x 256 x 256: 282 us backward, with
 // blocks of 64 383); 256 rows of a state in fp32 leave LDS for 64 only.
 inline int la_block(int dtype, int DK, int DV) {
-  return DV > 64 && (dtype == LSH_BF16 || DK <= 128) ? 128 : 64;
+  return DV > 64 && (dtype != LSH_F32 || DK <= 128) ? 128 : 64;
 }
 
 // Whether the walk's rows can be read and written in whole pieces: a chunk's byte offsets stay below

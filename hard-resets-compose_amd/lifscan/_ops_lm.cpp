@@ -435,7 +435,7 @@ std::tuple<Tensor, Tensor> distill_forward(const Tensor& z, const Tensor& values
   const c10::DeviceGuard guard(z.device());
   const int64_t rows = z.size(0), V = z.size(1);
   const auto f32 = z.options().dtype(torch::kFloat32);
-  const Tensor loss = torch::empty({rows}, f32), stats = torch::empty({2, rows}, f32);
+  const Tensor loss = torch::empty({rows}, f32), stats = torch::empty({4, rows}, f32);
   const size_t nb = g.lsh_distill_workspace(rows, V);
   const Tensor ws = workspace(nb, z);
   check(g.lsh_distill_fwd(code_of(z), raw(z), z.stride(0), code_of(values), raw(values), index.data_ptr<int64_t>(),
@@ -462,7 +462,7 @@ struct Distill : public torch::autograd::Function<Distill> {
     if (z.stride(1) != 1 && n[1] > 1) z = z.contiguous();
     const Tensor values = unpacked(saved[1], {n[0], n[2]}, (torch::ScalarType)n[4], gr).contiguous(),
                  index = unpacked(saved[2], {n[0], n[2]}, torch::kInt64, gr).contiguous(),
-                 stats = unpacked(saved[3], {2, n[0]}, torch::kFloat32, gr).contiguous();
+                 stats = unpacked(saved[3], {4, n[0]}, torch::kFloat32, gr).contiguous();
     const c10::DeviceGuard guard(z.device());
     const Tensor dz = torch::empty({n[0], n[1]}, z.options());
     check(g.lsh_distill_bwd(code_of(z), raw(z), z.stride(0), code_of(values), raw(values), index.data_ptr<int64_t>(),

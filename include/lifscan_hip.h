@@ -591,8 +591,8 @@ int lsh_embed_bwd(int dtype, const int64_t* tokens, const void* dout, void* dwei
  * entry; logits [rows, V] with a row stride in elements.  With p the softmax of values/tau over
  * the entries and q that of logits/tau over the vocabulary,
  *   loss = tau^2 * sum_k p_k (log p_k - log q_{index_k}),
- * 0 for a row without entries.  stats: [2, rows], what the gradient reads: log2(sum exp(logits/tau)) and
- * the teacher's log2(sum exp(values/tau)), -inf for a row without entries.
+ * 0 for a row without entries.  stats: [4, rows], what the gradient reads: the largest logit m and
+ * log2(sum exp((logits - m)/tau)), and the same of the teacher's values (-inf for a row without entries).
  *   dlogits = g * tau * (q - p at its ids), contiguous [rows, V]; g: [rows] with an element stride. */
 #define LSH_DISTILL_MAX_K 4096
 size_t lsh_distill_workspace(int64_t rows, int64_t V); /* 0: ws may be NULL */

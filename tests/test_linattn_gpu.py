@@ -342,6 +342,24 @@ def test_values_that_are_not_finite_stay_in_their_rows(dev):
         assert int((~torch.isfinite(s)).sum()) == 64
 
 
+@pytest.mark.parametrize("qk,vv", [(1e4, 1.0), (1e-3, 1.0), (1.0, 3000.0), (1.0, 2.0 ** -12)])
+def test_fp16_beyond_its_range_on_the_way(dev, qk, vv):
+    """Scores and states that fp16 cannot hold, or only among its smallest numbers, between operands and
+    results that it can: products of q and k of that size, values of that size."""
+    dtype, T, H, D = torch.float16, 150, 2, 64
+    q, k, v, beta, s0, do, ds = _inputs(dtype, T, 1, (H,) * 3, H, D, D, dev, seed=41)
+    q, k, v, s0 = q * qk ** 0.5, k * qk ** 0.5, v * vv, s0 * qk ** 0.5 * vv
+    do, ds, scale = do / max(vv, 1.0), ds / (qk ** 0.5 * vv), qk ** -0.5 / 16
+    got = run_all(q, k, v, beta, s0, scale, do, ds)
+    want = reference(q, k, v, beta, s0, scale, do, ds)
+    most = _absolute(q, k, v, beta, s0, scale, do, ds)
+    for g, w, m in zip(got, want, most):
+        assert g.dtype != dtype or float(w.abs().max()) < 65504
+        small = 2.0 ** -24 if g.dtype == dtype else 0.0  # fp16's smallest step
+        err = (g.detach().double().cpu() - w).abs()
+        assert bool((err <= U[g.dtype] * w.abs() + (2 * U[dtype] + (T + D + 64) * 2.0 ** -24) * m + small).all())
+
+
 def test_refusals(dev):
     from lifscan import hip_linattn as LA
     q = torch.randn(4, 2, 2, 8, device=dev)
