@@ -28,12 +28,12 @@ __global__ __launch_bounds__(256) void k_la_join(float* __restrict__ starts, con
   const float f = __builtin_amdgcn_exp2f(la_log2(beta[i / size % H]) * (float)L);
   float s = s0 ? s0[i] : 0.0f;
   starts[i] = s;
-  for (int j0 = 1; j0 < segs; j0 += 16) {
-    float x[16];  // the loads first: one latency for sixteen segments
+  for (int j0 = 1; j0 < segs; j0 += 8) {
+    float x[8];  // the loads first: one latency for eight segments
 #pragma unroll
-    for (int j = 0; j < 16; ++j) x[j] = starts[(size_t)min(j0 + j, segs - 1) * n + i];
+    for (int j = 0; j < 8; ++j) x[j] = starts[(size_t)min(j0 + j, segs - 1) * n + i];
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
+    for (int j = 0; j < 8; ++j) {
       s = __builtin_fmaf(f, s, x[j]);
       if (j0 + j < segs) starts[(size_t)(j0 + j) * n + i] = s;
     }

@@ -204,25 +204,30 @@ struct LaStage {
   static constexpr int N = C > ROWS ? C / ROWS : 1;
   static_assert(THREADS % PER_ROW == 0 && (C % ROWS == 0 || ROWS % C == 0), "whole rows");
   u32x4 x[N];
-  unsigned at;  // this thread's first piece, in bytes from the chunk's lowest row
+  const T* low;    // the lowest address of the chunk that is read next, as a whole one
+  int64_t ahead;   // elements from a chunk to the next
+  unsigned at;     // this thread's first piece, in bytes from low
+  unsigned step;   // bytes from a row of the walk to the next, modulo 2^32 where it goes back
   int r0;
-  // step: bytes from a row to the next in memory
-  __device__ __forceinline__ void init(unsigned step, int rev, int D) {
+  __device__ __forceinline__ void init(const T* lowest, int64_t st, int rev, int D) {
     r0 = threadIdx.x / PER_ROW;
+    low = lowest;
+    ahead = rev ? -C * st : C * st;
+    const unsigned bytes = (unsigned)st * (unsigned)sizeof(T);
+    step = rev ? 0u - bytes : bytes;
     const int c = threadIdx.x % PER_ROW * W;
-    at = (rev ? C - 1 - r0 : r0) * step + c * (unsigned)sizeof(T);
+    at = (rev ? C - 1 - r0 : r0) * bytes + c * (unsigned)sizeof(T);
     if (c >= D || r0 >= C) at = kLaNowhere;
   }
-  // the chunk's last n rows; low: the lowest address of a whole chunk
-  __device__ __forceinline__ void load(const T* low, unsigned step, int rev, int n) {
+  // the last n rows of the chunk at low
+  __device__ __forceinline__ void load(int n) {
     const LaRows rows(low);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const unsigned o = at == kLaNowhere || r0 + i * ROWS < C - n ? kLaNowhere
-                         : rev                                     ? at - i * ROWS * step
-                                                                   : at + i * ROWS * step;
-      x[i] = __builtin_amdgcn_raw_buffer_load_b128(rows.r, o, 0, 0);
+      const bool there = at != kLaNowhere && r0 + i * ROWS >= C - n;
+      x[i] = __builtin_amdgcn_raw_buffer_load_b128(rows.r, there ? at + i * ROWS * step : kLaNowhere, 0, 0);
     }
+    low += ahead;
   }
   __device__ __forceinline__ void put(L* lds, int pitch) const {
     const int c = threadIdx.x % PER_ROW * W;
@@ -252,9 +257,9 @@ struct LaStage {
 
 __device__ __forceinline__ bool la_odd(float x) { return !(fabsf(x) < INFINITY); }
 
-// Four columns of the chunk's rows i*16 + m to the output, o[i] to byte at + i*16*step (or -) from low.
+// Four columns of the chunk's rows i*16 + m to the output, o[i] to byte at + i*16*step (modulo 2^32) from low.
 template <class TO, int CT>
-__device__ __forceinline__ void la_store(TO* low, unsigned at, unsigned step, int rev, const f32x4 (&o)[CT],
+__device__ __forceinline__ void la_store(TO* low, unsigned at, unsigned step, const f32x4 (&o)[CT],
                                          int first) {
   const LaRows rows(low);
 #pragma unroll
@@ -262,9 +267,7 @@ __device__ __forceinline__ void la_store(TO* low, unsigned at, unsigned step, in
     Vec<TO, 4> y;
 #pragma unroll
     for (int e = 0; e < 4; ++e) y.v[e] = from_f<TO>(o[i][e]);
-    const unsigned b = at == kLaNowhere || i * 16 < first ? kLaNowhere
-                       : rev                              ? at - i * 16 * step
-                                                          : at + i * 16 * step;
+    const unsigned b = at != kLaNowhere && i * 16 >= first ? at + i * 16 * step : kLaNowhere;
     if constexpr (sizeof(TO) == 4)
       __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, y), rows.r, b, 0, 0);
     else
@@ -351,14 +354,22 @@ __global__ __launch_bounds__(W * 64, la_waves(sizeof(L), DKP, W)) void k_la_walk
   f32x4 S[KT];
   {
     const float* from = a.s_in + (size_t)(seg * BH + bh) * size;
+    if (!SUMS && a.s_in && a.sk == 1 && a.DK % 4 == 0) {
 #pragma unroll
-    for (int i = 0; i < KT; ++i)
+      for (int i = 0; i < KT; ++i)
+        S[i] = col && i * 16 + 4 * g < a.DK ? *(const f32x4*)(from + at0 + i * 16) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        S[i][e] = 0.0f;
-        if (!SUMS && a.s_in && col && i * 16 + 4 * g + e < a.DK) S[i][e] = from[at0 + (i * 16 + e) * a.sk];
-      }
+      for (int i = 0; i < KT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          S[i][e] = 0.0f;
+          if (!SUMS && a.s_in && col && i * 16 + 4 * g + e < a.DK) S[i][e] = from[at0 + (i * 16 + e) * a.sk];
+        }
+    }
   }
+  // the state is sigma*S: most chunks decay it by sigma alone, and weigh what they add by 1/sigma
+  float sigma = 1.0f;
   if (!SUMS) {
     for (int i = threadIdx.x; i < C * PP; i += W * 64) s_p[i] = (L)0.0f;  // tiles above the diagonal stay so
   }
@@ -383,13 +394,10 @@ __global__ __launch_bounds__(W * 64, la_waves(sizeof(L), DKP, W)) void k_la_walk
   LaStage<T, L, C, DKP, W * 64, true> xq;
   LaStage<T, L, C, DKP, W * 64, false> xk;
   LaStage<T, L, C, DVB, W * 64, false> xv;
-  // the row of lowest address of the chunk whose row 0 is at r
-  auto low = [&](int64_t r) { return a.rev ? a.T - r - C : r; };
-  const unsigned bq = (unsigned)a.q.st * sizeof(T), bk = (unsigned)a.k.st * sizeof(T), bv = (unsigned)a.v.st * sizeof(T);
-  auto fetch = [&](int64_t r, int n) {
-    if (!SUMS) xq.load(q + low(r) * a.q.st, bq, a.rev, n);
-    xk.load(k + low(r) * a.k.st, bk, a.rev, n);
-    xv.load(v + low(r) * a.v.st, bv, a.rev, n);
+  auto fetch = [&](int n) {
+    if (!SUMS) xq.load(n);
+    xk.load(n);
+    xv.load(n);
   };
   auto put = [&](int half) {
     if (!SUMS) xq.put(s_q + half * (C * PQ), PQ);
@@ -404,14 +412,20 @@ __global__ __launch_bounds__(W * 64, la_waves(sizeof(L), DKP, W)) void k_la_walk
   };
   const int64_t so = BH * a.DV;  // elements from a row of the output to the next
   const int dv = dv0 + wc + 4 * g;
-  const unsigned eo = a.out_f32 ? 4 : sizeof(T), bo = (unsigned)so * eo;
+  // the lowest address of the chunk's output, this lane's first byte from there, and bytes to the next row
+  const int64_t low = a.rev ? a.T - r - C : r;  // the chunk's row of lowest address
+  const unsigned eo = a.out_f32 ? 4 : sizeof(T), bo = (unsigned)so * eo, step_o = a.rev ? 0u - bo : bo;
+  const int64_t ahead_o = (a.rev ? -C : C) * so * eo;
+  char* out = (char*)a.out + ((low * BH + bh) * a.DV + dv0) * eo;
   const unsigned at_o = dv < a.DV ? (a.rev ? C - 1 - m : m) * bo + (wc + 4 * g) * eo : kLaNowhere;
   if (WIDE) {
-    xq.init(bq, a.rev, a.DK), xk.init(bk, a.rev, a.DK), xv.init(bv, a.rev, a.DV - dv0);
+    xq.init(q + low * a.q.st, a.q.st, a.rev, a.DK);
+    xk.init(k + low * a.k.st, a.k.st, a.rev, a.DK);
+    xv.init(v + low * a.v.st, a.v.st, a.rev, a.DV - dv0);
     if (n) {
-      fetch(r, n);
+      fetch(n);
       put(0);
-      fetch(r + C, r + 2 * C <= r1 ? C : 0);
+      fetch(r + 2 * C <= r1 ? C : 0);
     }
     __syncthreads();
   }
@@ -467,7 +481,7 @@ __global__ __launch_bounds__(W * 64, la_waves(sizeof(L), DKP, W)) void k_la_walk
       }
       const int first = C - n - m;  // a lane's rows of the chunk are those with 16i >= first
 #pragma unroll
-      for (int i = 0; i < CT; ++i) o[i] *= a.so * in.from * la_pow(l2, max(i * 16 - first, 0) + 1 - a.late);
+      for (int i = 0; i < CT; ++i) o[i] *= a.so * sigma * in.from * la_pow(l2, max(i * 16 - first, 0) + 1 - a.late);
       __syncthreads();  // the scores are there
 
       // what the chunk's own rows give
@@ -509,11 +523,11 @@ __global__ __launch_bounds__(W * 64, la_waves(sizeof(L), DKP, W)) void k_la_walk
           }
       }
       if (WIDE) {
-        const int64_t to = (low(r) * BH + bh) * a.DV + dv0;
         if (a.out_f32)
-          la_store<float, CT>((float*)a.out + to, at_o, bo, a.rev, o, first);
+          la_store<float, CT>((float*)out, at_o, step_o, o, first);
         else
-          la_store<T, CT>((T*)a.out + to, at_o, bo, a.rev, o, first);
+          la_store<T, CT>((T*)out, at_o, step_o, o, first);
+        out += ahead_o;
       } else {
         const int64_t to = ((a.rev ? a.T - 1 - r - m : r + m) * BH + bh) * a.DV + dv;
         if (a.out_f32)
@@ -523,9 +537,13 @@ __global__ __launch_bounds__(W * 64, la_waves(sizeof(L), DKP, W)) void k_la_walk
       }
     }
 
-    const float whole = la_pow(l2, n);
+    sigma *= la_pow(l2, n);
+    if (!(sigma > 0x1p-16f && sigma < 0x1p16f)) {
 #pragma unroll
-    for (int i = 0; i < KT; ++i) S[i] *= whole;
+      for (int i = 0; i < KT; ++i) S[i] *= sigma;
+      sigma = 1.0f;
+    }
+    const float weight = __builtin_amdgcn_rcpf(sigma);
 #pragma unroll
     for (int s = 0; s < CS; ++s) {
       const Frag x = X::col(&cv[s * KB * PV + wc], PV, g, m);
@@ -534,7 +552,7 @@ __global__ __launch_bounds__(W * 64, la_waves(sizeof(L), DKP, W)) void k_la_walk
       unsigned big = 0;
 #pragma unroll
       for (int e = 0; e < KB / 4; ++e) {
-        rest[e] = (float)x[e] * decay[s][e];
+        rest[e] = (float)x[e] * (decay[s][e] * weight);
         big = max(big, la_bits(rest[e]));
       }
       LaScale in = {1.0f, 1.0f};
@@ -566,7 +584,7 @@ __global__ __launch_bounds__(W * 64, la_waves(sizeof(L), DKP, W)) void k_la_walk
     if (WIDE) {
       half ^= 1;
       put(half);  // zeros after the last chunk
-      fetch(r + 2 * C, r + 3 * C <= r1 ? C : 0);
+      fetch(r + 3 * C <= r1 ? C : 0);
       __syncthreads();  // the next chunk is there, and the scores have been read
     }
   }
@@ -578,7 +596,7 @@ __global__ __launch_bounds__(W * 64, la_waves(sizeof(L), DKP, W)) void k_la_walk
     for (int i = 0; i < KT; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (col && i * 16 + 4 * g + e < a.DK) to[at0 + (i * 16 + e) * a.sk] = S[i][e];
+        if (col && i * 16 + 4 * g + e < a.DK) to[at0 + (i * 16 + e) * a.sk] = sigma * S[i][e];
   }
 }
 
