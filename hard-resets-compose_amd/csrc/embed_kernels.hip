@@ -36,7 +36,9 @@ __global__ __launch_bounds__(256) void k_embed(const int64_t* __restrict__ tok, 
 // that frequent neighbours go to different ones).  Each reads all tokens twice: it counts its rows'
 // tokens and those of the workgroups before it, which gives every row's place in the list, and then
 // puts its positions there in order.  The second reading needs no memory up to kEsTile tokens.
-// Bound by the reading, n * parts * 8 bytes from L2 (16384 tokens, 256 workgroups: 33 MB).
+// Bound by the latency of its steps (64 tokens 9 us, 16384 uniform ones 11, with Zipf's most frequent token
+// 16: one wave puts a workgroup's positions in order), beyond that by the reading, n * parts * 8 bytes
+// from L2 (65536 tokens: 134 MB, 60 us).
 constexpr int kEsThreads = 1024, kEsPer = 16, kEsTile = kEsThreads * kEsPer;
 constexpr int kEsRuns = kEsTile / 64;
 constexpr int kEsRows = 8192;  // table rows of a workgroup at most
@@ -195,9 +197,10 @@ __global__ __launch_bounds__(kEsThreads) void k_embed_sort(const int64_t* __rest
 // row's own lanes; longer rows are dealt to the workgroup's waves, up to kEbHot positions to one (its lane
 // groups take positions in turn), more to all, always joined in a fixed order.  Neighbouring rows, which
 // are often frequent together, go to different workgroups.
-// Bound by the rows read and written (16384 tokens, 32000 x 1024 bf16: 97 MB); what a Zipf text costs beyond
-// that is the chain of dependent loads of its longest rows.
-constexpr int kEbThreads = 1024, kEbLanes = 16, kEbFew = 4, kEbHot = 256, kEbGroups = 64;
+// Bound by the rows read and written (16384 tokens, 32000 x 1024 bf16: 97 MB, 26 us) and, with a Zipf text,
+// by the chain of dependent loads of its longest rows.  8 waves and 4 groups a wave measured best: 16 waves
+// 51 us with the sort, 4 waves 49, 8 waves 43.
+constexpr int kEbThreads = 512, kEbLanes = 16, kEbFew = 4, kEbHot = 256, kEbGroups = 32;
 
 // The sum of dout's rows at list[begin .. begin + n) in columns d.., dealt to `groups` lane groups, this
 // lane's the group-th, Q positions at once.
@@ -228,7 +231,7 @@ __global__ __launch_bounds__(kEbThreads) void k_embed_bwd(const int* __restrict_
   constexpr int P = kWide<T>, WAVES = kEbThreads / 64, EACH = kEbGroups / WAVES;
   // longer rows with their places and lengths, from the front; the longest from the back
   __shared__ int s_row[kEbGroups * 64], s_begin[kEbGroups * 64], s_count[kEbGroups * 64], s_n[2];
-  __shared__ int s_list[WAVES][kEbHot];
+  __shared__ int s_list[WAVES * kEbHot];
   __shared__ float s_sum[WAVES][kEbLanes * P];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int per = 64 / lanes, sub = lane / lanes, l = lane % lanes;  // rows of a wave, this lane's, its place
@@ -236,6 +239,7 @@ __global__ __launch_bounds__(kEbThreads) void k_embed_bwd(const int* __restrict_
   if (threadIdx.x < 2) s_n[threadIdx.x] = 0;
   __syncthreads();
   int c[EACH], at[EACH][kEbFew];
+  bool any[EACH];  // whether a row of the wave has positions
   int64_t row[EACH];
 #pragma unroll
   for (int k = 0; k < EACH; ++k) {
@@ -256,16 +260,19 @@ __global__ __launch_bounds__(kEbThreads) void k_embed_bwd(const int* __restrict_
       }
       c[k] = -1;
     }
+    any[k] = wave_ballot(c[k] > 0) != 0;
+    if (any[k])
 #pragma unroll
-    for (int q = kEbFew - 1; q >= 0; --q) at[k][q] = n > 0 ? list[min(at[k][0] + q, n - 1)] : 0;
+      for (int q = kEbFew - 1; q >= 0; --q) at[k][q] = n > 0 ? list[min(at[k][0] + q, n - 1)] : 0;
   }
-  if (n > 0) {
-    Raw<P, WIDE, T> x[EACH];
+  Raw<P, WIDE, T> x[EACH];
 #pragma unroll
-    for (int k = 0; k < EACH; ++k) x[k].load(dout + (size_t)(c[k] > 0 ? at[k][0] : 0) * D, d, D);
+  for (int k = 0; k < EACH; ++k)
+    if (any[k]) x[k].load(dout + (size_t)(c[k] > 0 ? at[k][0] : 0) * D, d, D);
 #pragma unroll
-    for (int k = 0; k < EACH; ++k) {
-      float s[P];
+  for (int k = 0; k < EACH; ++k) {
+    float s[P] = {};
+    if (any[k]) {
       x[k].get(s, d, D, c[k] > 0);
       if (wave_ballot(c[k] > 1)) {
         Raw<P, WIDE, T> y[kEbFew - 1];
@@ -279,25 +286,20 @@ __global__ __launch_bounds__(kEbThreads) void k_embed_bwd(const int* __restrict_
           for (int j = 0; j < P; ++j) s[j] += f[j];
         }
       }
-      if (c[k] < 0) continue;
-#pragma unroll
-      for (int j = 0; j < P; ++j) s[j] *= scale;
-      st_vals<P, WIDE>(s, dW + (size_t)row[k] * D, d, D);
     }
-  } else {
+    if (c[k] < 0) continue;
 #pragma unroll
-    for (int k = 0; k < EACH; ++k) {
-      const float s[P] = {};
-      if (c[k] == 0) st_vals<P, WIDE>(s, dW + (size_t)row[k] * D, d, D);
-    }
+    for (int j = 0; j < P; ++j) s[j] *= scale;
+    st_vals<P, WIDE>(s, dW + (size_t)row[k] * D, d, D);
   }
   __syncthreads();
   for (int h = w; h < s_n[0]; h += WAVES) {
     const int v = s_row[h], n = s_count[h], begin = s_begin[h];
-    for (int i = lane; i < n; i += 64) s_list[w][i] = list[begin + i];
+    int* mine = s_list + w * kEbHot;
+    for (int i = lane; i < n; i += 64) mine[i] = list[begin + i];
     __builtin_amdgcn_wave_barrier();
     float t[P] = {};
-    eb_sum<T, WIDE, 8>(t, [&](int i) { return s_list[w][i]; }, n, sub, per, dout, d, D);
+    eb_sum<T, WIDE, 8>(t, [&](int i) { return mine[i]; }, n, sub, per, dout, d, D);
     for (int o = lanes; o < 64; o *= 2)
 #pragma unroll
       for (int j = 0; j < P; ++j) t[j] += __shfl_xor(t[j], o, 64);
@@ -314,9 +316,9 @@ __global__ __launch_bounds__(kEbThreads) void k_embed_bwd(const int* __restrict_
     for (int i0 = 0; i0 < n; i0 += WAVES * kEbHot) {
       const int m = min(n - i0, WAVES * kEbHot);
       __syncthreads();  // s_list and s_sum have been read
-      for (int i = threadIdx.x; i < m; i += kEbThreads) s_list[0][i] = list[begin + i0 + i];
+      for (int i = threadIdx.x; i < m; i += kEbThreads) s_list[i] = list[begin + i0 + i];
       __syncthreads();
-      eb_sum<T, WIDE, 8>(t, [&](int i) { return s_list[0][i]; }, m, w * per + sub, per * WAVES, dout, d, D);
+      eb_sum<T, WIDE, 8>(t, [&](int i) { return s_list[i]; }, m, w * per + sub, per * WAVES, dout, d, D);
     }
     for (int o = lanes; o < 64; o *= 2)
 #pragma unroll

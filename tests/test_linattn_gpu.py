@@ -360,6 +360,53 @@ def test_fp16_beyond_its_range_on_the_way(dev, qk, vv):
         assert bool((err <= U[g.dtype] * w.abs() + (2 * U[dtype] + (T + D + 64) * 2.0 ** -24) * m + small).all())
 
 
+def _hooked(f, unpack):
+    with torch.autograd.graph.saved_tensors_hooks(lambda x: (x.device, x.cpu()), unpack):
+        outs, ins, grads = f()
+    return torch.autograd.grad(outs, ins, grads)
+
+
+def test_saved_tensors_that_come_back_changed(dev):
+    """Saved operands that went through host memory give the same gradients; ones that come back in
+    another type are refused, and so are second derivatives."""
+    from lifscan import hip_linattn as LA
+    from lifscan import hip_lm as LM
+    q, k, v, beta, s0, do, ds = _inputs(torch.bfloat16, 600, 1, (2, 1, 2), 2, 32, 64, dev, seed=43)
+    W, tok = torch.randn(50, 16, device=dev), torch.arange(40, device=dev) % 50
+    x, w = torch.randn(6, 40, device=dev), torch.ones(40, device=dev)
+    z, idx = torch.randn(5, 70, device=dev), torch.arange(15, device=dev).view(5, 3)
+
+    def attn():
+        ins = [t.detach().clone().requires_grad_(True) for t in (q, k, v, s0)]
+        return LA.lin_attn(*ins[:3], beta, s0=ins[3]), ins, (do, ds)
+
+    def norm():
+        ins = [t.detach().clone().requires_grad_(True) for t in (x, x, w, w)]
+        return LM.block_norm(ins[0], ins[1], ins[2], ins[3], gate=ins[1], res_scale=ins[2]), ins, (x, x)
+
+    def lookup():
+        a = W.clone().requires_grad_(True)
+        out = LM.embed(tok, a)
+        return out, [a], out.detach()
+
+    def loss():
+        a = z.clone().requires_grad_(True)
+        return LM.distill_topk(a, z[:, :3], idx), [a], torch.ones(5, device=dev)
+
+    for f in (attn, norm, lookup, loss):
+        outs, ins, grads = f()
+        want = torch.autograd.grad(outs, ins, grads)
+        for a, b in zip(_hooked(f, lambda p: p[1].to(p[0])), want):
+            assert torch.equal(a, b)
+        with pytest.raises(ValueError):
+            _hooked(f, lambda p: p[1].to(p[0]).double())
+        with pytest.raises(ValueError):
+            _hooked(f, lambda p: p[1])
+        outs, ins, grads = f()
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(outs, ins, grads, create_graph=True)
+
+
 def test_refusals(dev):
     from lifscan import hip_linattn as LA
     q = torch.randn(4, 2, 2, 8, device=dev)
