@@ -44,10 +44,28 @@ inline void with_dtype(int d, F&& f) {
     f(f16_t{});
 }
 
+// the value N lanes further in a row of 16
+template <int N>
+__device__ __forceinline__ float row_turned(float x) {
+  const int i = __builtin_bit_cast(int, x);
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, i, 0x120 + N, 0xf, 0xf, true));
+}
+
+// The sum over a wave, the same in every lane: a tree within the rows of 16 lanes, then over the rows, all
+// between registers.
 __device__ __forceinline__ float wave_sum_f(float v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, WAVE);
-  return v;
+  v += row_turned<8>(v);
+  v += row_turned<4>(v);
+  v += row_turned<2>(v);
+  v += row_turned<1>(v);
+  const unsigned a = __builtin_bit_cast(unsigned, v);
+  const auto x = __builtin_amdgcn_permlane16_swap(a, a, false, false);
+  const unsigned x0 = x[0], x1 = x[1];
+  v = __builtin_bit_cast(float, x0) + __builtin_bit_cast(float, x1);
+  const unsigned b = __builtin_bit_cast(unsigned, v);
+  const auto y = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+  const unsigned y0 = y[0], y1 = y[1];
+  return __builtin_bit_cast(float, y0) + __builtin_bit_cast(float, y1);
 }
 
 // V values of a row from column d on, as read: WIDE in 16-byte accesses (D a multiple of V), otherwise one
