@@ -14,7 +14,7 @@
 // Bound by the rows' bytes; x_new is computed again instead of being kept.  bf16, 8192 x 2048: forward
 // 26.6 us for 168 MB (6.3 TB/s, part of it from the Infinity Cache), gradients 48 us for 268 MB
 // (5.6 TB/s) and 7 for the parameters' sums; with an fp32 stream 35 and 75, all fp32 62 and 106.  Rows
-// that cannot be read in pieces go element by element: 8190 x 2047 forward 128, gradients 106.
+// that cannot be read in pieces go element by element: 8190 x 2047 forward 28, gradients 63.
 #include <type_traits>
 
 #include "lsh_lm.h"
@@ -73,7 +73,13 @@ struct BnRow {
 using u32x2 = unsigned __attribute__((ext_vector_type(2)));
 using u32x4 = unsigned __attribute__((ext_vector_type(4)));
 
-// V values from column d on, as read: WIDE in accesses of 8 or 16 bytes, otherwise one by one.
+// A lane's piece of V values, the d/V-th of the row.  WIDE: columns d.., in accesses of 8 or 16 bytes.
+// Otherwise one by one, the columns dealt out so that a wave's lanes read neighbours (8190 x 2047 forward
+// 28 us and gradients 63, with a lane's own columns side by side 128 and 106).
+template <int V, bool WIDE>
+__device__ __forceinline__ int bn_col(int d, int j) {
+  return WIDE ? d + j : (d / V & ~63) * V + j * 64 + (d / V & 63);
+}
 template <int V, bool WIDE, class T>
 struct BnRaw {
   static constexpr int P = V * sizeof(T) > 16 ? 16 / (int)sizeof(T) : V, BYTES = P * (int)sizeof(T);
@@ -81,7 +87,7 @@ struct BnRaw {
   __device__ __forceinline__ void load(const BnRow<T>& row, int d) {
 #pragma unroll
     for (int i = 0; i < V / P; ++i) {
-      const int at = (d + i * P) * (int)sizeof(T);
+      const int at = bn_col<V, WIDE>(d, i * P) * (int)sizeof(T);
       if constexpr (WIDE && BYTES == 16)
         x[i] = __builtin_bit_cast(Vec<T, P>, __builtin_amdgcn_raw_buffer_load_b128(row.r, at, 0, 0));
       else if constexpr (WIDE)
@@ -90,9 +96,9 @@ struct BnRaw {
 #pragma unroll
         for (int j = 0; j < P; ++j) {
           if constexpr (sizeof(T) == 4)
-            x[i].v[j] = __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b32(row.r, at + j * 4, 0, 0));
+            x[i].v[j] = __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b32(row.r, at + j * 64 * 4, 0, 0));
           else
-            x[i].v[j] = __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b16(row.r, at + j * 2, 0, 0));
+            x[i].v[j] = __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b16(row.r, at + j * 64 * 2, 0, 0));
         }
     }
   }
@@ -112,7 +118,7 @@ __device__ __forceinline__ void bn_put(const float (&f)[V], const BnRow<T>& row,
   using R = BnRaw<V, WIDE, T>;
 #pragma unroll
   for (int i = 0; i < V; i += R::P) {
-    const int at = (d + i) * (int)sizeof(T);
+    const int at = bn_col<V, WIDE>(d, i) * (int)sizeof(T);
     Vec<T, R::P> x;
 #pragma unroll
     for (int j = 0; j < R::P; ++j) x.v[j] = from_f<T>(f[i + j]);
@@ -124,9 +130,9 @@ __device__ __forceinline__ void bn_put(const float (&f)[V], const BnRow<T>& row,
 #pragma unroll
       for (int j = 0; j < R::P; ++j) {
         if constexpr (sizeof(T) == 4)
-          __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, x.v[j]), row.r, at + j * 4, 0, 0);
+          __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, x.v[j]), row.r, at + j * 64 * 4, 0, 0);
         else
-          __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(short, x.v[j]), row.r, at + j * 2, 0, 0);
+          __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(short, x.v[j]), row.r, at + j * 64 * 2, 0, 0);
       }
   }
 }
@@ -394,7 +400,7 @@ static void with_types(int tx, int ty, F&& f) {
 // 4 and a sixth with 8, which take 158 registers instead of 91.  Rows of 257 to 2048 channels in wide
 // accesses leave room for 3 waves a SIMD with 8 (bf16 8192 x 2048: 48 us, with 4 60).  Narrower rows would
 // leave lanes idle, wider ones are one workgroup a CU (4096 x 4096 with the sums: 83 us, with 4 78), and
-// element by element 8 take 190 registers (8190 x 2047: 165, with 4 114).
+// element by element 8 take 190 registers.
 template <bool BWD, bool WIDE, class F>
 static void with_row(int D, F&& f) {
   using std::integral_constant;

@@ -115,6 +115,17 @@ def test_block_norm(dev, types, rows, D):
     bn_check(got, bn_reference(x, y, gate, w_post, w_pre, a, 1e-6, act, gx, gz), rows)
 
 
+# more rows than workgroups: each kernel variant carries its parameters' sums and the next row over
+@pytest.mark.parametrize("types", [TYPES[0], TYPES[-1]], ids=[IDS[0], IDS[-1]])
+@pytest.mark.parametrize("rows,D", [(5000, 96), (3200, 320), (1700, 1000), (800, 2040), (700, 999), (300, 4096),
+                                    (300, 8184), (270, 16376), (260, 9001)])
+def test_block_norm_many_rows(dev, types, rows, D):
+    print(f"block_norm {rows}x{D} {types}", flush=True)
+    x, y, gate, w_post, w_pre, a, gx, gz = _bn_inputs(rows, D, *types, dev, seed=2)
+    got = bn_run(x, y, gate, w_post, w_pre, a, 1e-6, "silu", gx, gz)
+    bn_check(got, bn_reference(x, y, gate, w_post, w_pre, a, 1e-6, "silu", gx, gz), rows)
+
+
 @pytest.mark.parametrize("what", ["no_gate", "number", "only_x", "only_z", "large_eps"])
 def test_block_norm_parts(dev, what):
     rows, D = 37, 192
