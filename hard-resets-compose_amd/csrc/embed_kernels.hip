@@ -11,7 +11,8 @@
 
 namespace lsh {
 
-// One thread a piece of V columns.
+// One thread a piece of 16 bytes, or of as many columns a row's pieces apart (16384 x 1023 bf16: 12 us, with
+// a thread's own columns side by side 32; 16384 x 1024 10).
 template <class T, bool WIDE>
 __global__ __launch_bounds__(256) void k_embed(const int64_t* __restrict__ tok, const T* __restrict__ W,
                                                T* __restrict__ out, int64_t n, int64_t V, int D, int64_t pad,
@@ -20,15 +21,15 @@ __global__ __launch_bounds__(256) void k_embed(const int64_t* __restrict__ tok, 
   const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int64_t i = u / pieces;
   if (i >= n) return;
-  const int d = (int)(u - i * pieces) * P;
+  const int d = (int)(u - i * pieces) * (WIDE ? P : 1);
   const int64_t v = tok[i];
   float f[P] = {};
   if (v >= 0 && v < V && v != pad) {
-    ld_vals<P, WIDE>(f, W + (size_t)v * D, d, D);
+    ld_vals<P, WIDE>(f, W + (size_t)v * D, d, D, pieces);
 #pragma unroll
     for (int j = 0; j < P; ++j) f[j] *= scale;
   }
-  st_vals<P, WIDE>(f, out + (size_t)i * D, d, D);
+  st_vals<P, WIDE>(f, out + (size_t)i * D, d, D, pieces);
 }
 
 // ---- positions by token
@@ -199,23 +200,23 @@ __global__ __launch_bounds__(kEsThreads) void k_embed_sort(const int64_t* __rest
 // are often frequent together, go to different workgroups.
 // Bound by the rows read and written (16384 tokens, 32000 x 1024 bf16: 97 MB, 26 us) and, with a Zipf text,
 // by the chain of dependent loads of its longest rows.  8 waves and 4 groups a wave measured best: 16 waves
-// 51 us with the sort, 4 waves 49, 8 waves 43.
+// 51 us with the sort, 4 waves 49, 8 waves 43.  Rows of 1023 columns, element by element: 68 us.
 constexpr int kEbThreads = 512, kEbLanes = 16, kEbFew = 4, kEbHot = 256, kEbGroups = 32;
 
 // The sum of dout's rows at list[begin .. begin + n) in columns d.., dealt to `groups` lane groups, this
 // lane's the group-th, Q positions at once.
 template <class T, bool WIDE, int Q, class At>
 __device__ __forceinline__ void eb_sum(float (&t)[kWide<T>], At&& at, int n, int group, int groups,
-                                       const T* __restrict__ dout, int d, int D) {
+                                       const T* __restrict__ dout, int d, int D, int lanes) {
   constexpr int P = kWide<T>;
   for (int i = group; i < n; i += Q * groups) {
     Raw<P, WIDE, T> x[Q];
 #pragma unroll
-    for (int q = 0; q < Q; ++q) x[q].load(dout + (size_t)at(min(i + q * groups, n - 1)) * D, d, D);
+    for (int q = 0; q < Q; ++q) x[q].load(dout + (size_t)at(min(i + q * groups, n - 1)) * D, d, D, lanes);
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
       float f[P];
-      x[q].get(f, d, D, i + q * groups < n);
+      x[q].get(f, d, D, lanes, i + q * groups < n);
 #pragma unroll
       for (int j = 0; j < P; ++j) t[j] += f[j];
     }
@@ -235,7 +236,7 @@ __global__ __launch_bounds__(kEbThreads) void k_embed_bwd(const int* __restrict_
   __shared__ float s_sum[WAVES][kEbLanes * P];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int per = 64 / lanes, sub = lane / lanes, l = lane % lanes;  // rows of a wave, this lane's, its place
-  const int d0 = blockIdx.y * kEbLanes * P, d = d0 + l * P;
+  const int d0 = blockIdx.y * kEbLanes * P, d = d0 + (WIDE ? l * P : l);
   if (threadIdx.x < 2) s_n[threadIdx.x] = 0;
   __syncthreads();
   int c[EACH], at[EACH][kEbFew];
@@ -268,20 +269,20 @@ __global__ __launch_bounds__(kEbThreads) void k_embed_bwd(const int* __restrict_
   Raw<P, WIDE, T> x[EACH];
 #pragma unroll
   for (int k = 0; k < EACH; ++k)
-    if (any[k]) x[k].load(dout + (size_t)(c[k] > 0 ? at[k][0] : 0) * D, d, D);
+    if (any[k]) x[k].load(dout + (size_t)(c[k] > 0 ? at[k][0] : 0) * D, d, D, lanes);
 #pragma unroll
   for (int k = 0; k < EACH; ++k) {
     float s[P] = {};
     if (any[k]) {
-      x[k].get(s, d, D, c[k] > 0);
+      x[k].get(s, d, D, lanes, c[k] > 0);
       if (wave_ballot(c[k] > 1)) {
         Raw<P, WIDE, T> y[kEbFew - 1];
 #pragma unroll
-        for (int q = 1; q < kEbFew; ++q) y[q - 1].load(dout + (size_t)(q < c[k] ? at[k][q] : 0) * D, d, D);
+        for (int q = 1; q < kEbFew; ++q) y[q - 1].load(dout + (size_t)(q < c[k] ? at[k][q] : 0) * D, d, D, lanes);
 #pragma unroll
         for (int q = 1; q < kEbFew; ++q) {
           float f[P];
-          y[q - 1].get(f, d, D, q < c[k]);
+          y[q - 1].get(f, d, D, lanes, q < c[k]);
 #pragma unroll
           for (int j = 0; j < P; ++j) s[j] += f[j];
         }
@@ -290,7 +291,7 @@ __global__ __launch_bounds__(kEbThreads) void k_embed_bwd(const int* __restrict_
     if (c[k] < 0) continue;
 #pragma unroll
     for (int j = 0; j < P; ++j) s[j] *= scale;
-    st_vals<P, WIDE>(s, dW + (size_t)row[k] * D, d, D);
+    st_vals<P, WIDE>(s, dW + (size_t)row[k] * D, d, D, lanes);
   }
   __syncthreads();
   for (int h = w; h < s_n[0]; h += WAVES) {
@@ -299,14 +300,14 @@ __global__ __launch_bounds__(kEbThreads) void k_embed_bwd(const int* __restrict_
     for (int i = lane; i < n; i += 64) mine[i] = list[begin + i];
     __builtin_amdgcn_wave_barrier();
     float t[P] = {};
-    eb_sum<T, WIDE, 8>(t, [&](int i) { return mine[i]; }, n, sub, per, dout, d, D);
+    eb_sum<T, WIDE, 8>(t, [&](int i) { return mine[i]; }, n, sub, per, dout, d, D, lanes);
     for (int o = lanes; o < 64; o *= 2)
 #pragma unroll
       for (int j = 0; j < P; ++j) t[j] += __shfl_xor(t[j], o, 64);
     if (sub == 0) {
 #pragma unroll
       for (int j = 0; j < P; ++j) t[j] *= scale;
-      st_vals<P, WIDE>(t, dW + (size_t)v * D, d, D);
+      st_vals<P, WIDE>(t, dW + (size_t)v * D, d, D, lanes);
     }
     __builtin_amdgcn_wave_barrier();
   }
@@ -318,7 +319,7 @@ __global__ __launch_bounds__(kEbThreads) void k_embed_bwd(const int* __restrict_
       __syncthreads();  // s_list and s_sum have been read
       for (int i = threadIdx.x; i < m; i += kEbThreads) s_list[i] = list[begin + i0 + i];
       __syncthreads();
-      eb_sum<T, WIDE, 8>(t, [&](int i) { return s_list[i]; }, m, w * per + sub, per * WAVES, dout, d, D);
+      eb_sum<T, WIDE, 8>(t, [&](int i) { return s_list[i]; }, m, w * per + sub, per * WAVES, dout, d, D, lanes);
     }
     for (int o = lanes; o < 64; o *= 2)
 #pragma unroll
@@ -335,7 +336,7 @@ __global__ __launch_bounds__(kEbThreads) void k_embed_bwd(const int* __restrict_
         for (int j = 0; j < P; ++j) t[j] += s_sum[k][threadIdx.x * P + j];
 #pragma unroll
       for (int j = 0; j < P; ++j) t[j] *= scale;
-      st_vals<P, WIDE>(t, dW + (size_t)v * D, d, D);
+      st_vals<P, WIDE>(t, dW + (size_t)v * D, d, D, lanes);
     }
   }
 }

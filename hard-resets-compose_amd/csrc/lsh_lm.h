@@ -68,37 +68,38 @@ __device__ __forceinline__ float wave_sum_f(float v) {
   return __builtin_bit_cast(float, y0) + __builtin_bit_cast(float, y1);
 }
 
-// V values of a row from column d on, as read: WIDE in 16-byte accesses (D a multiple of V), otherwise one
-// by one.  Columns beyond D are read from the row's last ones, so that no branch stands around a wide
-// load: behind a branch the compiler waits for each load before it issues the next.
+// V values of a row of D: WIDE the columns d, d + 1, ... in 16-byte accesses (D a multiple of V), otherwise
+// the columns d, d + step, ... one by one, where lanes that are neighbours take neighbouring columns.
+// Columns beyond D are read from the row's last ones, so that no branch stands around a wide load: behind a
+// branch the compiler waits for each load before it issues the next.
 template <int V, bool WIDE, class T>
 struct Raw {
   static constexpr int P = V * sizeof(T) > 16 ? 16 / (int)sizeof(T) : V;
   Vec<T, P> x[V / P];
-  __device__ __forceinline__ void load(const T* p, int d, int D) {
+  __device__ __forceinline__ void load(const T* p, int d, int D, int step) {
     if constexpr (WIDE) {
       const int at = min(d, D - V);
 #pragma unroll
       for (int i = 0; i < V / P; ++i) x[i] = *(const Vec<T, P>*)(p + at + i * P);
     } else {
 #pragma unroll
-      for (int j = 0; j < V; ++j) x[j / P].v[j % P] = p[min(d + j, D - 1)];
+      for (int j = 0; j < V; ++j) x[j / P].v[j % P] = p[min(d + j * step, D - 1)];
     }
   }
   // as fp32, zeros beyond D or where `there` is false
-  __device__ __forceinline__ void get(float (&f)[V], int d, int D, bool there = true) const {
+  __device__ __forceinline__ void get(float (&f)[V], int d, int D, int step, bool there = true) const {
 #pragma unroll
-    for (int j = 0; j < V; ++j) f[j] = there && d + (WIDE ? 0 : j) < D ? to_f(x[j / P].v[j % P]) : 0.0f;
+    for (int j = 0; j < V; ++j) f[j] = there && d + (WIDE ? 0 : j * step) < D ? to_f(x[j / P].v[j % P]) : 0.0f;
   }
 };
 template <int V, bool WIDE, class T>
-__device__ __forceinline__ void ld_vals(float (&f)[V], const T* p, int d, int D) {
+__device__ __forceinline__ void ld_vals(float (&f)[V], const T* p, int d, int D, int step) {
   Raw<V, WIDE, T> x;
-  x.load(p, d, D);
-  x.get(f, d, D);
+  x.load(p, d, D, step);
+  x.get(f, d, D, step);
 }
 template <int V, bool WIDE, class T>
-__device__ __forceinline__ void st_vals(const float (&f)[V], T* p, int d, int D) {
+__device__ __forceinline__ void st_vals(const float (&f)[V], T* p, int d, int D, int step) {
   if constexpr (WIDE) {
     if (d < D) {
       constexpr int P = V * sizeof(T) > 16 ? 16 / sizeof(T) : V;
@@ -113,7 +114,7 @@ __device__ __forceinline__ void st_vals(const float (&f)[V], T* p, int d, int D)
   } else {
 #pragma unroll
     for (int j = 0; j < V; ++j)
-      if (d + j < D) p[d + j] = from_f<T>(f[j]);
+      if (d + j * step < D) p[d + j * step] = from_f<T>(f[j]);
   }
 }
 
