@@ -99,16 +99,19 @@ static int la_starts(LaWalk a, int dtype, LaSplit s, const float* s0, float* sta
   return LSH_OK;
 }
 
-// One token: the state is read, updated and written in place.  16 lanes cover 64 columns with
-// 16-byte accesses, the 16 row groups of a workgroup take the state's rows in turn, and o is
-// joined over the row groups in a fixed order.  Bound by the state's bytes.
+// One token: the state is read, updated and written in place.  16 lanes cover 64 columns, four a lane
+// (WIDE: one 16-byte access, otherwise 16 columns apart), the 16 row groups of a workgroup take the
+// state's rows in turn, and o is joined over the row groups in a fixed order.
+// Bound by the state's bytes: 64 x 16 states of 128 x 128 22.5 us for 134 MB (6.0 TB/s, from the Infinity
+// Cache); a single sequence by its launch (8 states of 64 x 64: 4 us).
 template <class T, bool WIDE>
 __global__ __launch_bounds__(256) void k_la_step(LaIn qi, LaIn ki, LaIn vi,
                                                  const float* __restrict__ betas,
                                                  float* __restrict__ state, T* __restrict__ out,
                                                  int64_t H, int DK, int DV, float scale) {
   __shared__ float s_o[16][64 + 4];
-  const int col = (threadIdx.x & 15) * 4, rg = threadIdx.x >> 4;
+  const int rg = threadIdx.x >> 4, col = (threadIdx.x & 15) * (WIDE ? 4 : 1);
+  constexpr int STEP = WIDE ? 1 : 16;
   const int dv0 = blockIdx.y * 64 + col;
   const int64_t bh = blockIdx.x, b = bh / H, h = bh % H;
   const T* q = la_row<T>(qi, b, h);
@@ -117,7 +120,7 @@ __global__ __launch_bounds__(256) void k_la_step(LaIn qi, LaIn ki, LaIn vi,
   const float beta = betas[h];
   float vt[4], o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-  for (int j = 0; j < 4; ++j) vt[j] = dv0 + j < DV ? to_f(v[dv0 + j]) : 0.0f;
+  for (int j = 0; j < 4; ++j) vt[j] = dv0 + j * STEP < DV ? to_f(v[dv0 + j * STEP]) : 0.0f;
   float* S = state + (size_t)bh * DK * DV + dv0;
   for (int dk = rg; dk < DK; dk += 16) {
     float* row = S + (size_t)dk * DV;
@@ -138,16 +141,16 @@ __global__ __launch_bounds__(256) void k_la_step(LaIn qi, LaIn ki, LaIn vi,
     } else {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        if (dv0 + j < DV) {
-          const float s = __builtin_fmaf(kt, vt[j], beta * row[j]);
-          row[j] = s;
+        if (dv0 + j * STEP < DV) {
+          const float s = __builtin_fmaf(kt, vt[j], beta * row[j * STEP]);
+          row[j * STEP] = s;
           o[j] = __builtin_fmaf(qt, s, o[j]);
         }
       }
     }
   }
 #pragma unroll
-  for (int j = 0; j < 4; ++j) s_o[rg][col + j] = o[j];
+  for (int j = 0; j < 4; ++j) s_o[rg][col + j * STEP] = o[j];
   __syncthreads();
   const int c = threadIdx.x;
   if (c < 64 && blockIdx.y * 64 + c < DV) {
