@@ -198,7 +198,7 @@ struct LaRows {
 // the rows before it and the columns from D on are zeros: the distance to a chunk's end is the same in
 // every chunk.  The loads have no branches around them (those cost the wait for all of them at the next
 // loop head).  PACKED: in the order of La::packed.
-template <class T, class L, int C, int DP, int THREADS, bool PACKED>
+template <class T, class L, int C, int DP, int THREADS, bool PACKED, bool WIDE>
 struct LaStage {
   static constexpr int W = kWide<T>, PER_ROW = DP / W, ROWS = THREADS / PER_ROW;  // rows a piece of all threads
   static constexpr int N = C > ROWS ? C / ROWS : 1;
@@ -244,14 +244,50 @@ struct LaStage {
         *(Vec<L, Q>*)&lds[(r0 + i * ROWS) * pitch + (PACKED ? La<L>::packed(c + j) : c + j)] = *(Vec<L, Q>*)&y.v[j];
     }
   }
-  // operands whose rows cannot be read 16 bytes at a time come straight from memory, element by element
-  static __device__ __forceinline__ void copy(L* lds, int pitch, const T* p, int64_t step, int D, int n) {
-#pragma unroll 1
-    for (int u = threadIdx.x; u < C * DP; u += THREADS) {
-      const int r = u / DP, c = u % DP;
-      lds[r * pitch + (PACKED ? La<L>::packed(c & ~3) + (c & 3) : c)] =
-          r >= C - n && c < D ? (L)p[r * step + c] : (L)0.0f;
+};
+
+// The same for operands whose rows cannot be read 16 bytes at a time, or lie far apart: element by element,
+// a thread's columns PER_ROW apart, so that neighbouring lanes read neighbours.  What is not there is read
+// from the last row and column that are.  4096 x 4 x 16 x 127 x 127 forward: fp32 341 us (128 columns 300),
+// bf16, where the accesses are half as wide again, 262 (125); without the chunk held ahead 817 and 370.
+template <class T, class L, int C, int DP, int THREADS, bool PACKED>
+struct LaStage<T, L, C, DP, THREADS, PACKED, false> {
+  static constexpr int W = kWide<T>, PER_ROW = DP / W, ROWS = THREADS / PER_ROW;
+  static constexpr int N = C > ROWS ? C / ROWS : 1;
+  T x[N][W];
+  const T* low;
+  int64_t ahead, step;  // elements, both signed
+  int r0, D, first;     // rows from `first` on are there
+  __device__ __forceinline__ void init(const T* lowest, int64_t st, int rev, int columns) {
+    r0 = threadIdx.x / PER_ROW;
+    step = rev ? -st : st;
+    ahead = C * step;
+    low = rev ? lowest + (C - 1) * st : lowest;  // the chunk's row 0
+    D = columns;
+  }
+  __device__ __forceinline__ void load(int n) {
+    first = C - n;
+    const T* from = n > 0 ? low : low - ahead;  // past the end, for good: the last chunk's last row again
+    const int c = threadIdx.x % PER_ROW;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int r = r0 + i * ROWS;
+      const T* row = from + (r >= first && r < C ? r : C - 1) * step;
+#pragma unroll
+      for (int j = 0; j < W; ++j) x[i][j] = row[min(c + j * PER_ROW, D - 1)];
     }
+    low = from + ahead;
+  }
+  __device__ __forceinline__ void put(L* lds, int pitch) const {
+    if (ROWS > C && r0 >= C) return;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int j = 0; j < W; ++j) {
+        const int r = r0 + i * ROWS, c = threadIdx.x % PER_ROW + j * PER_ROW;
+        lds[r * pitch + (PACKED ? La<L>::packed(c & ~3) + (c & 3) : c)] =
+            r >= first && c < D ? (L)x[i][j] : (L)0.0f;
+      }
   }
 };
 
@@ -334,8 +370,8 @@ __global__ __launch_bounds__(W * 64, la_waves(sizeof(L), DKP, W)) void k_la_walk
   constexpr int C = X::C, KB = X::KB, DVB = W * 16, KT = DKP / 16, CT = C / 16, KS = DKP / KB, CS = C / KB;
   static_assert(CT * (CT + 1) / 2 <= W, "a wave has one tile of the scores at most");
   constexpr int PQ = DKP + X::kPadRow, PK = DKP + X::kPadCol, PV = DVB + X::kPadCol, PP = C + X::kPadRow;
-  constexpr int HALVES = WIDE ? 2 : 1;  // of LDS: one is filled while the other is read
-  __shared__ alignas(16) L s_q[SUMS ? 8 : HALVES * C * PQ], s_k[HALVES * C * PK], s_v[HALVES * C * PV];
+  // of each two halves: one is filled while the other is read
+  __shared__ alignas(16) L s_q[SUMS ? 8 : 2 * C * PQ], s_k[2 * C * PK], s_v[2 * C * PV];
   __shared__ alignas(16) L s_p[SUMS ? 8 : C * PP];
   __shared__ float s_from[W];  // SCALED: what takes each tile of the scores back
 
@@ -395,9 +431,9 @@ __global__ __launch_bounds__(W * 64, la_waves(sizeof(L), DKP, W)) void k_la_walk
 #pragma unroll
   for (int e = 0; e < 4; ++e) fall[e] = a.so * a.su * la_pow(l2, max((ti - tj) * 16 + m - 4 * g - e, 0));
 
-  LaStage<T, L, C, DKP, W * 64, true> xq;
-  LaStage<T, L, C, DKP, W * 64, false> xk;
-  LaStage<T, L, C, DVB, W * 64, false> xv;
+  LaStage<T, L, C, DKP, W * 64, true, WIDE> xq;
+  LaStage<T, L, C, DKP, W * 64, false, WIDE> xk;
+  LaStage<T, L, C, DVB, W * 64, false, WIDE> xv;
   auto fetch = [&](int n) {
     if (!SUMS) xq.load(n);
     xk.load(n);
@@ -408,12 +444,6 @@ __global__ __launch_bounds__(W * 64, la_waves(sizeof(L), DKP, W)) void k_la_walk
     xk.put(s_k + half * (C * PK), PK);
     xv.put(s_v + half * (C * PV), PV);
   };
-  auto copy = [&](int64_t r, int n) {  // not WIDE
-    const int64_t t0 = a.rev ? a.T - 1 - r : r, sign = a.rev ? -1 : 1;
-    if (!SUMS) xq.copy(s_q, PQ, q + t0 * a.q.st, sign * a.q.st, a.DK, n);
-    xk.copy(s_k, PK, k + t0 * a.k.st, sign * a.k.st, a.DK, n);
-    xv.copy(s_v, PV, v + t0 * a.v.st, sign * a.v.st, a.DV - dv0, n);
-  };
   const int64_t so = BH * a.DV;  // elements from a row of the output to the next
   const int dv = dv0 + wc + 4 * g;
   // the lowest address of the chunk's output, this lane's first byte from there, and bytes to the next row
@@ -422,24 +452,17 @@ __global__ __launch_bounds__(W * 64, la_waves(sizeof(L), DKP, W)) void k_la_walk
   const int64_t ahead_o = (a.rev ? -C : C) * so * eo;
   char* out = (char*)a.out + ((low * BH + bh) * a.DV + dv0) * eo;
   const unsigned at_o = dv < a.DV ? (a.rev ? C - 1 - m : m) * bo + (wc + 4 * g) * eo : kLaNowhere;
-  if (WIDE) {
-    xq.init(q + low * a.q.st, a.q.st, a.rev, a.DK);
-    xk.init(k + low * a.k.st, a.k.st, a.rev, a.DK);
-    xv.init(v + low * a.v.st, a.v.st, a.rev, a.DV - dv0);
-    if (n) {
-      fetch(n);
-      put(0);
-      fetch(r + 2 * C <= r1 ? C : 0);
-    }
-    __syncthreads();
+  xq.init(q + low * a.q.st, a.q.st, a.rev, a.DK);
+  xk.init(k + low * a.k.st, a.k.st, a.rev, a.DK);
+  xv.init(v + low * a.v.st, a.v.st, a.rev, a.DV - dv0);
+  if (n) {
+    fetch(n);
+    put(0);
+    fetch(r + 2 * C <= r1 ? C : 0);
   }
+  __syncthreads();
   int half = 0;
   for (; n && r + C <= r1; r += C, n = C) {
-    if (!WIDE) {
-      __syncthreads();  // everyone has read the chunk before
-      copy(r, n);
-      __syncthreads();
-    }
     const L *cq = s_q + half * (C * PQ), *ck = s_k + half * (C * PK), *cv = s_v + half * (C * PV);
     if (!SUMS) {
       // scores with their decays
@@ -585,12 +608,10 @@ __global__ __launch_bounds__(W * 64, la_waves(sizeof(L), DKP, W)) void k_la_walk
         }
       }
     }
-    if (WIDE) {
-      half ^= 1;
-      put(half);  // zeros after the last chunk
-      fetch(r + 3 * C <= r1 ? C : 0);
-      __syncthreads();  // the next chunk is there, and the scores have been read
-    }
+    half ^= 1;
+    put(half);  // zeros after the last chunk
+    fetch(r + 3 * C <= r1 ? C : 0);
+    __syncthreads();  // the next chunk is there, and the scores have been read
   }
 
   if (SUMS || (a.s_out && seg == a.segs - 1)) {
