@@ -246,15 +246,29 @@ struct LaStage {
   }
 };
 
-// The same for operands whose rows cannot be read 16 bytes at a time, or lie far apart: element by element,
-// a thread's columns PER_ROW apart, so that neighbouring lanes read neighbours.  What is not there is read
-// from the last row and column that are.  4096 x 4 x 16 x 127 x 127 forward: fp32 341 us (128 columns 300),
-// bf16, where the accesses are half as wide again, 262 (125); without the chunk held ahead 817 and 370.
+// n of eight 16-bit values fall out at the low end, zeros come in at the high end.
+__device__ __forceinline__ u32x4 la_shift(u32x4 x, int n) {
+  x = n & 8 ? u32x4{0, 0, 0, 0} : x;
+  x = n & 4 ? u32x4{x[2], x[3], 0, 0} : x;
+  x = n & 2 ? u32x4{x[1], x[2], x[3], 0} : x;
+  return n & 1 ? u32x4{__builtin_amdgcn_alignbit(x[1], x[0], 16), __builtin_amdgcn_alignbit(x[2], x[1], 16),
+                       __builtin_amdgcn_alignbit(x[3], x[2], 16), x[3] >> 16}
+               : x;
+}
+
+// The same for operands whose rows do not begin at multiples of 16 bytes, or lie far apart.  Rows that are
+// not there are read from one that is.
+// 16 bits: a piece that would leave the row ends with it, and is shifted into place on its way to LDS (rows
+// shorter than a piece are read element by element).  32 bits: element by element, a thread's columns
+// PER_ROW apart, so that neighbouring lanes read neighbours.
+// 4096 x 4 x 16 x 127 x 127 forward: bf16 165 us, element by element 262 (128 columns 125); fp32 324 us, in
+// pieces 428 (128 columns 300).
 template <class T, class L, int C, int DP, int THREADS, bool PACKED>
 struct LaStage<T, L, C, DP, THREADS, PACKED, false> {
   static constexpr int W = kWide<T>, PER_ROW = DP / W, ROWS = THREADS / PER_ROW;
   static constexpr int N = C > ROWS ? C / ROWS : 1;
-  T x[N][W];
+  static constexpr bool PIECES = sizeof(T) == 2;
+  Vec<T, W> x[N];
   const T* low;
   int64_t ahead, step;  // elements, both signed
   int r0, D, first;     // rows from `first` on are there
@@ -273,21 +287,40 @@ struct LaStage<T, L, C, DP, THREADS, PACKED, false> {
     for (int i = 0; i < N; ++i) {
       const int r = r0 + i * ROWS;
       const T* row = from + (r >= first && r < C ? r : C - 1) * step;
+      if (PIECES && D >= W)
+        __builtin_memcpy(&x[i], row + min(c * W, D - W), 16);
+      else
 #pragma unroll
-      for (int j = 0; j < W; ++j) x[i][j] = row[min(c + j * PER_ROW, D - 1)];
+        for (int j = 0; j < W; ++j) x[i].v[j] = row[min(PIECES ? j : c + j * PER_ROW, D - 1)];
     }
     low = from + ahead;
   }
   __device__ __forceinline__ void put(L* lds, int pitch) const {
     if (ROWS > C && r0 >= C) return;
 #pragma unroll
-    for (int i = 0; i < N; ++i)
+    for (int i = 0; i < N; ++i) {
+      const bool there = r0 + i * ROWS >= first;
+      L* row = lds + (r0 + i * ROWS) * pitch;
+      if constexpr (PIECES) {
+        const int c = threadIdx.x % PER_ROW * W;
+        const int out = !there ? W : min(D >= W ? max(c - (D - W), 0) : c, W);
+        const Vec<L, W> y = __builtin_bit_cast(Vec<L, W>, la_shift(__builtin_bit_cast(u32x4, x[i]), out));
+        constexpr int Q = PACKED ? 4 : W;
 #pragma unroll
-      for (int j = 0; j < W; ++j) {
-        const int r = r0 + i * ROWS, c = threadIdx.x % PER_ROW + j * PER_ROW;
-        lds[r * pitch + (PACKED ? La<L>::packed(c & ~3) + (c & 3) : c)] =
-            r >= first && c < D ? (L)x[i][j] : (L)0.0f;
+        for (int j = 0; j < W; j += Q) {
+          Vec<L, Q> z;
+#pragma unroll
+          for (int e = 0; e < Q; ++e) z.v[e] = c + j + e < D ? y.v[j + e] : (L)0.0f;
+          *(Vec<L, Q>*)&row[PACKED ? La<L>::packed(c + j) : c + j] = z;
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < W; ++j) {
+          const int c = threadIdx.x % PER_ROW + j * PER_ROW;
+          row[PACKED ? La<L>::packed(c & ~3) + (c & 3) : c] = there && c < D ? (L)x[i].v[j] : (L)0.0f;
+        }
       }
+    }
   }
 };
 
@@ -310,14 +343,22 @@ __device__ __forceinline__ void la_store(TO* low, unsigned at, unsigned step, co
       __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, y), rows.r, b, 0, 0);
   }
 }
-// The same element by element: p is row m's first column, left of them are there.
+// The same where rows begin anywhere: p is row m's first column, left of them are there.
 template <class TO, int CT>
 __device__ __forceinline__ void la_store_some(TO* p, int64_t step, const f32x4 (&o)[CT], int first, int left) {
 #pragma unroll
-  for (int i = 0; i < CT; ++i)
+  for (int i = 0; i < CT; ++i) {
+    if (i * 16 < first) continue;
+    Vec<TO, 4> y;
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (i * 16 >= first && e < left) p[i * 16 * step + e] = from_f<TO>(o[i][e]);
+    for (int e = 0; e < 4; ++e) y.v[e] = from_f<TO>(o[i][e]);
+    if (left >= 4)
+      __builtin_memcpy(p + i * 16 * step, &y, sizeof(y));
+    else
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (e < left) p[i * 16 * step + e] = y.v[e];
+  }
 }
 
 // Whether any of a fragment's values is not finite: the exponent's bits, plus one in their last place; all
