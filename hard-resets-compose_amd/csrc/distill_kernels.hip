@@ -9,8 +9,8 @@
 // m the largest logit and l = log2(sum 2^(c*(z - m))), q_v = 2^(c*(z_v - m) - l).  (m stays apart from l:
 // their sum would round by a share of the logits' size where only their differences matter.)  The
 // forward reads the logits once, with the running maximum and sum of the softmax, and keeps m, l and the
-// teacher's two; the backward reads them once more and writes dz.  Both are bound by the logits' bytes
-// (4096 x 32000 bf16: 262 MB forward, 524 MB backward).  A row is split over several workgroups where there
+// teacher's two; the backward reads them once more and writes dz.  Both are bound by the logits' bytes:
+// 4096 x 32000 bf16 with 64 entries 47 us forward (262 MB, 5.6 TB/s) and 122 backward (524 MB, 4.3 TB/s).  A row is split over several workgroups where there
 // are too few rows for the chip, and the parts' maxima and sums are joined in order.
 #include <algorithm>
 
@@ -181,11 +181,21 @@ __global__ __launch_bounds__(64) void k_distill_join(DsArgs a) {
   ds_loss<T>(a, row, m, __builtin_amdgcn_logf(s));
 }
 
+// dz of a part of a row, then the teacher's entries in it once more with their p.  An id may come several
+// times; its p are summed in order by the first.  A bit for each place (modulo kDsBits) tells those that may
+// come again, and only they look through the others (4096 x 32000 bf16: 16 entries a row 113 us, 1024 entries
+// 293, with all looking 641; 8 x 131072 with 64 entries 4.9 and 7.4).
+constexpr int kDsBits = 32768;
 template <class T>
 __global__ __launch_bounds__(kDsThreads) void k_distill_bwd(DsArgs a) {
   constexpr int P = kWide<T>, U = 4;
-  extern __shared__ int s_id[];  // the teacher's ids of this part, as places in it (-1: none), then their p
+  extern __shared__ int s_id[];  // the teacher's ids of this part, as places in it (-1: none), then their p,
   float* s_p = (float*)(s_id + a.K);
+  int* s_again = s_id + 2 * a.K;  // and those whose place may come again, n_again of them
+  __shared__ unsigned s_once[kDsBits / 32], s_twice[kDsBits / 32];
+  __shared__ int n_again;
+  for (int b = threadIdx.x; b < kDsBits / 32; b += kDsThreads) s_once[b] = s_twice[b] = 0;
+  if (threadIdx.x == 0) n_again = 0;
   const int64_t row = blockIdx.x / a.splits, v0 = blockIdx.x % a.splits * a.len;
   const T* z = (const T*)a.z + row * a.stride + v0;
   T* dz = (T*)a.dz + row * a.V + v0;
@@ -212,16 +222,32 @@ __global__ __launch_bounds__(kDsThreads) void k_distill_bwd(DsArgs a) {
   for (; i < pieces; i += kDsThreads) put(ld_piece(z + (int64_t)i * P), i);
   if (const int e = pieces * P + threadIdx.x; e < n) dz[e] = from_f<T>(grad(to_f(z[e])));
   if (!some) return;
+  __syncthreads();  // the bits are clear
   for (int k = threadIdx.x; k < a.K; k += kDsThreads) {
     const int64_t id = a.id[row * a.K + k];
     const bool here = id >= v0 && id < v0 + n;
-    s_id[k] = here ? (int)(id - v0) : -1;
+    const int e = here ? (int)(id - v0) : -1;
+    s_id[k] = e;
     s_p[k] = here ? __builtin_amdgcn_exp2f(__builtin_fmaf(ds_value<T>(a, row * a.K + k) - tm, a.c, -tl)) : 0.0f;
+    if (!here) continue;
+    const unsigned bit = 1u << (e & 31), at = e % kDsBits / 32;
+    if (atomicOr(&s_once[at], bit) & bit) atomicOr(&s_twice[at], bit);
   }
   __syncthreads();  // also the part's stores: its entries are written again with the teacher's part
+  auto write = [&](int e, float p) {
+    dz[e] = from_f<T>(f * (__builtin_amdgcn_exp2f(__builtin_fmaf(to_f(z[e]) - zm, a.c, -l)) - p));
+  };
   for (int k = threadIdx.x; k < a.K; k += kDsThreads) {
     const int e = s_id[k];
     if (e < 0) continue;
+    if (s_twice[e % kDsBits / 32] & (1u << (e & 31)))
+      s_again[atomicAdd(&n_again, 1)] = k;
+    else
+      write(e, s_p[k]);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < n_again; i += kDsThreads) {
+    const int k = s_again[i], e = s_id[k];
     bool first = true;
     float p = 0.0f;
     for (int j = 0; j < a.K; ++j)
@@ -229,7 +255,7 @@ __global__ __launch_bounds__(kDsThreads) void k_distill_bwd(DsArgs a) {
         first = first && j >= k;
         p += s_p[j];
       }
-    if (first) dz[e] = from_f<T>(f * (__builtin_amdgcn_exp2f(__builtin_fmaf(to_f(z[e]) - zm, a.c, -l)) - p));
+    if (first) write(e, p);
   }
 }
 
@@ -305,7 +331,7 @@ extern "C" int lsh_distill_bwd(int dtype, const void* logits, int64_t stride, in
   a.stats = (float*)stats, a.g = g, a.g_stride = g_stride, a.dz = dlogits;
   with_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    k_distill_bwd<T><<<dim3((unsigned)(rows * a.splits)), kDsThreads, (size_t)K * 8, (hipStream_t)stream>>>(a);
+    k_distill_bwd<T><<<dim3((unsigned)(rows * a.splits)), kDsThreads, (size_t)K * 12, (hipStream_t)stream>>>(a);
   });
   LSH_CHECK_LAUNCH();
   return LSH_OK;
