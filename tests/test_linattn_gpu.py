@@ -132,6 +132,20 @@ def test_long_sequences_of_few_heads(dev, dtype, T, B, H, Dk, Dv):
         check(g, w, m, dtype, T, max(Dk, Dv))
 
 
+@pytest.mark.parametrize("dtype", list(U), ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("T,B,H,Dk,Dv", [(1500, 1, 1, 33, 127), (701, 2, 1, 63, 7), (400, 1, 2, 129, 65),
+                                         (333, 1, 1, 5, 3)])
+def test_odd_widths_in_segments(dev, dtype, T, B, H, Dk, Dv):
+    """Rows that begin anywhere, short first chunks, several segments, both directions."""
+    print(f"linattn odd {dtype} {T} {B} {H} {Dk} {Dv}", flush=True)
+    q, k, v, beta, s0, do, ds = _inputs(dtype, T, B, (H,) * 3, H, Dk, Dv, dev, seed=7)
+    got = run_all(q, k, v, beta, s0, 0.1, do, ds)
+    want = reference(q, k, v, beta, s0, 0.1, do, ds)
+    most = _absolute(q, k, v, beta, s0, 0.1, do, ds)
+    for g, w, m in zip(got, want, most):
+        check(g, w, m, dtype, T, max(Dk, Dv))
+
+
 @pytest.mark.parametrize("which", ["no_s0", "only_o", "only_state"])
 def test_parts_of_the_gradient(dev, which):
     dtype, T = torch.float32, 70

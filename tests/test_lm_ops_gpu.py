@@ -389,6 +389,20 @@ def test_distill(dev, dtype, rows, V, K, tau):
     assert bool((loss[(idx < 0).all(1)] == 0).all()) and bool((dz[(idx < 0).all(1)] == 0).all())
 
 
+@pytest.mark.parametrize("rows,V,K", [(520, 40000, 384), (2, 70001, 4096)])
+def test_distill_many_entries(dev, rows, V, K):
+    """Ids that lie 32768 apart, and ids that are named two to four times, among many."""
+    print(f"distill {rows}x{V} K={K}", flush=True)
+    gen = torch.Generator().manual_seed(V)
+    z = 3 * torch.randn(rows, V, generator=gen)
+    low = torch.rand(rows, V - 32768, generator=gen).topk(K // 3, 1).indices
+    idx = torch.cat([low, low + 32768, torch.randint(0, V, (rows, K - 2 * (K // 3) - 6), generator=gen),
+                     low[:, :3], low[:, :3]], 1)
+    idx = idx[:, torch.randperm(K, generator=gen)].contiguous()
+    t = torch.gather(z, 1, idx) + torch.randn(rows, K, generator=gen)
+    distill_check(z.to(dev), t.to(dev), idx.to(dev), 1.5, torch.randn(rows, generator=gen).to(dev), V)
+
+
 def test_distill_entries(dev):
     """No entry at all, K = 0, ids beyond the vocabulary, one id named twice, teacher logits of -inf, fp32
     teacher values with bf16 logits, logits of -inf that the teacher does not name."""
