@@ -38,12 +38,13 @@ __global__ __launch_bounds__(256) void k_embed(const int64_t* __restrict__ tok, 
 // tokens and those of the workgroups before it, which gives every row's place in the list, and then
 // puts its positions there in order.  The second reading needs no memory up to kEsTile tokens.
 // Bound by the latency of its steps (64 tokens 9 us, 16384 uniform ones 11, with Zipf's most frequent token
-// 16: one wave puts a workgroup's positions in order), beyond that by the reading, n * parts * 8 bytes
-// from L2 (65536 tokens: 134 MB, 60 us).
+// 13), beyond that by the reading, n * parts * 8 bytes from L2 (65536 tokens: 134 MB, 45 us).  Many positions
+// of few rows are put in order by all waves, which first count their shares (by one wave: 16 and 60 us).
 constexpr int kEsThreads = 1024, kEsPer = 16, kEsTile = kEsThreads * kEsPer;
 constexpr int kEsRuns = kEsTile / 64;
 constexpr int kEsRows = 8192;  // table rows of a workgroup at most
 constexpr int kEsList = 4096;  // positions on their way to the list
+constexpr int kEsFew = 256, kEsFine = 512;  // more positions of at most so many rows are put by all waves
 
 inline int es_parts(int64_t V) {
   int64_t p = 256;
@@ -57,6 +58,7 @@ __global__ __launch_bounds__(kEsThreads) void k_embed_sort(const int64_t* __rest
   __shared__ int s_row[kEsRows];   // a row's tokens, then where its next position goes
   __shared__ int s_at[kEsList];    // positions found, in order, with
   __shared__ short s_of[kEsList];  // the row of each
+  __shared__ int s_next[kEsThreads / 64][kEsFine];
   __shared__ int s_wave[kEsThreads / 64], s_sum[kEsThreads / 64];
   __shared__ int s_runs[kEsRuns + 1];  // runs of 64 tokens of a tile: how many are found before each, and in all
   const int p = blockIdx.x, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
@@ -114,29 +116,54 @@ __global__ __launch_bounds__(kEsThreads) void k_embed_sort(const int64_t* __rest
     __syncthreads();
   }
   int found = 0;
-  // the positions found so far to their places, by one wave, 64 at a time
-  auto flush = [&]() {
-    __syncthreads();
-    if (w == 0) {
-      for (int i0 = 0; i0 < found; i0 += 64) {
-        const bool there = i0 + lane < found;
-        const int row = there ? s_of[i0 + lane] : -1;
-        const int at = there ? s_at[i0 + lane] : 0;
-        // the lanes with this lane's row
-        unsigned long long same = wave_ballot(there);
-        if (wave_ballot(row == __shfl(row, 0, 64)) != ~0ull) {
+  // positions i0.. before i1 to their places by one wave, 64 at a time; next: a row's next place
+  auto place = [&](int i0, int i1, int* next) {
+    for (; i0 < i1; i0 += 64) {
+      const bool there = i0 + lane < i1;
+      const int row = there ? s_of[i0 + lane] : -1;
+      const int at = there ? s_at[i0 + lane] : 0;
+      // the lanes with this lane's row
+      unsigned long long same = wave_ballot(there);
+      if (wave_ballot(row == __shfl(row, 0, 64)) != ~0ull) {
 #pragma unroll
-          for (int b = 0; b < 13; ++b) {
-            const unsigned long long m = wave_ballot((row >> b) & 1);
-            same &= (row >> b) & 1 ? m : ~m;
-          }
-        }
-        if (there) {
-          const int to = s_row[row];
-          list[to + __popcll(same & lower)] = at;
-          if (!(same >> lane >> 1)) s_row[row] = to + __popcll(same);
+        for (int b = 0; b < 13; ++b) {
+          const unsigned long long m = wave_ballot((row >> b) & 1);
+          same &= (row >> b) & 1 ? m : ~m;
         }
       }
+      if (there) {
+        const int to = next[row];
+        list[to + __popcll(same & lower)] = at;
+        if (!(same >> lane >> 1)) next[row] = to + __popcll(same);
+      }
+    }
+  };
+  // the positions found so far to their places
+  auto flush = [&]() {
+    __syncthreads();
+    if (found <= kEsFew || rows > kEsFine) {
+      if (w == 0) place(0, found, s_row);
+    } else {
+      // a share for each wave, in order: what the shares before it hold of a row comes first
+      const int share = (found + kEsThreads - 1) / kEsThreads * 64;
+      const int i0 = min(w * share, found), i1 = min(i0 + share, found);
+      for (int i = threadIdx.x; i < (kEsThreads / 64) * kEsFine; i += kEsThreads) s_next[0][i] = 0;
+      __syncthreads();
+      for (int i = i0 + lane; i < i1; i += 64) atomicAdd(&s_next[w][s_of[i]], 1);
+      __syncthreads();
+      if ((int)threadIdx.x < rows) {
+        int c[kEsThreads / 64], at = s_row[threadIdx.x];
+#pragma unroll
+        for (int k = 0; k < kEsThreads / 64; ++k) c[k] = s_next[k][threadIdx.x];
+#pragma unroll
+        for (int k = 0; k < kEsThreads / 64; ++k) {
+          s_next[k][threadIdx.x] = at;
+          at += c[k];
+        }
+        s_row[threadIdx.x] = at;
+      }
+      __syncthreads();
+      place(i0, i1, s_next[w]);
     }
     __syncthreads();
     found = 0;
@@ -199,8 +226,8 @@ __global__ __launch_bounds__(kEsThreads) void k_embed_sort(const int64_t* __rest
 // groups take positions in turn), more to all, always joined in a fixed order.  Neighbouring rows, which
 // are often frequent together, go to different workgroups.
 // Bound by the rows read and written (16384 tokens, 32000 x 1024 bf16: 97 MB, 26 us) and, with a Zipf text,
-// by the chain of dependent loads of its longest rows.  8 waves and 4 groups a wave measured best: 16 waves
-// 51 us with the sort, 4 waves 49, 8 waves 43.  Rows of 1023 columns, element by element: 68 us.
+// by the chain of dependent loads of its longest rows.  8 waves and 4 groups a wave measured best: with
+// the sort 40 us; 16 waves took 8 us more, 4 waves 6.  Rows of 1023 columns, element by element: 65 us.
 constexpr int kEbThreads = 512, kEbLanes = 16, kEbFew = 4, kEbHot = 256, kEbGroups = 32;
 
 // The sum of dout's rows at list[begin .. begin + n) in columns d.., dealt to `groups` lane groups, this
