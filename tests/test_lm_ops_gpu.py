@@ -262,6 +262,12 @@ def test_embed(dev, dtype, kind, n, V, D):
     assert torch.equal(dW, again)
 
 
+@pytest.mark.parametrize("kind", ["zipf", "one"])
+def test_embed_many_tokens_of_a_large_table(dev, kind):
+    """More rows a workgroup than its waves can count apart, and more positions than its list holds."""
+    test_embed(dev, torch.float32, kind, 6000, 200000, 8)
+
+
 def test_embed_ids_outside_the_table(dev):
     """Ids below 0 and from V on read as zero rows and leave no gradient; also those that 32 bits fold."""
     from lifscan import hip_lm as LM
