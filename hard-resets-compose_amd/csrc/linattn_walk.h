@@ -508,6 +508,9 @@ __global__ __launch_bounds__(W * 64, la_waves(sizeof(L), DKP, W)) void k_la_walk
   int half = 0;
   for (; n && r + C <= r1; r += C, n = C) {
     const L *cq = s_q + half * (C * PQ), *ck = s_k + half * (C * PK), *cv = s_v + half * (C * PV);
+    Frag x[CS];  // the chunk's values in the wave's columns
+#pragma unroll
+    for (int s = 0; s < CS; ++s) x[s] = X::col(&cv[s * KB * PV + wc], PV, g, m);
     if (!SUMS) {
       // scores with their decays
       if (w < CT * (CT + 1) / 2) {
@@ -556,13 +559,9 @@ __global__ __launch_bounds__(W * 64, la_waves(sizeof(L), DKP, W)) void k_la_walk
       __syncthreads();  // the scores are there
 
       // what the chunk's own rows give
-      Frag x[CS];
       bool odd = false;
 #pragma unroll
-      for (int s = 0; s < CS; ++s) {
-        x[s] = X::col(&cv[s * KB * PV + wc], PV, g, m);
-        odd |= la_odd(x[s]);
-      }
+      for (int s = 0; s < CS; ++s) odd |= la_odd(x[s]);
       if (wave_ballot(odd)) {
         // values that are not finite must not meet the zero scores of the rows before them
 #pragma unroll 1
@@ -617,13 +616,12 @@ __global__ __launch_bounds__(W * 64, la_waves(sizeof(L), DKP, W)) void k_la_walk
     const float weight = __builtin_amdgcn_rcpf(sigma);
 #pragma unroll
     for (int s = 0; s < CS; ++s) {
-      const Frag x = X::col(&cv[s * KB * PV + wc], PV, g, m);
       Frag part[X::PARTS];
       float rest[KB / 4];
       unsigned big = 0;
 #pragma unroll
       for (int e = 0; e < KB / 4; ++e) {
-        rest[e] = (float)x[e] * (decay[s][e] * weight);
+        rest[e] = (float)x[s][e] * (decay[s][e] * weight);
         big = max(big, la_bits(rest[e]));
       }
       LaScale in = {1.0f, 1.0f};
