@@ -33,193 +33,294 @@ __global__ __launch_bounds__(256) void k_embed(const int64_t* __restrict__ tok, 
 }
 
 // ---- positions by token
-// The table's rows are dealt to `parts` workgroups (a power of two, row v to workgroup v % parts, so
-// that frequent neighbours go to different ones).  Each reads all tokens twice: it counts its rows'
-// tokens and those of the workgroups before it, which gives every row's place in the list, and then
-// puts its positions there in order.  The second reading needs no memory up to kEsTile tokens.
-// Bound by the latency of its steps (64 tokens 9 us, 16384 uniform ones 11, with Zipf's most frequent token
-// 13), beyond that by the reading, n * parts * 8 bytes from L2 (65536 tokens: 134 MB, 45 us).  Many positions
-// of few rows are put in order by all waves, which first count their shares (by one wave: 16 and 60 us).
-constexpr int kEsThreads = 1024, kEsPer = 16, kEsTile = kEsThreads * kEsPer;
+// The table's rows are dealt to `parts` workgroups (a power of two, row v to workgroup v % parts, so that
+// frequent neighbours go to different ones); a workgroup's rows lie together in the list of positions, part
+// after part.
+//
+// Up to kEsTile tokens one kernel does it: every workgroup reads all tokens, counts its rows' and those of
+// the workgroups before it, which gives every row's place in the list, and puts its positions there in
+// order.  Bound by the latency of its steps (64 tokens 9 us, 16384 uniform ones 11, with Zipf's most frequent
+// token 13; many positions of few rows are put in order by all waves, which first count their shares: by one
+// wave 16).
+// More tokens are also split over the workgroups, or each would look at all of them: one kernel counts every
+// (part, split)'s rows, the next puts its positions after those of the splits before it (65536 Zipf tokens
+// 21 us, with one kernel 45; 262144 33 and about 175).
+constexpr int kEsThreads = 1024, kEsPer = 16, kEsTile = kEsThreads * kEsPer, kEsWaves = kEsThreads / 64;
 constexpr int kEsRuns = kEsTile / 64;
 constexpr int kEsRows = 8192;  // table rows of a workgroup at most
 constexpr int kEsList = 4096;  // positions on their way to the list
 constexpr int kEsFew = 256, kEsFine = 512;  // more positions of at most so many rows are put by all waves
 
-inline int es_parts(int64_t V) {
-  int64_t p = 256;
+// How n tokens of V rows are dealt: splits == 0 is the one kernel.
+struct EsDeal {
+  int parts, splits;
+  int64_t rows;  // V up to a multiple of parts
+};
+inline EsDeal es_deal(int64_t n, int64_t V) {
+  int64_t p = n <= kEsTile ? 256 : 16;
   while ((V + p - 1) / p > kEsRows) p *= 2;
-  return (int)p;
+  const int splits = n <= kEsTile ? 0 : (int)std::max<int64_t>(1, std::min<int64_t>(256 / p, (n + 4095) / 4096));
+  return {(int)p, splits, (int64_t)align_up((size_t)V, (size_t)p)};
 }
 
-__global__ __launch_bounds__(kEsThreads) void k_embed_sort(const int64_t* __restrict__ tok, int n, int V,
-                                                           int64_t pad, int parts, int* __restrict__ start,
-                                                           int* __restrict__ count, int* __restrict__ list) {
-  __shared__ int s_row[kEsRows];   // a row's tokens, then where its next position goes
-  __shared__ int s_at[kEsList];    // positions found, in order, with
-  __shared__ short s_of[kEsList];  // the row of each
-  __shared__ int s_next[kEsThreads / 64][kEsFine];
-  __shared__ int s_wave[kEsThreads / 64], s_sum[kEsThreads / 64];
-  __shared__ int s_runs[kEsRuns + 1];  // runs of 64 tokens of a tile: how many are found before each, and in all
-  const int p = blockIdx.x, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int rows = (V - p + parts - 1) / parts, shift = __builtin_ctz(parts);
-  const unsigned long long lower = (1ull << lane) - 1;
-  // a token's row v, or -1; thread t has tokens t, t + 1024, ... of a tile
-  int v[kEsPer];
-  auto read = [&](int t0) {
+struct EsLds {
+  int row[kEsRows];              // a row's tokens, then where its next position goes
+  int at[kEsList];               // positions found, in order, with
+  short of[kEsList];             // the row of each
+  int next[kEsWaves][kEsFine];   // the same as row for each wave's share
+  int sum[kEsWaves];
+  int runs[kEsRuns + 1];         // runs of 64 tokens of a tile: how many are found before each, and in all
+};
+
+// The rows of a tile's tokens, -1 for none: thread t has tokens t0 + t, t0 + t + 1024, ... before end.
+__device__ __forceinline__ void es_read(int (&v)[kEsPer], const int64_t* __restrict__ tok, int t0, int end, int V,
+                                        int64_t pad) {
 #pragma unroll
-    for (int j = 0; j < kEsPer; ++j) {
-      const int i = t0 + j * kEsThreads + threadIdx.x;
-      const int64_t x = i < n ? tok[i] : -1;
-      v[j] = (uint64_t)x < (uint64_t)V && (int)x != (int)pad ? (int)x : -1;
-    }
-  };
-  for (int i = threadIdx.x; i < rows; i += kEsThreads) s_row[i] = 0;
-  __syncthreads();
-  int before = 0;
-  for (int t0 = 0; t0 < n; t0 += kEsTile) {
-    read(t0);
-#pragma unroll
-    for (int j = 0; j < kEsPer; ++j) {
-      const int part = v[j] & (parts - 1);
-      before += v[j] >= 0 && part < p;
-      if (v[j] >= 0 && part == p) atomicAdd(&s_row[v[j] >> shift], 1);
-    }
+  for (int j = 0; j < kEsPer; ++j) {
+    const int i = t0 + j * kEsThreads + threadIdx.x;
+    const int64_t x = i < end ? tok[i] : -1;
+    v[j] = (uint64_t)x < (uint64_t)V && (int)x != (int)pad ? (int)x : -1;
   }
-  before = wave_sum_i(before);
-  if (lane == 0) s_wave[w] = before;
+}
+
+// The sum of a workgroup's values, in every thread.
+__device__ __forceinline__ int es_sum(EsLds& s, int x) {
+  x = wave_sum_i(x);
   __syncthreads();
-  before = 0;
-  for (int i = 0; i < kEsThreads / 64; ++i) before += s_wave[i];
+  if ((threadIdx.x & 63) == 0) s.sum[threadIdx.x >> 6] = x;
   __syncthreads();
-  // each row's place: an exclusive sum over the rows, 1024 at a time
+  x = 0;
+#pragma unroll
+  for (int i = 0; i < kEsWaves; ++i) x += s.sum[i];
+  __syncthreads();
+  return x;
+}
+
+// Each row's place: an exclusive sum over the part's rows, 1024 at a time, behind `before` positions.  get(i,
+// own): a row's positions, and how many of them lie before this workgroup's.
+template <class Get>
+__device__ __forceinline__ void es_places(EsLds& s, Get&& get, int rows, int before, int p, int parts, bool write,
+                                          int* __restrict__ start, int* __restrict__ count) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   for (int i0 = 0; i0 < rows; i0 += kEsThreads) {
-    const int i = i0 + threadIdx.x, c = i < rows ? s_row[i] : 0;
+    const int i = i0 + threadIdx.x;
+    int own = 0;
+    const int c = i < rows ? get(i, own) : 0;
     int incl = c;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
       const int x = __shfl_up(incl, o, 64);
       if (lane >= o) incl += x;
     }
-    if (lane == 63) s_sum[w] = incl;
+    if (lane == 63) s.sum[w] = incl;
     __syncthreads();
     int at = before + incl - c;
-    for (int j = 0; j < kEsThreads / 64; ++j) {
-      if (j < w) at += s_sum[j];
-      before += s_sum[j];
+    for (int j = 0; j < kEsWaves; ++j) {
+      if (j < w) at += s.sum[j];
+      before += s.sum[j];
     }
     if (i < rows) {
-      s_row[i] = at;
-      start[(size_t)i * parts + p] = at;
-      count[(size_t)i * parts + p] = c;
-    }
-    __syncthreads();
-  }
-  int found = 0;
-  // positions i0.. before i1 to their places by one wave, 64 at a time; next: a row's next place
-  auto place = [&](int i0, int i1, int* next) {
-    for (; i0 < i1; i0 += 64) {
-      const bool there = i0 + lane < i1;
-      const int row = there ? s_of[i0 + lane] : -1;
-      const int at = there ? s_at[i0 + lane] : 0;
-      // the lanes with this lane's row
-      unsigned long long same = wave_ballot(there);
-      if (wave_ballot(row == __shfl(row, 0, 64)) != ~0ull) {
-#pragma unroll
-        for (int b = 0; b < 13; ++b) {
-          const unsigned long long m = wave_ballot((row >> b) & 1);
-          same &= (row >> b) & 1 ? m : ~m;
-        }
-      }
-      if (there) {
-        const int to = next[row];
-        list[to + __popcll(same & lower)] = at;
-        if (!(same >> lane >> 1)) next[row] = to + __popcll(same);
-      }
-    }
-  };
-  // the positions found so far to their places
-  auto flush = [&]() {
-    __syncthreads();
-    if (found <= kEsFew || rows > kEsFine) {
-      if (w == 0) place(0, found, s_row);
-    } else {
-      // a share for each wave, in order: what the shares before it hold of a row comes first
-      const int share = (found + kEsThreads - 1) / kEsThreads * 64;
-      const int i0 = min(w * share, found), i1 = min(i0 + share, found);
-      for (int i = threadIdx.x; i < (kEsThreads / 64) * kEsFine; i += kEsThreads) s_next[0][i] = 0;
-      __syncthreads();
-      for (int i = i0 + lane; i < i1; i += 64) atomicAdd(&s_next[w][s_of[i]], 1);
-      __syncthreads();
-      if ((int)threadIdx.x < rows) {
-        int c[kEsThreads / 64], at = s_row[threadIdx.x];
-#pragma unroll
-        for (int k = 0; k < kEsThreads / 64; ++k) c[k] = s_next[k][threadIdx.x];
-#pragma unroll
-        for (int k = 0; k < kEsThreads / 64; ++k) {
-          s_next[k][threadIdx.x] = at;
-          at += c[k];
-        }
-        s_row[threadIdx.x] = at;
-      }
-      __syncthreads();
-      place(i0, i1, s_next[w]);
-    }
-    __syncthreads();
-    found = 0;
-  };
-  for (int t0 = 0; t0 < n; t0 += kEsTile) {
-    if (n > kEsTile) read(t0);
-    // where each position found goes: those of earlier runs of 64 tokens, then of earlier lanes
-    unsigned long long hit[kEsPer];
-#pragma unroll
-    for (int j = 0; j < kEsPer; ++j) {
-      hit[j] = wave_ballot(v[j] >= 0 && (v[j] & (parts - 1)) == p);
-      if (lane == 0) s_runs[j * (kEsThreads / 64) + w] = __popcll(hit[j]);
-    }
-    __syncthreads();
-    if (w == 0) {
-      constexpr int E = kEsRuns / 64;
-      int c[E], sum = 0;
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        c[e] = s_runs[lane * E + e];
-        sum += c[e];
-      }
-      int incl = sum;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const int x = __shfl_up(incl, o, 64);
-        if (lane >= o) incl += x;
-      }
-      if (lane == 63) s_runs[kEsRuns] = incl;
-      int at = incl - sum;
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        s_runs[lane * E + e] = at;
-        at += c[e];
+      s.row[i] = at + own;
+      if (write) {
+        start[(size_t)i * parts + p] = at;
+        count[(size_t)i * parts + p] = c;
       }
     }
     __syncthreads();
-    const int total = s_runs[kEsRuns];
-    // the tile's positions pass through the list in windows of its size
-    for (int win = 0; win < total; win += kEsList) {
-#pragma unroll
-      for (int j = 0; j < kEsPer; ++j) {
-        const int at = s_runs[j * (kEsThreads / 64) + w] + __popcll(hit[j] & lower) - win;
-        if ((hit[j] >> lane & 1) && at >= 0 && at < kEsList) {
-          s_at[at] = t0 + j * kEsThreads + threadIdx.x;
-          s_of[at] = (short)(v[j] >> shift);
-        }
-      }
-      found = min(total - win, kEsList);
-      flush();
-    }
-    __syncthreads();  // s_runs has been read
   }
 }
 
-// ---- the sums
+// Positions i0.. before i1 of s.at to their places by one wave, 64 at a time; next: a row's next place.
+__device__ __forceinline__ void es_place(const EsLds& s, int i0, int i1, int* next, int* __restrict__ list) {
+  const int lane = threadIdx.x & 63;
+  const unsigned long long lower = (1ull << lane) - 1;
+  for (; i0 < i1; i0 += 64) {
+    const bool there = i0 + lane < i1;
+    const int row = there ? s.of[i0 + lane] : -1;
+    const int at = there ? s.at[i0 + lane] : 0;
+    // the lanes with this lane's row
+    unsigned long long same = wave_ballot(there);
+    if (wave_ballot(row == __shfl(row, 0, 64)) != ~0ull) {
+#pragma unroll
+      for (int b = 0; b < 13; ++b) {
+        const unsigned long long m = wave_ballot((row >> b) & 1);
+        same &= (row >> b) & 1 ? m : ~m;
+      }
+    }
+    if (there) {
+      const int to = next[row];
+      list[to + __popcll(same & lower)] = at;
+      if (!(same >> lane >> 1)) next[row] = to + __popcll(same);
+    }
+  }
+}
+
+// The `found` positions of s.at to their places.
+__device__ __forceinline__ void es_flush(EsLds& s, int found, int rows, int* __restrict__ list) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  __syncthreads();
+  if (found <= kEsFew || rows > kEsFine) {
+    if (w == 0) es_place(s, 0, found, s.row, list);
+  } else {
+    // a share for each wave, in order: what the shares before it hold of a row comes first
+    const int share = (found + kEsThreads - 1) / kEsThreads * 64;
+    const int i0 = min(w * share, found), i1 = min(i0 + share, found);
+    for (int i = threadIdx.x; i < kEsWaves * kEsFine; i += kEsThreads) s.next[0][i] = 0;
+    __syncthreads();
+    for (int i = i0 + lane; i < i1; i += 64) atomicAdd(&s.next[w][s.of[i]], 1);
+    __syncthreads();
+    if ((int)threadIdx.x < rows) {
+      int c[kEsWaves], at = s.row[threadIdx.x];
+#pragma unroll
+      for (int k = 0; k < kEsWaves; ++k) c[k] = s.next[k][threadIdx.x];
+#pragma unroll
+      for (int k = 0; k < kEsWaves; ++k) {
+        s.next[k][threadIdx.x] = at;
+        at += c[k];
+      }
+      s.row[threadIdx.x] = at;
+    }
+    __syncthreads();
+    es_place(s, i0, i1, s.next[w], list);
+  }
+  __syncthreads();
+}
+
+// A tile's positions of part p to the list.
+__device__ __forceinline__ void es_put(EsLds& s, const int (&v)[kEsPer], int t0, int rows, int p, int parts,
+                                       int shift, int* __restrict__ list) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const unsigned long long lower = (1ull << lane) - 1;
+  // where each position found goes: behind those of earlier runs of 64 tokens, then of earlier lanes
+  unsigned long long hit[kEsPer];
+#pragma unroll
+  for (int j = 0; j < kEsPer; ++j) {
+    hit[j] = wave_ballot(v[j] >= 0 && (v[j] & (parts - 1)) == p);
+    if (lane == 0) s.runs[j * kEsWaves + w] = __popcll(hit[j]);
+  }
+  __syncthreads();
+  if (w == 0) {
+    constexpr int E = kEsRuns / 64;
+    int c[E], sum = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      c[e] = s.runs[lane * E + e];
+      sum += c[e];
+    }
+    int incl = sum;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int x = __shfl_up(incl, o, 64);
+      if (lane >= o) incl += x;
+    }
+    if (lane == 63) s.runs[kEsRuns] = incl;
+    int at = incl - sum;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      s.runs[lane * E + e] = at;
+      at += c[e];
+    }
+  }
+  __syncthreads();
+  const int total = s.runs[kEsRuns];
+  // the tile's positions pass through the list in windows of its size
+  for (int win = 0; win < total; win += kEsList) {
+#pragma unroll
+    for (int j = 0; j < kEsPer; ++j) {
+      const int at = s.runs[j * kEsWaves + w] + __popcll(hit[j] & lower) - win;
+      if ((hit[j] >> lane & 1) && at >= 0 && at < kEsList) {
+        s.at[at] = t0 + j * kEsThreads + threadIdx.x;
+        s.of[at] = (short)(v[j] >> shift);
+      }
+    }
+    es_flush(s, min(total - win, kEsList), rows, list);
+  }
+  __syncthreads();  // s.runs has been read
+}
+
+// n up to kEsTile.
+__global__ __launch_bounds__(kEsThreads) void k_embed_sort(const int64_t* __restrict__ tok, int n, int V,
+                                                           int64_t pad, int parts, int* __restrict__ start,
+                                                           int* __restrict__ count, int* __restrict__ list) {
+  __shared__ EsLds s;
+  const int p = blockIdx.x, rows = (V - p + parts - 1) / parts, shift = __builtin_ctz(parts);
+  int v[kEsPer];
+  for (int i = threadIdx.x; i < rows; i += kEsThreads) s.row[i] = 0;
+  __syncthreads();
+  es_read(v, tok, 0, n, V, pad);
+  int before = 0;
+#pragma unroll
+  for (int j = 0; j < kEsPer; ++j) {
+    const int part = v[j] & (parts - 1);
+    before += v[j] >= 0 && part < p;
+    if (v[j] >= 0 && part == p) atomicAdd(&s.row[v[j] >> shift], 1);
+  }
+  before = es_sum(s, before);
+  es_places(s, [&](int i, int&) { return s.row[i]; }, rows, before, p, parts, true, start, count);
+  es_put(s, v, 0, rows, p, parts, shift, list);
+}
+
+// cnt [splits, parts, rows of a part]: the tokens of each row in each split; all [splits, parts]: their sums.
+__global__ __launch_bounds__(kEsThreads) void k_embed_count(const int64_t* __restrict__ tok, int n, int V,
+                                                            int64_t pad, int parts, int per, int* __restrict__ cnt,
+                                                            int* __restrict__ all) {
+  __shared__ EsLds s;
+  const int p = blockIdx.x, rows = (V - p + parts - 1) / parts, shift = __builtin_ctz(parts);
+  const int most = (V + parts - 1) / parts, t1 = (int)min((int64_t)n, (int64_t)(blockIdx.y + 1) * per);
+  int v[kEsPer], mine = 0;
+  for (int i = threadIdx.x; i < rows; i += kEsThreads) s.row[i] = 0;
+  __syncthreads();
+  for (int64_t t0 = (int64_t)blockIdx.y * per; t0 < t1; t0 += kEsTile) {
+    es_read(v, tok, (int)t0, t1, V, pad);
+#pragma unroll
+    for (int j = 0; j < kEsPer; ++j)
+      if (v[j] >= 0 && (v[j] & (parts - 1)) == p) {
+        atomicAdd(&s.row[v[j] >> shift], 1);
+        ++mine;
+      }
+  }
+  mine = es_sum(s, mine);
+  const size_t place = (size_t)blockIdx.y * parts + p;
+  if (threadIdx.x == 0) all[place] = mine;
+  for (int i = threadIdx.x; i < rows; i += kEsThreads) cnt[place * most + i] = s.row[i];
+}
+
+__global__ __launch_bounds__(kEsThreads) void k_embed_place(const int64_t* __restrict__ tok, int n, int V,
+                                                            int64_t pad, int parts, int per,
+                                                            const int* __restrict__ cnt, const int* __restrict__ all,
+                                                            int* __restrict__ start, int* __restrict__ count,
+                                                            int* __restrict__ list) {
+  __shared__ EsLds s;
+  const int p = blockIdx.x, rows = (V - p + parts - 1) / parts, shift = __builtin_ctz(parts);
+  const int most = (V + parts - 1) / parts, splits = gridDim.y, split = blockIdx.y;
+  const int t1 = (int)min((int64_t)n, (int64_t)(split + 1) * per);
+  int before = 0;
+  for (int i = threadIdx.x; i < splits * parts; i += kEsThreads)
+    if ((i & (parts - 1)) < p) before += all[i];
+  before = es_sum(s, before);
+  auto get = [&](int i, int& own) {
+    int c = 0;
+    for (int k0 = 0; k0 < splits; k0 += 8) {
+      int x[8];  // the loads first
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[k] = cnt[((size_t)min(k0 + k, splits - 1) * parts + p) * most + i];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        x[k] = k0 + k < splits ? x[k] : 0;
+        c += x[k];
+        own += k0 + k < split ? x[k] : 0;
+      }
+    }
+    return c;
+  };
+  es_places(s, get, rows, before, p, parts, split == 0, start, count);
+  for (int64_t t0 = (int64_t)split * per; t0 < t1; t0 += kEsTile) {
+    int v[kEsPer];
+    es_read(v, tok, (int)t0, t1, V, pad);
+    es_put(s, v, (int)t0, rows, p, parts, shift, list);
+  }
+}
+
 // A workgroup takes a block of kEbLanes*16 bytes of columns; a table row is taken by `lanes` lanes of a
 // wave, 16 bytes a lane, so a wave takes 4 rows or more at once.  Up to kEbFew positions are summed by the
 // row's own lanes; longer rows are dealt to the workgroup's waves, up to kEbHot positions to one (its lane
@@ -410,8 +511,8 @@ extern "C" int lsh_embed_fwd(int dtype, const int64_t* tokens, const void* weigh
 
 extern "C" size_t lsh_embed_bwd_workspace(int64_t n, int64_t V) {
   if (embed_check(LSH_F32, n, V, 1)) return 0;
-  const size_t rows = align_up((size_t)V, es_parts(V));
-  return (2 * rows + (size_t)n) * sizeof(int);
+  const EsDeal d = es_deal(n, V);
+  return (size_t)(2 * d.rows + n + d.splits * (d.rows + d.parts)) * sizeof(int);
 }
 
 extern "C" int lsh_embed_bwd(int dtype, const int64_t* tokens, const void* dout, void* dweight, int64_t n,
@@ -422,11 +523,20 @@ extern "C" int lsh_embed_bwd(int dtype, const int64_t* tokens, const void* dout,
   if (bad_ptr(dweight) || (n > 0 && (bad_ptr(tokens) || bad_ptr(dout)))) return LSH_ERR_ARG;
   if (bad_ptr(ws) || ws_bytes < lsh_embed_bwd_workspace(n, V)) return LSH_ERR_WORKSPACE;
   hipStream_t st = (hipStream_t)stream;
-  const int parts = es_parts(V);
-  const size_t rows = align_up((size_t)V, parts);
-  int *start = (int*)ws, *count = start + rows, *list = count + rows;
-  k_embed_sort<<<dim3((unsigned)parts), kEsThreads, 0, st>>>(tokens, (int)n, (int)V, padding, parts, start,
-                                                            count, list);
+  const EsDeal d = es_deal(n, V);
+  int *start = (int*)ws, *count = start + d.rows, *list = count + d.rows;
+  if (d.splits == 0) {
+    k_embed_sort<<<dim3((unsigned)d.parts), kEsThreads, 0, st>>>(tokens, (int)n, (int)V, padding, d.parts, start,
+                                                                count, list);
+  } else {
+    const int share = (int)((n + d.splits - 1) / d.splits);
+    const dim3 grid((unsigned)d.parts, (unsigned)d.splits);
+    int *all = list + n, *cnt = all + (size_t)d.splits * d.parts;
+    k_embed_count<<<grid, kEsThreads, 0, st>>>(tokens, (int)n, (int)V, padding, d.parts, share, cnt, all);
+    LSH_CHECK_LAUNCH();
+    k_embed_place<<<grid, kEsThreads, 0, st>>>(tokens, (int)n, (int)V, padding, d.parts, share, cnt, all, start,
+                                              count, list);
+  }
   LSH_CHECK_LAUNCH();
   const int per = 16 / lm_dtype_size(dtype);
   int lanes = 1;

@@ -268,6 +268,13 @@ def test_embed_many_tokens_of_a_large_table(dev, kind):
     test_embed(dev, torch.float32, kind, 6000, 200000, 8)
 
 
+@pytest.mark.parametrize("kind", ["zipf", "uniform", "one", "ordered"])
+@pytest.mark.parametrize("n,V,D", [(16385, 1, 1), (40000, 5, 3), (33333, 32000, 4), (70001, 200000, 2)])
+def test_embed_many_tokens(dev, kind, n, V, D):
+    """More tokens than one kernel sorts: split over the workgroups, with tables of few and of many rows."""
+    test_embed(dev, torch.bfloat16 if kind == "zipf" else torch.float32, kind, n, V, D)
+
+
 def test_embed_ids_outside_the_table(dev):
     """Ids below 0 and from V on read as zero rows and leave no gradient; also those that 32 bits fold."""
     from lifscan import hip_lm as LM
