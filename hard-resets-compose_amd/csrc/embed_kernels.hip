@@ -326,9 +326,11 @@ __global__ __launch_bounds__(kEsThreads) void k_embed_place(const int64_t* __res
 // row's own lanes; longer rows are dealt to the workgroup's waves, up to kEbHot positions to one (its lane
 // groups take positions in turn), more to all, always joined in a fixed order.  Neighbouring rows, which
 // are often frequent together, go to different workgroups.
-// Bound by the rows read and written (16384 tokens, 32000 x 1024 bf16: 97 MB, 26 us) and, with a Zipf text,
-// by the chain of dependent loads of its longest rows.  8 waves and 4 groups a wave measured best: with
-// the sort 40 us; 16 waves took 8 us more, 4 waves 6.  Rows of 1023 columns, element by element: 65 us.
+// Bound by the rows read and written (16384 tokens, 32000 x 1024 bf16: 97 MB, 26 us; 262144 uniform tokens 600
+// MB, 156 us) and, with a Zipf text, by its most frequent token, whose rows one workgroup sums for a block of
+// columns (262144 tokens: 213 us).  8 waves and 4 groups a wave measured best: with the sort 40 us; 16 waves
+// took 8 us more, 4 waves 6.  Blocks of 512 and 1024 bytes take 31 and 30 us with uniform tokens where 256
+// take 33, but 41 and 48 with Zipf's where 256 take 39.  Rows of 1023 columns, element by element: 65 us.
 constexpr int kEbThreads = 512, kEbLanes = 16, kEbFew = 4, kEbHot = 256, kEbGroups = 32;
 
 // The sum of dout's rows at list[begin .. begin + n) in columns d.., dealt to `groups` lane groups, this
