@@ -41,7 +41,7 @@ struct LaWalk {
 
 // Walks of one size class that do not wait for each other.  Neighbouring workgroups take the n walks of a
 // segment, which read some of the same operands and find them in the caches (bf16 4096 x 4 x 16 x 128: the
-// three gradient walks 177 us and 23% fewer bytes from memory than one walk after the other, 184 us).
+// three gradient walks with 4% less time and 23% fewer bytes from memory than one walk after the other).
 struct LaWalks {
   LaWalk w[3];
   int n;
@@ -60,9 +60,10 @@ using s16x4 = short __attribute__((ext_vector_type(4)));
 //
 // 16 bits: products of the type, fp32 sums.  A decayed value is taken in as many parts as hold the 24
 // bits of fp32 (bf16 three, fp16 two), so the state is kept to fp32; a score and the state that meets q
-// are rounded to the type once.  SCALED (fp16): what is rounded is first scaled by a power of two that
-// brings its largest value below 2^15, since scores, states and decayed values can leave fp16's range,
-// or sink below its normal numbers, where the results do not.
+// are taken in two parts (16 bits and more), so that the result's own rounding is nearly all of its error.
+// SCALED (fp16): what is split is first scaled by a power of two that brings its largest value below 2^15,
+// since scores, states and decayed values can leave fp16's range, or sink below its normal numbers, where
+// the results do not.
 // fp32: the fp32 matrix instruction, exact products.
 template <class L>
 struct La;
@@ -89,30 +90,45 @@ struct La16 {
     const F4 b = __builtin_bit_cast(F4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(at + 16 * pitch)));
     return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
   }
-  static __device__ __forceinline__ Frag of(const f32x4* acc, float scale) {
-    Frag f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = (L)(acc[e >> 2][e & 3] * scale);
-    return f;
-  }
   static __device__ __forceinline__ int at(int e) { return (e >> 2) * 16 + (e & 3); }  // + 4g
 };
 
 template <>
 struct La<bf16_t> : La16<bf16_t, bf16x4, bf16x8> {
-  static constexpr int PARTS = 3;
+  static constexpr int PARTS = 3, FINE = 2;
   static constexpr bool SCALED = false;
   static __device__ __forceinline__ f32x4 mma(Frag a, Frag b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+  // an accumulator's values as two fragments: the upper halves of the words, and what they leave
+  static __device__ __forceinline__ void of(const f32x4* acc, float, Frag (&f)[2]) {
+    unsigned top[4];
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      const float x = acc[e >> 2][e & 3], y = acc[e >> 2][(e & 3) + 1];
+      const unsigned a = __builtin_bit_cast(unsigned, x), b = __builtin_bit_cast(unsigned, y);
+      top[e / 2] = __builtin_amdgcn_perm(b, a, 0x07060302);
+      f[1][e] = (bf16_t)(x - __builtin_bit_cast(float, a & 0xffff0000u));
+      f[1][e + 1] = (bf16_t)(y - __builtin_bit_cast(float, b & 0xffff0000u));
+    }
+    f[0] = __builtin_bit_cast(Frag, top);
   }
 };
 
 template <>
 struct La<f16_t> : La16<f16_t, f16x4, f16x8> {
-  static constexpr int PARTS = 2;
+  static constexpr int PARTS = 2, FINE = 2;
   static constexpr bool SCALED = true;
   static __device__ __forceinline__ f32x4 mma(Frag a, Frag b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ void of(const f32x4* acc, float scale, Frag (&f)[2]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float x = acc[e >> 2][e & 3] * scale;
+      f[0][e] = (f16_t)x;
+      f[1][e] = (f16_t)(x - (float)f[0][e]);
+    }
   }
   // the same over half a fragment: rows 16*half.. of the 32
   static __device__ __forceinline__ f32x4 mma_half(Frag a, Frag b, int half, f32x4 c) {
@@ -151,7 +167,7 @@ __device__ __forceinline__ LaScale la_scale(unsigned t) {
 
 template <>
 struct La<float> {
-  static constexpr int KB = 16, C = 32, TILES = 1, PARTS = 1;
+  static constexpr int KB = 16, C = 32, TILES = 1, PARTS = 1, FINE = 1;
   static constexpr bool SCALED = false;
   using Frag = f32x4;
   using Quad = f32x4;
@@ -170,7 +186,7 @@ struct La<float> {
     for (int e = 0; e < 4; ++e) f[e] = p[(4 * g + e) * pitch + m];
     return f;
   }
-  static __device__ __forceinline__ Frag of(const f32x4* acc, float) { return acc[0]; }
+  static __device__ __forceinline__ void of(const f32x4* acc, float, Frag (&f)[1]) { f[0] = acc[0]; }
   static __device__ __forceinline__ int at(int e) { return e; }
 };
 
@@ -263,7 +279,7 @@ __device__ __forceinline__ u32x4 la_shift(u32x4 x, int n) {
 // 16 bits: a piece that would leave the row ends with it, and is shifted into place on its way to LDS (rows
 // shorter than a piece are read element by element).  32 bits: element by element, a thread's columns
 // PER_ROW apart, so that neighbouring lanes read neighbours.
-// 4096 x 4 x 16 x 127 x 127 forward: bf16 165 us, element by element 262 (128 columns 125); fp32 324 us, in
+// 4096 x 4 x 16 x 127 x 127 forward: bf16 171 us, element by element 268 (128 columns 132); fp32 322 us, in
 // pieces 428 (128 columns 300).
 template <class T, class L, int C, int DP, int THREADS, bool PACKED>
 struct LaStage<T, L, C, DP, THREADS, PACKED, false> {
@@ -402,9 +418,11 @@ constexpr int la_waves(int size, int DKP, int W) {
 // the 8 rows of 32 bytes that the transposing read takes at once, meet different banks.  Where rows are read
 // 4 dwords gave twice the conflicts (3.2 -> 6.0 million cycles of the forward walk below) and 1% of time.
 //
-// Bound by the bytes: bf16, 4096 x 4 x 16 x 128, forward 69 us for 302 MB with the states (4.4 TB/s; 4.9
-// without the 8 us in which the first chunk and state arrive), the gradients' three walks 177 us for 905 MB;
-// of a SIMD's cycles 37% issue vector instructions and 23% keep the matrix unit busy.
+// Bound by the bytes and by the latency of a chunk's steps between its barriers: bf16, 4096 x 4 x 16 x 128,
+// forward 75 us for 302 MB with the states (4.0 TB/s; 8 us pass until the first chunk and state arrive), the
+// gradients' three walks 190 us for 905 MB; with one part for scores and the state that meets q 69 and 170 us,
+// and 1.4 to 1.5 times the error.  Of a SIMD's cycles some 40% issue vector instructions and 30% keep the
+// matrix unit busy.
 template <class T, class L, int DKP, int W, bool SUMS, bool WIDE>
 __global__ __launch_bounds__(W * 64, la_waves(sizeof(L), DKP, W)) void k_la_walk(LaWalks all) {
   const int64_t turn = xcd_neuron(blockIdx.x, gridDim.x), job = turn / all.n;
@@ -416,7 +434,7 @@ __global__ __launch_bounds__(W * 64, la_waves(sizeof(L), DKP, W)) void k_la_walk
   constexpr int PQ = DKP + X::kPadRow, PK = DKP + X::kPadCol, PV = DVB + X::kPadCol, PP = C + X::kPadRow;
   // of each two halves: one is filled while the other is read
   __shared__ alignas(16) L s_q[SUMS ? 8 : 2 * C * PQ], s_k[2 * C * PK], s_v[2 * C * PV];
-  __shared__ alignas(16) L s_p[SUMS ? 8 : C * PP];
+  __shared__ alignas(16) L s_p[X::FINE][SUMS ? 8 : C * PP];
   __shared__ float s_from[W];  // SCALED: what takes each tile of the scores back
 
   const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
@@ -456,7 +474,7 @@ __global__ __launch_bounds__(W * 64, la_waves(sizeof(L), DKP, W)) void k_la_walk
   // the state is sigma*S: most chunks decay it by sigma alone, and weigh what they add by 1/sigma
   float sigma = 1.0f;
   if (!SUMS) {
-    for (int i = threadIdx.x; i < C * PP; i += W * 64) s_p[i] = (L)0.0f;  // tiles above the diagonal stay so
+    for (int i = threadIdx.x; i < X::FINE * C * PP; i += W * 64) s_p[0][i] = (L)0.0f;  // tiles above the diagonal stay so
   }
 
   // row r of the walk is row (rev ? T - 1 - r : r); the first chunk is the short one
@@ -531,8 +549,14 @@ __global__ __launch_bounds__(W * 64, la_waves(sizeof(L), DKP, W)) void k_la_walk
           if (lane == 0) s_from[w] = c.from;
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = (L)p[e];
-        *(typename X::Quad*)&s_p[(ti * 16 + m) * PP + X::packed(tj * 16 + 4 * g)] = y;
+        for (int c = 0; c < X::FINE; ++c) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            y[e] = (L)p[e];
+            p[e] -= (float)y[e];
+          }
+          *(typename X::Quad*)&s_p[c][(ti * 16 + m) * PP + X::packed(tj * 16 + 4 * g)] = y;
+        }
       }
       // what the state before the chunk gives
       f32x4 o[CT];
@@ -549,9 +573,14 @@ __global__ __launch_bounds__(W * 64, la_waves(sizeof(L), DKP, W)) void k_la_walk
       }
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
-        const Frag st = X::of(&S[s * X::TILES], in.to);
+        Frag st[X::FINE];
+        X::of(&S[s * X::TILES], in.to, st);
 #pragma unroll
-        for (int i = 0; i < CT; ++i) o[i] = X::mma(st, X::packed_row(&cq[(i * 16 + m) * PQ + s * KB], g), o[i]);
+        for (int i = 0; i < CT; ++i) {
+          const Frag y = X::packed_row(&cq[(i * 16 + m) * PQ + s * KB], g);
+#pragma unroll
+          for (int c = 0; c < X::FINE; ++c) o[i] = X::mma(st[c], y, o[i]);
+        }
       }
       const int first = C - n - m;  // a lane's rows of the chunk are those with 16i >= first
 #pragma unroll
@@ -569,7 +598,9 @@ __global__ __launch_bounds__(W * 64, la_waves(sizeof(L), DKP, W)) void k_la_walk
           const typename X::Quad y = *(const typename X::Quad*)&cv[j * PV + wc + 4 * g];
 #pragma unroll
           for (int i = 0; i < CT; ++i) {
-            float p = (float)s_p[(i * 16 + m) * PP + X::packed(j & ~3) + (j & 3)];
+            float p = 0.0f;
+#pragma unroll
+            for (int c = 0; c < X::FINE; ++c) p += (float)s_p[c][(i * 16 + m) * PP + X::packed(j & ~3) + (j & 3)];
             if constexpr (X::SCALED) p *= s_from[i * (i + 1) / 2 + min(j / 16, i)];
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[i][e] += i * 16 + m >= j ? p * (float)y[e] : 0.0f;
@@ -581,14 +612,21 @@ __global__ __launch_bounds__(W * 64, la_waves(sizeof(L), DKP, W)) void k_la_walk
 #pragma unroll
           for (int i = 0; i < CT; ++i) {
             if (s * X::TILES > i) continue;
-            const Frag p = X::packed_row(&s_p[(i * 16 + m) * PP + s * KB], g);
+            Frag p[X::FINE];
+#pragma unroll
+            for (int c = 0; c < X::FINE; ++c) p[c] = X::packed_row(&s_p[c][(i * 16 + m) * PP + s * KB], g);
             if constexpr (X::SCALED) {  // each 16 rows' scores have a scale of their own
 #pragma unroll
               for (int j = 0; j < 2; ++j)
-                if (s * 2 + j <= i)
-                  o[i] += X::mma_half(x[s], p, j, f32x4{0.0f, 0.0f, 0.0f, 0.0f}) * s_from[i * (i + 1) / 2 + s * 2 + j];
+                if (s * 2 + j <= i) {
+                  f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                  for (int c = 0; c < X::FINE; ++c) sum = X::mma_half(x[s], p[c], j, sum);
+                  o[i] += sum * s_from[i * (i + 1) / 2 + s * 2 + j];
+                }
             } else {
-              o[i] = X::mma(x[s], p, o[i]);
+#pragma unroll
+              for (int c = 0; c < X::FINE; ++c) o[i] = X::mma(x[s], p[c], o[i]);
             }
           }
       }

@@ -356,6 +356,22 @@ def test_values_that_are_not_finite_stay_in_their_rows(dev):
         assert int((~torch.isfinite(s)).sum()) == 64
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("T,Dk,Dv", [(5, 64, 64), (300, 64, 128), (97, 33, 20)])
+def test_the_error_is_that_of_one_rounding(dev, dtype, T, Dk, Dv):
+    """Scores and states enter the products with 16 bits and more (2^-16 of each term, the result is rounded to
+    2^-9 or 2^-12 of itself), so the error's norm is that of rounding the exact results, within a tenth."""
+    args = _inputs(dtype, T, 2, (3, 3, 3), 3, Dk, Dv, dev, seed=51)
+    q, k, v, beta, s0, do, ds = args
+    got = run_all(q, k, v, beta, s0, Dk ** -0.5, do, ds)
+    want = reference(q, k, v, beta, s0, Dk ** -0.5, do, ds)
+    for x, w in zip(got, want):
+        if x.dtype == dtype:
+            once = float((w.to(dtype).double() - w).norm())
+            err = float((x.detach().double().cpu() - w).norm())
+            assert err <= 1.1 * once, (err, once)
+
+
 @pytest.mark.parametrize("qk,vv", [(1e4, 1.0), (1e-3, 1.0), (1.0, 3000.0), (1.0, 2.0 ** -12)])
 def test_fp16_beyond_its_range_on_the_way(dev, qk, vv):
     """Scores and states that fp16 cannot hold, or only among its smallest numbers, between operands and
