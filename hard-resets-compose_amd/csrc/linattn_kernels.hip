@@ -46,17 +46,23 @@ __global__ __launch_bounds__(256) void k_la_join(float* __restrict__ starts, con
   }
 }
 
-// Gradients of a shared head: the sum over the heads that share it, in fp32 and head order, from
-// the walk's fp32 [rows, H, D] to [rows, H/share, D].
+// Gradients of shared heads: the sums over the heads that share one, in fp32 and head order, from the
+// walks' fp32 [rows, H, D] to [rows, H/share, D].  Workgroups (., i) take operand i.
+struct LaShares {
+  const float* x[3];
+  void* y[3];
+  int64_t n[3];
+  int D[3], share[3];
+};
 template <class T>
-__global__ __launch_bounds__(256) void k_la_share(const float* __restrict__ x, T* __restrict__ y,
-                                                  int64_t n, int D, int share) {
+__global__ __launch_bounds__(256) void k_la_share(LaShares a) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= n) return;
-  const float* p = x + (i / D) * share * D + i % D;
+  const int j = blockIdx.y, D = a.D[j], share = a.share[j];
+  if (i >= a.n[j]) return;
+  const float* p = a.x[j] + (i / D) * share * D + i % D;
   float s = 0.0f;
-  for (int j = 0; j < share; ++j) s += p[(int64_t)j * D];
-  y[i] = from_f<T>(s);
+  for (int k = 0; k < share; ++k) s += p[(int64_t)k * D];
+  ((T*)a.y[j])[i] = from_f<T>(s);
 }
 
 static int la_go(const LaWalks& all, int dtype, bool sums, hipStream_t st) {
@@ -310,14 +316,19 @@ extern "C" int lsh_linattn_bwd(const lsh_linattn* a, const void* starts, const v
   if (int rc = la_go(all, a->dtype, false, st)) return rc;
   if (!alike)
     if (int rc = la_go(w_v, a->dtype, false, st)) return rc;
+  LaShares shares = {};
+  int count = 0;
+  int64_t most = 0;
   for (const Out& o : outs) {
-    if (!o.f32 || a->T == 0) continue;
+    if (!o.f32) continue;
     const int64_t n = a->T * a->B * o.heads * o.D;
-    with_dtype(a->dtype, [&](auto t) {
-      using T = decltype(t);
-      k_la_share<T><<<dim3((unsigned)((n + 255) / 256)), 256, 0, st>>>(o.f32, (T*)o.to, n, o.D,
-                                                                      (int)(a->H / o.heads));
-    });
+    shares.x[count] = o.f32, shares.y[count] = o.to, shares.n[count] = n;
+    shares.D[count] = o.D, shares.share[count++] = (int)(a->H / o.heads);
+    most = most > n ? most : n;
+  }
+  if (most > 0) {
+    const dim3 grid((unsigned)((most + 255) / 256), (unsigned)count);
+    with_dtype(a->dtype, [&](auto t) { k_la_share<decltype(t)><<<grid, 256, 0, st>>>(shares); });
     LSH_CHECK_LAUNCH();
   }
   return LSH_OK;
