@@ -13,7 +13,7 @@
 //   dw_pre = sum gz*x_new*rx,  dw_post = sum dn*y*ry,  da = sum dx*h      over the rows
 // Bound by the rows' bytes; x_new is computed again instead of being kept.  bf16, 8192 x 2048: forward
 // 26.6 us for 168 MB (6.3 TB/s, part of it from the Infinity Cache), gradients 48 us for 268 MB
-// (5.6 TB/s) and 7 for the parameters' sums; with an fp32 stream 35 and 75, all fp32 62 and 106.  Rows
+// (5.6 TB/s) and 4.4 for the parameters' sums; with an fp32 stream 35 and 75, all fp32 62 and 106.  Rows
 // that cannot be read in pieces go element by element: 8190 x 2047 forward 28, gradients 63.
 #include <type_traits>
 
@@ -359,13 +359,15 @@ __global__ __launch_bounds__(W * 64) void k_block_norm_bwd(BnArgs a) {
   }
 }
 
-// dw_post, dw_pre and da: the workgroups' sums, 16 runs of workgroups at once and then in run order.
-__global__ __launch_bounds__(256) void k_block_norm_sums(const float* __restrict__ part, int P, int D,
-                                                         float* dw_post, float* dw_pre, float* da) {
-  __shared__ float s_run[16][16];
-  const int c = threadIdx.x & 15, run = threadIdx.x >> 4;
-  const int i = blockIdx.x * 16 + c;
-  const int per = (P + 15) / 16, p1 = min(P, (run + 1) * per);
+// dw_post, dw_pre and da: the workgroups' sums, kBnRuns runs of workgroups at once and then in run order.
+// 768 workgroups' sums of 2048 channels (19 MB): 4.4 us, with 16 columns and 16 runs a workgroup 7.2.
+constexpr int kBnCols = 32, kBnRuns = 32;
+__global__ __launch_bounds__(kBnCols* kBnRuns) void k_block_norm_sums(const float* __restrict__ part, int P, int D,
+                                                                     float* dw_post, float* dw_pre, float* da) {
+  __shared__ float s_run[kBnRuns][kBnCols];
+  const int c = threadIdx.x % kBnCols, run = threadIdx.x / kBnCols;
+  const int i = blockIdx.x * kBnCols + c;
+  const int per = (P + kBnRuns - 1) / kBnRuns, p1 = min(P, (run + 1) * per);
   float s = 0.0f;
   if (i < 3 * D)
 #pragma unroll 8
@@ -377,7 +379,7 @@ __global__ __launch_bounds__(256) void k_block_norm_sums(const float* __restrict
   if (!out) return;
   s = 0.0f;
 #pragma unroll
-  for (int r = 0; r < 16; ++r) s += s_run[r][c];
+  for (int r = 0; r < kBnRuns; ++r) s += s_run[r][c];
   out[i % D] = s;
 }
 
@@ -555,8 +557,8 @@ extern "C" int lsh_block_norm_bwd(const lsh_block_norm* p, const void* gx, const
     });
     LSH_CHECK_LAUNCH();
   }
-  k_block_norm_sums<<<dim3((3 * p->D + 15) / 16), 256, 0, st>>>((const float*)ws, (int)grid, p->D, dw_post,
-                                                              dw_pre, dscale);
+  k_block_norm_sums<<<dim3((3 * p->D + kBnCols - 1) / kBnCols), kBnCols * kBnRuns, 0, st>>>(
+      (const float*)ws, (int)grid, p->D, dw_post, dw_pre, dscale);
   LSH_CHECK_LAUNCH();
   return LSH_OK;
 }
