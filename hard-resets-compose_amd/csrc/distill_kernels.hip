@@ -169,15 +169,17 @@ __global__ __launch_bounds__(kDsThreads) void k_distill(DsArgs a) {
   }
 }
 
-// The parts of a row joined, one wave a row.
+// The parts of a row joined, one wave a row and one lane a part (48 rows of 21 parts: 3.7 us, one part after the
+// other 5.5).
+constexpr int kDsParts = 64;
 template <class T>
 __global__ __launch_bounds__(64) void k_distill_join(DsArgs a) {
   const int64_t row = blockIdx.x;
-  float m = -INFINITY, s = 0.0f;
-  for (int i = 0; i < a.splits; ++i) {
-    const float* p = a.part + (row * a.splits + i) * 2;
-    ds_join(m, s, p[0], p[1], a.c);
-  }
+  const int i = threadIdx.x;
+  const float* p = a.part + (row * a.splits + min(i, a.splits - 1)) * 2;
+  float m = i < a.splits ? p[0] : -INFINITY, s = i < a.splits ? p[1] : 0.0f;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) ds_join(m, s, __shfl_xor(m, o, 64), __shfl_xor(s, o, 64), a.c);
   ds_loss<T>(a, row, m, __builtin_amdgcn_logf(s));
 }
 
@@ -269,7 +271,7 @@ static int ds_check(int dtype, int v_dtype, int64_t rows, int64_t V, int K, floa
 
 // Parts of a row: about 1024 workgroups, none of less than 4096 logits.
 static int ds_splits(int64_t rows, int64_t V) {
-  const int64_t most = std::min<int64_t>((V + 4095) / 4096, 64);
+  const int64_t most = std::min<int64_t>((V + 4095) / 4096, kDsParts);
   return (int)std::max<int64_t>(1, std::min(most, 1024 / std::max<int64_t>(rows, 1)));
 }
 
