@@ -79,7 +79,8 @@ __device__ __forceinline__ void ds_loss(const DsArgs& a, int64_t row, float zm, 
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) ds_join(m, s, __shfl_xor(m, o, 64), __shfl_xor(s, o, 64), a.c);
-  const bool some = s != 0.0f && m != -INFINITY;  // a NaN counts
+  if (s != s) m = s;  // a NaN is an entry: it reaches the loss, also where it is the only one
+  const bool some = s != 0.0f && m != -INFINITY;
   const float tl = __builtin_amdgcn_logf(s);
   float sum = 0.0f;
   for (int k = lane; k < a.K && some; k += 64) {

@@ -546,3 +546,30 @@ def test_row_operators_in_a_graph(dev):
             assert torch.equal(a, b)
         work()
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", list(U), ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("V", [300, 9001])
+def test_distill_teacher_values_that_are_nan(dev, dtype, V):
+    """A NaN among a row's teacher values is an entry, also where every other one is NaN or -inf: the row's loss
+    is NaN, its gradient NaN at the entries' places, and other rows are as without it."""
+    from lifscan import hip_lm as LM
+    z, t, idx, g = _distill_inputs(5, V, 8, dtype, dev, seed=11)
+    idx[:] = torch.arange(8, device=dev) * 7
+    loss, dz = distill_check(z, t, idx, 2.0, g, V)
+    bad = t.clone()
+    bad[1] = float("nan")
+    bad[2, 0] = float("nan")
+    bad[3] = float("-inf")
+    bad[3, 5] = float("nan")
+    zg = z.clone().requires_grad_(True)
+    got = LM.distill_topk(zg, bad, idx, temperature=2.0)
+    (dbad,) = torch.autograd.grad(got, zg, g)
+    assert got.isnan().tolist() == [False, True, True, True, False]
+    for row in (0, 4):
+        assert got[row] == loss[row].detach() and torch.equal(dbad[row], dz[row])
+    for row in (1, 2, 3):
+        assert bool(dbad[row, idx[row]].isnan().all())
+        other = torch.ones(V, dtype=torch.bool, device=dev)
+        other[idx[row]] = False
+        assert bool(dbad[row, other].isfinite().all())
