@@ -268,6 +268,8 @@ Tensor lin_attn_step(const Tensor& q, const Tensor& k, const Tensor& v, const Te
   const Tensor o = torch::empty({r.a.B, r.a.H, r.a.Dv}, r.q.options());
   r.a.o = o.data_ptr();
   check(g.lsh_linattn_step(&r.a, fp(state), stream_of(r.q)), "lsh_linattn_step");
+  // a graph that has saved the state from before is told, as by torch's own in-place operations
+  if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();
   return o;
 }
 

@@ -466,3 +466,16 @@ def test_refusals(dev):
         with pytest.raises(ValueError):
             f()
             print("not refused:", i)
+
+
+def test_a_state_changed_in_place_is_noticed(dev):
+    """A graph that has saved a state must not take its gradients from the state after another token."""
+    from lifscan import hip_linattn as LA
+    q, k, v, beta, s0, _, _ = _inputs(torch.float32, 40, 1, (2, 2, 2), 2, 16, 16, dev, seed=31)
+    o, _ = LA.lin_attn(q.requires_grad_(True), k, v, beta, s0=s0)
+    with torch.no_grad():
+        LA.lin_attn_step(q[0], k[0], v[0], beta, s0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        o.sum().backward()
+    with torch.inference_mode():  # such tensors count no versions
+        LA.lin_attn_step(q[0], k[0], v[0], beta, s0.clone())
