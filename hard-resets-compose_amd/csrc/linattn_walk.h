@@ -195,9 +195,10 @@ __device__ __forceinline__ const T* la_row(const LaIn& x, int64_t b, int64_t h) 
   return (const T*)x.p + b * x.sb + (h / x.share) * x.sh;
 }
 
-// 2^(n * log2 beta); l2 is finite (la_log2), so beta = 0 gives 1 for n = 0 and 0 beyond
+// 2^(n * log2 beta); l2 is finite (la_log2), so beta = 0 gives 1 for n = 0 and 0 beyond.  What is no decay
+// (below 0, or NaN) gives NaN.
 __device__ __forceinline__ float la_pow(float l2, int n) { return __builtin_amdgcn_exp2f(l2 * (float)n); }
-__device__ __forceinline__ float la_log2(float beta) { return fmaxf(log2f(beta), -1e4f); }
+__device__ __forceinline__ float la_log2(float beta) { return beta >= 0.0f ? fmaxf(log2f(beta), -1e4f) : NAN; }
 
 using u32x2 = unsigned __attribute__((ext_vector_type(2)));
 using u32x4 = unsigned __attribute__((ext_vector_type(4)));

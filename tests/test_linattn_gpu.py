@@ -479,3 +479,20 @@ def test_a_state_changed_in_place_is_noticed(dev):
         o.sum().backward()
     with torch.inference_mode():  # such tensors count no versions
         LA.lin_attn_step(q[0], k[0], v[0], beta, s0.clone())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("beta", [-0.5, float("nan")])
+def test_what_is_no_decay_gives_nan(dev, dtype, beta):
+    """A decay below zero, or NaN, on the device: its head's results are NaN, the other heads' as they are."""
+    T, H = 70, 3
+    q, k, v, b, s0, do, ds = _inputs(dtype, T, 2, (H,) * 3, H, 32, 48, dev, seed=37)
+    want = run_all(q, k, v, b, s0, 0.3, do, ds)
+    b = b.clone()
+    b[1] = beta
+    got = run_all(q, k, v, b, s0, 0.3, do, ds)
+    for i, (x, w) in enumerate(zip(got, want)):
+        heads = 1 if i in (1, 5) else 2  # states [B, H, ...], the others [T, B, H, ...]
+        assert bool(x.select(heads, 1).isnan().all())
+        for h in (0, 2):
+            assert torch.equal(x.select(heads, h), w.select(heads, h))
