@@ -503,6 +503,7 @@ extern "C" int lsh_block_norm_fwd(const lsh_block_norm* p, void* x_new, void* z,
   BnArgs a = bn_args(p);
   a.x_new = x_new, a.z = z;
   const bool wide = bn_wide(a);
+  bool fits = true;
   with_types(p->x_dtype, p->dtype, [&](auto tx, auto ty) {
     with_row<false, true>(p->D, [&](auto, auto w, auto e) {
       using TX = decltype(tx);
@@ -510,12 +511,15 @@ extern "C" int lsh_block_norm_fwd(const lsh_block_norm* p, void* x_new, void* z,
       constexpr int W = decltype(w)::value, E = decltype(e)::value;
       const dim3 grid((unsigned)(W == 1 ? (p->rows + 3) / 4 : p->rows));
       const int threads = W == 1 ? 256 : W * 64;
+      fits = lm_grid_ok(grid.x, threads);
+      if (!fits) return;
       if (wide)
         k_block_norm<TX, TY, W, E, true><<<grid, threads, 0, (hipStream_t)stream>>>(a);
       else
         k_block_norm<TX, TY, W, E, false><<<grid, threads, 0, (hipStream_t)stream>>>(a);
     });
   });
+  if (!fits) return LSH_ERR_SHAPE;
   LSH_CHECK_LAUNCH();
   return LSH_OK;
 }

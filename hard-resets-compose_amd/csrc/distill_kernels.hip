@@ -265,7 +265,7 @@ __global__ __launch_bounds__(kDsThreads) void k_distill_bwd(DsArgs a) {
 static int ds_check(int dtype, int v_dtype, int64_t rows, int64_t V, int K, float tau) {
   if (!lm_dtype_ok(dtype) || (v_dtype != LSH_F32 && v_dtype != dtype) || !(tau > 0.0f) || !(tau < INFINITY))
     return LSH_ERR_ARG;
-  if (rows < 0 || rows > 0x7fffffff / 64 || V < 1 || V > 0x7fffffff / 2 || K < 0 || K > LSH_DISTILL_MAX_K)
+  if (rows < 0 || !lm_grid_ok(rows, kDsThreads) || V < 1 || V > 0x7fffffff / 2 || K < 0 || K > LSH_DISTILL_MAX_K)
     return LSH_ERR_SHAPE;
   return LSH_OK;
 }

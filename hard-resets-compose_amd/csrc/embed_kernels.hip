@@ -494,7 +494,7 @@ extern "C" int lsh_embed_fwd(int dtype, const int64_t* tokens, const void* weigh
   if (bad_ptr(tokens) || (V > 0 && bad_ptr(weight)) || bad_ptr(out)) return LSH_ERR_ARG;
   const int per = 16 / lm_dtype_size(dtype), pieces = (int)((D + per - 1) / per);
   const int64_t blocks = (n * pieces + 255) / 256;
-  if (blocks > 0x7fffffff) return LSH_ERR_SHAPE;
+  if (!lm_grid_ok(blocks, 256)) return LSH_ERR_SHAPE;
   const bool wide = embed_wide(dtype, D, weight, out);
   with_dtype(dtype, [&](auto t) {
     using T = decltype(t);

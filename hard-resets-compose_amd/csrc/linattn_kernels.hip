@@ -56,14 +56,15 @@ struct LaShares {
 };
 template <class T>
 __global__ __launch_bounds__(256) void k_la_share(LaShares a) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int j = blockIdx.y, D = a.D[j], share = a.share[j];
-  if (i >= a.n[j]) return;
-  const float* p = a.x[j] + (i / D) * share * D + i % D;
-  float s = 0.0f;
-  for (int k = 0; k < share; ++k) s += p[(int64_t)k * D];
-  ((T*)a.y[j])[i] = from_f<T>(s);
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.n[j]; i += (int64_t)gridDim.x * 256) {
+    const float* p = a.x[j] + (i / D) * share * D + i % D;
+    float s = 0.0f;
+    for (int k = 0; k < share; ++k) s += p[(int64_t)k * D];
+    ((T*)a.y[j])[i] = from_f<T>(s);
+  }
 }
+constexpr int64_t kLaShareGroups = 1 << 20;  // at most; a grid has fewer than 2^32 threads
 
 static int la_go(const LaWalks& all, int dtype, bool sums, hipStream_t st) {
   return dtype == LSH_F32    ? la_launch_f32(all, sums, st)
@@ -186,7 +187,7 @@ static int la_check(const lsh_linattn* a) {
   if (a->T < 0 || a->B < 0 || a->H < 0 || a->Dk < 1 || a->Dv < 1 || a->Dk > LSH_LINATTN_MAX_D ||
       a->Dv > LSH_LINATTN_MAX_D)
     return LSH_ERR_SHAPE;
-  if (a->B * a->H > 0x7fffffff / 64 || a->T > ((int64_t)1 << 40)) return LSH_ERR_SHAPE;
+  if (!lm_grid_ok(a->B * a->H, 256) || a->T > ((int64_t)1 << 40)) return LSH_ERR_SHAPE;
   if (a->H > 0) {
     for (int n : {a->q_heads, a->k_heads, a->v_heads})
       if (n < 1 || a->H % n) return LSH_ERR_SHAPE;
@@ -327,7 +328,7 @@ extern "C" int lsh_linattn_bwd(const lsh_linattn* a, const void* starts, const v
     most = most > n ? most : n;
   }
   if (most > 0) {
-    const dim3 grid((unsigned)((most + 255) / 256), (unsigned)count);
+    const dim3 grid((unsigned)std::min((most + 255) / 256, kLaShareGroups), (unsigned)count);
     with_dtype(a->dtype, [&](auto t) { k_la_share<decltype(t)><<<grid, 256, 0, st>>>(shares); });
     LSH_CHECK_LAUNCH();
   }

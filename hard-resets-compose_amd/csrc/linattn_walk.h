@@ -740,6 +740,7 @@ inline int la_launch(const LaWalks& all, bool sums, hipStream_t st) {
     wide = wide && la_wide(all.w[i], La<L>::C);
     blocks = blocks > (all.w[i].DV + block - 1) / block ? blocks : (all.w[i].DV + block - 1) / block;
   }
+  if (!lm_grid_ok(n * blocks * all.n, block * 4)) return LSH_ERR_SHAPE;
   const dim3 grid((unsigned)(n * blocks * all.n));
   auto go = [&](auto dkp, auto waves) {
     constexpr int DKP = decltype(dkp)::value, W = decltype(waves)::value;

@@ -33,6 +33,9 @@ __device__ __forceinline__ T from_f(float x) {
 inline bool lm_dtype_ok(int d) { return d == LSH_F32 || d == LSH_BF16 || d == LSH_F16; }
 inline int lm_dtype_size(int d) { return d == LSH_F32 ? 4 : 2; }
 
+// Whether a launch of so many workgroups fits: along an axis a grid has fewer than 2^32 threads.
+inline bool lm_grid_ok(int64_t groups, int threads) { return groups < ((int64_t)1 << 32) / threads; }
+
 // Calls f with a value of the C++ type of a dtype code.
 template <class F>
 inline void with_dtype(int d, F&& f) {

@@ -87,3 +87,17 @@ def test_model_parameters():
     assert S.shape == (3, 2, 8, 16) and u.shape == (72,)
     d = m.blocks[0].decay
     assert bool((d > 0).all()) and bool((d < 1).all()) and "blocks.0.decay" in dict(m.named_buffers())
+
+
+def test_more_threads_than_a_grid_holds_are_refused():
+    """A grid has fewer than 2^32 threads along an axis: what would need more is refused before the launch."""
+    from lifscan import _native as n
+    L = n.lib()
+    assert L.lsh_linattn_step(_attn(T=1, B=2 ** 22), P, None) == SHAPE
+    assert L.lsh_linattn_fwd(_attn(T=1, B=2 ** 22), None, 0, None) == SHAPE
+    assert L.lsh_linattn_fwd(_attn(T=1, B=2 ** 21, Dv=128), None, 0, None) == SHAPE  # 512 threads a state
+    norm = n.BlockNorm(x_dtype=0, dtype=1, act=1, D=2048, rows=2 ** 24, x=P, y=P, gate=P, w_post=P, w_pre=P, eps=1e-6)
+    assert L.lsh_block_norm_fwd(ctypes.byref(norm), P, P, None) == SHAPE
+    assert L.lsh_embed_fwd(1, P, P, P, 2 ** 26, 8, 512, -1, 1.0, None) == SHAPE
+    assert L.lsh_distill_fwd(1, P, 8, 0, P, P, P, P, 2 ** 24, 8, 1, 1.0, None, 0, None) == SHAPE
+    assert L.lsh_distill_bwd(1, P, 8, 0, P, P, P, P, 1, P, 2 ** 24, 8, 1, 1.0, None) == SHAPE
