@@ -138,7 +138,7 @@ __global__ __launch_bounds__(256) void k_la_step(LaIn qi, LaIn ki, LaIn vi,
   const T* q = la_row<T>(qi, b, h);
   const T* k = la_row<T>(ki, b, h);
   const T* v = la_row<T>(vi, b, h);
-  const float beta = betas[h];
+  const float beta = betas[h] >= 0.0f ? betas[h] : NAN;  // as in the walks (la_log2)
   float vt[4], o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
   for (int j = 0; j < 4; ++j) vt[j] = dv0 + j * STEP < DV ? to_f(v[dv0 + j * STEP]) : 0.0f;

@@ -37,7 +37,7 @@ def lin_attn(q, k, v, beta, s0=None, scale=1.0):
     q [T, B, Hq, Dk], k [T, B, Hk, Dk], v [T, B, Hv, Dv]: float32, bfloat16 or float16, one type;
     widths 1 to 256.  beta: [H] decays on the device (>= 0, of any float type), or one number for all
     heads; Hq, Hk and Hv divide H, and consecutive heads share one.  s0: the fp32 state before the
-    first row, or None (zeros).  A decay gets no gradient.
+    first row, or None (zeros).  A decay gets no gradient; a negative one on the device gives NaN.
 
     A value of v that is not finite reaches its own row and the later ones, and no earlier row."""
     return _n.lm_ops().lin_attn(q, k, v, _decays(beta, q, k, v), s0, scale)

@@ -496,3 +496,18 @@ def test_what_is_no_decay_gives_nan(dev, dtype, beta):
         assert bool(x.select(heads, 1).isnan().all())
         for h in (0, 2):
             assert torch.equal(x.select(heads, h), w.select(heads, h))
+
+
+@pytest.mark.parametrize("Dv", [48, 50])
+@pytest.mark.parametrize("beta", [-0.5, float("nan")])
+def test_what_is_no_decay_gives_nan_in_a_step(dev, beta, Dv):
+    from lifscan import hip_linattn as LA
+    q, k, v, b, s0, _, _ = _inputs(torch.float32, 1, 2, (3,) * 3, 3, 32, Dv, dev, seed=41)
+    good, bad = s0.clone(), s0.clone()
+    want = LA.lin_attn_step(q[0], k[0], v[0], b, good)
+    b = b.clone()
+    b[1] = beta
+    got = LA.lin_attn_step(q[0], k[0], v[0], b, bad)
+    assert bool(got[:, 1].isnan().all()) and bool(bad[:, 1].isnan().all())
+    for h in (0, 2):
+        assert torch.equal(got[:, h], want[:, h]) and torch.equal(bad[:, h], good[:, h])
