@@ -58,9 +58,9 @@ using s16x4 = short __attribute__((ext_vector_type(4)));
 // rows: lane l has row l%16 and, with g = l/16, the values 4g..4g+3 of each 16 (the order in which an
 // accumulator holds its rows, so that an accumulator turns into a fragment in registers).
 //
-// 16 bits: products of the type, fp32 sums.  A decayed value is taken in as many parts as hold the 24
-// bits of fp32 (bf16 three, fp16 two), so the state is kept to fp32; a score and the state that meets q
-// are taken in two parts (16 bits and more), so that the result's own rounding is nearly all of its error.
+// 16 bits: products of the type, fp32 sums.  What the walk holds in fp32 (a decayed value, a score, the state that
+// meets q) is taken in parts: bf16 in three, which hold its 24 bits; fp16 in two, which hold 23 (one value in four
+// is off by its last place).
 // SCALED (fp16): what is split is first scaled by a power of two that brings its largest value below 2^15,
 // since scores, states and decayed values can leave fp16's range, or sink below its normal numbers, where
 // the results do not.
@@ -95,23 +95,28 @@ struct La16 {
 
 template <>
 struct La<bf16_t> : La16<bf16_t, bf16x4, bf16x8> {
-  static constexpr int PARTS = 3, FINE = 2;
+  static constexpr int PARTS = 3, FINE = 3;
   static constexpr bool SCALED = false;
   static __device__ __forceinline__ f32x4 mma(Frag a, Frag b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
   }
-  // an accumulator's values as two fragments: the upper halves of the words, and what they leave
-  static __device__ __forceinline__ void of(const f32x4* acc, float, Frag (&f)[2]) {
-    unsigned top[4];
+  // an accumulator's values as three fragments of eight bits each: the upper halves of the words, those of what
+  // they leave, and the rest, which has no lower half
+  static __device__ __forceinline__ void of(const f32x4* acc, float, Frag (&f)[3]) {
+    unsigned top[3][4];
 #pragma unroll
     for (int e = 0; e < 8; e += 2) {
-      const float x = acc[e >> 2][e & 3], y = acc[e >> 2][(e & 3) + 1];
-      const unsigned a = __builtin_bit_cast(unsigned, x), b = __builtin_bit_cast(unsigned, y);
-      top[e / 2] = __builtin_amdgcn_perm(b, a, 0x07060302);
-      f[1][e] = (bf16_t)(x - __builtin_bit_cast(float, a & 0xffff0000u));
-      f[1][e + 1] = (bf16_t)(y - __builtin_bit_cast(float, b & 0xffff0000u));
+      float x = acc[e >> 2][e & 3], y = acc[e >> 2][(e & 3) + 1];
+#pragma unroll
+      for (int c = 0; c < 3; ++c) {
+        const unsigned a = __builtin_bit_cast(unsigned, x), b = __builtin_bit_cast(unsigned, y);
+        top[c][e / 2] = __builtin_amdgcn_perm(b, a, 0x07060302);
+        x -= __builtin_bit_cast(float, a & 0xffff0000u);
+        y -= __builtin_bit_cast(float, b & 0xffff0000u);
+      }
     }
-    f[0] = __builtin_bit_cast(Frag, top);
+#pragma unroll
+    for (int c = 0; c < 3; ++c) f[c] = __builtin_bit_cast(Frag, top[c]);
   }
 };
 

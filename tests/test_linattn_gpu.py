@@ -511,3 +511,40 @@ def test_what_is_no_decay_gives_nan_in_a_step(dev, beta, Dv):
     assert bool(got[:, 1].isnan().all()) and bool(bad[:, 1].isnan().all())
     for h in (0, 2):
         assert torch.equal(got[:, h], want[:, h]) and torch.equal(bad[:, h], good[:, h])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("what", ["state", "scores"])
+def test_cancelling_terms_keep_the_digits_of_fp32(dev, dtype, what):
+    """Two terms of an output that cancel but for their last digits, from the state or from two scores: scores
+    and states are fp32 numbers, so an output is off by its own rounding and a few 2^-24 of its terms (six
+    products at most that are added in fp32, fp16's parts of 22 bits and more, and the factors of the decays: 16
+    in all).  Sixteen bits would leave some 2^-17 of them."""
+    from lifscan import hip_linattn as LA
+    B, H, Dv = 3, 4, 80
+    g = torch.Generator().manual_seed(61)
+    beta = 1 - torch.exp2(-torch.linspace(2, 9, H))
+    if what == "state":
+        T, Dk = 1, 2
+        q, k = torch.ones(T, B, H, Dk), torch.zeros(T, B, H, Dk)
+        v = torch.randn(T, B, H, Dv, generator=g)
+        s0 = 1 + torch.rand(B, H, Dk, Dv, generator=g)
+        s0[:, :, 1] = -s0[:, :, 0] + 2.0 ** -12 * torch.rand(B, H, Dv, generator=g)
+    else:
+        T, Dk = 2, 4
+        beta = torch.ones(H)
+        q = 1 + torch.rand(T, B, H, Dk, generator=g)
+        k = (1 + torch.rand(1, B, H, Dk, generator=g)).to(dtype).float().repeat(T, 1, 1, 1)
+        k[:, ..., 3] = torch.tensor([2.0 ** -11, 2.0 ** -12])[:, None, None]
+        v = torch.ones(T, B, H, Dv)
+        v[1] = -1
+        s0 = None
+    q, k, v, beta = q.to(dtype).to(dev), k.to(dtype).to(dev), v.to(dtype).to(dev), beta.to(dev)
+    s0 = None if s0 is None else s0.to(dev)
+    o, _ = LA.lin_attn(q, k, v, beta, s0=s0)
+    want, _ = reference(q, k, v, beta, s0, 1.0)
+    most, _ = _absolute(q, k, v, beta, s0, 1.0)
+    err = (o.double().cpu() - want)[-1].abs()
+    bound = U[dtype] * want[-1].abs() + 16 * 2.0 ** -24 * most[-1] + (2.0 ** -25 if dtype == torch.float16 else 0.0)
+    assert float((want[-1].abs() / most[-1]).max()) < 2.0 ** -10
+    assert bool((err <= bound).all()), float((err / bound).max())
