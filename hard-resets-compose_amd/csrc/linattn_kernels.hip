@@ -30,7 +30,7 @@ __global__ __launch_bounds__(256) void k_la_join(float* __restrict__ starts, con
   using X = float __attribute__((ext_vector_type(V)));
   const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V;
   if (i >= n) return;
-  const float f = __builtin_amdgcn_exp2f(la_log2(beta[i / size % H]) * (float)L);
+  const float l2 = la_log2(beta[i / size % H]), f = __builtin_amdgcn_exp2f(l2 * (float)L);
   X s = s0 ? *(const X*)(s0 + i) : X(0.0f);
   *(X*)(starts + i) = s;
   for (int j0 = 1; j0 < segs; j0 += AHEAD) {
@@ -40,7 +40,8 @@ __global__ __launch_bounds__(256) void k_la_join(float* __restrict__ starts, con
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) s[e] = __builtin_fmaf(f, s[e], x[j][e]);
+      for (int e = 0; e < V; ++e)
+        s[e] = f == INFINITY ? la_grow(s[e], l2, (float)L) + x[j][e] : __builtin_fmaf(f, s[e], x[j][e]);
       if (j0 + j < segs) *(X*)(starts + (size_t)(j0 + j) * n + i) = s;
     }
   }

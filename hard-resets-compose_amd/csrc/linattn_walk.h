@@ -204,6 +204,11 @@ __device__ __forceinline__ const T* la_row(const LaIn& x, int64_t b, int64_t h) 
 // (below 0, or NaN) gives NaN.
 __device__ __forceinline__ float la_pow(float l2, int n) { return __builtin_amdgcn_exp2f(l2 * (float)n); }
 __device__ __forceinline__ float la_log2(float beta) { return beta >= 0.0f ? fmaxf(log2f(beta), -1e4f) : NAN; }
+// x * 2^(l2 * n), l2 > 0, where the power alone may leave fp32: zeros stay zeros, and what fp32 holds is finite.
+__device__ __forceinline__ float la_grow(float x, float l2, float n) {
+  const float t = fminf(l2 * n, 1024.0f), whole = floorf(t);
+  return __builtin_amdgcn_ldexpf(x * __builtin_amdgcn_exp2f(t - whole), (int)whole);
+}
 
 using u32x2 = unsigned __attribute__((ext_vector_type(2)));
 using u32x4 = unsigned __attribute__((ext_vector_type(4)));
@@ -229,14 +234,14 @@ struct LaStage {
   static_assert(THREADS % PER_ROW == 0 && (C % ROWS == 0 || ROWS % C == 0), "whole rows");
   u32x4 x[N];
   const T* low;    // the lowest address of the chunk that is read next, as a whole one
-  int64_t ahead;   // elements from a chunk to the next
+  int64_t ahead;   // elements from a chunk to the next, `rows` rows on
   unsigned at;     // this thread's first piece, in bytes from low
   unsigned step;   // bytes from a row of the walk to the next, modulo 2^32 where it goes back
   int r0;
-  __device__ __forceinline__ void init(const T* lowest, int64_t st, int rev, int D) {
+  __device__ __forceinline__ void init(const T* lowest, int64_t st, int rev, int D, int rows) {
     r0 = threadIdx.x / PER_ROW;
     low = lowest;
-    ahead = rev ? -C * st : C * st;
+    ahead = rev ? -rows * st : rows * st;
     const unsigned bytes = (unsigned)st * (unsigned)sizeof(T);
     step = rev ? 0u - bytes : bytes;
     const int c = threadIdx.x % PER_ROW * W;
@@ -296,10 +301,10 @@ struct LaStage<T, L, C, DP, THREADS, PACKED, false> {
   const T* low;
   int64_t ahead, step;  // elements, both signed
   int r0, D, first;     // rows from `first` on are there
-  __device__ __forceinline__ void init(const T* lowest, int64_t st, int rev, int columns) {
+  __device__ __forceinline__ void init(const T* lowest, int64_t st, int rev, int columns, int rows) {
     r0 = threadIdx.x / PER_ROW;
     step = rev ? -st : st;
-    ahead = C * step;
+    ahead = rows * step;
     low = rev ? lowest + (C - 1) * st : lowest;  // the chunk's row 0
     D = columns;
   }
@@ -483,21 +488,30 @@ __global__ __launch_bounds__(W * 64, la_waves(sizeof(L), DKP, W)) void k_la_walk
     for (int i = threadIdx.x; i < X::FINE * C * PP; i += W * 64) s_p[0][i] = (L)0.0f;  // tiles above the diagonal stay so
   }
 
-  // row r of the walk is row (rev ? T - 1 - r : r); the first chunk is the short one
-  int n = r0 < r1 ? (int)((r1 - r0 - 1) % C) + 1 : 0;
-  int64_t r = r0 + n - C;  // where the chunk's row 0 would be
+  // A chunk's powers reach beta^C, and sigma adds to them: with beta = 4 less than 2^81.  Heads that grow faster take
+  // one row at a time, as if each were a short chunk, so that no power is formed that overflows where the results
+  // do not (beta^31 of rows that hold zeros, or are not there).
   const float l2 = la_log2(a.beta[h]);
-  float decay[CS][KB / 4];  // of the rows to the chunk's end
+  const int step = __builtin_amdgcn_readfirstlane(l2 > 2.0f ? 1 : C);
+  // row r of the walk is row (rev ? T - 1 - r : r); the first chunk is the short one
+  int n = r0 < r1 ? step == 1 ? 1 : (int)((r1 - r0 - 1) % C) + 1 : 0;
+  int64_t r = r0 + n - C;  // where the chunk's row 0 would be
+  float decay[CS][KB / 4];  // of the rows to the chunk's end; where step is 1, of the last row only
 #pragma unroll
   for (int s = 0; s < CS; ++s)
 #pragma unroll
-    for (int e = 0; e < KB / 4; ++e)
-      decay[s][e] = a.su * la_pow(l2, C - 1 - (s * KB + X::at(e) + 4 * g) + a.late);
+    for (int e = 0; e < KB / 4; ++e) {
+      const int left = C - 1 - (s * KB + X::at(e) + 4 * g);
+      decay[s][e] = left < step ? a.su * la_pow(l2, left + a.late) : 0.0f;
+    }
   // this wave's tile of the scores: rows 16*ti + m against rows 16*tj + 4g + e
   const int ti = w == 0 ? 0 : w < 3 ? 1 : w < 6 ? 2 : 3, tj = w - ti * (ti + 1) / 2;
   float fall[4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) fall[e] = a.so * a.su * la_pow(l2, max((ti - tj) * 16 + m - 4 * g - e, 0));
+  for (int e = 0; e < 4; ++e) {
+    const int far = max((ti - tj) * 16 + m - 4 * g - e, 0);
+    fall[e] = far < step ? a.so * a.su * la_pow(l2, far) : 0.0f;
+  }
 
   LaStage<T, L, C, DKP, W * 64, true, WIDE> xq;
   LaStage<T, L, C, DKP, W * 64, false, WIDE> xk;
@@ -517,20 +531,20 @@ __global__ __launch_bounds__(W * 64, la_waves(sizeof(L), DKP, W)) void k_la_walk
   // the lowest address of the chunk's output, this lane's first byte from there, and bytes to the next row
   const int64_t low = a.rev ? a.T - r - C : r;  // the chunk's row of lowest address
   const unsigned eo = a.out_f32 ? 4 : sizeof(T), bo = (unsigned)so * eo, step_o = a.rev ? 0u - bo : bo;
-  const int64_t ahead_o = (a.rev ? -C : C) * so * eo;
+  const int64_t ahead_o = (a.rev ? -step : step) * so * eo;
   char* out = (char*)a.out + ((low * BH + bh) * a.DV + dv0) * eo;
   const unsigned at_o = dv < a.DV ? (a.rev ? C - 1 - m : m) * bo + (wc + 4 * g) * eo : kLaNowhere;
-  xq.init(q + low * a.q.st, a.q.st, a.rev, a.DK);
-  xk.init(k + low * a.k.st, a.k.st, a.rev, a.DK);
-  xv.init(v + low * a.v.st, a.v.st, a.rev, a.DV - dv0);
+  xq.init(q + low * a.q.st, a.q.st, a.rev, a.DK, step);
+  xk.init(k + low * a.k.st, a.k.st, a.rev, a.DK, step);
+  xv.init(v + low * a.v.st, a.v.st, a.rev, a.DV - dv0, step);
   if (n) {
     fetch(n);
     put(0);
-    fetch(r + 2 * C <= r1 ? C : 0);
+    fetch(r + C + step <= r1 ? step : 0);
   }
   __syncthreads();
   int half = 0;
-  for (; n && r + C <= r1; r += C, n = C) {
+  for (; n && r + C <= r1; r += step, n = step) {
     const L *cq = s_q + half * (C * PQ), *ck = s_k + half * (C * PK), *cv = s_v + half * (C * PV);
     Frag x[CS];  // the chunk's values in the wave's columns
 #pragma unroll
@@ -696,7 +710,7 @@ __global__ __launch_bounds__(W * 64, la_waves(sizeof(L), DKP, W)) void k_la_walk
     }
     half ^= 1;
     put(half);  // zeros after the last chunk
-    fetch(r + 3 * C <= r1 ? C : 0);
+    fetch(r + C + 2 * step <= r1 ? step : 0);
     __syncthreads();  // the next chunk is there, and the scores have been read
   }
 

@@ -35,8 +35,9 @@ def lin_attn(q, k, v, beta, s0=None, scale=1.0):
     """Linear attention over a sequence -> (o [T, B, H, Dv], state after the last row [B, H, Dk, Dv]).
 
     q [T, B, Hq, Dk], k [T, B, Hk, Dk], v [T, B, Hv, Dv]: float32, bfloat16 or float16, one type;
-    widths 1 to 256.  beta: [H] decays on the device (>= 0, of any float type), or one number for all
-    heads; Hq, Hk and Hv divide H, and consecutive heads share one.  s0: the fp32 state before the
+    widths 1 to 256.  beta: [H] decays on the device (finite, >= 0, of any float type), or one number for
+    all heads; Hq, Hk and Hv divide H, and consecutive heads share one.  (A head that grows, beta > 1, is
+    right as far as fp32 holds its state; above 4 it is walked row by row.)  s0: the fp32 state before the
     first row, or None (zeros).  A decay gets no gradient; a negative one on the device gives NaN.
 
     A value of v that is not finite reaches its own row and the later ones, and no earlier row."""

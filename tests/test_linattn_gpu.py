@@ -548,3 +548,53 @@ def test_cancelling_terms_keep_the_digits_of_fp32(dev, dtype, what):
     bound = U[dtype] * want[-1].abs() + 16 * 2.0 ** -24 * most[-1] + (2.0 ** -25 if dtype == torch.float16 else 0.0)
     assert float((want[-1].abs() / most[-1]).max()) < 2.0 ** -10
     assert bool((err <= bound).all()), float((err / bound).max())
+
+
+@pytest.mark.parametrize("dtype", list(U), ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("T,beta", [(1, 20.0), (2, 20.0), (5, 20.0), (3, 300.0), (1, 1e30), (27, 20.0), (64, 3.0)])
+def test_decays_that_grow(dev, dtype, T, beta):
+    """Any finite factor is a decay: what a chunk has no rows for must not overflow where the results do not."""
+    H, D = 2, 24
+    q, k, v, b, s0, do, ds = _inputs(dtype, T, 2, (H,) * 3, H, D, D, dev, seed=67)
+    b = torch.tensor([beta, 0.5], device=dev)
+    size = beta ** -(T - 1)  # so that 16-bit results stay in their type's range
+    scale = min(max(size, 2.0 ** -100), 1.0)
+    s0, ds = s0 / 2 ** 10, ds * scale
+    if dtype == torch.float16:
+        scale = scale / 2 ** 8 / beta if beta < 1e10 else 1e-30
+        ds = ds / 2 ** 8 / beta if beta < 1e10 else ds * 1e-30
+        s0 = s0 / beta
+    got = run_all(q, k, v, b, s0, scale, do, ds)
+    want = reference(q, k, v, b, s0, scale, do, ds)
+    most = _absolute(q, k, v, b, s0, scale, do, ds)
+    for x, w, m in zip(got, want, most):
+        small = 2.0 ** -24 if x.dtype == torch.float16 else 0.0
+        err = (x.detach().double().cpu() - w).abs()
+        u = U[x.dtype]
+        # a power of beta: its exponent, up to log2(beta^T) <= 128, is an fp32 number
+        bound = u * w.abs() + ((2 * u if u > 1e-6 else 0.0) + (T + D + 64 + 128) * 2.0 ** -24) * m + small
+        assert bool((err <= bound).all()), float((err / bound.clamp(min=1e-300)).max())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("T,Dk", [(70, 64), (330, 128)])
+def test_rows_of_zeros_do_not_grow(dev, dtype, T, Dk):
+    """Zeros times any power of a decay are zeros: a sequence whose first rows (for the gradients: last rows) are
+    zeros, in one segment and in several."""
+    from lifscan import hip_linattn as LA
+    H, Dv, beta = 1, 64, 20.0
+    q, k, v, _, _, do, _ = _inputs(dtype, T, 1, (H,) * 3, H, Dk, Dv, dev, seed=71, s0=False)
+    b = torch.full((H,), beta, device=dev)
+    late, early = v.clone(), do.clone()
+    late[:-4] = 0
+    early[4:] = 0
+    o, s = LA.lin_attn(q, k, late, b, scale=2.0 ** -20)
+    want, s_want = reference(q, k, late, b, None, 2.0 ** -20)
+    most, s_most = _absolute(q, k, late, b, None, 2.0 ** -20)
+    check(o, want, most, dtype, T, Dk)
+    check(s, s_want, s_most, dtype, T, Dk)
+    got = run_all(q, k, late * 0, b, None, 2.0 ** -20, early, None)
+    want = reference(q, k, late * 0, b, None, 2.0 ** -20, early, None)
+    most = _absolute(q, k, late * 0, b, None, 2.0 ** -20, early, None)
+    for i in (2, 3, 4):
+        check(got[i], want[i], most[i], dtype, T, Dk)
