@@ -482,8 +482,10 @@ __global__ __launch_bounds__(W * 64, la_waves(sizeof(L), DKP, W)) void k_la_walk
         }
     }
   }
-  // the state is sigma*S: most chunks decay it by sigma alone, and weigh what they add by 1/sigma
+  // the state is sigma*S: most chunks decay it by sigma alone, and weigh what they add by 1/sigma.  sigma is a power
+  // of its own, not a product of the chunks' (whose one rounding would come again in every chunk: 6.5e-6 after 512).
   float sigma = 1.0f;
+  int since = 0;  // the rows that sigma stands for
   if (!SUMS) {
     for (int i = threadIdx.x; i < X::FINE * C * PP; i += W * 64) s_p[0][i] = (L)0.0f;  // tiles above the diagonal stay so
   }
@@ -665,11 +667,13 @@ __global__ __launch_bounds__(W * 64, la_waves(sizeof(L), DKP, W)) void k_la_walk
       }
     }
 
-    sigma *= la_pow(l2, n);
-    if (!(sigma > 0x1p-16f && sigma < 0x1p16f)) {
+    since += n;
+    sigma = la_pow(l2, since);
+    if (!(sigma > 0x1p-16f && sigma < 0x1p16f && since < 1 << 22)) {
 #pragma unroll
       for (int i = 0; i < KT; ++i) S[i] *= sigma;
       sigma = 1.0f;
+      since = 0;
     }
     const float weight = __builtin_amdgcn_rcpf(sigma);
 #pragma unroll

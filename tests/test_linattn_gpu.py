@@ -598,3 +598,21 @@ def test_rows_of_zeros_do_not_grow(dev, dtype, T, Dk):
     most = _absolute(q, k, late * 0, b, None, 2.0 ** -20, early, None)
     for i in (2, 3, 4):
         check(got[i], want[i], most[i], dtype, T, Dk)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_slow_decays_of_long_sequences_do_not_drift(dev, dtype):
+    """The first state after T rows without values is beta^T times it.  Bound: beta^T = 2^(T*log2 beta) with
+    T*log2 beta up to 6, the logarithm off by 2^-23 of itself and its product by 2^-24 (12 * 2^-24 of the result),
+    the power by 2^-23, and one rounding each for its product with the state and where the state is rescaled: below
+    24 * 2^-24.  Heads enough that no row is split."""
+    from lifscan import hip_linattn as LA
+    T, B, D = 16384, 172, 8
+    beta = torch.tensor([1 - 2.0 ** -12, 1 - 2.0 ** -14, 1 - 2.0 ** -16])
+    g = torch.Generator().manual_seed(73)
+    s0 = 1 + torch.rand(B, 3, D, D, generator=g)
+    z = torch.zeros(T, B, 3, D, dtype=dtype, device=dev)
+    _, s = LA.lin_attn(z, z, z, beta.to(dev), s0=s0.to(dev))
+    want = s0.double() * beta.double()[:, None, None] ** T
+    err = (s.double().cpu() - want).abs() / want
+    assert float(err.max()) <= 24 * 2.0 ** -24, [float(e) / 2.0 ** -24 for e in err.amax((0, 2, 3))]
