@@ -5,6 +5,7 @@
 #include <torch/extension.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <algorithm>
 #include <map>
@@ -87,13 +88,28 @@ bool grad_wanted(std::initializer_list<Tensor> ts) {
     if (t.defined() && t.requires_grad()) return true;
   return false;
 }
+// What looks at the calls from outside sees none of the kernels: a trace would record outputs that nothing fills,
+// and a forward-mode tangent would be lost.
+template <class Tensors>
+void check_plain(const char* what, const Tensors& ts) {
+  TORCH_CHECK(!torch::jit::tracer::isTracing(), what, " cannot be recorded by a trace (torch.jit.trace)");
+  for (const Tensor& t : ts) {
+    if (!t.defined()) continue;
+    TORCH_CHECK(!t._fw_grad(0).defined(), what, " has no forward-mode derivatives");
+  }
+}
+void check_plain(const char* what, std::initializer_list<Tensor> ts) {
+  check_plain<std::initializer_list<Tensor>>(what, ts);
+}
 Tensor of(const Maybe& t) { return t.has_value() ? *t : Tensor(); }
 // autograd functions take no undefined tensors
 Maybe maybe(const Tensor& t) { return t.defined() ? Maybe(t) : Maybe(); }
 
 // The kernels' gradients have no graph of their own.
-void check_first_order() {
+variable_list first_order(variable_list grads) {
   TORCH_CHECK(!at::GradMode::is_enabled(), "the language-model operators have no second derivatives (create_graph)");
+  check_plain("a language-model operator's gradient", grads);
+  return grads;
 }
 // A saved tensor as the kernels read it: a saved-tensor hook may hand back another one than it was given.
 Tensor unpacked(const Tensor& t, torch::IntArrayRef sizes, torch::ScalarType type, const Tensor& like) {
@@ -192,8 +208,8 @@ struct LinAttn : public torch::autograd::Function<LinAttn> {
     return {out.o, out.s_end};
   }
 
-  static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    check_first_order();
+  static variable_list backward(AutogradContext* ctx, variable_list grads_in) {
+    const variable_list grads = first_order(std::move(grads_in));
     variable_list none(6);
     const Tensor &d_o = grads[0], &d_s = grads[1];
     if (!d_o.defined() && !d_s.defined()) return none;
@@ -238,6 +254,7 @@ struct LinAttn : public torch::autograd::Function<LinAttn> {
 std::tuple<Tensor, Tensor> lin_attn(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& beta,
                                     const Maybe& s0_in, double scale) {
   Tensor s0 = of(s0_in);
+  check_plain("lin_attn", {q, k, v, beta, s0});
   if (grad_wanted({q, k, v, beta, s0})) {
     TORCH_CHECK_VALUE(!beta.requires_grad(), "beta is a constant of lin_attn: it gets no gradient (pass beta.detach())");
     const Attn r = attn(q, k, v, beta, scale, 4);
@@ -259,6 +276,7 @@ std::tuple<Tensor, Tensor> lin_attn(const Tensor& q, const Tensor& k, const Tens
 
 Tensor lin_attn_step(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& beta, const Tensor& state,
                      double scale) {
+  check_plain("lin_attn_step", {q, k, v, beta, state});
   TORCH_CHECK_VALUE(!grad_wanted({q, k, v, state}),
                     "lin_attn_step has no gradients: call it under torch.no_grad, or lin_attn");
   Attn r = attn(q, k, v, beta, scale, 3);
@@ -313,8 +331,8 @@ struct BlockNorm : public torch::autograd::Function<BlockNorm> {
     return norm_forward(norm_args(x, y, gate, w_post, w_pre, scale, scale1, eps, act), x, y);
   }
 
-  static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    check_first_order();
+  static variable_list backward(AutogradContext* ctx, variable_list grads_in) {
+    const variable_list grads = first_order(std::move(grads_in));
     if (!grads[0].defined() && !grads[1].defined()) return variable_list(9);
     const auto saved = ctx->get_saved_variables();
     const auto n = ctx->saved_data["n"].toIntVector();
@@ -351,6 +369,7 @@ struct BlockNorm : public torch::autograd::Function<BlockNorm> {
 std::tuple<Tensor, Tensor> block_norm(const Tensor& x_in, const Tensor& y_in, const Tensor& w_post_in,
                                       const Tensor& w_pre_in, const Maybe& gate_in, const Maybe& scale_in,
                                       double scale1, double eps, int64_t act) {
+  check_plain("block_norm", {x_in, y_in, w_post_in, w_pre_in, of(gate_in), of(scale_in)});
   check_float(x_in, "x");
   check_float(y_in, "y");
   TORCH_CHECK_VALUE(x_in.dim() >= 1 && x_in.sizes() == y_in.sizes() && x_in.device() == y_in.device(),
@@ -398,8 +417,8 @@ struct Embed : public torch::autograd::Function<Embed> {
     ctx->saved_data["sizes"] = tokens.sizes().vec();
     return embed_forward(tokens, weight, scale, padding);
   }
-  static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    check_first_order();
+  static variable_list backward(AutogradContext* ctx, variable_list grads_in) {
+    const variable_list grads = first_order(std::move(grads_in));
     const auto n = ctx->saved_data["n"].toIntVector();
     const Tensor dout = grads[0].contiguous();
     const Tensor tokens = unpacked(ctx->get_saved_variables()[0], ctx->saved_data["sizes"].toIntVector(),
@@ -416,6 +435,7 @@ struct Embed : public torch::autograd::Function<Embed> {
 };
 
 Tensor embed(const Tensor& tokens_in, const Tensor& weight_in, double scale, c10::optional<int64_t> padding_idx) {
+  check_plain("embed", {weight_in});
   check_float(weight_in, "weight");
   TORCH_CHECK_VALUE(weight_in.dim() == 2 && weight_in.size(1) >= 1, "weight must be a [V, D] tensor");
   TORCH_CHECK_VALUE(tokens_in.device() == weight_in.device(), "tokens must be on ", weight_in.device());
@@ -455,8 +475,8 @@ struct Distill : public torch::autograd::Function<Distill> {
                                                 (int64_t)values.scalar_type()};
     return loss;
   }
-  static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    check_first_order();
+  static variable_list backward(AutogradContext* ctx, variable_list grads_in) {
+    const variable_list grads = first_order(std::move(grads_in));
     const auto saved = ctx->get_saved_variables();
     const auto n = ctx->saved_data["n"].toIntVector();
     const Tensor& gr = grads[0];
@@ -476,6 +496,7 @@ struct Distill : public torch::autograd::Function<Distill> {
 };
 
 Tensor distill_topk(const Tensor& logits, const Tensor& values_in, const Tensor& index_in, double tau) {
+  check_plain("distill_topk", {logits, values_in});
   check_float(logits, "logits");
   TORCH_CHECK_VALUE(logits.dim() >= 1 && logits.size(-1) >= 1, "logits must be [*rows, V]");
   const auto lead = logits.sizes().slice(0, logits.dim() - 1);

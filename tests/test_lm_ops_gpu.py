@@ -573,3 +573,49 @@ def test_distill_teacher_values_that_are_nan(dev, dtype, V):
         other = torch.ones(V, dtype=torch.bool, device=dev)
         other[idx[row]] = False
         assert bool(dbad[row, other].isfinite().all())
+
+
+def test_forward_mode_and_traces_are_refused(dev):
+    """A dual tensor's tangent would be lost, and a trace would record none of the kernels."""
+    import torch.autograd.forward_ad as fw
+    from lifscan import hip_linattn as LA
+    from lifscan import hip_lm as LM
+    x, w, q = torch.randn(4, 8, device=dev), torch.ones(8, device=dev), torch.randn(4, 1, 2, 8, device=dev)
+    s, b = torch.zeros(1, 2, 8, 8, device=dev), torch.full((2,), 0.9, device=dev)
+    tok = torch.zeros(3, dtype=torch.int64, device=dev)
+    idx = torch.zeros(4, 2, dtype=torch.int64, device=dev)
+    calls = [
+        (lambda *a: LA.lin_attn(*a)[0], (q, q, q, b, s)),
+        (lambda *a: LA.lin_attn_step(*a), (q[0], q[0], q[0], b, s)),
+        (lambda *a: LM.block_norm(*a)[0], (x, x, w, w, x, w)),
+        (lambda a: LM.embed(tok, a), (x,)),
+        (lambda a, v: LM.distill_topk(a, v, idx), (x, x[:, :2].contiguous())),
+    ]
+    for f, args in calls:
+        f(*args)
+        for i in range(len(args)):
+            with fw.dual_level():
+                duals = [fw.make_dual(t, torch.ones_like(t)) if i == j else t for j, t in enumerate(args)]
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    f(*duals)
+        with pytest.raises(RuntimeError, match="trace"):
+            torch.jit.trace(f, args, check_trace=False)
+        f(*args)
+
+
+def test_gradients_that_arrive_in_other_forms(dev):
+    """A dual gradient is refused in the backward too."""
+    import torch.autograd.forward_ad as fw
+    from lifscan import hip_linattn as LA
+    from lifscan import hip_lm as LM
+    x, q = torch.randn(4, 8, device=dev), torch.randn(4, 1, 2, 8, device=dev)
+    w = torch.ones(8, device=dev)
+    tok, idx = torch.zeros(3, dtype=torch.int64, device=dev), torch.zeros(4, 2, dtype=torch.int64, device=dev)
+    for f, a in ((lambda a: LA.lin_attn(a, a, a, 0.9)[0], q), (lambda a: LM.block_norm(a, a, w, w)[1], x),
+                 (lambda a: LM.embed(tok, a), x), (lambda a: LM.distill_topk(a, x[:, :2], idx), x)):
+        a = a.clone().requires_grad_(True)
+        out = f(a)
+        g = torch.randn_like(out)
+        with fw.dual_level():
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                torch.autograd.grad(out, a, fw.make_dual(g, g))
