@@ -89,13 +89,14 @@ bool grad_wanted(std::initializer_list<Tensor> ts) {
   return false;
 }
 // What looks at the calls from outside sees none of the kernels: a trace would record outputs that nothing fills,
-// and a forward-mode tangent would be lost.
+// a forward-mode tangent would be lost, and the values behind a lazily negated view have the other sign.
 template <class Tensors>
 void check_plain(const char* what, const Tensors& ts) {
   TORCH_CHECK(!torch::jit::tracer::isTracing(), what, " cannot be recorded by a trace (torch.jit.trace)");
   for (const Tensor& t : ts) {
     if (!t.defined()) continue;
     TORCH_CHECK(!t._fw_grad(0).defined(), what, " has no forward-mode derivatives");
+    TORCH_CHECK_VALUE(!t.is_neg(), what, ": an argument is a lazily negated view (pass its resolve_neg())");
   }
 }
 void check_plain(const char* what, std::initializer_list<Tensor> ts) {
@@ -105,9 +106,11 @@ Tensor of(const Maybe& t) { return t.has_value() ? *t : Tensor(); }
 // autograd functions take no undefined tensors
 Maybe maybe(const Tensor& t) { return t.defined() ? Maybe(t) : Maybe(); }
 
-// The kernels' gradients have no graph of their own.
+// The kernels' gradients have no graph of their own.  What arrives may be a lazily negated view.
 variable_list first_order(variable_list grads) {
   TORCH_CHECK(!at::GradMode::is_enabled(), "the language-model operators have no second derivatives (create_graph)");
+  for (Tensor& t : grads)
+    if (t.defined() && t.is_neg()) t = t.resolve_neg();
   check_plain("a language-model operator's gradient", grads);
   return grads;
 }

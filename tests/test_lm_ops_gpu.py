@@ -604,7 +604,7 @@ def test_forward_mode_and_traces_are_refused(dev):
 
 
 def test_gradients_that_arrive_in_other_forms(dev):
-    """A dual gradient is refused in the backward too."""
+    """A dual gradient is refused in the backward too; a lazily negated one is read with its sign."""
     import torch.autograd.forward_ad as fw
     from lifscan import hip_linattn as LA
     from lifscan import hip_lm as LM
@@ -616,6 +616,13 @@ def test_gradients_that_arrive_in_other_forms(dev):
         a = a.clone().requires_grad_(True)
         out = f(a)
         g = torch.randn_like(out)
+        (want,) = torch.autograd.grad(out, a, -g, retain_graph=True)
+        (got,) = torch.autograd.grad(out, a, torch._neg_view(g), retain_graph=True)
+        assert torch.equal(got, want)
         with fw.dual_level():
             with pytest.raises(RuntimeError, match="forward-mode"):
                 torch.autograd.grad(out, a, fw.make_dual(g, g))
+    for f in (lambda: LM.block_norm(torch._neg_view(x), x, w, w), lambda: LA.lin_attn(q, torch._neg_view(q), q, 0.9),
+              lambda: LM.embed(tok, torch._neg_view(x)), lambda: LM.distill_topk(torch._neg_view(x), x[:, :2], idx)):
+        with pytest.raises(ValueError):
+            f()
