@@ -280,8 +280,9 @@ std::tuple<Tensor, Tensor> lin_attn(const Tensor& q, const Tensor& k, const Tens
 Tensor lin_attn_step(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& beta, const Tensor& state,
                      double scale) {
   check_plain("lin_attn_step", {q, k, v, beta, state});
-  TORCH_CHECK_VALUE(!grad_wanted({q, k, v, state}),
-                    "lin_attn_step has no gradients: call it under torch.no_grad, or lin_attn");
+  TORCH_CHECK_VALUE(!grad_wanted({q, k, v, beta, state}),
+                    "lin_attn_step has no gradients (q, k, v, beta or the state asks for one): call it under "
+                    "torch.no_grad, or lin_attn");
   Attn r = attn(q, k, v, beta, scale, 3);
   r.check_state(state, "state");
   TORCH_CHECK_VALUE(state.is_contiguous(), "state must be contiguous: it is updated in place");

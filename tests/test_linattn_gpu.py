@@ -616,3 +616,15 @@ def test_slow_decays_of_long_sequences_do_not_drift(dev, dtype):
     want = s0.double() * beta.double()[:, None, None] ** T
     err = (s.double().cpu() - want).abs() / want
     assert float(err.max()) <= 24 * 2.0 ** -24, [float(e) / 2.0 ** -24 for e in err.amax((0, 2, 3))]
+
+
+def test_step_refuses_a_decay_that_asks_for_a_gradient(dev):
+    from lifscan import hip_linattn as LA
+    q, s = torch.randn(2, 2, 8, device=dev), torch.zeros(2, 2, 8, 8, device=dev)
+    b = torch.full((2,), 0.9, device=dev, requires_grad=True)
+    with pytest.raises(ValueError, match="beta"):
+        LA.lin_attn_step(q, q, q, b, s)
+    assert bool((s == 0).all())
+    with torch.no_grad():
+        LA.lin_attn_step(q, q, q, b, s)
+    assert not bool((s == 0).all())
