@@ -13,8 +13,9 @@ token by token: ``forward(tokens, state)`` takes and returns the state (the matr
 membranes), ``step`` is its form for one token.  ``loss`` is the distillation from a teacher's top
 logits, the usual way to train spiking language models.
 
-Training runs the exact scan layers with the surrogate gradient (``lif_auto``) from resting neurons; with
-a state, and without gradients, the serial forward carries the membranes.
+Training runs the exact scan layers with the surrogate gradient (``lif_auto``) from resting neurons and
+returns no state.  Without gradients (``torch.no_grad``, or a call with a state, which has none) the serial
+forward carries the membranes, and every call returns the state after it.
 """
 import torch
 import torch.nn as nn
@@ -60,20 +61,22 @@ class Block(nn.Module):
         return LM.block_norm(x, y, self.spike_post, self.spike_pre, res_scale=self.spike_scale)
 
     def forward(self, x, z, state=None):
-        """x (fp32), z [T, B, D] -> x, z, the state after the last row.  state: (matrix states, membranes)
-        or None for a start at rest; only a call with a state carries the membranes on."""
+        """x (fp32), z [T, B, D] -> x, z, the state after the last row (None with gradients).  state: (matrix
+        states, membranes) or None for a start at rest."""
         T, B, _ = x.shape
         o, S = LA.lin_attn(*self._split(z), self.decay, s0=state and state[0], scale=self.dk ** -0.5)
         x, z = self._mixed(x, z, o)
         currents = self.up(z.float()).view(T, -1)
-        if state is None:
-            u = None
-            s = L.lif_auto(currents, currents.new_zeros(currents.shape[1]), self.beta, THETA, RESET, SURROGATE)
+        rest = currents.new_zeros(currents.shape[1])
+        if torch.is_grad_enabled():
+            after = None
+            s = L.lif_auto(currents, rest, self.beta, THETA, RESET, SURROGATE)
         else:
-            U, s = L.serial_forward(currents, self.beta, THETA, RESET, state[1])
-            u = U[-1]
+            u = state[1] if state else rest
+            U, s = L.serial_forward(currents, self.beta, THETA, RESET, u)
+            after = S, U[-1] if T else u
         x, z = self._spiked(x, s.view(T, B, -1))
-        return x, z, (S, u)
+        return x, z, after
 
     def step(self, x, z, state):
         """One token: x, z [B, D]; the matrix states are updated in place."""
@@ -99,6 +102,21 @@ class SpikeLM(nn.Module):
         like = self.table
         return [(like.new_zeros(B, b.heads, b.dk, b.dv), like.new_zeros(B * b.up.out_features)) for b in self.blocks]
 
+    def _check_state(self, state, B, in_place=False):
+        """Before anything is changed: a state of B sequences, whole."""
+        def fits(t, shape):
+            return torch.is_tensor(t) and tuple(t.shape) == shape and t.dtype == torch.float32 \
+                and t.device == self.table.device
+
+        if len(state) != len(self.blocks):
+            raise ValueError(f"a state of {len(self.blocks)} blocks is needed, got {len(state)}")
+        for i, (s, b) in enumerate(zip(state, self.blocks)):
+            shapes = (B, b.heads, b.dk, b.dv), (B * b.up.out_features,)
+            if s is None or len(s) != 2 or not all(fits(t, n) for t, n in zip(s, shapes)) \
+                    or in_place and not s[0].is_contiguous():
+                raise ValueError(f"block {i}: the state must be a matrix state {shapes[0]} and membranes {shapes[1]}, "
+                                 f"as a call without gradients returns them")
+
     def _start(self, tokens):
         e = LM.embed(tokens, self.table, scale=self.D ** 0.5).to(self.dtype)
         return LM.block_norm(torch.zeros(e.shape, device=e.device), e, self.start_post, self.start_pre)
@@ -107,18 +125,23 @@ class SpikeLM(nn.Module):
         return F.linear(z, self.table.to(self.dtype))
 
     def forward(self, tokens, state=None):
-        """tokens [T, B] -> logits [T, B, vocab], and the state after the last token.  state: as returned
-        (or ``state(B)``), to continue sequences without gradients; None in training."""
-        x, z = self._start(tokens)
-        after = []
-        for i, block in enumerate(self.blocks):
-            x, z, s = block(x, z, None if state is None else state[i])
-            after.append(s)
-        return self._logits(z), after
+        """tokens [T, B] -> logits [T, B, vocab], and the state after the last token (None with gradients).
+        state: as returned (or ``state(B)``), to continue sequences, without gradients; None: from their
+        start."""
+        if state is not None:
+            self._check_state(state, tokens.shape[1])
+        with torch.set_grad_enabled(torch.is_grad_enabled() and state is None):
+            x, z = self._start(tokens)
+            after = []
+            for i, block in enumerate(self.blocks):
+                x, z, s = block(x, z, None if state is None else state[i])
+                after.append(s)
+            return self._logits(z), None if torch.is_grad_enabled() else after
 
     @torch.no_grad()
     def step(self, tokens, state):
         """One token of each sequence: tokens [B] -> logits [B, vocab]; `state` is updated in place."""
+        self._check_state(state, tokens.shape[0], in_place=True)
         x, z = self._start(tokens)
         for i, block in enumerate(self.blocks):
             x, z, state[i] = block.step(x, z, state[i])

@@ -50,3 +50,38 @@ def test_training_by_distillation(dev, dtype):
         opt.step()
         losses.append(float(loss.detach()))
     assert losses[-1] < 0.7 * losses[0], losses
+
+
+def test_a_prompt_then_its_next_tokens(dev):
+    """The state that forward returns without gradients continues the sequence, token by token or in pieces."""
+    model = _model(dev)
+    tokens = torch.randint(0, 200, (45, 2), generator=torch.Generator().manual_seed(1)).to(dev)
+    with torch.no_grad():
+        whole, _ = model(tokens, model.state(2))
+        prompt, state = model(tokens[:30])
+        piece, state = model(tokens[30:40], state)
+        last = [model.step(tokens[t], state) for t in range(40, 45)]
+    pieces = torch.cat([prompt, piece, torch.stack(last)])
+    assert float((pieces - whole).abs().max()) < 1e-4 * float(whole.abs().max())
+
+
+def test_states_that_do_not_continue_a_sequence(dev):
+    """Training returns no state; a state that is not whole is refused before any of it is changed; a call with a
+    state has no gradients."""
+    model = _model(dev)
+    tokens = torch.randint(0, 200, (5, 2), generator=torch.Generator().manual_seed(1)).to(dev)
+    logits, state = model(tokens)
+    assert logits.requires_grad and state is None
+    with torch.no_grad():
+        _, good = model(tokens, model.state(2))
+    S = good[0][0].clone()
+    for bad in ([good[0], (good[1][0], None)], good[:1], [good[0], (good[1][0][:1], good[1][1])],
+                [good[0], (good[1][0], good[1][1][:-1])], [good[0], None],
+                [good[0], (good[1][0].double(), good[1][1])], [good[0], (good[1][0], good[1][1].cpu())]):
+        with pytest.raises(ValueError):
+            model.step(tokens[0], list(bad))
+        with pytest.raises(ValueError):
+            model(tokens, list(bad))
+    assert torch.equal(S, good[0][0])
+    logits, _ = model(tokens, good)
+    assert not logits.requires_grad
