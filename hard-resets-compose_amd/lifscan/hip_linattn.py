@@ -40,7 +40,9 @@ def lin_attn(q, k, v, beta, s0=None, scale=1.0):
     right as far as fp32 holds its state; above 4 it is walked row by row.)  s0: the fp32 state before the
     first row, or None (zeros).  A decay gets no gradient; a negative one on the device gives NaN.
 
-    A value of v that is not finite reaches its own row and the later ones, and no earlier row."""
+    A value of v, or an element of s0, that is not finite reaches its own row and the later ones in its
+    column, and no earlier row.  What it reaches is not finite, but which of NaN and infinity it is is
+    not that of the recurrence: sums run in other orders, and 16-bit products take values in parts."""
     return _n.lm_ops().lin_attn(q, k, v, _decays(beta, q, k, v), s0, scale)
 
 

@@ -522,6 +522,8 @@ int lsh_alif_bwd_recompute(const float* I, const float* U, const float* W, const
  *   S_t = beta[h]*S_{t-1} + k_t v_t^T,  o_t = scale * q_t^T S_t,  S a [Dk, Dv] matrix per (b, h).
  * H query/state heads; q_heads, k_heads and v_heads divide H, head h reads head h/(H/heads).
  * beta: [H] fp32 on the device, 0 <= beta (a head whose decay is not gives NaN).  s0: [B, H, Dk, Dv] fp32 or NULL (zeros).
+ * What depends on a value that is not finite is not finite, and nothing else; NaN may stand where the
+ * recurrence has an infinity (not in lsh_linattn_step, which is the recurrence).
  * o: contiguous [T, B, H, Dv].  s_end: the state after the last row, [B, H, Dk, Dv], or NULL;
  * 1 <= Dk, Dv <= LSH_LINATTN_MAX_D; T = 0 is allowed (s_end = s0). */
 #define LSH_LINATTN_MAX_D 256

@@ -628,3 +628,19 @@ def test_step_refuses_a_decay_that_asks_for_a_gradient(dev):
     with torch.no_grad():
         LA.lin_attn_step(q, q, q, b, s)
     assert not bool((s == 0).all())
+
+
+@pytest.mark.parametrize("dtype", list(U), ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("T,H", [(100, 600), (300, 1)])
+def test_infinite_values_reach_what_depends_on_them(dev, dtype, T, H):
+    """An infinite value, or element of the first state: its column from its row on (the state's element alone) is
+    not finite, whole and in segments, and nothing else."""
+    from lifscan import hip_linattn as LA
+    q, k, v, beta, s0, _, _ = _inputs(dtype, T, 1, (1, 1, 1), H, 32, 48, dev, seed=79)
+    v[20, 0, 0, 5], v[T - 1, 0, 0, 11] = float("inf"), float("-inf")
+    s0[0, 0, 3, 9] = float("inf")
+    o, s = LA.lin_attn(q, k, v, beta, s0=s0, scale=0.1)
+    want_o, want_s = torch.ones_like(o, dtype=torch.bool), torch.ones_like(s, dtype=torch.bool)
+    want_o[20:, 0, :, 5] = want_o[T - 1, 0, :, 11] = want_o[:, 0, 0, 9] = False
+    want_s[0, :, :, 5] = want_s[0, :, :, 11] = want_s[0, 0, 3, 9] = False
+    assert torch.equal(o.isfinite(), want_o) and torch.equal(s.isfinite(), want_s)
