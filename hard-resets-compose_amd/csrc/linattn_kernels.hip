@@ -192,8 +192,8 @@ static int la_check(const lsh_linattn* a) {
   if (a->H > 0) {
     for (int n : {a->q_heads, a->k_heads, a->v_heads})
       if (n < 1 || a->H % n) return LSH_ERR_SHAPE;
-    if (a->B > 0 && a->T > 0 && (bad_ptr(a->q) || bad_ptr(a->k) || bad_ptr(a->v) || bad_ptr(a->beta)))
-      return LSH_ERR_ARG;
+    if (a->B > 0 && (bad_ptr(a->beta) || (a->T > 0 && (bad_ptr(a->q) || bad_ptr(a->k) || bad_ptr(a->v)))))
+      return LSH_ERR_ARG;  // the decays are read without rows too
   }
   return LSH_OK;
 }

@@ -101,3 +101,13 @@ def test_more_threads_than_a_grid_holds_are_refused():
     assert L.lsh_embed_fwd(1, P, P, P, 2 ** 26, 8, 512, -1, 1.0, None) == SHAPE
     assert L.lsh_distill_fwd(1, P, 8, 0, P, P, P, P, 2 ** 24, 8, 1, 1.0, None, 0, None) == SHAPE
     assert L.lsh_distill_bwd(1, P, 8, 0, P, P, P, P, 1, P, 2 ** 24, 8, 1, 1.0, None) == SHAPE
+
+
+def test_linattn_without_rows_still_needs_decays():
+    """The walk reads its head's decay before it looks for rows."""
+    from lifscan import _native as n
+    L = n.lib()
+    none = dict(T=0, q=None, k=None, v=None, beta=None)
+    assert L.lsh_linattn_fwd(_attn(**none), None, 0, None) == ARG
+    assert L.lsh_linattn_bwd(_attn(**none), None, None, 1, 1, 1, None, None, None, None, None, None, 0, None) == ARG
+    assert L.lsh_linattn_fwd(_attn(**none, B=0), None, 0, None) == 0
