@@ -79,7 +79,7 @@ __device__ __forceinline__ void es_read(int (&v)[kEsPer], const int64_t* __restr
   for (int j = 0; j < kEsPer; ++j) {
     const int i = t0 + j * kEsThreads + threadIdx.x;
     const int64_t x = i < end ? tok[i] : -1;
-    v[j] = (uint64_t)x < (uint64_t)V && (int)x != (int)pad ? (int)x : -1;
+    v[j] = (uint64_t)x < (uint64_t)V && x != pad ? (int)x : -1;
   }
 }
 

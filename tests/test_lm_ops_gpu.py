@@ -626,3 +626,21 @@ def test_gradients_that_arrive_in_other_forms(dev):
               lambda: LM.embed(tok, torch._neg_view(x)), lambda: LM.distill_topk(torch._neg_view(x), x[:, :2], idx)):
         with pytest.raises(ValueError):
             f()
+
+
+def test_embed_padding_beyond_32_bits(dev):
+    """A padding id that no token of the table has takes no row away, whatever its lower 32 bits."""
+    from lifscan import _native as n
+    L = n.lib()
+    V, D = 10, 8
+    tok = torch.tensor([3, 3, 5, 0], device=dev)
+    W, dout = torch.randn(V, D, device=dev), torch.randn(4, D, device=dev)
+    out, dW = torch.empty(4, D, device=dev), torch.empty(V, D, device=dev)
+    nb = L.lsh_embed_bwd_workspace(4, V)
+    ws = torch.empty(nb, dtype=torch.uint8, device=dev)
+    st = n.stream_of(W)
+    for pad in (2 ** 32 + 3, -(2 ** 32) + 5, 2 ** 32 - 1):
+        assert L.lsh_embed_fwd(0, n.ptr(tok), n.ptr(W), n.ptr(out), 4, V, D, pad, 1.0, st) == 0
+        assert L.lsh_embed_bwd(0, n.ptr(tok), n.ptr(dout), n.ptr(dW), 4, V, D, pad, 1.0, n.ptr(ws), nb, st) == 0
+        assert torch.equal(out, W[tok])
+        assert torch.equal(dW[3], dout[0] + dout[1]) and torch.equal(dW[5], dout[2]) and torch.equal(dW[0], dout[3])
