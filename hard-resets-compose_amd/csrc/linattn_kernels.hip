@@ -72,6 +72,12 @@ static int la_go(const LaWalks& all, int dtype, bool sums, hipStream_t st) {
          : dtype == LSH_BF16 ? la_launch_bf16(all, sums, st)
                              : la_launch_f16(all, sums, st);
 }
+// Whether the walks' threads fit one launch.
+static bool la_fits(const LaWalks& all, int dtype) {
+  const LaWalk& a = all.w[0];
+  const int block = la_block(dtype, a.DK, a.DV);
+  return lm_grid_ok(a.B * a.H * a.segs * la_blocks(all, block) * all.n, block * 4);
+}
 static int la_go(const LaWalk& a, int dtype, bool sums, hipStream_t st) {
   LaWalks all = {};
   all.w[0] = a;
@@ -315,9 +321,14 @@ extern "C" int lsh_linattn_bwd(const lsh_linattn* a, const void* starts, const v
   all.w[0] = w_q, all.w[1] = w_k, all.w[2] = w_v;
   const bool alike = la_rows(w_v.DK) == la_rows(w_q.DK) && la_block(a->dtype, w_v.DK, w_v.DV) == la_block(a->dtype, w_q.DK, w_q.DV);
   all.n = alike ? 3 : 2;
-  if (int rc = la_go(all, a->dtype, false, st)) return rc;
-  if (!alike)
-    if (int rc = la_go(w_v, a->dtype, false, st)) return rc;
+  if (la_fits(all, a->dtype)) {
+    if (int rc = la_go(all, a->dtype, false, st)) return rc;
+    if (!alike)
+      if (int rc = la_go(w_v, a->dtype, false, st)) return rc;
+  } else {  // more pairs than a launch of several walks has threads for: one after the other, as the forward's
+    for (const LaWalk& x : all.w)
+      if (int rc = la_go(x, a->dtype, false, st)) return rc;
+  }
   LaShares shares = {};
   int count = 0;
   int64_t most = 0;

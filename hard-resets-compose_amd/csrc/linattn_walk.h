@@ -749,6 +749,14 @@ inline bool la_wide(const LaWalk& a, int chunk) {
 // State rows that a kernel is built for, by the walk's DK.
 inline int la_rows(int DK) { return DK <= 64 ? 64 : DK <= 128 ? 128 : 256; }
 
+// Blocks of columns of the walk that has most.
+inline int la_blocks(const LaWalks& all, int block) {
+  int most = 0;
+  for (int i = 0; i < all.n; ++i)
+    if (const int n = (all.w[i].DV + block - 1) / block; n > most) most = n;
+  return most;
+}
+
 // Launches walks of one la_rows and la_block (their sums: SUMS) for operands of T computed in L.
 template <class T, class L>
 inline int la_launch(const LaWalks& all, bool sums, hipStream_t st) {
@@ -758,11 +766,8 @@ inline int la_launch(const LaWalks& all, bool sums, hipStream_t st) {
   constexpr int dtype = sizeof(L) == 2 ? LSH_BF16 : LSH_F32;
   const int block = la_block(dtype, a.DK, a.DV);
   bool wide = true;
-  int blocks = 0;
-  for (int i = 0; i < all.n; ++i) {
-    wide = wide && la_wide(all.w[i], La<L>::C);
-    blocks = blocks > (all.w[i].DV + block - 1) / block ? blocks : (all.w[i].DV + block - 1) / block;
-  }
+  const int blocks = la_blocks(all, block);
+  for (int i = 0; i < all.n; ++i) wide = wide && la_wide(all.w[i], La<L>::C);
   if (!lm_grid_ok(n * blocks * all.n, block * 4)) return LSH_ERR_SHAPE;
   const dim3 grid((unsigned)(n * blocks * all.n));
   auto go = [&](auto dkp, auto waves) {

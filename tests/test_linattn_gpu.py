@@ -644,3 +644,22 @@ def test_infinite_values_reach_what_depends_on_them(dev, dtype, T, H):
     want_o[20:, 0, :, 5] = want_o[T - 1, 0, :, 11] = want_o[:, 0, 0, 9] = False
     want_s[0, :, :, 5] = want_s[0, :, :, 11] = want_s[0, 0, 3, 9] = False
     assert torch.equal(o.isfinite(), want_o) and torch.equal(s.isfinite(), want_s)
+
+
+def test_more_pairs_than_one_launch_of_the_three_walks_holds(dev):
+    """What the forward takes the gradients take: 6 million (batch, head) pairs, whose three walks have too many
+    threads for one launch."""
+    from lifscan import hip_linattn as LA
+    T, B, H = 2, 3 << 20, 2
+    q, k, v, do = (torch.rand(T, B, H, 1, device=dev, generator=torch.Generator(dev).manual_seed(i)) for i in range(4))
+    beta = torch.tensor([0.5, 0.25], device=dev)
+    ins = [t.requires_grad_(True) for t in (q, k, v)]
+    o, s = LA.lin_attn(*ins, beta)
+    dq, dk, dv = torch.autograd.grad(o, ins, do)
+    q, k, v = (t.detach() for t in (q, k, v))
+    b = beta[:, None]
+    kv = k * v
+    S1 = b * kv[0] + kv[1]
+    G0 = q[0] * do[0] + b * q[1] * do[1]
+    for got, want in ((o[1], q[1] * S1), (s[..., 0], S1), (dq[1], S1 * do[1]), (dk[0], G0 * v[0]), (dv[0], G0 * k[0])):
+        assert float((got.detach() - want).abs().max()) < 1e-6
