@@ -581,7 +581,8 @@ int lsh_block_norm_bwd(const lsh_block_norm* a, const void* gx, const void* gz, 
 
 /* Embedding lookup: out[i] = scale * weight[tokens[i]] ([n, D] from [V, D]); rows of `padding` (-1: no
  * padding id) and of ids outside 0..V-1 are zero.  The gradient dweight [V, D] = scale * the sum of
- * dout over each token's positions, in fp32 and position order (every row is written). */
+ * dout over each token's positions, in fp32 and an order that depends on the tokens alone (every row is
+ * written). */
 int lsh_embed_fwd(int dtype, const int64_t* tokens, const void* weight, void* out, int64_t n, int64_t V,
                   int64_t D, int64_t padding, float scale, void* stream);
 size_t lsh_embed_bwd_workspace(int64_t n, int64_t V);

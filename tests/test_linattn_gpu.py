@@ -663,3 +663,55 @@ def test_more_pairs_than_one_launch_of_the_three_walks_holds(dev):
     G0 = q[0] * do[0] + b * q[1] * do[1]
     for got, want in ((o[1], q[1] * S1), (s[..., 0], S1), (dq[1], S1 * do[1]), (dk[0], G0 * v[0]), (dv[0], G0 * k[0])):
         assert float((got.detach() - want).abs().max()) < 1e-6
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("first", ["none", "aligned", "odd_offset"])
+def test_many_states_in_segments(dev, dtype, first):
+    """2^19 state elements in eight segments (fp32) and eleven, joined four elements and eight segments at a time; a
+    first state that does not begin at a multiple of 16 bytes is joined one by one.  A decay of its own for each head."""
+    T, B, H, Dk, Dv = 700, 2, 16, 128, 128
+    print(f"linattn join {dtype} {first}", flush=True)
+    q, k, v, beta, s0, do, ds = _inputs(dtype, T, B, (H,) * 3, H, Dk, Dv, dev, seed=83)
+    if first == "none":
+        s0 = None
+    elif first == "odd_offset":
+        s0 = torch.cat([s0.flatten()[:1], s0.flatten()])[1:].view(s0.shape)
+    got = run_all(q, k, v, beta, s0, 0.1, do, ds)
+    want = reference(q, k, v, beta, s0, 0.1, do, ds)
+    most = _absolute(q, k, v, beta, s0, 0.1, do, ds)
+    for g, w, m in zip(got, want, most):
+        check(g, w, m, dtype, T, Dk)
+
+
+@pytest.mark.parametrize("T,H,Dk,Dv", [(150, 2, 129, 256), (150, 1, 256, 140), (40, 2, 200, 130)])
+def test_walks_of_unequal_column_blocks_in_one_launch(dev, T, H, Dk, Dv):
+    """fp32 gradients whose walks have three and four (four and three) blocks of columns."""
+    q, k, v, beta, s0, do, ds = _inputs(torch.float32, T, 2, (H,) * 3, H, Dk, Dv, dev, seed=89)
+    got = run_all(q, k, v, beta, s0, 0.1, do, ds)
+    want = reference(q, k, v, beta, s0, 0.1, do, ds)
+    most = _absolute(q, k, v, beta, s0, 0.1, do, ds)
+    for g, w, m in zip(got, want, most):
+        check(g, w, m, torch.float32, T, 256)
+
+
+@pytest.mark.parametrize("qk,vv", [(2.0 ** -10, 1.0), (1.0, 2.0 ** -20), (2.0 ** -8, 2.0 ** -18), (1e4, 1.0), (1.0, 3000.0)])
+def test_fp16_states_and_scores_hold_22_bits_at_any_size(dev, qk, vv):
+    """fp16 operands far below (and above) one: states, outputs and gradients that are scaled back to about one.
+    An output is off by its own rounding and 2^-22 of its terms for a score's and a state's parts, a state by 2^-22
+    for the decayed values' parts; both by fp32 sums.  Parts that were not scaled would leave 2^-25 of an absolute
+    size to each, which at values of 2^-20 is 2^-5 of them."""
+    dtype, T, H, D = torch.float16, 150, 2, 64
+    q, k, v, beta, s0, do, ds = _inputs(dtype, T, 1, (H,) * 3, H, D, D, dev, seed=97)
+    q, k, v, s0 = q * qk ** 0.5, k * qk ** 0.5, v * vv, s0 * (qk ** 0.5 * vv)
+    scale = 2.0 ** -4 / (qk * vv)
+    do, ds = do * min(vv * qk ** 0.5 * 2.0 ** 4, 1.0), ds * min(1.0 / (qk ** 0.5 * vv), 2.0 ** 8)
+    got = run_all(q, k, v, beta, s0, scale, do, ds)
+    want = reference(q, k, v, beta, s0, scale, do, ds)
+    most = _absolute(q, k, v, beta, s0, scale, do, ds)
+    for x, w, m in zip(got, want, most):
+        assert x.dtype != dtype or float(w.abs().max()) < 65504
+        small = 2.0 ** -25 if x.dtype == dtype else 0.0  # half of fp16's smallest step
+        err = (x.detach().double().cpu() - w).abs()
+        bound = U[x.dtype] * w.abs() + (2 * 2.0 ** -22 + (T + D + 64) * 2.0 ** -24) * m + small
+        assert bool((err <= bound).all()), float((err / bound.clamp(min=1e-300)).max())
