@@ -66,16 +66,17 @@ class Block(nn.Module):
         T, B, _ = x.shape
         o, S = LA.lin_attn(*self._split(z), self.decay, s0=state and state[0], scale=self.dk ** -0.5)
         x, z = self._mixed(x, z, o)
-        currents = self.up(z.float()).view(T, -1)
-        rest = currents.new_zeros(currents.shape[1])
-        if torch.is_grad_enabled():
-            after = None
-            s = L.lif_auto(currents, rest, self.beta, THETA, RESET, SURROGATE)
+        currents = self.up(z.float()).flatten(1)
+        u = state[1] if state else currents.new_zeros(currents.shape[1])
+        if T == 0:
+            s = currents  # the neurons take one row at least
+        elif torch.is_grad_enabled():
+            s = L.lif_auto(currents, u, self.beta, THETA, RESET, SURROGATE)
         else:
-            u = state[1] if state else rest
             U, s = L.serial_forward(currents, self.beta, THETA, RESET, u)
-            after = S, U[-1] if T else u
-        x, z = self._spiked(x, s.view(T, B, -1))
+            u = U[-1].clone()  # not a view that keeps all rows
+        after = None if torch.is_grad_enabled() else (S, u)
+        x, z = self._spiked(x, s.unflatten(1, (B, -1)))
         return x, z, after
 
     def step(self, x, z, state):

@@ -85,3 +85,20 @@ def test_states_that_do_not_continue_a_sequence(dev):
     assert torch.equal(S, good[0][0])
     logits, _ = model(tokens, good)
     assert not logits.requires_grad
+
+
+def test_no_tokens(dev):
+    """A sequence without tokens: no logits, the state that it began with, gradients of zero."""
+    model = _model(dev)
+    none = torch.zeros(0, 2, dtype=torch.int64, device=dev)
+    logits, state = model(none)
+    assert logits.shape == (0, 2, 200) and state is None
+    logits.sum().backward()
+    assert all(p.grad is None or bool((p.grad == 0).all()) for p in model.parameters())
+    with torch.no_grad():
+        logits, state = model(none)
+        assert logits.shape == (0, 2, 200) and all(bool((t == 0).all()) for s in state for t in s)
+        _, good = model(torch.ones(3, 2, dtype=torch.int64, device=dev))
+        _, same = model(none, good)
+    for a, b in zip(good, same):
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
