@@ -96,9 +96,10 @@ static LaSplit la_split(int dtype, int64_t T, int64_t BH, int DK, int DV) {
   const int64_t C = la_chunk(), chunks = (T + C - 1) / C;
   const int block = la_block(dtype, DK, DV);
   const int64_t groups = BH * ((DV + block - 1) / block);
-  // LDS holds two workgroups a CU in 16 bits, one in fp32 from 65 state rows on.  Measured with 256 and 512
-  // workgroups: bf16 4096 x 4 x 16 x 128 forward 137 and 127 us, fp32 2048 x 4 x 16 x 128 168 and 183 us.
-  const int64_t fill = dtype != LSH_F32 || std::max(DK, DV) <= 64 ? 512 : 256;
+  // LDS holds two workgroups a CU up to 128 state rows in 16 bits, up to 64 in fp32, and one above.  Measured with 256
+  // and 512 workgroups, forward: bf16 4096 x 4 x 16 x 128 142 and 138 us, fp32 2048 x 4 x 16 x 128 152 and 169, bf16
+  // 4096 x 16 x 256 x 256 130 and 147.
+  const int64_t fill = std::max(DK, DV) <= (dtype == LSH_F32 ? 64 : 128) ? 512 : 256;
   int64_t segs = std::min<int64_t>((fill + groups - 1) / std::max<int64_t>(groups, 1), chunks / 2);
   if (segs < 2) return {1, std::max<int64_t>(T, 1)};
   const int64_t per = (chunks + segs - 1) / segs;
