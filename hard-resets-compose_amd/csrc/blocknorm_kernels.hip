@@ -219,7 +219,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * 64) void k_block_norm(BnArgs a) 
 // h = a*act*n it is <h*dx>/ry, whose sums do not, so a row has two reductions.
 // HOLD: a row is read once, ahead, while the one before is worked on; without it (rows of more than 4096
 // channels, which do not fit the registers) each sweep over the row reads it, mostly from the caches (bf16
-// 2048 x 8192: 87 us, held 106 with spilled registers; 2048 x 16384: 189, with all sums in registers 417).
+// 2048 x 8192: 89 us, held 106 with spilled registers; 2048 x 16384: 196, with all sums in registers 417).
 //
 // What bounds it next to the bytes are the instructions a row (376 vector ones a wave of 64 x 4 columns):
 // hence buffer accesses whose bounds replace selects and branches, sums over lanes without LDS, and a
@@ -401,8 +401,11 @@ static void with_types(int tx, int ty, F&& f) {
 // Gradients: what a wave does once a row (reductions, roots) is a third of its instructions with pieces of
 // 4 and a sixth with 8, which take 158 registers instead of 91.  Rows of 257 to 2048 channels in wide
 // accesses leave room for 3 waves a SIMD with 8 (bf16 8192 x 2048: 48 us, with 4 60).  Narrower rows would
-// leave lanes idle, wider ones are one workgroup a CU (4096 x 4096 with the sums: 83 us, with 4 78), and
-// element by element 8 take 190 registers.
+// leave lanes idle, and element by element 8 take 190 registers.  Wider ones are one workgroup a CU, where 8 gain in
+// some types what they lose in others (whole calls: bf16 4096 x 4096 101 us, with 4 103; 8192 x 2560 bf16 146 and 151,
+// with an fp32 stream 180 and 171).  One workgroup a CU is also what bounds them: nothing runs while it waits at a
+// row's two barriers (bf16 4096 x 4096 64 us and 4 for the sums, 2048 x 8192 89 and 6), and above 8192 channels 1024
+// threads leave 128 registers, of which 6 to 64 too few (2048 x 16384: 196 and 10).
 template <bool BWD, bool WIDE, class F>
 static void with_row(int D, F&& f) {
   using std::integral_constant;

@@ -10,8 +10,9 @@
 // their sum would round by a share of the logits' size where only their differences matter.)  The
 // forward reads the logits once, with the running maximum and sum of the softmax, and keeps m, l and the
 // teacher's two; the backward reads them once more and writes dz.  Both are bound by the logits' bytes:
-// 4096 x 32000 bf16 with 64 entries 47 us forward (262 MB, 5.6 TB/s) and 122 backward (524 MB, 4.3 TB/s).  A row is split over several workgroups where there
-// are too few rows for the chip, and the parts' maxima and sums are joined in order.
+// 4096 x 32000 bf16 with 64 entries, one after the other in training, 81 us forward (262 MB; 53 where no gradient of
+// before is still on its way to memory) and 92 backward (524 MB): 4.5 TB/s over both.  A row is split over several
+// workgroups where there are too few rows for the chip, and the parts' maxima and sums are joined in order.
 #include <algorithm>
 
 #include "lsh_lm.h"
@@ -186,8 +187,8 @@ __global__ __launch_bounds__(64) void k_distill_join(DsArgs a) {
 
 // dz of a part of a row, then the teacher's entries in it once more with their p.  An id may come several
 // times; its p are summed in order by the first.  A bit for each place (modulo kDsBits) tells those that may
-// come again, and only they look through the others (4096 x 32000 bf16: 16 entries a row 113 us, 1024 entries
-// 293, with all looking 641; 8 x 131072 with 64 entries 4.9 and 7.4).
+// come again, and only they look through the others (4096 x 32000 bf16: 16 entries a row 89 us, 64 92, 1024 177; with
+// all looking 1024 took more than twice as long).
 constexpr int kDsBits = 32768;
 template <class T>
 __global__ __launch_bounds__(kDsThreads) void k_distill_bwd(DsArgs a) {

@@ -22,7 +22,7 @@ namespace lsh {
 // beta^L starts[s-1] + sum of segment s-1, in place.  One thread V elements, AHEAD segments' loads at once.
 // Bound by the bytes where there are many heads (64 states of 128 x 128, 8 segments: 12.3 us for 62 MB, with one
 // element a thread 16.0), by the chain of segments where there are few (8 of 64 x 128, 64 segments: one element
-// and 16 ahead 8.6 us, 8 ahead 9.4, four elements 10.6).
+// and 16 ahead 9.0 us, with 8 ahead or four elements 1 to 2 more).
 template <int V, int AHEAD>
 __global__ __launch_bounds__(256) void k_la_join(float* __restrict__ starts, const float* __restrict__ s0,
                                                  const float* __restrict__ beta, int64_t n, int64_t size,

@@ -41,7 +41,7 @@ struct LaWalk {
 
 // Walks of one size class that do not wait for each other.  Neighbouring workgroups take the n walks of a
 // segment, which read some of the same operands and find them in the caches (bf16 4096 x 4 x 16 x 128: the
-// three gradient walks with 4% less time and 23% fewer bytes from memory than one walk after the other).
+// three gradient walks with 23% fewer bytes from memory, 271 MB, than one walk after the other).
 struct LaWalks {
   LaWalk w[3];
   int n;
@@ -290,8 +290,8 @@ __device__ __forceinline__ u32x4 la_shift(u32x4 x, int n) {
 // 16 bits: a piece that would leave the row ends with it, and is shifted into place on its way to LDS (rows
 // shorter than a piece are read element by element).  32 bits: element by element, a thread's columns
 // PER_ROW apart, so that neighbouring lanes read neighbours.
-// 4096 x 4 x 16 x 127 x 127 forward: bf16 171 us, element by element 268 (128 columns 132); fp32 322 us, in
-// pieces 428 (128 columns 300).
+// 4096 x 4 x 16 x 127 x 127 forward: bf16 175 us (128 columns 138), fp32 322 us (128 columns 275).  Element by element
+// bf16 took half as long again, and fp32 in pieces a third.
 template <class T, class L, int C, int DP, int THREADS, bool PACKED>
 struct LaStage<T, L, C, DP, THREADS, PACKED, false> {
   static constexpr int W = kWide<T>, PER_ROW = DP / W, ROWS = THREADS / PER_ROW;
@@ -429,11 +429,12 @@ constexpr int la_waves(int size, int DKP, int W) {
 // the 8 rows of 32 bytes that the transposing read takes at once, meet different banks.  Where rows are read
 // 4 dwords gave twice the conflicts (3.2 -> 6.0 million cycles of the forward walk below) and 1% of time.
 //
-// Bound by the bytes and by the latency of a chunk's steps between its barriers: bf16, 4096 x 4 x 16 x 128,
-// forward 75 us for 302 MB with the states (4.0 TB/s; 8 us pass until the first chunk and state arrive), the
-// gradients' three walks 190 us for 905 MB; with one part for scores and the state that meets q 69 and 170 us,
-// and 1.4 to 1.5 times the error.  Of a SIMD's cycles some 40% issue vector instructions and 30% keep the
-// matrix unit busy.
+// Bound by the vector instructions, the bytes and the latency of a chunk's steps between its barriers: bf16,
+// 4096 x 4 x 16 x 128, forward 88 us for 302 MB with the states (3.4 TB/s; 8 us pass until the first chunk and state
+// arrive), the gradients' three walks 230 us for 905 MB (3.9 TB/s).  Of a SIMD's cycles 53% issue vector instructions
+// (gradients 66%) and 28% keep the matrix unit busy (35%); nearly half of the vector instructions take the state apart
+// for q.  With two parts for scores and that state the walks take 78 and 200 us, but hold 16 of fp32's 24 bits.
+// fp16 103 and 270 us.  fp32 192 and 554 us, with the matrix unit busy for 67% and 71% of it.
 template <class T, class L, int DKP, int W, bool SUMS, bool WIDE>
 __global__ __launch_bounds__(W * 64, la_waves(sizeof(L), DKP, W)) void k_la_walk(LaWalks all) {
   const int64_t turn = xcd_neuron(blockIdx.x, gridDim.x), job = turn / all.n;
@@ -732,8 +733,8 @@ __global__ __launch_bounds__(W * 64, la_waves(sizeof(L), DKP, W)) void k_la_walk
 // Rows of a chunk (of every type), and columns of a workgroup's block for widths DK, DV.
 inline int la_chunk() { return La<float>::C; }
 // 128 columns read Q and K and form the scores once where two blocks of 64 do it twice (bf16 4096 x 4 x 16
-// x 128, forward and backward: 425 us, with blocks of 64 461; 4096 x 16 x 256 x 256: 282 us backward, with
-// blocks of 64 383); 256 rows of a state in fp32 leave LDS for 64 only.
+// x 128, forward and backward: 398 us, with blocks of 64 448; 4096 x 16 x 256 x 256: 377 us, with
+// blocks of 64 542); 256 rows of a state in fp32 leave LDS for 64 only.
 inline int la_block(int dtype, int DK, int DV) {
   return DV > 64 && (dtype != LSH_F32 || DK <= 128) ? 128 : 64;
 }
