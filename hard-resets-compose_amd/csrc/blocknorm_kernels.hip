@@ -142,14 +142,15 @@ __device__ __forceinline__ float bn_rsqrt(float x) {
   return x > 0x1p-100f && x < 0x1p100f ? __builtin_amdgcn_rsqf(x) : 1.0f / sqrtf(x);
 }
 
-// act(g) and its derivative
+// act(g) and its derivative.  1 - sigmoid(g) is taken as exp(-g)*sigmoid(g) where the difference would cancel (at
+// g = 10 it left 10 of 24 bits).
 __device__ __forceinline__ float bn_act(int act, float g, float& d) {
   if (act == LSH_GATE_NONE) {
     d = 0.0f;
     return 1.0f;
   }
-  const float sg = sigmoid_neg(g);
-  const float ds = sg * (1.0f - sg);
+  const float e = __expf(-g), sg = __builtin_amdgcn_rcpf(1.0f + e);
+  const float ds = sg * (g > 0.0f ? e * sg : 1.0f - sg);
   d = act == LSH_GATE_SILU ? __builtin_fmaf(g, ds, sg) : ds;
   return act == LSH_GATE_SILU ? g * sg : sg;
 }

@@ -644,3 +644,19 @@ def test_embed_padding_beyond_32_bits(dev):
         assert L.lsh_embed_bwd(0, n.ptr(tok), n.ptr(dout), n.ptr(dW), 4, V, D, pad, 1.0, n.ptr(ws), nb, st) == 0
         assert torch.equal(out, W[tok])
         assert torch.equal(dW[3], dout[0] + dout[1]) and torch.equal(dW[5], dout[2]) and torch.equal(dW[0], dout[3])
+
+
+@pytest.mark.parametrize("act", ["silu", "sigmoid"])
+@pytest.mark.parametrize("types", [TYPES[0], TYPES[3]], ids=[IDS[0], IDS[3]])
+def test_block_norm_wide_gates(dev, types, act):
+    """Gates far from zero: a sigmoid's derivative keeps its digits where the sigmoid is nearly one."""
+    rows, D = 40, 512
+    x, y, gate, w_post, w_pre, a, gx, gz = _bn_inputs(rows, D, *types, dev, seed=4)
+    gate = torch.linspace(-30, 30, rows * D).view(D, rows).t().contiguous().to(types[1]).to(dev)
+    got = bn_run(x, y, gate, w_post, w_pre, a, 1e-6, act, gx, gz)
+    want = bn_reference(x, y, gate, w_post, w_pre, a, 1e-6, act, gx, gz)
+    if act == "sigmoid":  # 1 - sg has lost its digits at 30 in 64 bits too: sigmoid(-gate) in its place
+        g = gate.double().cpu()
+        right = (1 / (1 + torch.exp(g))) / (1 - 1 / (1 + torch.exp(-g)))
+        want["dgate"], want["size"]["dgate"] = want["dgate"] * right, want["size"]["dgate"] * right
+    bn_check(got, want, rows)
