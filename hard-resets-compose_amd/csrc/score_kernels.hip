@@ -1,0 +1,424 @@
+// Log probabilities of given tokens, the entropy of each row and its most likely alternatives.  With a temperature
+// tau and z the logits,
+//
+//   p = softmax(z/tau),  logp = log p_y (0 where the row has no token y),  H = -sum_v p_v log p_v
+//   top: the K largest logits, ties to the lower id, as log p and ids
+//   dz_v = (g*([v = y] - p_v) - gH*p_v*(log p_v + H)) / tau       g, gH: gradients of logp and H; g is 0 without a token
+//
+// One pass over the logits holds the running maximum m, s = sum e and t = sum e*d, with d = (z - m)*c, e = 2^d and
+// c = log2(e)/tau; then l = log2(s), log p = ln2*(d - l) and H = ln2*(l - t/s).  A logit of -inf has p = 0, and a row of
+// nothing else has log p = -inf, H = 0 and no gradient.  A row with NaN or +inf has NaN.
+//
+// The K largest: each thread knows the largest of the logits that it read.  The K-th largest of those is a bound that
+// K logits reach, so only the K threads whose largest reaches it can hold one of the row's K: they read their share again
+// (from the caches), and a handful more than K values come out, which are ranked by counting.  Values and ids are one
+// whole number of 64 bits, no two alike, so the order in which they are found does not matter.
+#include <algorithm>
+#include <type_traits>
+
+#include "lsh_lm.h"
+
+namespace lsh {
+
+constexpr int kScThreads = 256, kScUnroll = 4, kScParts = 64, kScList = 1024;
+constexpr float kScLog2e = 1.4426950408889634f, kScLn2 = 0.6931471805599453f;
+
+struct ScArgs {
+  const void* z;
+  int64_t stride;
+  const int64_t* token;
+  float *logp, *entropy;
+  float* stats;  // [3, rows]: m, l and H
+  float* top_logp;
+  int64_t* top_id;
+  float* part;               // [rows, splits, 3]: m, s and t of each part
+  unsigned long long* keys;  // [rows, splits, K]: each part's largest, in order
+  const float *g, *gh;
+  int64_t g_stride, gh_stride;
+  void* dz;
+  int64_t rows, V;
+  int K, splits;
+  int64_t len;  // logits of a part
+  float c, tau;
+};
+
+// A value and its id as a number: larger values first, then lower ids; NaN before all values; never 0.
+using Key = unsigned long long;
+__device__ __forceinline__ Key sc_key(float x, unsigned id) {
+  unsigned b = __builtin_bit_cast(unsigned, x + 0.0f);  // one zero
+  if (x != x) b = 0x7fc00000u;
+  b = b & 0x80000000u ? ~b : b | 0x80000000u;
+  return (Key)b << 32 | (0xffffffffu - id);
+}
+__device__ __forceinline__ float sc_value(Key k) {
+  const unsigned b = (unsigned)(k >> 32);
+  return __builtin_bit_cast(float, b & 0x80000000u ? b & 0x7fffffffu : ~b);
+}
+__device__ __forceinline__ unsigned sc_id(Key k) { return 0xffffffffu - (unsigned)k; }
+
+// (m, s, t) of two parts; a part without values has m = -inf, s = t = 0
+__device__ __forceinline__ void sc_join(float& m, float& s, float& t, float m2, float s2, float t2, float c) {
+  const float top = fmaxf(m, m2), at = top > -INFINITY ? top : 0.0f;
+  const float d1 = fmaxf((m - at) * c, -1000.0f), d2 = fmaxf((m2 - at) * c, -1000.0f);
+  const float e1 = __builtin_amdgcn_exp2f(d1), e2 = __builtin_amdgcn_exp2f(d2);
+  t = e1 * __builtin_fmaf(d1, s, t) + e2 * __builtin_fmaf(d2, s2, t2);
+  s = s * e1 + s2 * e2;
+  m = top;
+}
+
+// 16 bytes at the address of any element
+template <class T>
+using ScPiece = Vec<T, kWide<T>>;
+template <class T>
+__device__ __forceinline__ ScPiece<T> sc_load(const T* p) {
+  ScPiece<T> x;
+  __builtin_memcpy(&x, p, 16);
+  return x;
+}
+
+// The K largest of keys that the threads of a workgroup hold between them, in order, to out (0: none).  own: a thread's
+// largest (0: it has none).  scan(bound, f) calls f with each key of the thread that reaches bound.
+// One call a kernel: its LDS is not shared.
+template <class Scan, class Out>
+__device__ __forceinline__ void sc_select(Key own, int K, Scan&& scan, Out&& out) {
+  __shared__ Key s_own[kScThreads], s_list[kScList], s_bound;
+  __shared__ int s_count;
+  const int tid = threadIdx.x;
+  s_own[tid] = own;
+  if (tid == 0) s_bound = 0, s_count = 0;
+  __syncthreads();
+  int above = 0;
+#pragma unroll 8
+  for (int i = 0; i < kScThreads; ++i) above += s_own[i] > own;
+  if (above == K - 1 && own) s_bound = own;
+  __syncthreads();
+  const Key bound = s_bound;
+  if (own && own >= bound)
+    scan(bound, [&](Key k) {
+      const int at = atomicAdd(&s_count, 1);
+      if (at < kScList) s_list[at] = k;
+    });
+  __syncthreads();
+  const int n = s_count;
+  if (n <= kScList) {
+    for (int i = tid; i < n; i += kScThreads) {
+      const Key mine = s_list[i];
+      int rank = 0;
+      for (int j = 0; j < n; ++j) rank += s_list[j] > mine;
+      if (rank < K) out(rank, mine);
+    }
+    for (int i = n + tid; i < K; i += kScThreads) out(i, (Key)0);
+    return;
+  }
+  // more than the list holds reach the bound (long runs of large values that a few threads share): one after the other
+  Key last = ~(Key)0;
+  for (int k = 0; k < K; ++k) {
+    Key best = 0;
+    if (own && own >= bound)
+      scan(bound, [&](Key x) {
+        if (x < last && x > best) best = x;
+      });
+    __syncthreads();  // s_own was read
+    s_own[tid] = best;
+    __syncthreads();
+    for (int o = kScThreads / 2; o > 0; o >>= 1) {
+      if (tid < o && s_own[tid + o] > s_own[tid]) s_own[tid] = s_own[tid + o];
+      __syncthreads();
+    }
+    last = s_own[0];
+    if (tid == 0) out(k, last);
+  }
+}
+
+// What a row's statistics give: by one thread
+__device__ __forceinline__ float sc_logp(float z, float m, float l, float c) {
+  return l == -INFINITY ? -INFINITY : kScLn2 * ((z - m) * c - l);
+}
+template <class T>
+__device__ __forceinline__ void sc_finish(const ScArgs& a, int64_t row, float m, float s, float t) {
+  const float l = __builtin_amdgcn_logf(s), H = s == 0.0f ? 0.0f : kScLn2 * (l - t / s);
+  const int64_t y = a.token[row];
+  const bool there = y >= 0 && y < a.V;
+  a.logp[row] = there ? sc_logp(to_f(((const T*)a.z)[row * a.stride + y]), m, l, a.c) : 0.0f;
+  a.entropy[row] = H;
+  if (a.stats) a.stats[row] = m, a.stats[a.rows + row] = l, a.stats[2 * a.rows + row] = H;
+}
+__device__ __forceinline__ void sc_put(const ScArgs& a, int64_t row, int k, Key key, float m, float l) {
+  a.top_logp[row * a.K + k] = sc_logp(sc_value(key), m, l, a.c);
+  a.top_id[row * a.K + k] = sc_id(key);
+}
+
+template <class T, bool SPLIT, bool TOP>
+__global__ __launch_bounds__(kScThreads) void k_score(ScArgs a) {
+  constexpr int P = kWide<T>, U = kScUnroll, STEP = U * kScThreads * P;
+  __shared__ float s_stat[kScThreads / 64][3];
+  const int64_t row = SPLIT ? blockIdx.x / a.splits : blockIdx.x, part = SPLIT ? blockIdx.x % a.splits : 0;
+  const int64_t v0 = part * a.len;
+  const T* z = (const T*)a.z + row * a.stride + v0;
+  const int n = (int)max((int64_t)0, min(a.len, a.V - v0));
+  const int tid = threadIdx.x;
+  // element j of piece u of a thread in block b: ((b*U + u)*kScThreads + tid)*P + j
+  auto place = [&](int b, int u) { return b * STEP + (u * kScThreads + tid) * P; };
+  float m = -INFINITY, s = 0.0f, t = 0.0f;
+  int best = 0;  // the block of the largest
+  auto take = [&](const float (&f)[U][P], int b) {
+    float top = m;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < P; ++j) top = fmaxf(top, f[u][j]);
+    if (TOP && top > m) best = b;
+    const float at = top > -INFINITY ? top : 0.0f;
+    const float d0 = fmaxf((m - at) * a.c, -1000.0f), e0 = __builtin_amdgcn_exp2f(d0);
+    t = e0 * __builtin_fmaf(d0, s, t);
+    s *= e0;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < P; ++j) {
+        const float d = (f[u][j] - at) * a.c, e = __builtin_amdgcn_exp2f(d);
+        s += e;
+        t = __builtin_fmaf(e, fmaxf(d, -1000.0f), t);
+      }
+    m = top;
+  };
+  const int whole = n / STEP;
+  for (int b = 0; b < whole; ++b) {
+    ScPiece<T> y[U];
+    float f[U][P];
+#pragma unroll
+    for (int u = 0; u < U; ++u) y[u] = sc_load(z + place(b, u));
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < P; ++j) f[u][j] = to_f(y[u].v[j]);
+    take(f, b);
+  }
+  // what is left of a block, the pieces that are whole and the one that is not
+  auto rest = [&](int b, float (&f)[U][P]) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int e = place(b, u);
+#pragma unroll
+      for (int j = 0; j < P; ++j) f[u][j] = -INFINITY;
+      if (e + P <= n) {
+        const ScPiece<T> y = sc_load(z + e);
+#pragma unroll
+        for (int j = 0; j < P; ++j) f[u][j] = to_f(y.v[j]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < P; ++j)
+          if (e + j < n) f[u][j] = to_f(z[e + j]);
+      }
+    }
+  };
+  if (place(whole, 0) < n) {
+    float f[U][P];
+    rest(whole, f);
+    take(f, whole);
+  }
+  const bool odd = s != s;  // a NaN, or +inf
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1)
+    sc_join(m, s, t, __shfl_xor(m, o, 64), __shfl_xor(s, o, 64), __shfl_xor(t, o, 64), a.c);
+  if ((tid & 63) == 0) s_stat[tid >> 6][0] = m, s_stat[tid >> 6][1] = s, s_stat[tid >> 6][2] = t;
+  __syncthreads();
+  m = s_stat[0][0], s = s_stat[0][1], t = s_stat[0][2];
+#pragma unroll
+  for (int w = 1; w < kScThreads / 64; ++w) sc_join(m, s, t, s_stat[w][0], s_stat[w][1], s_stat[w][2], a.c);
+  if (tid == 0) {
+    if (SPLIT) {
+      float* to = a.part + (row * a.splits + part) * 3;
+      to[0] = m, to[1] = s, to[2] = t;
+    } else {
+      sc_finish<T>(a, row, m, s, t);
+    }
+  }
+  if constexpr (TOP) {
+    // the thread's keys of a block that reach a bound
+    auto block = [&](int b, Key bound, auto&& f) {
+      float x[U][P];
+      rest(b, x);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+          const int e = place(b, u) + j;
+          const Key k = sc_key(x[u][j], (unsigned)(v0 + e));
+          if (e < n && k >= bound) f(k);
+        }
+    };
+    const int blocks = place(whole, 0) < n ? whole + 1 : whole;
+    Key own = 0;
+    auto largest = [&](Key k) { own = k > own ? k : own; };
+    if (odd)
+      for (int b = 0; b < blocks; ++b) block(b, 0, largest);
+    else if (blocks)
+      block(best, 0, largest);
+    const float l = __builtin_amdgcn_logf(s);
+    sc_select(
+        own, a.K,
+        [&](Key bound, auto&& f) {
+          for (int b = 0; b < blocks; ++b) block(b, bound, f);
+        },
+        [&](int k, Key key) {
+          if (SPLIT)
+            a.keys[(row * a.splits + part) * a.K + k] = key;
+          else
+            sc_put(a, row, k, key, m, l);
+        });
+  }
+}
+
+// The parts of a row: a wave joins their statistics, and the workgroup their largest.
+template <class T, bool TOP>
+__global__ __launch_bounds__(kScThreads) void k_score_join(ScArgs a) {
+  const int64_t row = blockIdx.x;
+  const int tid = threadIdx.x, i = tid & 63;
+  const float* p = a.part + (row * a.splits + min(i, a.splits - 1)) * 3;
+  float m = i < a.splits ? p[0] : -INFINITY, s = i < a.splits ? p[1] : 0.0f, t = i < a.splits ? p[2] : 0.0f;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1)
+    sc_join(m, s, t, __shfl_xor(m, o, 64), __shfl_xor(s, o, 64), __shfl_xor(t, o, 64), a.c);
+  if (tid == 0) sc_finish<T>(a, row, m, s, t);
+  if constexpr (TOP) {
+    const Key* keys = a.keys + row * a.splits * a.K;
+    const int n = a.splits * a.K;
+    Key own = 0;
+    for (int k = tid; k < n; k += kScThreads) own = max(own, keys[k]);
+    const float l = __builtin_amdgcn_logf(s);
+    sc_select(
+        own, a.K,
+        [&](Key bound, auto&& f) {
+          for (int k = tid; k < n; k += kScThreads)
+            if (const Key x = keys[k]; x && x >= bound) f(x);
+        },
+        [&](int k, Key key) { sc_put(a, row, k, key, m, l); });
+  }
+}
+
+template <class T>
+__global__ __launch_bounds__(kScThreads) void k_score_bwd(ScArgs a) {
+  constexpr int P = kWide<T>, U = kScUnroll;
+  const int64_t row = blockIdx.x / a.splits, v0 = blockIdx.x % a.splits * a.len;
+  const T* z = (const T*)a.z + row * a.stride + v0;
+  T* dz = (T*)a.dz + row * a.V + v0;
+  const int n = (int)max((int64_t)0, min(a.len, a.V - v0)), pieces = n / P;
+  const float m = a.stats[row], l = a.stats[a.rows + row], H = a.stats[2 * a.rows + row];
+  const int64_t y = a.token[row];
+  const bool some = l != -INFINITY, there = some && y >= 0 && y < a.V;
+  const float per = 1.0f / a.tau;
+  const float g = there ? a.g ? a.g[row * a.g_stride] * per : 0.0f : 0.0f;
+  const float gh = some && a.gh ? a.gh[row * a.gh_stride] * per : 0.0f;
+  const float flat = __builtin_fmaf(gh, H, g), slope = gh * kScLn2;
+  const int at = there && y >= v0 && y < v0 + n ? (int)(y - v0) : -1;
+  auto grad = [&](float v, int e) {
+    float x = __builtin_fmaf(v - m, a.c, -l);
+    x = x < -1000.0f ? -1000.0f : x;  // p = 0; a NaN stays
+    const float d = -__builtin_amdgcn_exp2f(x) * __builtin_fmaf(slope, x, flat);
+    return some ? e == at ? d + g : d : 0.0f;
+  };
+  auto put = [&](const ScPiece<T>& q, int i) {
+    ScPiece<T> d;
+#pragma unroll
+    for (int j = 0; j < P; ++j) d.v[j] = from_f<T>(grad(to_f(q.v[j]), i * P + j));
+    __builtin_memcpy(dz + (int64_t)i * P, &d, 16);
+  };
+  int i = threadIdx.x;
+  for (; i + (U - 1) * kScThreads < pieces; i += U * kScThreads) {
+    ScPiece<T> q[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) q[u] = sc_load(z + (int64_t)(i + u * kScThreads) * P);
+#pragma unroll
+    for (int u = 0; u < U; ++u) put(q[u], i + u * kScThreads);
+  }
+  for (; i < pieces; i += kScThreads) put(sc_load(z + (int64_t)i * P), i);
+  if (const int e = pieces * P + threadIdx.x; e < n) dz[e] = from_f<T>(grad(to_f(z[e]), e));
+}
+
+static int sc_check(int dtype, int64_t rows, int64_t V, int K, float tau) {
+  if (!lm_dtype_ok(dtype) || !(tau > 0.0f) || !(tau < INFINITY)) return LSH_ERR_ARG;
+  if (rows < 0 || !lm_grid_ok(rows, kScThreads) || V < 1 || V > 0x7fffffff / 2 || K < 0 || K > LSH_SCORE_MAX_TOP ||
+      K > V)
+    return LSH_ERR_SHAPE;
+  return LSH_OK;
+}
+
+// Parts of a row: about 1024 workgroups, none of less than 4096 logits.
+static int sc_splits(int64_t rows, int64_t V) {
+  const int64_t most = std::min<int64_t>((V + 4095) / 4096, kScParts);
+  return (int)std::max<int64_t>(1, std::min(most, 1024 / std::max<int64_t>(rows, 1)));
+}
+
+static ScArgs sc_args(const void* logits, int64_t stride, const int64_t* tokens, int64_t rows, int64_t V, int K,
+                      float tau) {
+  ScArgs a = {};
+  a.z = logits, a.stride = stride, a.token = tokens, a.rows = rows, a.V = V, a.K = K;
+  a.splits = sc_splits(rows, V);
+  a.len = align_up((size_t)((V + a.splits - 1) / a.splits), 8);
+  a.c = kScLog2e / tau, a.tau = tau;
+  return a;
+}
+
+}  // namespace lsh
+
+using namespace lsh;
+
+extern "C" size_t lsh_score_workspace(int64_t rows, int64_t V, int K) {
+  if (sc_check(LSH_F32, rows, V, K, 1.0f)) return 0;
+  const int64_t splits = sc_splits(rows, V);
+  return splits > 1 ? (size_t)(rows * splits) * (K * sizeof(Key) + 3 * sizeof(float)) : 0;
+}
+
+extern "C" int lsh_score_fwd(int dtype, const void* logits, int64_t stride, const int64_t* tokens, float* logp,
+                             float* entropy, float* stats, float* top_logp, int64_t* top_index, int64_t rows,
+                             int64_t V, int K, float tau, void* ws, size_t ws_bytes, void* stream) {
+  if (int rc = sc_check(dtype, rows, V, K, tau)) return rc;
+  if (rows == 0) return LSH_OK;
+  if (bad_ptr(logits) || bad_ptr(tokens) || bad_ptr(logp) || bad_ptr(entropy) ||
+      (K > 0 && (bad_ptr(top_logp) || bad_ptr(top_index))))
+    return LSH_ERR_ARG;
+  const size_t need = lsh_score_workspace(rows, V, K);
+  if (need && (bad_ptr(ws) || ws_bytes < need)) return LSH_ERR_WORKSPACE;
+  ScArgs a = sc_args(logits, stride, tokens, rows, V, K, tau);
+  a.logp = logp, a.entropy = entropy, a.stats = stats, a.top_logp = top_logp, a.top_id = top_index;
+  a.keys = (Key*)ws, a.part = (float*)((Key*)ws + rows * a.splits * K);
+  if (!lm_grid_ok(rows * a.splits, kScThreads)) return LSH_ERR_SHAPE;
+  hipStream_t st = (hipStream_t)stream;
+  with_dtype(dtype, [&](auto t) {
+    using T = decltype(t);
+    auto go = [&](auto top) {
+      constexpr bool TOP = decltype(top)::value;
+      if (a.splits > 1) {
+        k_score<T, true, TOP><<<dim3((unsigned)(rows * a.splits)), kScThreads, 0, st>>>(a);
+        k_score_join<T, TOP><<<dim3((unsigned)rows), TOP ? kScThreads : 64, 0, st>>>(a);
+      } else {
+        k_score<T, false, TOP><<<dim3((unsigned)rows), kScThreads, 0, st>>>(a);
+      }
+    };
+    if (K > 0)
+      go(std::true_type{});
+    else
+      go(std::false_type{});
+  });
+  LSH_CHECK_LAUNCH();
+  return LSH_OK;
+}
+
+extern "C" int lsh_score_bwd(int dtype, const void* logits, int64_t stride, const int64_t* tokens, const float* stats,
+                             const float* g_logp, int64_t g_stride, const float* g_entropy, int64_t ge_stride,
+                             void* dlogits, int64_t rows, int64_t V, float tau, void* stream) {
+  if (int rc = sc_check(dtype, rows, V, 0, tau)) return rc;
+  if (rows == 0) return LSH_OK;
+  if (bad_ptr(logits) || bad_ptr(tokens) || bad_ptr(stats) || bad_ptr(dlogits)) return LSH_ERR_ARG;
+  ScArgs a = sc_args(logits, stride, tokens, rows, V, 0, tau);
+  a.stats = (float*)stats, a.g = g_logp, a.g_stride = g_stride, a.gh = g_entropy, a.gh_stride = ge_stride;
+  a.dz = dlogits;
+  if (!lm_grid_ok(rows * a.splits, kScThreads)) return LSH_ERR_SHAPE;
+  with_dtype(dtype, [&](auto t) {
+    using T = decltype(t);
+    k_score_bwd<T><<<dim3((unsigned)(rows * a.splits)), kScThreads, 0, (hipStream_t)stream>>>(a);
+  });
+  LSH_CHECK_LAUNCH();
+  return LSH_OK;
+}

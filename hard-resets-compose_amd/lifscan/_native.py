@@ -85,6 +85,20 @@ class BlockNorm(ctypes.Structure):
         [(n, c_p) for n in ("x", "y", "gate", "w_post", "w_pre", "scale")] + [("scale1", c_f), ("eps", c_f)]
 
 
+class Gated(ctypes.Structure):
+    _fields_ = [(n, c_i) for n in ("dtype", "decay", "mix")] + [(n, c_i64) for n in ("T", "B", "D")] + \
+        [(n, c_p) for n in ("x", "gate")] + [(n, c_i64) for n in ("x_st", "x_sb", "g_st", "g_sb")] + \
+        [(n, c_p) for n in ("starts", "h0")]
+
+
+class Rotate(ctypes.Structure):
+    _fields_ = [(n, c_i) for n in ("dtype", "D", "rot", "neighbours")] + \
+        [(n, c_i64) for n in ("T", "B", "H", "HK")] + [(n, c_p) for n in ("q", "k")] + \
+        [(n, c_i64) for n in ("q_st", "q_sb", "q_sh", "k_st", "k_sb", "k_sh")] + \
+        [("positions", c_p), ("p_st", c_i64), ("p_sb", c_i64)] + \
+        [(n, c_p) for n in ("inv_freq", "q_weight", "k_weight")] + [("eps", c_f)]
+
+
 # name -> (restype, argtypes); mirrors include/lifscan_hip.h
 SIGNATURES = {
     "lsh_abi_version": (c_i, []),
@@ -193,6 +207,17 @@ SIGNATURES = {
     "lsh_distill_workspace": (c_sz, [c_i64, c_i64]),
     "lsh_distill_fwd": (c_i, [c_i, c_p, c_i64, c_i, c_p, c_p, c_p, c_p, c_i64, c_i64, c_i, c_f, c_p, c_sz, c_p]),
     "lsh_distill_bwd": (c_i, [c_i, c_p, c_i64, c_i, c_p, c_p, c_p, c_p, c_i64, c_p, c_i64, c_i64, c_i, c_f, c_p]),
+    "lsh_gated_workspace": (c_sz, [c_p]),
+    "lsh_gated_saved": (c_i64, [c_p]),
+    "lsh_gated_fwd": (c_i, [c_p] * 5 + [c_sz, c_p]),
+    "lsh_gated_bwd": (c_i, [c_p, c_p, c_p, c_i64, c_i64] + [c_p] * 5 + [c_sz, c_p]),
+    "lsh_gated_step": (c_i, [c_p] * 4),
+    "lsh_rotate_fwd": (c_i, [c_p] * 4),
+    "lsh_rotate_bwd_workspace": (c_sz, [c_p]),
+    "lsh_rotate_bwd": (c_i, [c_p, c_p, c_i64, c_i64, c_i64, c_p, c_i64, c_i64, c_i64] + [c_p] * 5 + [c_sz, c_p]),
+    "lsh_score_workspace": (c_sz, [c_i64, c_i64, c_i]),
+    "lsh_score_fwd": (c_i, [c_i, c_p, c_i64] + [c_p] * 6 + [c_i64, c_i64, c_i, c_f, c_p, c_sz, c_p]),
+    "lsh_score_bwd": (c_i, [c_i, c_p, c_i64, c_p, c_p, c_p, c_i64, c_p, c_i64, c_p, c_i64, c_i64, c_f, c_p]),
 }
 
 

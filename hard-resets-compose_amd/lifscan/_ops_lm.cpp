@@ -1,4 +1,4 @@
-// The language-model operators (lifscan/hip_linattn.py, hip_lm.py) over the lifscan C ABI: argument
+// The language-model operators (lifscan/hip_linattn.py, hip_lm.py, hip_gated.py) over the lifscan C ABI: argument
 // checks, workspaces and autograd functions in C++, one Python -> C++ crossing a call.  (From Python the
 // checks and the engine's calls back into the interpreter cost some 60 us a forward and backward, several
 // times the kernels of small steps.)
@@ -37,7 +37,18 @@ struct Entry {
   X(lsh_embed_bwd)                \
   X(lsh_distill_workspace)        \
   X(lsh_distill_fwd)              \
-  X(lsh_distill_bwd)
+  X(lsh_distill_bwd)              \
+  X(lsh_gated_workspace)          \
+  X(lsh_gated_saved)              \
+  X(lsh_gated_fwd)                \
+  X(lsh_gated_bwd)                \
+  X(lsh_gated_step)               \
+  X(lsh_rotate_fwd)               \
+  X(lsh_rotate_bwd_workspace)     \
+  X(lsh_rotate_bwd)               \
+  X(lsh_score_workspace)          \
+  X(lsh_score_fwd)                \
+  X(lsh_score_bwd)
 #define LSH_MEMBER(name) decltype(&::name) name = nullptr;
   LSH_ENTRIES(LSH_MEMBER)
 #undef LSH_MEMBER
@@ -527,6 +538,364 @@ Tensor distill_topk(const Tensor& logits, const Tensor& values_in, const Tensor&
   return logits.dim() == 2 ? loss : loss.reshape(lead);
 }
 
+// ------------------------------------------------------------------------------- log probabilities of tokens
+struct Scores {
+  Tensor logp, entropy, stats, top_logp, top_index;
+  variable_list outputs() const {
+    if (!top_logp.defined()) return {logp, entropy};
+    return {logp, entropy, top_logp, top_index};
+  }
+};
+Scores score_forward(const Tensor& z, const Tensor& tokens, double tau, int64_t K, bool train) {
+  const c10::DeviceGuard guard(z.device());
+  const int64_t rows = z.size(0), V = z.size(1);
+  const auto f32 = z.options().dtype(torch::kFloat32);
+  Scores r;
+  r.logp = torch::empty({rows}, f32), r.entropy = torch::empty({rows}, f32);
+  if (train) r.stats = torch::empty({3, rows}, f32);
+  if (K > 0) r.top_logp = torch::empty({rows, K}, f32), r.top_index = torch::empty({rows, K}, tokens.options());
+  const size_t nb = g.lsh_score_workspace(rows, V, (int)K);
+  const Tensor ws = workspace(nb, z);
+  check(g.lsh_score_fwd(code_of(z), raw(z), z.stride(0), tokens.data_ptr<int64_t>(), fp(r.logp), fp(r.entropy),
+                        fp(r.stats), fp(r.top_logp), K > 0 ? r.top_index.data_ptr<int64_t>() : nullptr, rows, V, (int)K,
+                        (float)tau, raw(ws), nb, stream_of(z)),
+        "lsh_score_fwd");
+  return r;
+}
+
+struct Score : public torch::autograd::Function<Score> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& z, const Tensor& tokens, double tau, int64_t K) {
+    const Scores r = score_forward(z, tokens, tau, K, true);
+    ctx->save_for_backward({z, tokens, r.stats});
+    ctx->saved_data["tau"] = tau;
+    ctx->saved_data["n"] = std::vector<int64_t>{z.size(0), z.size(1), (int64_t)z.scalar_type()};
+    if (K > 0) ctx->mark_non_differentiable({r.top_logp, r.top_index});
+    ctx->set_materialize_grads(false);
+    return r.outputs();
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads_in) {
+    const variable_list grads = first_order(std::move(grads_in));
+    const Tensor &gl = grads[0], &ge = grads[1];
+    if (!gl.defined() && !ge.defined()) return variable_list(4);
+    const auto saved = ctx->get_saved_variables();
+    const auto n = ctx->saved_data["n"].toIntVector();
+    const Tensor& like = gl.defined() ? gl : ge;
+    Tensor z = unpacked(saved[0], {n[0], n[1]}, (torch::ScalarType)n[2], like);
+    if (z.stride(1) != 1 && n[1] > 1) z = z.contiguous();
+    const Tensor tokens = unpacked(saved[1], {n[0]}, torch::kInt64, like).contiguous(),
+                 stats = unpacked(saved[2], {3, n[0]}, torch::kFloat32, like).contiguous();
+    const c10::DeviceGuard guard(z.device());
+    const Tensor dz = torch::empty({n[0], n[1]}, z.options());
+    check(g.lsh_score_bwd(code_of(z), raw(z), z.stride(0), tokens.data_ptr<int64_t>(), fp(stats), fp(gl),
+                          gl.defined() ? gl.stride(0) : 0, fp(ge), ge.defined() ? ge.stride(0) : 0, raw(dz), n[0], n[1],
+                          (float)ctx->saved_data["tau"].toDouble(), stream_of(z)),
+          "lsh_score_bwd");
+    return {dz, Tensor(), Tensor(), Tensor()};
+  }
+};
+
+variable_list token_logprobs(const Tensor& logits, const Tensor& tokens_in, double tau, int64_t K) {
+  check_plain("token_logprobs", {logits});
+  check_float(logits, "logits");
+  TORCH_CHECK_VALUE(logits.dim() >= 1 && logits.size(-1) >= 1, "logits must be [*rows, V]");
+  const auto lead = logits.sizes().slice(0, logits.dim() - 1);
+  const int64_t V = logits.size(-1);
+  TORCH_CHECK_VALUE(tokens_in.device() == logits.device() && tokens_in.sizes() == lead, "tokens must be ", lead, " on ",
+                    logits.device(), ", one for each row of logits");
+  TORCH_CHECK_VALUE(tokens_in.scalar_type() == torch::kInt64 || tokens_in.scalar_type() == torch::kInt32,
+                    "tokens must be int64 or int32");
+  TORCH_CHECK_VALUE(tau > 0 && tau < std::numeric_limits<double>::infinity(), "temperature=", tau,
+                    " must be positive and finite");
+  TORCH_CHECK_VALUE(K >= 0 && K <= LSH_SCORE_MAX_TOP && K <= V, "top=", K, ": 0 to ",
+                    std::min<int64_t>(LSH_SCORE_MAX_TOP, V), " alternatives of ", V, " are supported");
+  const int64_t rows = logits.numel() / V;
+  Tensor z = logits.dim() == 2 ? logits : logits.reshape({rows, V});
+  if (z.stride(1) != 1 && V > 1) z = z.contiguous();
+  const Tensor tokens = tokens_in.to(torch::kInt64).reshape({rows}).contiguous();
+  variable_list out =
+      grad_wanted({z}) ? Score::apply(z, tokens, tau, K) : score_forward(z, tokens, tau, K, false).outputs();
+  if (logits.dim() == 2) return out;
+  auto wide = lead.vec();
+  wide.push_back(K);
+  for (size_t i = 0; i < out.size(); ++i) out[i] = out[i].reshape(i < 2 ? lead : torch::IntArrayRef(wide));
+  return out;
+}
+
+// ------------------------------------------------------------------------------- gated linear recurrence
+// A stride, 0 where it leads nowhere: the kernels ask that strides are whole pieces.
+int64_t step_of(const Tensor& t, int64_t dim) { return t.size(dim) == 1 ? 0 : t.stride(dim); }
+
+struct Gates {
+  Tensor x, gate, starts;
+  lsh_gated a = {};
+  std::vector<int64_t> state() const { return {a.B, a.D}; }
+  void check_state(const Tensor& s, const char* name) const {
+    TORCH_CHECK_VALUE(s.scalar_type() == torch::kFloat32 && s.device() == x.device() && s.sizes() == state(), name,
+                      " must be float32 ", state(), " on ", x.device());
+  }
+};
+Gates gates(const Tensor& x, const Tensor& gate, const Tensor& starts, int64_t decay, bool mix, int64_t dims) {
+  check_float(x, "x");
+  TORCH_CHECK_VALUE(x.dim() == dims && x.size(-1) >= 1, "x must be a ", dims, "-D [", dims == 3 ? "T, " : "", "B, D] tensor");
+  TORCH_CHECK_VALUE(gate.sizes() == x.sizes() && gate.scalar_type() == x.scalar_type() && gate.device() == x.device(),
+                    "gate must be ", x.scalar_type(), " ", x.sizes(), " on ", x.device());
+  Gates r;
+  r.x = rows_of(x), r.gate = rows_of(gate);
+  lsh_gated& a = r.a;
+  a.dtype = code_of(x), a.decay = (int)decay, a.mix = mix;
+  a.T = dims == 3 ? x.size(0) : 1, a.B = x.size(-2), a.D = x.size(-1);
+  a.x = raw(r.x), a.gate = raw(r.gate);
+  a.x_sb = step_of(r.x, -2), a.g_sb = step_of(r.gate, -2);
+  if (dims == 3) a.x_st = step_of(r.x, 0), a.g_st = step_of(r.gate, 0);
+  if (starts.defined()) {
+    TORCH_CHECK_VALUE((starts.scalar_type() == torch::kBool || starts.scalar_type() == torch::kUInt8) &&
+                          starts.device() == x.device() && starts.dim() == 2 && starts.size(0) == a.T &&
+                          starts.size(1) == a.B, "starts must be bool [", a.T, ", ", a.B, "] on ", x.device());
+    r.starts = starts.contiguous();
+    a.starts = static_cast<const uint8_t*>(r.starts.data_ptr());
+  }
+  return r;
+}
+struct GatedOut {
+  Tensor h, h_end, saved;
+};
+GatedOut gated_forward(Gates& r, const Tensor& h0, bool train) {
+  const c10::DeviceGuard guard(r.x.device());
+  const auto f32 = r.x.options().dtype(torch::kFloat32);
+  GatedOut out;
+  out.h = torch::empty({r.a.T, r.a.B, r.a.D}, r.x.options());
+  out.h_end = torch::empty(r.state(), f32);
+  r.a.h0 = fp(h0);
+  if (train) out.saved = torch::empty({g.lsh_gated_saved(&r.a)}, f32);
+  const size_t nb = g.lsh_gated_workspace(&r.a);
+  const Tensor ws = workspace(nb, r.x);
+  check(g.lsh_gated_fwd(&r.a, raw(out.h), fp(out.h_end), fp(out.saved), raw(ws), nb, stream_of(r.x)), "lsh_gated_fwd");
+  return out;
+}
+
+struct Gated : public torch::autograd::Function<Gated> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& gate, const Maybe& h0_in,
+                               const Maybe& starts_in, int64_t decay, bool mix) {
+    const Tensor h0 = of(h0_in);
+    Gates r = gates(x, gate, of(starts_in), decay, mix, 3);
+    const GatedOut out = gated_forward(r, h0, true);
+    ctx->save_for_backward({r.x, r.gate, r.starts, out.saved});
+    ctx->saved_data["n"] = std::vector<int64_t>{r.a.T, r.a.B, r.a.D, decay, mix, r.starts.defined(),
+                                                h0.defined() && h0.requires_grad(), out.saved.numel(),
+                                                r.starts.defined() ? (int64_t)r.starts.scalar_type() : 0};
+    ctx->set_materialize_grads(false);
+    return {out.h, out.h_end};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads_in) {
+    const variable_list grads = first_order(std::move(grads_in));
+    const Tensor& d_end = grads[1];
+    if (!grads[0].defined() && !d_end.defined()) return variable_list(6);
+    const auto saved = ctx->get_saved_variables();
+    const auto n = ctx->saved_data["n"].toIntVector();
+    const Tensor& like = grads[0].defined() ? grads[0] : d_end;
+    const auto type = saved[0].scalar_type();
+    TORCH_CHECK_VALUE(!grads[0].defined() || type == grads[0].scalar_type(), "a saved tensor was unpacked to another type");
+    const Tensor x = unpacked(saved[0], {n[0], n[1], n[2]}, type, like),
+                 gate = unpacked(saved[1], {n[0], n[1], n[2]}, type, like);
+    const Tensor starts = n[5] ? unpacked(saved[2], {n[0], n[1]}, (torch::ScalarType)n[8], like) : Tensor();
+    const Tensor states = unpacked(saved[3], {n[7]}, torch::kFloat32, like).contiguous();
+    const Gates r = gates(x, gate, starts, n[3], n[4], 3);
+    const c10::DeviceGuard guard(r.x.device());
+    Tensor dh, gs, dh0;
+    if (grads[0].defined()) dh = rows_of(grads[0]);
+    if (d_end.defined()) {
+      r.check_state(d_end, "the final state's gradient");
+      gs = d_end.contiguous();
+    }
+    const Tensor dx = torch::empty(r.x.sizes(), r.x.options()), dgate = torch::empty(r.x.sizes(), r.x.options());
+    if (n[6]) dh0 = torch::empty(r.state(), states.options());
+    const size_t nb = g.lsh_gated_workspace(&r.a);
+    const Tensor ws = workspace(nb, r.x);
+    check(g.lsh_gated_bwd(&r.a, fp(states), raw(dh), dh.defined() ? step_of(dh, 0) : 0, dh.defined() ? step_of(dh, 1) : 0,
+                          fp(gs), raw(dx), raw(dgate), fp(dh0), raw(ws), nb, stream_of(r.x)),
+          "lsh_gated_bwd");
+    return {dx, dgate, dh0, Tensor(), Tensor(), Tensor()};
+  }
+};
+
+std::tuple<Tensor, Tensor> gated_scan(const Tensor& x, const Tensor& gate, const Maybe& h0_in, const Maybe& starts_in,
+                                      int64_t decay, bool mix) {
+  Tensor h0 = of(h0_in);
+  check_plain("gated_scan", {x, gate, h0});
+  const bool train = grad_wanted({x, gate, h0});
+  Gates r = train ? gates(x, gate, of(starts_in), decay, mix, 3)
+                  : gates(x.detach(), gate.detach(), of(starts_in), decay, mix, 3);
+  if (h0.defined()) {
+    r.check_state(h0, "h0");
+    h0 = train ? h0.contiguous() : h0.detach().contiguous();
+  }
+  if (train) {
+    const auto out = Gated::apply(x, gate, maybe(h0), starts_in, decay, mix);
+    return {out[0], out[1]};
+  }
+  const GatedOut out = gated_forward(r, h0, false);
+  return {out.h, out.h_end};
+}
+
+Tensor gated_scan_step(const Tensor& x, const Tensor& gate, const Tensor& state, int64_t decay, bool mix) {
+  check_plain("gated_scan_step", {x, gate, state});
+  TORCH_CHECK_VALUE(!grad_wanted({x, gate, state}),
+                    "gated_scan_step has no gradients (x, gate or the state asks for one): call it under torch.no_grad, "
+                    "or gated_scan");
+  const Gates r = gates(x, gate, Tensor(), decay, mix, 2);
+  r.check_state(state, "state");
+  TORCH_CHECK_VALUE(state.is_contiguous(), "state must be contiguous: it is updated in place");
+  const c10::DeviceGuard guard(r.x.device());
+  const Tensor h = torch::empty({r.a.B, r.a.D}, r.x.options());
+  check(g.lsh_gated_step(&r.a, fp(state), raw(h), stream_of(r.x)), "lsh_gated_step");
+  // a graph that has saved the state from before is told, as by torch's own in-place operations
+  if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();
+  return h;
+}
+
+// ------------------------------------------------------------------------------- norms and rotation of heads
+struct Heads {
+  Tensor q, k, positions, freq, wq, wk;
+  lsh_rotate a = {};
+};
+// The sizes and what does not depend on q's and k's values.  lead: [T, B], or [B].
+void heads_of(Heads& r, torch::IntArrayRef lead, int64_t H, int64_t HK, int64_t D, double eps, bool neighbours) {
+  lsh_rotate& a = r.a;
+  const bool one = lead.size() == 1;
+  a.T = one ? 1 : lead[0], a.B = lead[one ? 0 : 1], a.H = H, a.HK = HK, a.D = (int)D;
+  a.neighbours = neighbours, a.eps = (float)eps;
+  if (r.freq.defined()) {
+    a.rot = 2 * (int)r.freq.size(0), a.inv_freq = r.freq.data_ptr<double>();
+    a.positions = r.positions.data_ptr<int64_t>();
+    if (one)
+      a.p_sb = r.positions.stride(0);
+    else
+      a.p_st = r.positions.stride(0), a.p_sb = r.positions.dim() == 2 ? r.positions.stride(1) : 0;
+  }
+  a.q_weight = fp(r.wq), a.k_weight = fp(r.wk);
+}
+void heads_data(Heads& r, const Tensor& q, const Tensor& k) {
+  lsh_rotate& a = r.a;
+  r.q = rows_of(q), r.k = rows_of(k);
+  a.dtype = code_of(q), a.q = raw(r.q), a.k = raw(r.k);
+  a.q_sb = step_of(r.q, -3), a.q_sh = step_of(r.q, -2), a.k_sb = step_of(r.k, -3), a.k_sh = step_of(r.k, -2);
+  if (q.dim() == 4) a.q_st = step_of(r.q, 0), a.k_st = step_of(r.k, 0);
+}
+variable_list rotate_forward(const Heads& r) {
+  const c10::DeviceGuard guard(r.q.device());
+  const Tensor qo = torch::empty(r.q.sizes(), r.q.options()), ko = torch::empty(r.k.sizes(), r.k.options());
+  check(g.lsh_rotate_fwd(&r.a, raw(qo), raw(ko), stream_of(r.q)), "lsh_rotate_fwd");
+  return {qo, ko};
+}
+
+struct NormRotate : public torch::autograd::Function<NormRotate> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Maybe& positions,
+                               const Maybe& freq, const Maybe& wq, const Maybe& wk, double eps, bool neighbours) {
+    Heads r;
+    r.positions = of(positions), r.freq = of(freq), r.wq = of(wq), r.wk = of(wk);
+    heads_data(r, q, k);
+    heads_of(r, q.sizes().slice(0, q.dim() - 2), q.size(-2), k.size(-2), q.size(-1), eps, neighbours);
+    const bool norm = r.wq.defined();
+    // a rotation alone needs no operand to go back
+    ctx->save_for_backward({norm ? r.q : Tensor(), norm ? r.k : Tensor(), r.positions, r.freq, r.wq, r.wk});
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["q"] = q.sizes().vec();
+    ctx->saved_data["k"] = k.sizes().vec();
+    ctx->saved_data["p"] = r.positions.defined() ? r.positions.sizes().vec() : std::vector<int64_t>{};
+    ctx->saved_data["n"] = std::vector<int64_t>{neighbours, norm, r.freq.defined(), r.freq.defined() ? r.freq.size(0) : 0,
+                                                (int64_t)q.scalar_type()};
+    ctx->set_materialize_grads(false);
+    return rotate_forward(r);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads_in) {
+    const variable_list grads = first_order(std::move(grads_in));
+    if (!grads[0].defined() && !grads[1].defined()) return variable_list(8);
+    const auto saved = ctx->get_saved_variables();
+    const auto n = ctx->saved_data["n"].toIntVector();
+    const auto qs = ctx->saved_data["q"].toIntVector(), ks = ctx->saved_data["k"].toIntVector();
+    const Tensor& like = grads[0].defined() ? grads[0] : grads[1];
+    const auto type = (torch::ScalarType)n[4];
+    const int64_t D = qs.back();
+    const auto lead = torch::IntArrayRef(qs).slice(0, qs.size() - 2);
+    Heads r;
+    if (n[2]) {
+      r.positions = unpacked(saved[2], ctx->saved_data["p"].toIntVector(), torch::kInt64, like);
+      r.freq = unpacked(saved[3], {n[3]}, torch::kFloat64, like).contiguous();
+    }
+    const c10::DeviceGuard guard(like.device());
+    if (n[1]) {
+      r.wq = unpacked(saved[4], {D}, torch::kFloat32, like).contiguous();
+      r.wk = unpacked(saved[5], {D}, torch::kFloat32, like).contiguous();
+      heads_data(r, unpacked(saved[0], qs, type, like), unpacked(saved[1], ks, type, like));
+    }
+    // heads whose outputs were not used leave no gradient
+    heads_of(r, lead, grads[0].defined() ? qs[qs.size() - 2] : 0, grads[1].defined() ? ks[ks.size() - 2] : 0, D,
+             ctx->saved_data["eps"].toDouble(), n[0]);
+    r.a.dtype = code_of(like);
+    Tensor gq, gk, dq, dk;
+    int64_t st[6] = {};
+    auto strides = [&](const Tensor& t, int64_t* to) {
+      to[0] = t.dim() == 4 ? step_of(t, 0) : 0, to[1] = step_of(t, -3), to[2] = step_of(t, -2);
+    };
+    if (grads[0].defined()) {
+      gq = rows_of(grads[0]), dq = torch::empty(qs, gq.options());
+      strides(gq, st);
+    }
+    if (grads[1].defined()) {
+      gk = rows_of(grads[1]), dk = torch::empty(ks, gk.options());
+      strides(gk, st + 3);
+    }
+    Tensor dwq, dwk;
+    if (n[1]) dwq = torch::empty({D}, r.wq.options()), dwk = torch::empty({D}, r.wk.options());
+    const size_t nb = g.lsh_rotate_bwd_workspace(&r.a);
+    const Tensor ws = workspace(nb, like);
+    check(g.lsh_rotate_bwd(&r.a, raw(gq), st[0], st[1], st[2], raw(gk), st[3], st[4], st[5], raw(dq), raw(dk), fp(dwq),
+                           fp(dwk), raw(ws), nb, stream_of(like)),
+          "lsh_rotate_bwd");
+    return {dq, dk, Tensor(), Tensor(), dwq, dwk, Tensor(), Tensor()};
+  }
+};
+
+std::tuple<Tensor, Tensor> norm_rotate(const Tensor& q, const Tensor& k, const Maybe& positions_in, const Maybe& freq_in,
+                                       const Maybe& wq_in, const Maybe& wk_in, double eps, bool neighbours) {
+  check_plain("norm_rotate", {q, k, of(freq_in), of(wq_in), of(wk_in)});
+  check_float(q, "q");
+  TORCH_CHECK_VALUE(q.dim() == 4 || q.dim() == 3, "q must be a [T, B, heads, D] tensor, or [B, heads, D]");
+  const auto lead = q.sizes().slice(0, q.dim() - 2);
+  const int64_t D = q.size(-1);
+  TORCH_CHECK_VALUE(k.dim() == q.dim() && k.sizes().slice(0, k.dim() - 2) == lead && k.size(-1) == D &&
+                        k.scalar_type() == q.scalar_type() && k.device() == q.device(),
+                    "k must be ", q.scalar_type(), " with the rows, batches and width of q on ", q.device(), ", got ",
+                    k.sizes(), " for ", q.sizes());
+  TORCH_CHECK_VALUE(D >= 2 && D % 2 == 0 && D <= LSH_ROTATE_MAX_D, "heads of ", D, ": even widths from 2 to ",
+                    LSH_ROTATE_MAX_D, " are supported");
+  TORCH_CHECK_VALUE(wq_in.has_value() == wk_in.has_value(), "q_weight and k_weight come together");
+  TORCH_CHECK_VALUE(eps >= 0, "eps=", eps, " must not be negative");
+  Heads r;
+  if (freq_in.has_value()) {
+    TORCH_CHECK_VALUE(positions_in.has_value(), "a rotation needs positions");
+    const Tensor &f = *freq_in, &p = *positions_in;
+    TORCH_CHECK_VALUE(f.dim() == 1 && f.device() == q.device() && f.is_floating_point() && f.size(0) <= D / 2,
+                      "inv_freq must be a float tensor of up to ", D / 2, " frequencies on ", q.device());
+    TORCH_CHECK_VALUE(!grad_wanted({f}), "inv_freq is a constant of norm_rotate: it gets no gradient (pass inv_freq.detach())");
+    TORCH_CHECK_VALUE((p.scalar_type() == torch::kInt64 || p.scalar_type() == torch::kInt32) && p.device() == q.device(),
+                      "positions must be int64 or int32 on ", q.device());
+    TORCH_CHECK_VALUE(p.sizes() == lead || (lead.size() == 2 && p.dim() == 1 && p.size(0) == lead[0]),
+                      "positions must be ", lead, lead.size() == 2 ? ", or one for each row" : "", ", got ", p.sizes());
+    r.freq = f.detach().to(torch::kFloat64).contiguous();
+    r.positions = p.to(torch::kInt64);
+  }
+  if (wq_in.has_value()) r.wq = channel(*wq_in, D, q, "q_weight"), r.wk = channel(*wk_in, D, q, "k_weight");
+  if (grad_wanted({q, k, r.wq, r.wk})) {
+    const auto out = NormRotate::apply(q, k, maybe(r.positions), maybe(r.freq), maybe(r.wq), maybe(r.wk), eps, neighbours);
+    return {out[0], out[1]};
+  }
+  heads_data(r, q.detach(), k.detach());
+  heads_of(r, lead, q.size(-2), k.size(-2), D, eps, neighbours);
+  const auto out = rotate_forward(r);
+  return {out[0], out[1]};
+}
+
 }  // namespace
 
 void register_lm_ops(pybind11::module_& m) {
@@ -536,4 +905,8 @@ void register_lm_ops(pybind11::module_& m) {
   m.def("block_norm", &block_norm, "norm after a block, gate, residual scale, norm before the next: x_new, z");
   m.def("embed", &embed, "embedding lookup with scaling");
   m.def("distill_topk", &distill_topk, "loss against a teacher's top logits, by row");
+  m.def("token_logprobs", &token_logprobs, "log probabilities of given tokens, entropy, top alternatives, by row");
+  m.def("gated_scan", &gated_scan, "gated linear recurrence over a sequence: h, state after the last row");
+  m.def("gated_scan_step", &gated_scan_step, "gated linear recurrence of one token, the state updated in place: h");
+  m.def("norm_rotate", &norm_rotate, "norms of queries and keys for each head and their rotation by position: q, k");
 }

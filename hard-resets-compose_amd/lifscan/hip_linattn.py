@@ -10,9 +10,10 @@ batch-major array, are not copied.
 
   lin_attn        a prompt or a training step, with gradients for q, k, v and the first state
   lin_attn_step   one new token; the state is updated in place
+  norm_rotate     before either: norms of queries and keys for each head and their rotation by position
 
 No counterpart in the reference.  There is no fallback: every call runs the HIP kernels of
-liblifscan_hip.so (linattn_kernels.hip) through the C++ operators of ``_ops_lm.cpp``, which check the
+liblifscan_hip.so (linattn_kernels.hip, rotate_kernels.hip) through the C++ operators of ``_ops_lm.cpp``, which check the
 arguments and raise ValueError.
 """
 import torch
@@ -50,3 +51,20 @@ def lin_attn_step(q, k, v, beta, state, scale=1.0):
     """One token: q [B, Hq, Dk], k [B, Hk, Dk], v [B, Hv, Dv] -> o [B, H, Dv]; `state` [B, H, Dk, Dv]
     (fp32, contiguous) is updated in place.  No gradients: train with lin_attn."""
     return _n.lm_ops().lin_attn_step(q, k, v, _decays(beta, q, k, v), state, scale)
+
+
+def norm_rotate(q, k, positions=None, inv_freq=None, q_weight=None, k_weight=None, eps=1e-6, pairs="halves"):
+    """Queries and keys as they enter attention -> (q, k), contiguous, of the same shapes and type:
+
+        y = x / sqrt(mean(x^2) + eps) * weight                           each head by itself
+        (y_i, y_j) -> (y_i cos a - y_j sin a, y_i sin a + y_j cos a)     a = position * inv_freq[p] for pair p
+
+    q [T, B, Hq, D], k [T, B, Hk, D], or [B, heads, D] for one token each: float32, bfloat16 or float16, one
+    type; even D from 2 to 256.  positions: int64 or int32, [T], [T, B], or [B] for one token each; any size,
+    also negative: angles are formed in 64 bits.  inv_freq: up to D/2 frequencies on the device (float64 keeps
+    them as they are); the first 2*len columns rotate, the others pass; None: no rotation.  pairs: "halves"
+    (column p with p + len) or "neighbours" (2p with 2p + 1).  q_weight, k_weight: [D] each; both None: no norm.
+    Gradients for q, k and the weights."""
+    if pairs not in ("halves", "neighbours"):
+        raise ValueError(f"pairs {pairs!r}: 'halves' or 'neighbours'")
+    return _n.lm_ops().norm_rotate(q, k, positions, inv_freq, q_weight, k_weight, eps, pairs == "neighbours")

@@ -4,6 +4,7 @@
   block_norm    the norm after a block, its gate and residual scale, and the norm before the next block
   embed         embedding lookup with scaling; the table's gradient sums by token
   distill_topk  the loss against a teacher's top logits
+  token_logprobs  log probabilities of given tokens, the entropy, the most likely alternatives
 
 Tensors are float32, bfloat16 or float16; sums and statistics are fp32 and every result is rounded to
 its tensor's type once.  Every operator is deterministic (no floating-point atomics).  No counterpart
@@ -51,3 +52,17 @@ def distill_topk(logits, top_values, top_index, temperature=1.0):
     An index outside the vocabulary is no entry (-1 pads short lists); a row without entries has loss 0
     and gradient 0; entries that name one id add up.  Only the logits get a gradient."""
     return _n.lm_ops().distill_topk(logits, top_values, top_index, temperature)
+
+
+def token_logprobs(logits, tokens, temperature=1.0, top=0):
+    """What a model says about given tokens -> (logp, entropy), fp32 [*rows]; with top = K > 0 also the most
+    likely alternatives (top_logp fp32, top_index int64), [*rows, K]:
+
+        p = softmax(logits / tau),  logp = log p[token],  entropy = -sum p log p
+
+    logits [*rows, V], read through its row stride; tokens [*rows], int64 or int32.  A token outside the
+    vocabulary is none: logp 0 without a gradient.  Alternatives come in order, equal logits by their id, NaN
+    first; top up to 64 and V.  The logits get a gradient from logp and from the entropy, not from the
+    alternatives.  A logit of -inf has probability 0; a row of nothing else has logp -inf, entropy 0 and no
+    gradient, and a row with NaN or +inf has NaN."""
+    return tuple(_n.lm_ops().token_logprobs(logits, tokens, temperature, top))

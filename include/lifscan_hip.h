@@ -606,6 +606,77 @@ int lsh_distill_bwd(int dtype, const void* logits, int64_t stride, int v_dtype, 
                     const int64_t* index, const float* stats, const float* g, int64_t g_stride,
                     void* dlogits, int64_t rows, int64_t V, int K, float tau, void* stream);
 
+/* A gated linear recurrence over time-major [T, B, D]:
+ *   a_t = sigmoid(gate_t) or exp(min(gate_t, 0)),  h_t = a_t*h_{t-1} + w_t*x_t,  w_t = 1 - a_t (mix) or 1
+ * and h_t = w_t*x_t where starts ([T, B] bytes, contiguous, or NULL) is not 0: what was before is dropped there.
+ * x, gate: of one type, with row and batch strides in elements.  h0: [B, D] fp32 or NULL (zeros).
+ * h: contiguous [T, B, D]; h_end: [B, D] fp32, the state after the last row (T = 0: h0). */
+#define LSH_DECAY_SIGMOID 0
+#define LSH_DECAY_LOG 1
+typedef struct lsh_gated {
+  int dtype, decay, mix;
+  int64_t T, B, D;
+  const void *x, *gate;
+  int64_t x_st, x_sb, g_st, g_sb;
+  const uint8_t* starts;
+  const float* h0;
+} lsh_gated;
+size_t lsh_gated_workspace(const lsh_gated* a); /* 0: ws may be NULL; the same for both directions */
+/* Floats that the gradients need of the forward (`saved`: the states before every 128 rows). */
+int64_t lsh_gated_saved(const lsh_gated* a);
+int lsh_gated_fwd(const lsh_gated* a, void* h, float* h_end, float* saved /* or NULL */, void* ws,
+                  size_t ws_bytes, void* stream);
+/* Its gradients from dh (with strides; NULL: zeros) and dh_end (NULL: zeros): contiguous dx and dgate
+ * [T, B, D], and dh0 [B, D] fp32 (or NULL).  h0 is not read. */
+int lsh_gated_bwd(const lsh_gated* a, const float* saved, const void* dh, int64_t dh_st, int64_t dh_sb,
+                  const float* dh_end, void* dx, void* dgate, float* dh0, void* ws, size_t ws_bytes,
+                  void* stream);
+/* One token (T = 1; row strides, starts and h0 are not read): `state` [B, D] fp32 is updated in place, h is
+ * [B, D]. */
+int lsh_gated_step(const lsh_gated* a, float* state, void* h, void* stream);
+
+/* Norms of queries and keys for each head and their rotation by position, over [T, B, heads, D]:
+ *   y = x / sqrt(mean(x^2) + eps) * weight  (weights NULL: y = x)
+ *   (y_i, y_j) -> (y_i cos - y_j sin, y_i sin + y_j cos),  angle = positions[t, b] * inv_freq[p]
+ * for the pairs p of the first rot columns: (p, p + rot/2), or (2p, 2p + 1) with neighbours; the other
+ * columns pass.  q and k have H and HK heads (either may be 0), strides in elements and a contiguous last
+ * axis; positions strides in elements; inv_freq [rot/2].  D and rot are even, 2 <= D <= LSH_ROTATE_MAX_D.
+ * q_out, k_out: contiguous. */
+#define LSH_ROTATE_MAX_D 256
+typedef struct lsh_rotate {
+  int dtype, D, rot, neighbours;
+  int64_t T, B, H, HK;
+  const void *q, *k;
+  int64_t q_st, q_sb, q_sh, k_st, k_sb, k_sh;
+  const int64_t* positions;
+  int64_t p_st, p_sb;
+  const double* inv_freq;
+  const float *q_weight, *k_weight;
+  float eps;
+} lsh_rotate;
+int lsh_rotate_fwd(const lsh_rotate* a, void* q_out, void* k_out, void* stream);
+/* Its gradients from gq and gk (with strides): contiguous dq and dk, and the weights' [D] fp32 (each may be
+ * NULL), summed in a fixed order.  Without weights q and k are not read. */
+size_t lsh_rotate_bwd_workspace(const lsh_rotate* a); /* 0: ws may be NULL */
+int lsh_rotate_bwd(const lsh_rotate* a, const void* gq, int64_t gq_st, int64_t gq_sb, int64_t gq_sh,
+                   const void* gk, int64_t gk_st, int64_t gk_sb, int64_t gk_sh, void* dq, void* dk,
+                   float* dq_weight, float* dk_weight, void* ws, size_t ws_bytes, void* stream);
+
+/* Log probabilities of given tokens over logits [rows, V] (a row stride in elements), with p the softmax of
+ * logits/tau: logp = log p[tokens] (0 for a token outside 0..V-1), entropy = -sum p log p, and the K largest
+ * logits of each row in order, ties to the lower id (NaN before all), as log p and ids [rows, K].  K <= V.
+ * A row of -inf alone has log p = -inf and entropy 0.  stats: [3, rows], what the gradient reads, or NULL.
+ *   dlogits = (g*([v = token] - p) - ge*p*(log p + entropy)) / tau, contiguous [rows, V]; g (without a token:
+ * 0) and ge: [rows] with element strides, each may be NULL (zeros). */
+#define LSH_SCORE_MAX_TOP 64
+size_t lsh_score_workspace(int64_t rows, int64_t V, int K); /* 0: ws may be NULL */
+int lsh_score_fwd(int dtype, const void* logits, int64_t stride, const int64_t* tokens, float* logp,
+                  float* entropy, float* stats, float* top_logp, int64_t* top_index, int64_t rows, int64_t V,
+                  int K, float tau, void* ws, size_t ws_bytes, void* stream);
+int lsh_score_bwd(int dtype, const void* logits, int64_t stride, const int64_t* tokens, const float* stats,
+                  const float* g_logp, int64_t g_stride, const float* g_entropy, int64_t ge_stride,
+                  void* dlogits, int64_t rows, int64_t V, float tau, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
