@@ -23,7 +23,8 @@
 
 namespace lsh {
 
-constexpr int kGsR = 16, kGsW = 8, kGsRows = kGsR * kGsW;
+// Rows of a wave forwards and backwards, waves of a workgroup, rows of a forward round, and rows between saved states.
+constexpr int kGsR = 16, kGsB = 8, kGsW = 8, kGsRows = kGsR * kGsW, kGsSave = kGsB * kGsW;
 
 struct GsArgs {
   const void *x, *g;
@@ -31,7 +32,7 @@ struct GsArgs {
   const uint8_t* starts;  // [T, B], or NULL
   const float* h0;        // [n], or NULL
   void* h;
-  float *h_end, *saved;   // saved: [ceil(T / kGsRows), n], or NULL
+  float *h_end, *saved;   // saved: the states before every kGsSave rows, or NULL
   const void* dh;
   int64_t d_st, d_sb;
   const float* d_end;
@@ -42,10 +43,13 @@ struct GsArgs {
   int groups, S, sigmoid, mix;
 };
 
-// e^x for x <= 0: the hardware's power of two with what the product x*log2(e) loses put back
+// e^x for x <= 0: the hardware's power of two with what the product x*log2(e) loses put back.  16-bit gates go without
+// (6 instructions of 30 an element): it is |x|*2^-24 of a weight, of which 2^-8 or 2^-11 is seen.
+template <bool FINE>
 __device__ __forceinline__ float gs_exp(float x) {
-  x = x < -150.0f ? -150.0f : x;  // 0, and no inf - inf; a NaN stays
   constexpr float kHi = 1.44269502f, kLo = 1.92596299e-8f;  // log2(e)
+  if constexpr (!FINE) return __builtin_amdgcn_exp2f(x * kHi);
+  x = x < -150.0f ? -150.0f : x;  // 0, and no inf - inf; a NaN stays
   const float t = x * kHi, r = __builtin_fmaf(x, kHi, -t) + x * kLo;
   const float y = __builtin_amdgcn_exp2f(t);
   return __builtin_fmaf(y, r * 0.693147181f, y);
@@ -54,9 +58,10 @@ __device__ __forceinline__ float gs_exp(float x) {
 // (a, 1 - a).  Of a sigmoid the smaller one is e/(1 + e) with e = exp(-|g|), 1 - e^g is a Taylor sum where it would
 // cancel, and a decay near one is what is left of one: it is raised to hundreds of rows, so it is rounded once (with
 // the hardware's 1/(1 + e) and 2^x in its place the results of 1000 rows in fp32 were off by 7.2e-7 of their norm, so 2.2e-7).
-__device__ __forceinline__ void gs_gate(int sigmoid, float g, float& a, float& w) {
-  if (sigmoid) {
-    const float e = gs_exp(-__builtin_fabsf(g)), s = e * __builtin_amdgcn_rcpf(1.0f + e), r = 1.0f - s;
+template <bool FINE, bool SIGMOID>
+__device__ __forceinline__ void gs_gate(float g, float& a, float& w) {
+  if constexpr (SIGMOID) {
+    const float e = gs_exp<FINE>(-__builtin_fabsf(g)), s = e * __builtin_amdgcn_rcpf(1.0f + e), r = 1.0f - s;
     a = g >= 0.0f ? r : s;
     w = g >= 0.0f ? s : r;
   } else {
@@ -67,7 +72,7 @@ __device__ __forceinline__ void gs_gate(int sigmoid, float g, float& a, float& w
     p = __builtin_fmaf(g, p, 1.0f / 6);
     p = __builtin_fmaf(g, p, 0.5f);
     p = __builtin_fmaf(g, p, 1.0f);
-    const float e = gs_exp(g);
+    const float e = gs_exp<FINE>(g);
     w = g > -0.35f ? -g * p : 1.0f - e;
     a = g > -0.35f ? 1.0f - w : e;
   }
@@ -85,99 +90,180 @@ __device__ __forceinline__ float gs_product(float first, float then) {
   return MASK && gs_marked(then) ? then : MASK && gs_marked(first) ? first : first * then;
 }
 
-// A lane's channels
-template <class T, int V>
+// FAST: 4 bytes a lane and row (two channels of 16 bits), and a row's lanes within 4 GB of each other, so that an address
+// is a scalar and an offset.  Otherwise a channel a lane, wherever it lies.
+template <class T, bool FAST>
+constexpr int kGsV = FAST && sizeof(T) == 2 ? 2 : 1;
+template <bool FAST>
+using GsOff = std::conditional_t<FAST, uint32_t, uint64_t>;
+
+// A lane's channels.  A lane beyond the last channel does the last ones once more, to the same values.
+template <class T, bool FAST>
 struct GsLane {
-  bool there;
-  int64_t c, b, x_at, g_at, d_at;  // the first channel, its batch, and where they lie in a row
+  static constexpr int V = kGsV<T, FAST>;
+  int64_t c0, c, b0, b, d;  // the first channel of the wave and of the lane, their batches, the lane's column
   __device__ __forceinline__ GsLane(const GsArgs& a, int group) {
-    const int64_t p = (int64_t)group * 64 + (threadIdx.x & 63);
-    there = p < a.pieces;
-    c = (there ? p : a.pieces - 1) * V;
-    b = c / a.D;
-    const int64_t d = c - b * a.D;
-    x_at = b * a.x_sb + d, g_at = b * a.g_sb + d, d_at = b * a.d_sb + d;
+    const int64_t p0 = (int64_t)group * 64, p = min(p0 + (threadIdx.x & 63), a.pieces - 1);
+    c0 = p0 * V, c = p * V;
+    b0 = c0 / a.D, b = c / a.D, d = c - b * a.D;
   }
 };
 
-// kGsR rows of a lane as read; rows from `end` on are read from the one before it
+// A lane's V values of a row as they lie in memory: two of 16 bits stay in one register.
 template <class T, int V>
-struct GsRows {
-  Vec<T, V> v[kGsR];
-  __device__ __forceinline__ void load(const T* p, int64_t stride, int64_t t, int64_t end) {
-    if (t + kGsR <= end) {
-      p += t * stride;
+struct GsRaw {
+  std::conditional_t<V * sizeof(T) == 4, uint32_t, uint16_t> x;
+  __device__ __forceinline__ float get(int j) const {
+    if constexpr (sizeof(T) == 4)
+      return __builtin_bit_cast(float, x);
+    else if constexpr (V == 1)
+      return to_f(__builtin_bit_cast(T, x));
+    else if constexpr (std::is_same_v<T, bf16_t>)
+      return __builtin_bit_cast(float, j ? x & 0xffff0000u : x << 16);
+    else
+      return to_f(__builtin_bit_cast(T, (uint16_t)(x >> 16 * j)));
+  }
+  __device__ __forceinline__ void set(const float (&f)[V]) {
+    Vec<T, V> y;
 #pragma unroll
-      for (int i = 0; i < kGsR; ++i) v[i] = *(const Vec<T, V>*)(p + i * stride);
+    for (int j = 0; j < V; ++j) y.v[j] = from_f<T>(f[j]);
+    x = __builtin_bit_cast(decltype(x), y);
+  }
+};
+
+// One operand as a lane reads it, row by row
+template <class T, bool FAST>
+struct GsIn {
+  static constexpr int V = kGsV<T, FAST>;
+  const T* base;
+  int64_t stride;
+  GsOff<FAST> off;
+  __device__ __forceinline__ GsIn(const void* p, int64_t st, int64_t sb, const GsLane<T, FAST>& at)
+      : base((const T*)p + at.b0 * sb), stride(st), off((GsOff<FAST>)(((at.b - at.b0) * sb + at.d) * sizeof(T))) {}
+  __device__ __forceinline__ GsRaw<T, V> row(int64_t t) const {
+    return *(const GsRaw<T, V>*)((const char*)(base + t * stride) + off);
+  }
+};
+template <class T, bool FAST>
+struct GsOut {
+  static constexpr int V = kGsV<T, FAST>;
+  T* base;
+  int64_t n;
+  uint32_t off;
+  __device__ __forceinline__ GsOut(void* p, int64_t n, const GsLane<T, FAST>& at)
+      : base((T*)p + at.c0), n(n), off((uint32_t)((at.c - at.c0) * sizeof(T))) {}
+  __device__ __forceinline__ void put(int64_t t, const float (&f)[V]) const {
+    GsRaw<T, V> x;
+    x.set(f);
+    *(GsRaw<T, V>*)((char*)(base + t * n) + off) = x;
+  }
+};
+
+// R rows of a lane as read; rows from `end` on are read from the one before it
+template <class T, bool FAST, int R>
+struct GsRows {
+  GsRaw<T, kGsV<T, FAST>> v[R];
+  __device__ __forceinline__ void load(const GsIn<T, FAST>& in, int64_t t, int64_t end) {
+    if (t + R <= end) {
+#pragma unroll
+      for (int i = 0; i < R; ++i) v[i] = in.row(t + i);
     } else {
 #pragma unroll
-      for (int i = 0; i < kGsR; ++i) {
-        const int64_t at = t + i < end ? t + i : end - 1;
-        v[i] = *(const Vec<T, V>*)(p + at * stride);
-      }
+      for (int i = 0; i < R; ++i) v[i] = in.row(t + i < end ? t + i : end - 1);
     }
   }
+  __device__ __forceinline__ float get(int i, int j) const { return v[i].get(j); }
 };
-struct GsStarts {
-  uint8_t v[kGsR];
-  __device__ __forceinline__ void load(const GsArgs& a, int64_t b, int64_t t, int64_t end) {
+// A bit for each of R rows that starts a sequence
+template <bool MASK, int R>
+__device__ __forceinline__ unsigned gs_starts(const GsArgs& a, int64_t b, int64_t t, int64_t end) {
+  unsigned bits = 0;
+  if constexpr (MASK)
+    if (t < end) {
+      uint8_t v[R];
 #pragma unroll
-    for (int i = 0; i < kGsR; ++i) v[i] = a.starts[(t + i < end ? t + i : end - 1) * a.B + b];
-  }
-};
+      for (int i = 0; i < R; ++i) v[i] = a.starts[(t + i < end ? t + i : end - 1) * a.B + b];
+#pragma unroll
+      for (int i = 0; i < R; ++i) bits |= (v[i] != 0) << i;
+    }
+  return bits;
+}
+__device__ __forceinline__ bool gs_bit(unsigned bits, int i) { return bits >> i & 1; }
 
-// Where segments are needed: the map of each, forwards (x, gate) or backwards (gate, dh).  A wave takes its share of the
-// segment's rows, its map in registers.
-template <class T, int V, bool MASK, bool BWD>
-__global__ __launch_bounds__(kGsW * 64) void k_gated_sums(GsArgs a) {
-  __shared__ float s_map[kGsW][2][64 * V];
+// Calls f with whether the decay is a sigmoid and whether inputs are weighed, as constants: the branch stands once
+// around a chunk of rows.
+template <class F>
+__device__ __forceinline__ void gs_form(const GsArgs& a, F&& f) {
+  if (a.sigmoid) {
+    if (a.mix)
+      f(std::true_type{}, std::true_type{});
+    else
+      f(std::true_type{}, std::false_type{});
+  } else {
+    if (a.mix)
+      f(std::false_type{}, std::true_type{});
+    else
+      f(std::false_type{}, std::false_type{});
+  }
+}
+
+// Where segments are needed: the map of each but the last, forwards (x, gate), or of each but the first, backwards
+// (gate, dh).  A wave takes its share of the segment's rows, its map in registers; backwards the map is summed with
+// the product of the decays so far, from the first row on.
+constexpr int kGsSumW = 4;
+template <class T, bool FAST, bool MASK, bool BWD>
+__global__ __launch_bounds__(kGsSumW * 64, 4) void k_gated_sums(GsArgs a) {
+  constexpr int V = kGsV<T, FAST>;
+  __shared__ float s_map[kGsSumW][2][64 * V];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int group = blockIdx.x % a.groups, seg = blockIdx.x / a.groups;
-  const GsLane<T, V> at(a, group);
-  const T* x = BWD ? (const T*)a.dh + at.d_at : (const T*)a.x + at.x_at;
-  const int64_t x_st = BWD ? a.d_st : a.x_st;
-  const T* g = (const T*)a.g + at.g_at;
+  const int group = blockIdx.x % a.groups, seg = blockIdx.x / a.groups + (BWD ? 1 : 0);
+  const GsLane<T, FAST> at(a, group);
+  const GsIn<T, FAST> x = BWD ? GsIn<T, FAST>(a.dh, a.d_st, a.d_sb, at) : GsIn<T, FAST>(a.x, a.x_st, a.x_sb, at);
+  const GsIn<T, FAST> g(a.g, a.g_st, a.g_sb, at);
   const int64_t t1 = min(a.T, (seg + 1) * a.len);
-  const int64_t per = a.len / kGsW, lo = seg * a.len + wave * per, hi = min(t1, lo + per);
+  const int64_t per = a.len / kGsSumW, lo = seg * a.len + wave * per, hi = min(t1, lo + per);
   float P[V], H[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) P[j] = 1.0f, H[j] = 0.0f;
   const bool zeros = BWD && !a.dh;
-  for (int64_t k = lo; k < hi; k += kGsR) {
-    const int64_t t = BWD ? lo + (hi - lo - 1) / kGsR * kGsR - (k - lo) : k;
-    GsRows<T, V> rx, rg;
-    GsStarts rs;
-    if (!zeros) rx.load(x, x_st, t, hi);
-    rg.load(g, a.g_st, t, hi);
-    if (MASK) rs.load(a, at.b, t, hi);
+  GsRows<T, FAST, kGsR> nx, ng;
+  auto load = [&](int64_t t) {
+    if (!zeros) nx.load(x, t, hi);
+    ng.load(g, t, hi);
+  };
+  if (lo < hi) load(lo);
+  for (int64_t t = lo; t < hi; t += kGsR) {
+    const GsRows<T, FAST, kGsR> rx = nx, rg = ng;
+    const unsigned starts = gs_starts<MASK, kGsR>(a, at.b, t, hi);
+    if (t + kGsR < hi) load(t + kGsR);
+    gs_form(a, [&](auto sig, auto mix) {
 #pragma unroll
-    for (int n = 0; n < kGsR; ++n) {
-      const int i = BWD ? kGsR - 1 - n : n;
-      if (t + i >= hi) continue;
+      for (int i = 0; i < kGsR; ++i) {
+        if (t + i >= hi) break;
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        float f, w;
-        gs_gate(a.sigmoid, to_f(rg.v[i].v[j]), f, w);
-        if (MASK && rs.v[i]) f = __builtin_bit_cast(float, kGsStart);
-        if constexpr (BWD) {
-          const float d = zeros ? 0.0f : to_f(rx.v[i].v[j]);
-          H[j] = MASK && gs_marked(f) ? 0.0f : f * (d + H[j]);
-        } else {
-          const float v = to_f(rx.v[i].v[j]);
-          H[j] = gs_apply<MASK>(f, a.mix ? w * v : v, H[j]);
+        for (int j = 0; j < V; ++j) {
+          float f, w;
+          gs_gate<sizeof(T) == 4, decltype(sig)::value>(rg.get(i, j), f, w);
+          if (MASK && gs_bit(starts, i)) f = __builtin_bit_cast(float, kGsStart);
+          P[j] = gs_product<MASK>(P[j], f);
+          const float v = BWD && zeros ? 0.0f : rx.get(i, j);
+          if constexpr (BWD)
+            H[j] = MASK && gs_marked(P[j]) ? H[j] : __builtin_fmaf(P[j], v, H[j]);
+          else
+            H[j] = gs_apply<MASK>(f, decltype(mix)::value ? w * v : v, H[j]);
         }
-        P[j] = gs_product<MASK>(P[j], f);
       }
-    }
+    });
   }
 #pragma unroll
   for (int j = 0; j < V; ++j) s_map[wave][0][lane * V + j] = P[j], s_map[wave][1][lane * V + j] = H[j];
   __syncthreads();
-  if (wave != 0 || !at.there) return;
+  if (wave != 0) return;
 #pragma unroll
   for (int j = 0; j < V; ++j) P[j] = 1.0f, H[j] = 0.0f;
-  for (int n = 0; n < kGsW; ++n) {
-    const int w = BWD ? kGsW - 1 - n : n;
+#pragma unroll
+  for (int n = 0; n < kGsSumW; ++n) {
+    const int w = BWD ? kGsSumW - 1 - n : n;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       const float p = s_map[w][0][lane * V + j];
@@ -223,125 +309,143 @@ __device__ __forceinline__ void gs_enter(const GsArgs& a, int seg, int64_t c, co
   __syncthreads();
 }
 
-template <class T, int V, bool MASK>
-__global__ __launch_bounds__(kGsW * 64) void k_gated(GsArgs a) {
-  __shared__ float s_map[2][kGsW][2][64 * V];
+// One barrier a round: what a wave writes for the next round goes to the other half of the LDS.  The state after a
+// round is what its last wave ends with.
+template <class T, bool FAST, bool MASK>
+__global__ __launch_bounds__(kGsW * 64, 4) void k_gated(GsArgs a) {
+  constexpr int V = kGsV<T, FAST>;
+  __shared__ float s_map[2][kGsW][2][64 * V], s_carry[2][64 * V];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), W = blockDim.x >> 6;
   const int group = blockIdx.x % a.groups, seg = blockIdx.x / a.groups;
-  const GsLane<T, V> at(a, group);
-  const T *x = (const T*)a.x + at.x_at, *g = (const T*)a.g + at.g_at;
-  T* out = (T*)a.h + at.c;
+  const GsLane<T, FAST> at(a, group);
+  const GsIn<T, FAST> x(a.x, a.x_st, a.x_sb, at), g(a.g, a.g_st, a.g_sb, at);
+  const GsOut<T, FAST> out(a.h, a.n, at);
   const int64_t t0 = seg * a.len, t1 = min(a.T, t0 + a.len);
-  float h[V];  // before the round
-  gs_enter<V, MASK, false>(a, seg, at.c, a.h0, h, s_map[0]);
-  GsRows<T, V> rx, rg;
-  GsStarts rs;
+  GsRows<T, FAST, kGsR> rx, rg;
   int64_t t = t0 + wave * kGsR;
-  if (t < t1) {
-    rx.load(x, a.x_st, t, t1), rg.load(g, a.g_st, t, t1);
-    if (MASK) rs.load(a, at.b, t, t1);
-  }
+  auto load = [&](int64_t t) { rx.load(x, t, t1), rg.load(g, t, t1); };
+  if (t < t1) load(t);
+  float h[V];  // before the round, then before the wave's rows
+  gs_enter<V, MASK, false>(a, seg, at.c, a.h0, h, s_map[0]);
+  if (wave == W - 1)
+#pragma unroll
+    for (int j = 0; j < V; ++j) s_carry[0][lane * V + j] = h[j];
   int buf = 0;
   for (int64_t r = t0; r < t1; r += W * kGsR, t += W * kGsR, buf ^= 1) {
     float f[kGsR][V], b[kGsR][V], P[V], H[V];
+    const unsigned starts = gs_starts<MASK, kGsR>(a, at.b, t, t1);
+    gs_form(a, [&](auto sig, auto mix) {
+#pragma unroll
+      for (int i = 0; i < kGsR; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          float w;
+          gs_gate<sizeof(T) == 4, decltype(sig)::value>(rg.get(i, j), f[i][j], w);
+          b[i][j] = decltype(mix)::value ? w * rx.get(i, j) : rx.get(i, j);
+        }
+    });
+#pragma unroll
+    for (int i = 0; i < kGsR; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (MASK && gs_bit(starts, i)) f[i][j] = __builtin_bit_cast(float, kGsStart);
+    if (t + kGsR > t1)
+#pragma unroll
+      for (int i = 0; i < kGsR; ++i)
+        if (t + i >= t1)
+#pragma unroll
+          for (int j = 0; j < V; ++j) f[i][j] = 1.0f, b[i][j] = 0.0f;
+    if (const int64_t next = t + W * kGsR; next < t1) load(next);
 #pragma unroll
     for (int j = 0; j < V; ++j) P[j] = 1.0f, H[j] = 0.0f;
 #pragma unroll
     for (int i = 0; i < kGsR; ++i)
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        float w;
-        gs_gate(a.sigmoid, to_f(rg.v[i].v[j]), f[i][j], w);
-        const float v = to_f(rx.v[i].v[j]);
-        b[i][j] = a.mix ? w * v : v;
-        if (MASK && rs.v[i]) f[i][j] = __builtin_bit_cast(float, kGsStart);
-        if (t + i >= t1) f[i][j] = 1.0f, b[i][j] = 0.0f;
         H[j] = gs_apply<MASK>(f[i][j], b[i][j], H[j]);
         P[j] = gs_product<MASK>(P[j], f[i][j]);
       }
-    if (const int64_t next = t + W * kGsR; next < t1) {
-      rx.load(x, a.x_st, next, t1), rg.load(g, a.g_st, next, t1);
-      if (MASK) rs.load(a, at.b, next, t1);
-    }
 #pragma unroll
     for (int j = 0; j < V; ++j) s_map[buf][wave][0][lane * V + j] = P[j], s_map[buf][wave][1][lane * V + j] = H[j];
     __syncthreads();
-    if (a.saved && wave == 0 && at.there)
 #pragma unroll
-      for (int j = 0; j < V; ++j) a.saved[r / kGsRows * a.n + at.c + j] = h[j];
-    float mine[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) mine[j] = h[j];
-    for (int w = 0; w < W; ++w) {
-      if (w == wave)
-#pragma unroll
-        for (int j = 0; j < V; ++j) mine[j] = h[j];
+    for (int j = 0; j < V; ++j) h[j] = s_carry[buf][lane * V + j];
+    for (int w = 0; w < wave; ++w)
 #pragma unroll
       for (int j = 0; j < V; ++j)
         h[j] = gs_apply<MASK>(s_map[buf][w][0][lane * V + j], s_map[buf][w][1][lane * V + j], h[j]);
-    }
+    if (a.saved && t % kGsSave == 0 && t < t1)
+#pragma unroll
+      for (int j = 0; j < V; ++j) a.saved[t / kGsSave * a.n + at.c + j] = h[j];
 #pragma unroll
     for (int i = 0; i < kGsR; ++i) {
-      Vec<T, V> y;
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        mine[j] = gs_apply<MASK>(f[i][j], b[i][j], mine[j]);
-        y.v[j] = from_f<T>(mine[j]);
-      }
-      if (at.there && t + i < t1) *(Vec<T, V>*)(out + (t + i) * a.n) = y;
+      for (int j = 0; j < V; ++j) h[j] = gs_apply<MASK>(f[i][j], b[i][j], h[j]);
+      if (t + i < t1) out.put(t + i, h);
     }
+    if (wave == W - 1)
+#pragma unroll
+      for (int j = 0; j < V; ++j) s_carry[buf ^ 1][lane * V + j] = h[j];
   }
-  if (t1 == a.T && wave == 0 && at.there)
+  if (t1 == a.T && wave == W - 1)
 #pragma unroll
     for (int j = 0; j < V; ++j) a.h_end[at.c + j] = h[j];
 }
 
-template <class T, int V, bool MASK>
-__global__ __launch_bounds__(kGsW * 64) void k_gated_bwd(GsArgs a) {
-  __shared__ float s_map[2][kGsW][3][64 * V];
+// The gradients, the rounds from the last.  A first sweep over the rows in registers forms the wave's maps of both
+// directions, a second one forwards the states and what multiplies the adjoint, a third one backwards the adjoint: the
+// gates' powers are formed twice, which is cheaper than keeping them (two workgroups a CU need 128 registers).
+template <class T, bool FAST, bool MASK>
+__global__ __launch_bounds__(kGsW * 64, 4) void k_gated_bwd(GsArgs a) {
+  constexpr int V = kGsV<T, FAST>;
+  __shared__ float s_map[2][kGsW][3][64 * V], s_carry[2][64 * V];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), W = blockDim.x >> 6;
   const int group = blockIdx.x % a.groups, seg = blockIdx.x / a.groups;
-  const GsLane<T, V> at(a, group);
-  const T *x = (const T*)a.x + at.x_at, *g = (const T*)a.g + at.g_at, *d = (const T*)a.dh + at.d_at;
-  T *dx = (T*)a.dx + at.c, *dg = (T*)a.dg + at.c;
-  const int64_t t0 = seg * a.len, t1 = min(a.T, t0 + a.len), rows = W * kGsR;
-  float F[V];  // behind the round
+  const GsLane<T, FAST> at(a, group);
+  const GsIn<T, FAST> x(a.x, a.x_st, a.x_sb, at), g(a.g, a.g_st, a.g_sb, at), d(a.dh, a.d_st, a.d_sb, at);
+  const GsOut<T, FAST> dx(a.dx, a.n, at), dg(a.dg, a.n, at);
+  const int64_t t0 = seg * a.len, t1 = min(a.T, t0 + a.len), rows = W * kGsB;
+  float F[V];  // behind the round, then behind the wave's rows
   gs_enter<V, MASK, true>(a, seg, at.c, a.d_end, F, (float(*)[2][64 * V])s_map[0]);
+  if (wave == 0)
+#pragma unroll
+    for (int j = 0; j < V; ++j) s_carry[0][lane * V + j] = F[j];
   int buf = 0;
   for (int64_t r = t0 + (t1 - t0 - 1) / rows * rows; r >= t0 && t1 > t0; r -= rows, buf ^= 1) {
-    const int64_t t = r + wave * kGsR;
-    GsRows<T, V> rx, rg, rd;
-    GsStarts rs;
+    const int64_t t = r + wave * kGsB;
+    GsRows<T, FAST, kGsB> rx, rg, rd;
     if (t < t1) {
-      rx.load(x, a.x_st, t, t1), rg.load(g, a.g_st, t, t1);
-      if (a.dh) rd.load(d, a.d_st, t, t1);
-      if (MASK) rs.load(a, at.b, t, t1);
+      rx.load(x, t, t1), rg.load(g, t, t1);
+      if (a.dh) rd.load(d, t, t1);
     }
-    float h[V];  // before the round
+    const unsigned starts = gs_starts<MASK, kGsB>(a, at.b, t, t1);
+    float h[V];  // before the round, then before the wave's rows
 #pragma unroll
-    for (int j = 0; j < V; ++j) h[j] = a.saved[r / kGsRows * a.n + at.c + j];
-    float f[kGsR][V], hp[kGsR][V], P[V], H[V], Q[V];
+    for (int j = 0; j < V; ++j) h[j] = a.saved[r / kGsSave * a.n + at.c + j];
+    // rows that are not there: a decay of 1, an input and a gradient of 0
+    const bool tail = t + kGsB > t1;
+    if (tail || !a.dh)
+#pragma unroll
+      for (int i = 0; i < kGsB; ++i)
+        if (t + i >= t1 || !a.dh) rd.v[i].x = 0;
+    float P[V], H[V], Q[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) P[j] = 1.0f, H[j] = Q[j] = 0.0f;
+    gs_form(a, [&](auto sig, auto mix) {
 #pragma unroll
-    for (int i = 0; i < kGsR; ++i)
+      for (int i = 0; i < kGsB; ++i) {
+        if (tail && t + i >= t1) break;
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        float w;
-        gs_gate(a.sigmoid, to_f(rg.v[i].v[j]), f[i][j], w);
-        const float v = to_f(rx.v[i].v[j]);
-        hp[i][j] = a.mix ? w * v : v;  // the row's input, until its state stands here
-        if (MASK && rs.v[i]) f[i][j] = __builtin_bit_cast(float, kGsStart);
-        if (t + i >= t1) f[i][j] = 1.0f, hp[i][j] = 0.0f;
-        H[j] = gs_apply<MASK>(f[i][j], hp[i][j], H[j]);
-        P[j] = gs_product<MASK>(P[j], f[i][j]);
+        for (int j = 0; j < V; ++j) {
+          float f, w;
+          gs_gate<sizeof(T) == 4, decltype(sig)::value>(rg.get(i, j), f, w);
+          if (MASK && gs_bit(starts, i)) f = __builtin_bit_cast(float, kGsStart);
+          H[j] = gs_apply<MASK>(f, decltype(mix)::value ? w * rx.get(i, j) : rx.get(i, j), H[j]);
+          P[j] = gs_product<MASK>(P[j], f);
+          Q[j] = MASK && gs_marked(P[j]) ? Q[j] : __builtin_fmaf(P[j], rd.get(i, j), Q[j]);
+        }
       }
-    auto grad = [&](int i, int j) { return a.dh && t + i < t1 ? to_f(rd.v[i].v[j]) : 0.0f; };
-#pragma unroll
-    for (int i = kGsR - 1; i >= 0; --i)
-#pragma unroll
-      for (int j = 0; j < V; ++j)
-        Q[j] = MASK && gs_marked(f[i][j]) ? 0.0f : f[i][j] * (grad(i, j) + Q[j]);
+    });
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       s_map[buf][wave][0][lane * V + j] = P[j];
@@ -353,43 +457,58 @@ __global__ __launch_bounds__(kGsW * 64) void k_gated_bwd(GsArgs a) {
 #pragma unroll
       for (int j = 0; j < V; ++j)
         h[j] = gs_apply<MASK>(s_map[buf][w][0][lane * V + j], s_map[buf][w][1][lane * V + j], h[j]);
-    float mine[V];
-    for (int w = W - 1; w >= 0; --w) {
-      if (w == wave)
 #pragma unroll
-        for (int j = 0; j < V; ++j) mine[j] = F[j];
+    for (int j = 0; j < V; ++j) F[j] = s_carry[buf][lane * V + j];
+    for (int w = W - 1; w > wave; --w)
 #pragma unroll
       for (int j = 0; j < V; ++j)
         F[j] = gs_apply<MASK>(s_map[buf][w][0][lane * V + j], s_map[buf][w][2][lane * V + j], F[j]);
-    }
+    // the first sweep's values are not to be kept for the second
 #pragma unroll
-    for (int i = 0; i < kGsR; ++i)
+    for (int i = 0; i < kGsB; ++i) asm volatile("" : "+v"(rg.v[i].x), "+v"(rx.v[i].x));
+    // dx = w*E, dgate = u*E, F = f*E
+    float f[kGsB][V], w[kGsB][V], u[kGsB][V];
+    gs_form(a, [&](auto sig, auto mix) {
+      constexpr bool SIG = decltype(sig)::value, MIX = decltype(mix)::value;
+#pragma unroll
+      for (int i = 0; i < kGsB; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const float gate = rg.get(i, j), v = rx.get(i, j);
+          float p, q;
+          gs_gate<sizeof(T) == 4, SIG>(gate, p, q);
+          const float slope = SIG ? p * q : gate > 0.0f ? 0.0f : p;
+          const bool start = MASK && gs_bit(starts, i);
+          const float before = start ? 0.0f : h[j];
+          u[i][j] = (MIX ? before - v : before) * slope;
+          w[i][j] = MIX ? q : 1.0f;
+          f[i][j] = start ? __builtin_bit_cast(float, kGsStart) : p;
+          h[j] = __builtin_fmaf(p, before, MIX ? q * v : v);
+        }
+    });
+    if (tail)
+#pragma unroll
+      for (int i = 0; i < kGsB; ++i)
+        if (t + i >= t1)
+#pragma unroll
+          for (int j = 0; j < V; ++j) f[i][j] = 1.0f;
+#pragma unroll
+    for (int i = kGsB - 1; i >= 0; --i) {
+      float yx[V], yg[V];
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float b = hp[i][j];
-        hp[i][j] = MASK && gs_marked(f[i][j]) ? 0.0f : h[j];
-        h[j] = gs_apply<MASK>(f[i][j], b, h[j]);
+        const float E = rd.get(i, j) + F[j];
+        yx[j] = w[i][j] * E;
+        yg[j] = u[i][j] * E;
+        F[j] = MASK && gs_marked(f[i][j]) ? 0.0f : f[i][j] * E;
       }
-#pragma unroll
-    for (int i = kGsR - 1; i >= 0; --i) {
-      Vec<T, V> yx, yg;
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float gate = to_f(rg.v[i].v[j]), v = to_f(rx.v[i].v[j]), E = grad(i, j) + mine[j];
-        float p, w;
-        gs_gate(a.sigmoid, gate, p, w);
-        const float slope = a.sigmoid ? p * w : gate > 0.0f ? 0.0f : p;
-        yx.v[j] = from_f<T>(a.mix ? w * E : E);
-        yg.v[j] = from_f<T>(E * (a.mix ? hp[i][j] - v : hp[i][j]) * slope);
-        mine[j] = MASK && gs_marked(f[i][j]) ? 0.0f : f[i][j] * E;
-      }
-      if (at.there && t + i < t1) {
-        *(Vec<T, V>*)(dx + (t + i) * a.n) = yx;
-        *(Vec<T, V>*)(dg + (t + i) * a.n) = yg;
-      }
+      if (t + i < t1) dx.put(t + i, yx), dg.put(t + i, yg);
     }
+    if (wave == 0)
+#pragma unroll
+      for (int j = 0; j < V; ++j) s_carry[buf ^ 1][lane * V + j] = F[j];
   }
-  if (a.dh0 && seg == 0 && wave == 0 && at.there)
+  if (a.dh0 && seg == 0 && wave == 0)
 #pragma unroll
     for (int j = 0; j < V; ++j) a.dh0[at.c + j] = F[j];
 }
@@ -408,7 +527,10 @@ __global__ __launch_bounds__(kGsStep) void k_gated_step(GsArgs a, float* __restr
 #pragma unroll
   for (int j = 0; j < V; ++j) {
     float f, w;
-    gs_gate(a.sigmoid, to_f(g.v[j]), f, w);
+    if (a.sigmoid)
+      gs_gate<sizeof(T) == 4, true>(to_f(g.v[j]), f, w);
+    else
+      gs_gate<sizeof(T) == 4, false>(to_f(g.v[j]), f, w);
     const float v = to_f(x.v[j]);
     s.v[j] = __builtin_fmaf(f, s.v[j], a.mix ? w * v : v);
     y.v[j] = from_f<T>(s.v[j]);
@@ -476,23 +598,33 @@ static size_t gs_workspace(const lsh_gated* p) {
   return most;
 }
 
-// Calls f<T, V, MASK>(threads of a workgroup, workgroups), everything about the launch in *a.  False: too many.
-template <class F>
+// Whether a wave's lanes lie within 32-bit offsets of each other in each operand: it may reach over several batches.
+static bool gs_near(const GsArgs& a, int size, int V) {
+  const int64_t over = std::min<int64_t>(a.B - 1, 64 * V / a.D + 1);
+  for (int64_t sb : {a.x_sb, a.g_sb, a.d_sb})
+    if (sb < 0 || (over > 0 && sb > (((int64_t)1 << 32) / size - a.D) / over)) return false;
+  return a.D < ((int64_t)1 << 32) / size;
+}
+
+// Calls f(type, FAST, MASK, threads of a workgroup, channel groups), everything about the launch in *a.  False: too
+// many workgroups.  R: rows of a wave.
+template <int R, class F>
 static bool gs_launch(GsArgs& a, int dtype, F&& f) {
-  const bool two = gs_wide(a, lm_dtype_size(dtype), 2);
-  a.pieces = a.n / (two ? 2 : 1);
+  const int size = lm_dtype_size(dtype), V = size == 2 ? 2 : 1;
+  const bool fast = (V == 1 || gs_wide(a, size, V)) && gs_near(a, size, V);
+  a.pieces = a.n / (fast ? V : 1);
   const int64_t groups = (a.pieces + 63) / 64;
   a.len = gs_len(a.T, groups, &a.S);
   if (!lm_grid_ok(groups * a.S, kGsW * 64)) return false;
   a.groups = (int)groups;
   // of short sequences as many waves as there are rows for
-  const int W = a.T > kGsRows / 2 ? kGsW : a.T > kGsRows / 4 ? kGsW / 2 : a.T > kGsR ? kGsW / 4 : 1;
+  const int W = a.T > 4 * R ? 8 : a.T > 2 * R ? 4 : a.T > R ? 2 : 1;
   with_dtype(dtype, [&](auto t) {
     with_mask(a.starts != nullptr, [&](auto mask) {
-      if (two)
-        f(t, std::integral_constant<int, 2>{}, mask, W * 64, (unsigned)(groups * a.S));
+      if (fast)
+        f(t, std::true_type{}, mask, W * 64, (unsigned)groups);
       else
-        f(t, std::integral_constant<int, 1>{}, mask, W * 64, (unsigned)(groups * a.S));
+        f(t, std::false_type{}, mask, W * 64, (unsigned)groups);
     });
   });
   return true;
@@ -504,7 +636,7 @@ using namespace lsh;
 
 extern "C" int64_t lsh_gated_saved(const lsh_gated* p) {
   if (gs_check(p)) return 0;
-  return (p->T + kGsRows - 1) / kGsRows * p->B * p->D;
+  return (p->T + kGsSave - 1) / kGsSave * p->B * p->D;
 }
 
 extern "C" size_t lsh_gated_workspace(const lsh_gated* p) { return gs_check(p) ? 0 : gs_workspace(p); }
@@ -519,12 +651,11 @@ extern "C" int lsh_gated_fwd(const lsh_gated* p, void* h, float* h_end, float* s
   GsArgs a = gs_args(p);
   a.h = h, a.h_end = h_end, a.saved = saved, a.part = (float*)ws;
   hipStream_t st = (hipStream_t)stream;
-  if (!gs_launch(a, p->dtype, [&](auto t, auto v, auto mask, int threads, unsigned grid) {
+  if (!gs_launch<kGsR>(a, p->dtype, [&](auto t, auto fast, auto mask, int threads, unsigned groups) {
         using T = decltype(t);
-        constexpr int V = decltype(v)::value;
-        constexpr bool MASK = decltype(mask)::value;
-        if (a.S > 1) k_gated_sums<T, V, MASK, false><<<dim3(grid), kGsW * 64, 0, st>>>(a);
-        k_gated<T, V, MASK><<<dim3(grid), threads, 0, st>>>(a);
+        constexpr bool FAST = decltype(fast)::value, MASK = decltype(mask)::value;
+        if (a.S > 1) k_gated_sums<T, FAST, MASK, false><<<dim3(groups * (a.S - 1)), kGsSumW * 64, 0, st>>>(a);
+        k_gated<T, FAST, MASK><<<dim3(groups * a.S), threads, 0, st>>>(a);
       }))
     return LSH_ERR_SHAPE;
   LSH_CHECK_LAUNCH();
@@ -543,12 +674,11 @@ extern "C" int lsh_gated_bwd(const lsh_gated* p, const float* saved, const void*
   a.saved = (float*)saved, a.dh = dh, a.d_st = dh ? dh_st : 0, a.d_sb = dh ? dh_sb : 0, a.d_end = dh_end;
   a.dx = dx, a.dg = dgate, a.dh0 = dh0, a.part = (float*)ws;
   hipStream_t st = (hipStream_t)stream;
-  if (!gs_launch(a, p->dtype, [&](auto t, auto v, auto mask, int threads, unsigned grid) {
+  if (!gs_launch<kGsB>(a, p->dtype, [&](auto t, auto fast, auto mask, int threads, unsigned groups) {
         using T = decltype(t);
-        constexpr int V = decltype(v)::value;
-        constexpr bool MASK = decltype(mask)::value;
-        if (a.S > 1) k_gated_sums<T, V, MASK, true><<<dim3(grid), kGsW * 64, 0, st>>>(a);
-        k_gated_bwd<T, V, MASK><<<dim3(grid), threads, 0, st>>>(a);
+        constexpr bool FAST = decltype(fast)::value, MASK = decltype(mask)::value;
+        if (a.S > 1) k_gated_sums<T, FAST, MASK, true><<<dim3(groups * (a.S - 1)), kGsSumW * 64, 0, st>>>(a);
+        k_gated_bwd<T, FAST, MASK><<<dim3(groups * a.S), threads, 0, st>>>(a);
       }))
     return LSH_ERR_SHAPE;
   LSH_CHECK_LAUNCH();

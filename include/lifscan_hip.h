@@ -622,7 +622,7 @@ typedef struct lsh_gated {
   const float* h0;
 } lsh_gated;
 size_t lsh_gated_workspace(const lsh_gated* a); /* 0: ws may be NULL; the same for both directions */
-/* Floats that the gradients need of the forward (`saved`: the states before every 128 rows). */
+/* Floats that the gradients need of the forward (`saved`: the states before every 64 rows). */
 int64_t lsh_gated_saved(const lsh_gated* a);
 int lsh_gated_fwd(const lsh_gated* a, void* h, float* h_end, float* saved /* or NULL */, void* ws,
                   size_t ws_bytes, void* stream);

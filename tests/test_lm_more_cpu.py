@@ -29,7 +29,7 @@ def test_gated_checks():
     need = L.lsh_gated_workspace(_gated(T=4096))
     assert need > 0 and need % (2 * 2 * 8 * 4) == 0 and L.lsh_gated_workspace(_gated()) == 0
     assert fwd(T=4096) == WS and fwd(T=4096, ws=P, nb=need - 1) == WS
-    assert L.lsh_gated_saved(_gated(T=129)) == 2 * 16 and L.lsh_gated_saved(_gated(T=0)) == 0
+    assert L.lsh_gated_saved(_gated(T=129)) == 3 * 16 and L.lsh_gated_saved(_gated(T=0)) == 0
     bwd = lambda a, saved=P, dx=P, dg=P, ws=None, nb=0: L.lsh_gated_bwd(a, saved, P, 1, 1, None, dx, dg, None, ws, nb, None)  # noqa: E731
     assert bwd(_gated(), saved=None) == ARG and bwd(_gated(), dx=None) == ARG and bwd(_gated(), dg=None) == ARG
     assert bwd(_gated(T=4096)) == WS and bwd(_gated(B=0)) == 0 and bwd(_gated(dtype=7)) == ARG
