@@ -9,10 +9,11 @@
 // c = log2(e)/tau; then l = log2(s), log p = ln2*(d - l) and H = ln2*(l - t/s).  A logit of -inf has p = 0, and a row of
 // nothing else has log p = -inf, H = 0 and no gradient.  A row with NaN or +inf has NaN.
 //
-// The K largest: each thread knows the largest of the logits that it read.  The K-th largest of those is a bound that
-// K logits reach, so only the K threads whose largest reaches it can hold one of the row's K: they read their share again
-// (from the caches), and a handful more than K values come out, which are ranked by counting.  Values and ids are one
-// whole number of 64 bits, no two alike, so the order in which they are found does not matter.
+// The K largest: each thread knows the largest of the logits that it read, and of its block of 4 pieces where that
+// stands.  The K-th largest of those 256 is a bound that K logits reach, so only the few threads whose largest reaches it
+// can hold one of the row's K: they read that block once more (others of theirs only if one of those reaches it too),
+// and a handful more than K values come out, which are ranked by counting.  Values and ids are one whole number of 64
+// bits, no two alike, so the order in which they are found does not matter.
 #include <algorithm>
 #include <type_traits>
 
@@ -42,16 +43,18 @@ struct ScArgs {
   float c, tau;
 };
 
-// A value and its id as a number: larger values first, then lower ids; NaN before all values; never 0.
-using Key = unsigned long long;
-__device__ __forceinline__ Key sc_key(float x, unsigned id) {
-  unsigned b = __builtin_bit_cast(unsigned, x + 0.0f);  // one zero
+// A value as a whole number in the same order, never 0; NaN before all, and one zero.
+__device__ __forceinline__ unsigned sc_order(float x) {
+  unsigned b = __builtin_bit_cast(unsigned, x + 0.0f);
   if (x != x) b = 0x7fc00000u;
-  b = b & 0x80000000u ? ~b : b | 0x80000000u;
-  return (Key)b << 32 | (0xffffffffu - id);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
+// A value and its id as a number: larger values first, then lower ids.
+using Key = unsigned long long;
+__device__ __forceinline__ Key sc_key(float x, unsigned id) { return (Key)sc_order(x) << 32 | (0xffffffffu - id); }
+__device__ __forceinline__ unsigned sc_order(Key k) { return (unsigned)(k >> 32); }
 __device__ __forceinline__ float sc_value(Key k) {
-  const unsigned b = (unsigned)(k >> 32);
+  const unsigned b = sc_order(k);
   return __builtin_bit_cast(float, b & 0x80000000u ? b & 0x7fffffffu : ~b);
 }
 __device__ __forceinline__ unsigned sc_id(Key k) { return 0xffffffffu - (unsigned)k; }
@@ -76,56 +79,86 @@ __device__ __forceinline__ ScPiece<T> sc_load(const T* p) {
   return x;
 }
 
-// The K largest of keys that the threads of a workgroup hold between them, in order, to out (0: none).  own: a thread's
-// largest (0: it has none).  scan(bound, f) calls f with each key of the thread that reaches bound.
-// One call a kernel: its LDS is not shared.
+// The K largest of keys that the threads of a workgroup hold between them, in order, to out (0: none).  own: the value of
+// a thread's largest, as sc_order (0: it has none).  scan(bound, f) calls f with each key of the thread whose value
+// reaches bound.  One call a kernel: its LDS is not shared.
 template <class Scan, class Out>
-__device__ __forceinline__ void sc_select(Key own, int K, Scan&& scan, Out&& out) {
-  __shared__ Key s_own[kScThreads], s_list[kScList], s_bound;
+__device__ __forceinline__ void sc_select(unsigned own, int K, Scan&& scan, Out&& out) {
+  __shared__ unsigned s_value[kScThreads], s_bound;
+  __shared__ Key s_list[kScList], s_key;
   __shared__ int s_count;
+  static_assert(kScList >= kScThreads, "the list holds a key of each thread");
   const int tid = threadIdx.x;
-  s_own[tid] = own;
-  if (tid == 0) s_bound = 0, s_count = 0;
+  s_value[tid] = own;
   __syncthreads();
-  int above = 0;
-#pragma unroll 8
-  for (int i = 0; i < kScThreads; ++i) above += s_own[i] > own;
-  if (above == K - 1 && own) s_bound = own;
+  if (tid < 64) {  // the K-th largest, bit by bit
+    unsigned v[kScThreads / 64], bound = 0;
+#pragma unroll
+    for (int i = 0; i < kScThreads / 64; ++i) v[i] = s_value[tid + 64 * i];
+    for (unsigned bit = 0x80000000u; bit; bit >>= 1) {
+      const unsigned t = bound | bit;
+      int reach = 0;
+#pragma unroll
+      for (int i = 0; i < kScThreads / 64; ++i) reach += __popcll(__ballot(v[i] >= t));
+      if (reach >= K) bound = t;
+      if (reach == K) break;
+    }
+    if (tid == 0) s_bound = bound, s_key = 0, s_count = 0;
+  }
   __syncthreads();
-  const Key bound = s_bound;
-  if (own && own >= bound)
-    scan(bound, [&](Key k) {
-      const int at = atomicAdd(&s_count, 1);
-      if (at < kScList) s_list[at] = k;
-    });
-  __syncthreads();
-  const int n = s_count;
+  const unsigned bound = s_bound;
+  const bool mine = own && own >= bound;
+  auto collect = [&](Key least) {
+    if (mine)
+      scan(bound, [&](Key k) {
+        if (k < least) return;
+        const int at = atomicAdd(&s_count, 1);
+        if (at < kScList) s_list[at] = k;
+      });
+    __syncthreads();
+    return s_count;
+  };
+  int n = collect(0);
+  if (n > kScList) {
+    // long runs of equal values, as where most of a row is masked: the K-th largest of the threads' keys
+    Key best = 0;
+    if (mine) scan(bound, [&](Key k) { best = max(best, k); });
+    __syncthreads();
+    s_list[tid] = best;
+    if (tid == 0) s_count = 0;
+    __syncthreads();
+    int above = 0;
+    for (int i = 0; i < kScThreads; ++i) above += s_list[i] > best;
+    if (above == K - 1 && best) s_key = best;
+    __syncthreads();
+    n = collect(s_key);
+  }
   if (n <= kScList) {
     for (int i = tid; i < n; i += kScThreads) {
-      const Key mine = s_list[i];
+      const Key k = s_list[i];
       int rank = 0;
-      for (int j = 0; j < n; ++j) rank += s_list[j] > mine;
-      if (rank < K) out(rank, mine);
+      for (int j = 0; j < n; ++j) rank += s_list[j] > k;
+      if (rank < K) out(rank, k);
     }
     for (int i = n + tid; i < K; i += kScThreads) out(i, (Key)0);
     return;
   }
-  // more than the list holds reach the bound (long runs of large values that a few threads share): one after the other
+  // a few threads hold more than the list: one after the other
   Key last = ~(Key)0;
   for (int k = 0; k < K; ++k) {
     Key best = 0;
-    if (own && own >= bound)
+    if (mine)
       scan(bound, [&](Key x) {
-        if (x < last && x > best) best = x;
+        if (x < last) best = max(best, x);
       });
-    __syncthreads();  // s_own was read
-    s_own[tid] = best;
+    __syncthreads();  // the list was read
+    s_list[tid] = best;
     __syncthreads();
     for (int o = kScThreads / 2; o > 0; o >>= 1) {
-      if (tid < o && s_own[tid + o] > s_own[tid]) s_own[tid] = s_own[tid + o];
+      if (tid < o) s_list[tid] = max(s_list[tid], s_list[tid + o]);
       __syncthreads();
     }
-    last = s_own[0];
+    last = s_list[0];
     if (tid == 0) out(k, last);
   }
 }
@@ -157,17 +190,22 @@ __global__ __launch_bounds__(kScThreads) void k_score(ScArgs a) {
   const T* z = (const T*)a.z + row * a.stride + v0;
   const int n = (int)max((int64_t)0, min(a.len, a.V - v0));
   const int tid = threadIdx.x;
-  // element j of piece u of a thread in block b: ((b*U + u)*kScThreads + tid)*P + j
+  // the first element of piece u of a thread in block b
   auto place = [&](int b, int u) { return b * STEP + (u * kScThreads + tid) * P; };
   float m = -INFINITY, s = 0.0f, t = 0.0f;
-  int best = 0;  // the block of the largest
+  int best = 0;             // the block of the largest
+  float other = -INFINITY;  // the largest of the other blocks
   auto take = [&](const float (&f)[U][P], int b) {
-    float top = m;
+    float top = f[0][0];
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int j = 0; j < P; ++j) top = fmaxf(top, f[u][j]);
-    if (TOP && top > m) best = b;
+    if (TOP) {
+      other = fmaxf(other, fminf(m, top));
+      best = top > m ? b : best;
+    }
+    top = fmaxf(m, top);
     const float at = top > -INFINITY ? top : 0.0f;
     const float d0 = fmaxf((m - at) * a.c, -1000.0f), e0 = __builtin_amdgcn_exp2f(d0);
     t = e0 * __builtin_fmaf(d0, s, t);
@@ -183,41 +221,49 @@ __global__ __launch_bounds__(kScThreads) void k_score(ScArgs a) {
     m = top;
   };
   const int whole = n / STEP;
-  for (int b = 0; b < whole; ++b) {
+  // a block that is whole; f(place of the first element of a piece, its values)
+  auto read = [&](int b, float (&f)[U][P]) {
     ScPiece<T> y[U];
-    float f[U][P];
 #pragma unroll
     for (int u = 0; u < U; ++u) y[u] = sc_load(z + place(b, u));
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int j = 0; j < P; ++j) f[u][j] = to_f(y[u].v[j]);
-    take(f, b);
-  }
-  // what is left of a block, the pieces that are whole and the one that is not
-  auto rest = [&](int b, float (&f)[U][P]) {
+  };
+  // what is left behind the whole blocks, -inf where nothing is.  A piece that reaches over the end is read from P before
+  // the end on (from[u]), without branches around the loads; what another thread reads too is left out.
+  auto read_rest = [&](int b, float (&f)[U][P], int (&from)[U]) {
+    if (n >= P) {
+      ScPiece<T> y[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int e = place(b, u);
+      for (int u = 0; u < U; ++u) from[u] = min(place(b, u), n - P), y[u] = sc_load(z + from[u]);
 #pragma unroll
-      for (int j = 0; j < P; ++j) f[u][j] = -INFINITY;
-      if (e + P <= n) {
-        const ScPiece<T> y = sc_load(z + e);
+      for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int j = 0; j < P; ++j) f[u][j] = to_f(y.v[j]);
-      } else {
+        for (int j = 0; j < P; ++j) f[u][j] = from[u] + j >= place(b, u) ? to_f(y[u].v[j]) : -INFINITY;
+    } else {
 #pragma unroll
-        for (int j = 0; j < P; ++j)
-          if (e + j < n) f[u][j] = to_f(z[e + j]);
+      for (int u = 0; u < U; ++u) {
+        from[u] = place(b, u);
+#pragma unroll
+        for (int j = 0; j < P; ++j) f[u][j] = from[u] + j < n ? to_f(z[from[u] + j]) : -INFINITY;
       }
     }
   };
+  for (int b = 0; b < whole; ++b) {
+    float f[U][P];
+    read(b, f);
+    take(f, b);
+  }
   if (place(whole, 0) < n) {
     float f[U][P];
-    rest(whole, f);
+    int from[U];
+    read_rest(whole, f, from);
     take(f, whole);
   }
   const bool odd = s != s;  // a NaN, or +inf
+  const float mine = m;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1)
     sc_join(m, s, t, __shfl_xor(m, o, 64), __shfl_xor(s, o, 64), __shfl_xor(t, o, 64), a.c);
@@ -235,31 +281,39 @@ __global__ __launch_bounds__(kScThreads) void k_score(ScArgs a) {
     }
   }
   if constexpr (TOP) {
-    // the thread's keys of a block that reach a bound
-    auto block = [&](int b, Key bound, auto&& f) {
+    const int blocks = place(whole, 0) < n ? whole + 1 : whole;
+    // the thread's keys of a block whose values reach a bound
+    auto block = [&](int b, unsigned bound, auto&& f) {
       float x[U][P];
-      rest(b, x);
+      int from[U];
+      if (b < whole) {
+        read(b, x);
+#pragma unroll
+        for (int u = 0; u < U; ++u) from[u] = place(b, u);
+      } else {
+        read_rest(b, x, from);
+      }
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int j = 0; j < P; ++j) {
-          const int e = place(b, u) + j;
-          const Key k = sc_key(x[u][j], (unsigned)(v0 + e));
-          if (e < n && k >= bound) f(k);
+          const int e = from[u] + j;
+          if (sc_order(x[u][j]) >= bound && e >= place(b, u) && e < n) f(sc_key(x[u][j], (unsigned)(v0 + e)));
         }
     };
-    const int blocks = place(whole, 0) < n ? whole + 1 : whole;
-    Key own = 0;
-    auto largest = [&](Key k) { own = k > own ? k : own; };
-    if (odd)
-      for (int b = 0; b < blocks; ++b) block(b, 0, largest);
-    else if (blocks)
-      block(best, 0, largest);
+    unsigned own = blocks ? sc_order(mine) : 0;
+    if (odd) {  // the maximum leaves NaN out
+      own = 0;
+      for (int b = 0; b < blocks; ++b) block(b, 0, [&](Key k) { own = max(own, sc_order(k)); });
+    }
     const float l = __builtin_amdgcn_logf(s);
     sc_select(
         own, a.K,
-        [&](Key bound, auto&& f) {
-          for (int b = 0; b < blocks; ++b) block(b, bound, f);
+        [&](unsigned bound, auto&& f) {
+          if (odd || sc_order(other) >= bound)
+            for (int b = 0; b < blocks; ++b) block(b, bound, f);
+          else
+            block(best, bound, f);
         },
         [&](int k, Key key) {
           if (SPLIT)
@@ -284,14 +338,14 @@ __global__ __launch_bounds__(kScThreads) void k_score_join(ScArgs a) {
   if constexpr (TOP) {
     const Key* keys = a.keys + row * a.splits * a.K;
     const int n = a.splits * a.K;
-    Key own = 0;
-    for (int k = tid; k < n; k += kScThreads) own = max(own, keys[k]);
+    unsigned own = 0;
+    for (int k = tid; k < n; k += kScThreads) own = max(own, sc_order(keys[k]));
     const float l = __builtin_amdgcn_logf(s);
     sc_select(
         own, a.K,
-        [&](Key bound, auto&& f) {
+        [&](unsigned bound, auto&& f) {
           for (int k = tid; k < n; k += kScThreads)
-            if (const Key x = keys[k]; x && x >= bound) f(x);
+            if (const Key x = keys[k]; x && sc_order(x) >= bound) f(x);
         },
         [&](int k, Key key) { sc_put(a, row, k, key, m, l); });
   }
