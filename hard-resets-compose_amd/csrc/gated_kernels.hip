@@ -8,7 +8,7 @@
 //   dx_t = w_t*E_t,  dgate_t = E_t*(h_{t-1} - [w = 1 - a]*x_t)*da/dgate
 //
 // A step is an affine map, and so is a run of steps: (P, H) with h_end = P*h_begin + H, and backwards (P, Q) with
-// F_begin = P*F_end + Q and the same P.  A lane has V neighbouring channels, a wave kGsR rows of them in registers,
+// F_begin = P*F_end + Q and the same P.  A lane has V neighbouring channels, a wave 8 or 16 rows of them in registers,
 // and a workgroup's waves hold consecutive rows: the waves' maps meet in LDS, each wave composes those before its own,
 // and then writes its rows from the state before them.  Where there are too few channels for the chip the rows are cut
 // into segments, whose maps an extra pass over the operands forms.  The gradients take h_{t-1} from the state before
@@ -23,8 +23,12 @@
 
 namespace lsh {
 
-// Rows of a wave forwards and backwards, waves of a workgroup, rows of a forward round, and rows between saved states.
-constexpr int kGsR = 16, kGsB = 8, kGsW = 8, kGsRows = kGsR * kGsW, kGsSave = kGsB * kGsW;
+// Waves of a workgroup, what the rows of a segment are a multiple of, and the rows between saved states.
+constexpr int kGsW = 8, kGsRows = 128, kGsSave = 64;
+// Rows that a wave holds: forwards, backwards, and for a segment's map with so many bytes a lane and row
+constexpr int kGsFwd = 16, kGsBwd = 8;
+template <int BYTES>
+constexpr int kGsSum = BYTES == 8 ? 8 : 16;
 
 struct GsArgs {
   const void *x, *g;
@@ -90,17 +94,19 @@ __device__ __forceinline__ float gs_product(float first, float then) {
   return MASK && gs_marked(then) ? then : MASK && gs_marked(first) ? first : first * then;
 }
 
-// FAST: 4 bytes a lane and row (two channels of 16 bits), and a row's lanes within 4 GB of each other, so that an address
-// is a scalar and an offset.  Otherwise a channel a lane, wherever it lies.
-template <class T, bool FAST>
-constexpr int kGsV = FAST && sizeof(T) == 2 ? 2 : 1;
-template <bool FAST>
-using GsOff = std::conditional_t<FAST, uint32_t, uint64_t>;
+// Bytes of a lane in a row: 8, 4, or one element of either size.  The first two have a row's lanes within 4 GB of each
+// other, so that an address is a scalar and an offset; the last reads a channel wherever it lies.  Wider is faster for
+// the maps (4096 x 4 x 2048 bf16: 36 us with 8 bytes, 41 with 4, 54 with 2), but the passes themselves have not the
+// registers for 8 (forward 61 us with 8 rows a wave of 8 bytes, 41 with 16 rows of 4, 55 with 2 bytes).
+template <class T, int BYTES>
+constexpr int kGsV = BYTES > (int)sizeof(T) ? BYTES / (int)sizeof(T) : 1;
+template <int BYTES>
+using GsOff = std::conditional_t<BYTES != 0, uint32_t, uint64_t>;
 
 // A lane's channels.  A lane beyond the last channel does the last ones once more, to the same values.
-template <class T, bool FAST>
+template <class T, int BYTES>
 struct GsLane {
-  static constexpr int V = kGsV<T, FAST>;
+  static constexpr int V = kGsV<T, BYTES>;
   int64_t c0, c, b0, b, d;  // the first channel of the wave and of the lane, their batches, the lane's column
   __device__ __forceinline__ GsLane(const GsArgs& a, int group) {
     const int64_t p0 = (int64_t)group * 64, p = min(p0 + (threadIdx.x & 63), a.pieces - 1);
@@ -111,46 +117,47 @@ struct GsLane {
 
 // A lane's V values of a row as they lie in memory: two of 16 bits stay in one register.
 template <class T, int V>
-struct GsRaw {
-  std::conditional_t<V * sizeof(T) == 4, uint32_t, uint16_t> x;
+struct alignas(V * sizeof(T)) GsRaw {
+  using Word = std::conditional_t<V * sizeof(T) >= 4, uint32_t, uint16_t>;
+  static constexpr int N = V * sizeof(T) / sizeof(Word), PER = sizeof(Word) / sizeof(T);
+  Word x[N];
   __device__ __forceinline__ float get(int j) const {
-    if constexpr (sizeof(T) == 4)
-      return __builtin_bit_cast(float, x);
-    else if constexpr (V == 1)
-      return to_f(__builtin_bit_cast(T, x));
+    const Word w = x[j / PER];
+    if constexpr (PER == 1)
+      return to_f(__builtin_bit_cast(T, w));
     else if constexpr (std::is_same_v<T, bf16_t>)
-      return __builtin_bit_cast(float, j ? x & 0xffff0000u : x << 16);
+      return __builtin_bit_cast(float, j % 2 ? w & 0xffff0000u : w << 16);
     else
-      return to_f(__builtin_bit_cast(T, (uint16_t)(x >> 16 * j)));
+      return to_f(__builtin_bit_cast(T, (uint16_t)(w >> 16 * (j % 2))));
   }
   __device__ __forceinline__ void set(const float (&f)[V]) {
     Vec<T, V> y;
 #pragma unroll
     for (int j = 0; j < V; ++j) y.v[j] = from_f<T>(f[j]);
-    x = __builtin_bit_cast(decltype(x), y);
+    __builtin_memcpy(x, &y, sizeof(y));
   }
 };
 
 // One operand as a lane reads it, row by row
-template <class T, bool FAST>
+template <class T, int BYTES>
 struct GsIn {
-  static constexpr int V = kGsV<T, FAST>;
+  static constexpr int V = kGsV<T, BYTES>;
   const T* base;
   int64_t stride;
-  GsOff<FAST> off;
-  __device__ __forceinline__ GsIn(const void* p, int64_t st, int64_t sb, const GsLane<T, FAST>& at)
-      : base((const T*)p + at.b0 * sb), stride(st), off((GsOff<FAST>)(((at.b - at.b0) * sb + at.d) * sizeof(T))) {}
+  GsOff<BYTES> off;
+  __device__ __forceinline__ GsIn(const void* p, int64_t st, int64_t sb, const GsLane<T, BYTES>& at)
+      : base((const T*)p + at.b0 * sb), stride(st), off((GsOff<BYTES>)(((at.b - at.b0) * sb + at.d) * sizeof(T))) {}
   __device__ __forceinline__ GsRaw<T, V> row(int64_t t) const {
     return *(const GsRaw<T, V>*)((const char*)(base + t * stride) + off);
   }
 };
-template <class T, bool FAST>
+template <class T, int BYTES>
 struct GsOut {
-  static constexpr int V = kGsV<T, FAST>;
+  static constexpr int V = kGsV<T, BYTES>;
   T* base;
   int64_t n;
   uint32_t off;
-  __device__ __forceinline__ GsOut(void* p, int64_t n, const GsLane<T, FAST>& at)
+  __device__ __forceinline__ GsOut(void* p, int64_t n, const GsLane<T, BYTES>& at)
       : base((T*)p + at.c0), n(n), off((uint32_t)((at.c - at.c0) * sizeof(T))) {}
   __device__ __forceinline__ void put(int64_t t, const float (&f)[V]) const {
     GsRaw<T, V> x;
@@ -160,10 +167,10 @@ struct GsOut {
 };
 
 // R rows of a lane as read; rows from `end` on are read from the one before it
-template <class T, bool FAST, int R>
+template <class T, int BYTES, int R>
 struct GsRows {
-  GsRaw<T, kGsV<T, FAST>> v[R];
-  __device__ __forceinline__ void load(const GsIn<T, FAST>& in, int64_t t, int64_t end) {
+  GsRaw<T, kGsV<T, BYTES>> v[R];
+  __device__ __forceinline__ void load(const GsIn<T, BYTES>& in, int64_t t, int64_t end) {
     if (t + R <= end) {
 #pragma unroll
       for (int i = 0; i < R; ++i) v[i] = in.row(t + i);
@@ -210,35 +217,36 @@ __device__ __forceinline__ void gs_form(const GsArgs& a, F&& f) {
 // Where segments are needed: the map of each but the last, forwards (x, gate), or of each but the first, backwards
 // (gate, dh).  A wave takes its share of the segment's rows, its map in registers; backwards the map is summed with
 // the product of the decays so far, from the first row on.
-constexpr int kGsSumW = 4;
-template <class T, bool FAST, bool MASK, bool BWD>
-__global__ __launch_bounds__(kGsSumW * 64, 4) void k_gated_sums(GsArgs a) {
-  constexpr int V = kGsV<T, FAST>;
-  __shared__ float s_map[kGsSumW][2][64 * V];
+template <int BYTES>
+constexpr int kGsSumW = BYTES == 8 ? 8 : 4;
+template <class T, int BYTES, bool MASK, bool BWD>
+__global__ __launch_bounds__(kGsSumW<BYTES> * 64, 4) void k_gated_sums(GsArgs a) {
+  constexpr int V = kGsV<T, BYTES>, R = kGsSum<BYTES>;
+  __shared__ float s_map[kGsSumW<BYTES>][2][64 * V];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int group = blockIdx.x % a.groups, seg = blockIdx.x / a.groups + (BWD ? 1 : 0);
-  const GsLane<T, FAST> at(a, group);
-  const GsIn<T, FAST> x = BWD ? GsIn<T, FAST>(a.dh, a.d_st, a.d_sb, at) : GsIn<T, FAST>(a.x, a.x_st, a.x_sb, at);
-  const GsIn<T, FAST> g(a.g, a.g_st, a.g_sb, at);
+  const GsLane<T, BYTES> at(a, group);
+  const GsIn<T, BYTES> x = BWD ? GsIn<T, BYTES>(a.dh, a.d_st, a.d_sb, at) : GsIn<T, BYTES>(a.x, a.x_st, a.x_sb, at);
+  const GsIn<T, BYTES> g(a.g, a.g_st, a.g_sb, at);
   const int64_t t1 = min(a.T, (seg + 1) * a.len);
-  const int64_t per = a.len / kGsSumW, lo = seg * a.len + wave * per, hi = min(t1, lo + per);
+  const int64_t per = a.len / kGsSumW<BYTES>, lo = seg * a.len + wave * per, hi = min(t1, lo + per);
   float P[V], H[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) P[j] = 1.0f, H[j] = 0.0f;
   const bool zeros = BWD && !a.dh;
-  GsRows<T, FAST, kGsR> nx, ng;
+  GsRows<T, BYTES, R> nx, ng;
   auto load = [&](int64_t t) {
     if (!zeros) nx.load(x, t, hi);
     ng.load(g, t, hi);
   };
   if (lo < hi) load(lo);
-  for (int64_t t = lo; t < hi; t += kGsR) {
-    const GsRows<T, FAST, kGsR> rx = nx, rg = ng;
-    const unsigned starts = gs_starts<MASK, kGsR>(a, at.b, t, hi);
-    if (t + kGsR < hi) load(t + kGsR);
+  for (int64_t t = lo; t < hi; t += R) {
+    const GsRows<T, BYTES, R> rx = nx, rg = ng;
+    const unsigned starts = gs_starts<MASK, R>(a, at.b, t, hi);
+    if (t + R < hi) load(t + R);
     gs_form(a, [&](auto sig, auto mix) {
 #pragma unroll
-      for (int i = 0; i < kGsR; ++i) {
+      for (int i = 0; i < R; ++i) {
         if (t + i >= hi) break;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
@@ -262,8 +270,8 @@ __global__ __launch_bounds__(kGsSumW * 64, 4) void k_gated_sums(GsArgs a) {
 #pragma unroll
   for (int j = 0; j < V; ++j) P[j] = 1.0f, H[j] = 0.0f;
 #pragma unroll
-  for (int n = 0; n < kGsSumW; ++n) {
-    const int w = BWD ? kGsSumW - 1 - n : n;
+  for (int n = 0; n < kGsSumW<BYTES>; ++n) {
+    const int w = BWD ? kGsSumW<BYTES> - 1 - n : n;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       const float p = s_map[w][0][lane * V + j];
@@ -311,18 +319,18 @@ __device__ __forceinline__ void gs_enter(const GsArgs& a, int seg, int64_t c, co
 
 // One barrier a round: what a wave writes for the next round goes to the other half of the LDS.  The state after a
 // round is what its last wave ends with.
-template <class T, bool FAST, bool MASK>
+template <class T, int BYTES, bool MASK>
 __global__ __launch_bounds__(kGsW * 64, 4) void k_gated(GsArgs a) {
-  constexpr int V = kGsV<T, FAST>;
+  constexpr int V = kGsV<T, BYTES>, R = kGsFwd;
   __shared__ float s_map[2][kGsW][2][64 * V], s_carry[2][64 * V];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), W = blockDim.x >> 6;
   const int group = blockIdx.x % a.groups, seg = blockIdx.x / a.groups;
-  const GsLane<T, FAST> at(a, group);
-  const GsIn<T, FAST> x(a.x, a.x_st, a.x_sb, at), g(a.g, a.g_st, a.g_sb, at);
-  const GsOut<T, FAST> out(a.h, a.n, at);
+  const GsLane<T, BYTES> at(a, group);
+  const GsIn<T, BYTES> x(a.x, a.x_st, a.x_sb, at), g(a.g, a.g_st, a.g_sb, at);
+  const GsOut<T, BYTES> out(a.h, a.n, at);
   const int64_t t0 = seg * a.len, t1 = min(a.T, t0 + a.len);
-  GsRows<T, FAST, kGsR> rx, rg;
-  int64_t t = t0 + wave * kGsR;
+  GsRows<T, BYTES, R> rx, rg;
+  int64_t t = t0 + wave * R;
   auto load = [&](int64_t t) { rx.load(x, t, t1), rg.load(g, t, t1); };
   if (t < t1) load(t);
   float h[V];  // before the round, then before the wave's rows
@@ -331,12 +339,12 @@ __global__ __launch_bounds__(kGsW * 64, 4) void k_gated(GsArgs a) {
 #pragma unroll
     for (int j = 0; j < V; ++j) s_carry[0][lane * V + j] = h[j];
   int buf = 0;
-  for (int64_t r = t0; r < t1; r += W * kGsR, t += W * kGsR, buf ^= 1) {
-    float f[kGsR][V], b[kGsR][V], P[V], H[V];
-    const unsigned starts = gs_starts<MASK, kGsR>(a, at.b, t, t1);
+  for (int64_t r = t0; r < t1; r += W * R, t += W * R, buf ^= 1) {
+    float f[R][V], b[R][V], P[V], H[V];
+    const unsigned starts = gs_starts<MASK, R>(a, at.b, t, t1);
     gs_form(a, [&](auto sig, auto mix) {
 #pragma unroll
-      for (int i = 0; i < kGsR; ++i)
+      for (int i = 0; i < R; ++i)
 #pragma unroll
         for (int j = 0; j < V; ++j) {
           float w;
@@ -345,21 +353,21 @@ __global__ __launch_bounds__(kGsW * 64, 4) void k_gated(GsArgs a) {
         }
     });
 #pragma unroll
-    for (int i = 0; i < kGsR; ++i)
+    for (int i = 0; i < R; ++i)
 #pragma unroll
       for (int j = 0; j < V; ++j)
         if (MASK && gs_bit(starts, i)) f[i][j] = __builtin_bit_cast(float, kGsStart);
-    if (t + kGsR > t1)
+    if (t + R > t1)
 #pragma unroll
-      for (int i = 0; i < kGsR; ++i)
+      for (int i = 0; i < R; ++i)
         if (t + i >= t1)
 #pragma unroll
           for (int j = 0; j < V; ++j) f[i][j] = 1.0f, b[i][j] = 0.0f;
-    if (const int64_t next = t + W * kGsR; next < t1) load(next);
+    if (const int64_t next = t + W * R; next < t1) load(next);
 #pragma unroll
     for (int j = 0; j < V; ++j) P[j] = 1.0f, H[j] = 0.0f;
 #pragma unroll
-    for (int i = 0; i < kGsR; ++i)
+    for (int i = 0; i < R; ++i)
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         H[j] = gs_apply<MASK>(f[i][j], b[i][j], H[j]);
@@ -378,7 +386,7 @@ __global__ __launch_bounds__(kGsW * 64, 4) void k_gated(GsArgs a) {
 #pragma unroll
       for (int j = 0; j < V; ++j) a.saved[t / kGsSave * a.n + at.c + j] = h[j];
 #pragma unroll
-    for (int i = 0; i < kGsR; ++i) {
+    for (int i = 0; i < R; ++i) {
 #pragma unroll
       for (int j = 0; j < V; ++j) h[j] = gs_apply<MASK>(f[i][j], b[i][j], h[j]);
       if (t + i < t1) out.put(t + i, h);
@@ -395,16 +403,16 @@ __global__ __launch_bounds__(kGsW * 64, 4) void k_gated(GsArgs a) {
 // The gradients, the rounds from the last.  A first sweep over the rows in registers forms the wave's maps of both
 // directions, a second one forwards the states and what multiplies the adjoint, a third one backwards the adjoint: the
 // gates' powers are formed twice, which is cheaper than keeping them (two workgroups a CU need 128 registers).
-template <class T, bool FAST, bool MASK>
+template <class T, int BYTES, bool MASK>
 __global__ __launch_bounds__(kGsW * 64, 4) void k_gated_bwd(GsArgs a) {
-  constexpr int V = kGsV<T, FAST>;
+  constexpr int V = kGsV<T, BYTES>, R = kGsBwd;
   __shared__ float s_map[2][kGsW][3][64 * V], s_carry[2][64 * V];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), W = blockDim.x >> 6;
   const int group = blockIdx.x % a.groups, seg = blockIdx.x / a.groups;
-  const GsLane<T, FAST> at(a, group);
-  const GsIn<T, FAST> x(a.x, a.x_st, a.x_sb, at), g(a.g, a.g_st, a.g_sb, at), d(a.dh, a.d_st, a.d_sb, at);
-  const GsOut<T, FAST> dx(a.dx, a.n, at), dg(a.dg, a.n, at);
-  const int64_t t0 = seg * a.len, t1 = min(a.T, t0 + a.len), rows = W * kGsB;
+  const GsLane<T, BYTES> at(a, group);
+  const GsIn<T, BYTES> x(a.x, a.x_st, a.x_sb, at), g(a.g, a.g_st, a.g_sb, at), d(a.dh, a.d_st, a.d_sb, at);
+  const GsOut<T, BYTES> dx(a.dx, a.n, at), dg(a.dg, a.n, at);
+  const int64_t t0 = seg * a.len, t1 = min(a.T, t0 + a.len), rows = W * R;
   float F[V];  // behind the round, then behind the wave's rows
   gs_enter<V, MASK, true>(a, seg, at.c, a.d_end, F, (float(*)[2][64 * V])s_map[0]);
   if (wave == 0)
@@ -412,28 +420,30 @@ __global__ __launch_bounds__(kGsW * 64, 4) void k_gated_bwd(GsArgs a) {
     for (int j = 0; j < V; ++j) s_carry[0][lane * V + j] = F[j];
   int buf = 0;
   for (int64_t r = t0 + (t1 - t0 - 1) / rows * rows; r >= t0 && t1 > t0; r -= rows, buf ^= 1) {
-    const int64_t t = r + wave * kGsB;
-    GsRows<T, FAST, kGsB> rx, rg, rd;
+    const int64_t t = r + wave * R;
+    GsRows<T, BYTES, R> rx, rg, rd;
     if (t < t1) {
       rx.load(x, t, t1), rg.load(g, t, t1);
       if (a.dh) rd.load(d, t, t1);
     }
-    const unsigned starts = gs_starts<MASK, kGsB>(a, at.b, t, t1);
+    const unsigned starts = gs_starts<MASK, R>(a, at.b, t, t1);
     float h[V];  // before the round, then before the wave's rows
 #pragma unroll
     for (int j = 0; j < V; ++j) h[j] = a.saved[r / kGsSave * a.n + at.c + j];
     // rows that are not there: a decay of 1, an input and a gradient of 0
-    const bool tail = t + kGsB > t1;
+    const bool tail = t + R > t1;
     if (tail || !a.dh)
 #pragma unroll
-      for (int i = 0; i < kGsB; ++i)
-        if (t + i >= t1 || !a.dh) rd.v[i].x = 0;
+      for (int i = 0; i < R; ++i)
+        if (t + i >= t1 || !a.dh)
+#pragma unroll
+          for (auto& word : rd.v[i].x) word = 0;
     float P[V], H[V], Q[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) P[j] = 1.0f, H[j] = Q[j] = 0.0f;
     gs_form(a, [&](auto sig, auto mix) {
 #pragma unroll
-      for (int i = 0; i < kGsB; ++i) {
+      for (int i = 0; i < R; ++i) {
         if (tail && t + i >= t1) break;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
@@ -465,13 +475,15 @@ __global__ __launch_bounds__(kGsW * 64, 4) void k_gated_bwd(GsArgs a) {
         F[j] = gs_apply<MASK>(s_map[buf][w][0][lane * V + j], s_map[buf][w][2][lane * V + j], F[j]);
     // the first sweep's values are not to be kept for the second
 #pragma unroll
-    for (int i = 0; i < kGsB; ++i) asm volatile("" : "+v"(rg.v[i].x), "+v"(rx.v[i].x));
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+      for (int k = 0; k < GsRaw<T, V>::N; ++k) asm volatile("" : "+v"(rg.v[i].x[k]), "+v"(rx.v[i].x[k]));
     // dx = w*E, dgate = u*E, F = f*E
-    float f[kGsB][V], w[kGsB][V], u[kGsB][V];
+    float f[R][V], w[R][V], u[R][V];
     gs_form(a, [&](auto sig, auto mix) {
       constexpr bool SIG = decltype(sig)::value, MIX = decltype(mix)::value;
 #pragma unroll
-      for (int i = 0; i < kGsB; ++i)
+      for (int i = 0; i < R; ++i)
 #pragma unroll
         for (int j = 0; j < V; ++j) {
           const float gate = rg.get(i, j), v = rx.get(i, j);
@@ -488,12 +500,12 @@ __global__ __launch_bounds__(kGsW * 64, 4) void k_gated_bwd(GsArgs a) {
     });
     if (tail)
 #pragma unroll
-      for (int i = 0; i < kGsB; ++i)
+      for (int i = 0; i < R; ++i)
         if (t + i >= t1)
 #pragma unroll
           for (int j = 0; j < V; ++j) f[i][j] = 1.0f;
 #pragma unroll
-    for (int i = kGsB - 1; i >= 0; --i) {
+    for (int i = R - 1; i >= 0; --i) {
       float yx[V], yg[V];
 #pragma unroll
       for (int j = 0; j < V; ++j) {
@@ -560,7 +572,6 @@ static int64_t gs_len(int64_t T, int64_t groups, int* S) {
   *S = (int)(per ? (rounds + per - 1) / per : 1);
   return per * kGsRows;
 }
-static int64_t gs_groups(const lsh_gated* a, int V) { return (a->B * a->D + 64 * V - 1) / (64 * V); }
 
 static GsArgs gs_args(const lsh_gated* p) {
   GsArgs a = {};
@@ -592,7 +603,7 @@ static size_t gs_workspace(const lsh_gated* p) {
   if (p->B == 0) return 0;
   for (int V : {1, 2}) {
     int S;
-    gs_len(p->T, gs_groups(p, V), &S);
+    gs_len(p->T, (p->B * p->D + 64 * V - 1) / (64 * V), &S);
     if (S > 1) most = std::max(most, (size_t)S * 2 * p->B * p->D * sizeof(float));
   }
   return most;
@@ -606,28 +617,62 @@ static bool gs_near(const GsArgs& a, int size, int V) {
   return a.D < ((int64_t)1 << 32) / size;
 }
 
-// Calls f(type, FAST, MASK, threads of a workgroup, channel groups), everything about the launch in *a.  False: too
-// many workgroups.  R: rows of a wave.
-template <int R, class F>
-static bool gs_launch(GsArgs& a, int dtype, F&& f) {
-  const int size = lm_dtype_size(dtype), V = size == 2 ? 2 : 1;
-  const bool fast = (V == 1 || gs_wide(a, size, V)) && gs_near(a, size, V);
-  a.pieces = a.n / (fast ? V : 1);
-  const int64_t groups = (a.pieces + 63) / 64;
-  a.len = gs_len(a.T, groups, &a.S);
-  if (!lm_grid_ok(groups * a.S, kGsW * 64)) return false;
-  a.groups = (int)groups;
-  // of short sequences as many waves as there are rows for
-  const int W = a.T > 4 * R ? 8 : a.T > 2 * R ? 4 : a.T > R ? 2 : 1;
+// Bytes of a lane in a row, at most `most`: 8 or 4 where all operands allow it, else 0 (one channel anywhere).
+static int gs_bytes(const GsArgs& a, int size, int most) {
+  for (int bytes = most; bytes >= 4; bytes /= 2)
+    if (const int V = bytes / size; (V == 1 || gs_wide(a, size, V)) && gs_near(a, size, V)) return bytes;
+  return 0;
+}
+template <class F>
+static void with_bytes(int bytes, F&& f) {
+  if (bytes == 8)
+    f(std::integral_constant<int, 8>{});
+  else if (bytes == 4)
+    f(std::integral_constant<int, 4>{});
+  else
+    f(std::integral_constant<int, 0>{});
+}
+// The channels in groups of 64 pieces
+static void gs_group(GsArgs& a, int size, int bytes) {
+  a.pieces = a.n / (bytes ? bytes / size : 1);
+  a.groups = (int)((a.pieces + 63) / 64);
+}
+
+template <bool BWD>
+static int gs_run(GsArgs& a, int dtype, hipStream_t st) {
+  const int size = lm_dtype_size(dtype);
+  if (!lm_grid_ok(a.n / 64 + 1, kGsW * 64)) return LSH_ERR_SHAPE;
+  const int bytes = gs_bytes(a, size, 4), sums = gs_bytes(a, size, 8);
+  gs_group(a, size, bytes);
+  a.len = gs_len(a.T, a.groups, &a.S);
+  if (!lm_grid_ok((int64_t)a.groups * a.S, kGsW * 64)) return LSH_ERR_SHAPE;
   with_dtype(dtype, [&](auto t) {
+    using T = decltype(t);
     with_mask(a.starts != nullptr, [&](auto mask) {
-      if (fast)
-        f(t, std::true_type{}, mask, W * 64, (unsigned)groups);
-      else
-        f(t, std::false_type{}, mask, W * 64, (unsigned)groups);
+      constexpr bool MASK = decltype(mask)::value;
+      if (a.S > 1)
+        with_bytes(sums, [&](auto n) {
+          constexpr int N = decltype(n)::value;
+          GsArgs b = a;
+          gs_group(b, size, N);
+          k_gated_sums<T, N, MASK, BWD><<<dim3(b.groups * (b.S - 1)), kGsSumW<N> * 64, 0, st>>>(b);
+        });
+      with_bytes(bytes, [&](auto n) {
+        constexpr int N = decltype(n)::value;
+        if constexpr (N <= 4) {
+          constexpr int R = BWD ? kGsBwd : kGsFwd;
+          // of short sequences as many waves as there are rows for
+          const int W = a.T > 4 * R ? 8 : a.T > 2 * R ? 4 : a.T > R ? 2 : 1;
+          if constexpr (BWD)
+            k_gated_bwd<T, N, MASK><<<dim3(a.groups * a.S), W * 64, 0, st>>>(a);
+          else
+            k_gated<T, N, MASK><<<dim3(a.groups * a.S), W * 64, 0, st>>>(a);
+        }
+      });
     });
   });
-  return true;
+  LSH_CHECK_LAUNCH();
+  return LSH_OK;
 }
 
 }  // namespace lsh
@@ -650,16 +695,7 @@ extern "C" int lsh_gated_fwd(const lsh_gated* p, void* h, float* h_end, float* s
   if (need && (bad_ptr(ws) || ws_bytes < need)) return LSH_ERR_WORKSPACE;
   GsArgs a = gs_args(p);
   a.h = h, a.h_end = h_end, a.saved = saved, a.part = (float*)ws;
-  hipStream_t st = (hipStream_t)stream;
-  if (!gs_launch<kGsR>(a, p->dtype, [&](auto t, auto fast, auto mask, int threads, unsigned groups) {
-        using T = decltype(t);
-        constexpr bool FAST = decltype(fast)::value, MASK = decltype(mask)::value;
-        if (a.S > 1) k_gated_sums<T, FAST, MASK, false><<<dim3(groups * (a.S - 1)), kGsSumW * 64, 0, st>>>(a);
-        k_gated<T, FAST, MASK><<<dim3(groups * a.S), threads, 0, st>>>(a);
-      }))
-    return LSH_ERR_SHAPE;
-  LSH_CHECK_LAUNCH();
-  return LSH_OK;
+  return gs_run<false>(a, p->dtype, (hipStream_t)stream);
 }
 
 extern "C" int lsh_gated_bwd(const lsh_gated* p, const float* saved, const void* dh, int64_t dh_st, int64_t dh_sb,
@@ -673,16 +709,7 @@ extern "C" int lsh_gated_bwd(const lsh_gated* p, const float* saved, const void*
   GsArgs a = gs_args(p);
   a.saved = (float*)saved, a.dh = dh, a.d_st = dh ? dh_st : 0, a.d_sb = dh ? dh_sb : 0, a.d_end = dh_end;
   a.dx = dx, a.dg = dgate, a.dh0 = dh0, a.part = (float*)ws;
-  hipStream_t st = (hipStream_t)stream;
-  if (!gs_launch<kGsB>(a, p->dtype, [&](auto t, auto fast, auto mask, int threads, unsigned groups) {
-        using T = decltype(t);
-        constexpr bool FAST = decltype(fast)::value, MASK = decltype(mask)::value;
-        if (a.S > 1) k_gated_sums<T, FAST, MASK, true><<<dim3(groups * (a.S - 1)), kGsSumW * 64, 0, st>>>(a);
-        k_gated_bwd<T, FAST, MASK><<<dim3(groups * a.S), threads, 0, st>>>(a);
-      }))
-    return LSH_ERR_SHAPE;
-  LSH_CHECK_LAUNCH();
-  return LSH_OK;
+  return gs_run<true>(a, p->dtype, (hipStream_t)stream);
 }
 
 extern "C" int lsh_gated_step(const lsh_gated* p, float* state, void* h, void* stream) {
