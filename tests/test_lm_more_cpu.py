@@ -107,3 +107,27 @@ def test_host_tensors_are_refused():
               lambda: LA.norm_rotate(q, q, tok, torch.ones(4), pairs="none"), lambda: LM.token_logprobs(x[:, 0], tok)):
         with pytest.raises(ValueError):
             f()
+
+
+def test_models_with_other_mixers():
+    from lifscan.spikelm import SpikeLM
+    kw = dict(D=32, layers=2, heads=2, dk=8, dv=16, neurons=24)
+    plain = set(dict(SpikeLM(50, **kw).named_parameters()))
+    assert not any("norm" in n or "vg" in n for n in plain)
+    m = SpikeLM(50, rotary=True, **kw)
+    assert set(dict(m.named_parameters())) - plain == {f"blocks.{i}.{n}" for i in range(2) for n in ("q_norm", "k_norm")}
+    S, u, at = m.state(3)[0]
+    assert S.shape == (3, 2, 8, 16) and u.shape == (72,) and at.shape == (3,) and at.dtype == torch.int64
+    want = [10000.0 ** (-2 * i / 8) for i in range(4)]
+    for n in (m, SpikeLM(50, rotary=True, **kw).bfloat16()):
+        f = n.blocks[1].inv_freq
+        assert f.dtype == torch.float64 and torch.allclose(f, torch.tensor(want, dtype=torch.float64), rtol=1e-15)
+        assert not any("inv_freq" in k for k in n.state_dict())
+    m = SpikeLM(50, mixer="gated", **kw)
+    names = dict(m.named_parameters())
+    assert names["blocks.0.vg.weight"].shape == (64, 32) and names["blocks.1.gate_bias"].shape == (32,) and "blocks.0.qkv.weight" not in names
+    S, u = m.state(3)[1]
+    assert S.shape == (3, 32) and u.shape == (72,)
+    for bad in (dict(mixer="none"), dict(mixer="gated", rotary=True)):
+        with pytest.raises(ValueError):
+            SpikeLM(50, **kw, **bad)
