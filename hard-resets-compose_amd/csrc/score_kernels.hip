@@ -80,10 +80,11 @@ __device__ __forceinline__ ScPiece<T> sc_load(const T* p) {
 }
 
 // The K largest of keys that the threads of a workgroup hold between them, in order, to out (0: none).  own: the value of
-// a thread's largest, as sc_order (0: it has none).  scan(bound, f) calls f with each key of the thread whose value
-// reaches bound.  One call a kernel: its LDS is not shared.
+// a thread's largest, as sc_order (0: it has none); not known: the values of own are not to be relied on.  scan(bound, f)
+// calls f with each key of the thread whose value reaches bound (and others only where bound is none, or a NaN).  One
+// call a kernel: its LDS is not shared.
 template <class Scan, class Out>
-__device__ __forceinline__ void sc_select(unsigned own, int K, Scan&& scan, Out&& out) {
+__device__ __forceinline__ void sc_select(unsigned own, bool known, int K, Scan&& scan, Out&& out) {
   __shared__ unsigned s_value[kScThreads], s_bound;
   __shared__ Key s_list[kScList], s_key;
   __shared__ int s_count;
@@ -95,7 +96,7 @@ __device__ __forceinline__ void sc_select(unsigned own, int K, Scan&& scan, Out&
     unsigned v[kScThreads / 64], bound = 0;
 #pragma unroll
     for (int i = 0; i < kScThreads / 64; ++i) v[i] = s_value[tid + 64 * i];
-    for (unsigned bit = 0x80000000u; bit; bit >>= 1) {
+    for (unsigned bit = known ? 0x80000000u : 0; bit; bit >>= 1) {
       const unsigned t = bound | bit;
       int reach = 0;
 #pragma unroll
@@ -103,63 +104,65 @@ __device__ __forceinline__ void sc_select(unsigned own, int K, Scan&& scan, Out&
       if (reach >= K) bound = t;
       if (reach == K) break;
     }
-    if (tid == 0) s_bound = bound, s_key = 0, s_count = 0;
+    if (tid == 0) s_bound = bound, s_count = 0;
   }
   __syncthreads();
   const unsigned bound = s_bound;
   const bool mine = own && own >= bound;
-  auto collect = [&](Key least) {
-    if (mine)
-      scan(bound, [&](Key k) {
-        if (k < least) return;
-        const int at = atomicAdd(&s_count, 1);
-        if (at < kScList) s_list[at] = k;
-      });
-    __syncthreads();
-    return s_count;
-  };
-  int n = collect(0);
-  if (n > kScList) {
-    // long runs of equal values, as where most of a row is masked: the K-th largest of the threads' keys
-    Key best = 0;
-    if (mine) scan(bound, [&](Key k) { best = max(best, k); });
-    __syncthreads();
-    s_list[tid] = best;
-    if (tid == 0) s_count = 0;
-    __syncthreads();
-    int above = 0;
-    for (int i = 0; i < kScThreads; ++i) above += s_list[i] > best;
-    if (above == K - 1 && best) s_key = best;
-    __syncthreads();
-    n = collect(s_key);
-  }
-  if (n <= kScList) {
-    for (int i = tid; i < n; i += kScThreads) {
-      const Key k = s_list[i];
-      int rank = 0;
-      for (int j = 0; j < n; ++j) rank += s_list[j] > k;
-      if (rank < K) out(rank, k);
-    }
-    for (int i = n + tid; i < K; i += kScThreads) out(i, (Key)0);
-    return;
-  }
-  // a few threads hold more than the list: one after the other
-  Key last = ~(Key)0;
-  for (int k = 0; k < K; ++k) {
+  // The list of all keys that reach the bound.  Where it does not hold them (long runs of equal values, as where most of
+  // a row is masked): the K-th largest of the threads' largest keys, and the list of all that reach that.  Where it does
+  // not hold those either (a few threads hold most): the keys one after the other.  One place in the code looks
+  // through a thread's keys for all of these: copies of it cost registers, and so waves.
+  enum { kList, kLargest, kBounded, kNext } what = known ? kList : kLargest;
+  Key least = 0, last = ~(Key)0;
+  for (int k = 0;;) {
     Key best = 0;
     if (mine)
       scan(bound, [&](Key x) {
-        if (x < last) best = max(best, x);
+        if (what == kList || what == kBounded) {
+          if (x < least) return;
+          const int at = atomicAdd(&s_count, 1);
+          if (at < kScList) s_list[at] = x;
+        } else if (x < last) {
+          best = max(best, x);
+        }
       });
-    __syncthreads();  // the list was read
-    s_list[tid] = best;
     __syncthreads();
-    for (int o = kScThreads / 2; o > 0; o >>= 1) {
-      if (tid < o) s_list[tid] = max(s_list[tid], s_list[tid + o]);
+    if (what == kList || what == kBounded) {
+      const int n = s_count;
+      if (n <= kScList) {
+        for (int i = tid; i < n; i += kScThreads) {
+          const Key x = s_list[i];
+          int rank = 0;
+          for (int j = 0; j < n; ++j) rank += s_list[j] > x;
+          if (rank < K) out(rank, x);
+        }
+        for (int i = n + tid; i < K; i += kScThreads) out(i, (Key)0);
+        return;
+      }
+      what = what == kList ? kLargest : kNext;
+    } else if (what == kLargest) {
+      s_list[tid] = best;
+      if (tid == 0) s_count = 0, s_key = 0;
       __syncthreads();
+      int above = 0;
+      for (int i = 0; i < kScThreads; ++i) above += s_list[i] > best;
+      if (above == K - 1 && best) s_key = best;
+      __syncthreads();
+      least = s_key;
+      what = kBounded;
+    } else {
+      s_list[tid] = best;
+      __syncthreads();
+      for (int o = kScThreads / 2; o > 0; o >>= 1) {
+        if (tid < o) s_list[tid] = max(s_list[tid], s_list[tid + o]);
+        __syncthreads();
+      }
+      last = s_list[0];
+      __syncthreads();
+      if (tid == 0) out(k, last);
+      if (++k == K) return;
     }
-    last = s_list[0];
-    if (tid == 0) out(k, last);
   }
 }
 
@@ -181,8 +184,10 @@ __device__ __forceinline__ void sc_put(const ScArgs& a, int64_t row, int k, Key 
   a.top_id[row * a.K + k] = sc_id(key);
 }
 
+// 8 waves a SIMD: while some workgroups select, others stream (2048 x 32000 bf16 with 5 alternatives: 37 us, with the 5
+// waves that the compiler would leave 39, without alternatives 28).
 template <class T, bool SPLIT, bool TOP>
-__global__ __launch_bounds__(kScThreads) void k_score(ScArgs a) {
+__global__ __launch_bounds__(kScThreads, 8) void k_score(ScArgs a) {
   constexpr int P = kWide<T>, U = kScUnroll, STEP = U * kScThreads * P;
   __shared__ float s_stat[kScThreads / 64][3];
   const int64_t row = SPLIT ? blockIdx.x / a.splits : blockIdx.x, part = SPLIT ? blockIdx.x % a.splits : 0;
@@ -221,7 +226,9 @@ __global__ __launch_bounds__(kScThreads) void k_score(ScArgs a) {
     m = top;
   };
   const int whole = n / STEP;
-  // a block that is whole; f(place of the first element of a piece, its values)
+  // where piece u of block b is read from: a piece that reaches over the end from P before the end on, so that no branch
+  // stands around the loads.  What another thread reads too is left out.
+  auto from = [&](int b, int u) { return b < whole || n < P ? place(b, u) : min(place(b, u), n - P); };
   auto read = [&](int b, float (&f)[U][P]) {
     ScPiece<T> y[U];
 #pragma unroll
@@ -231,24 +238,21 @@ __global__ __launch_bounds__(kScThreads) void k_score(ScArgs a) {
 #pragma unroll
       for (int j = 0; j < P; ++j) f[u][j] = to_f(y[u].v[j]);
   };
-  // what is left behind the whole blocks, -inf where nothing is.  A piece that reaches over the end is read from P before
-  // the end on (from[u]), without branches around the loads; what another thread reads too is left out.
-  auto read_rest = [&](int b, float (&f)[U][P], int (&from)[U]) {
+  // what is left behind the whole blocks, -inf where nothing is
+  auto read_rest = [&](int b, float (&f)[U][P]) {
     if (n >= P) {
       ScPiece<T> y[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) from[u] = min(place(b, u), n - P), y[u] = sc_load(z + from[u]);
+      for (int u = 0; u < U; ++u) y[u] = sc_load(z + from(b, u));
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int j = 0; j < P; ++j) f[u][j] = from[u] + j >= place(b, u) ? to_f(y[u].v[j]) : -INFINITY;
+        for (int j = 0; j < P; ++j) f[u][j] = from(b, u) + j >= place(b, u) ? to_f(y[u].v[j]) : -INFINITY;
     } else {
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        from[u] = place(b, u);
+      for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int j = 0; j < P; ++j) f[u][j] = from[u] + j < n ? to_f(z[from[u] + j]) : -INFINITY;
-      }
+        for (int j = 0; j < P; ++j) f[u][j] = place(b, u) + j < n ? to_f(z[place(b, u) + j]) : -INFINITY;
     }
   };
   for (int b = 0; b < whole; ++b) {
@@ -258,11 +262,9 @@ __global__ __launch_bounds__(kScThreads) void k_score(ScArgs a) {
   }
   if (place(whole, 0) < n) {
     float f[U][P];
-    int from[U];
-    read_rest(whole, f, from);
+    read_rest(whole, f);
     take(f, whole);
   }
-  const bool odd = s != s;  // a NaN, or +inf
   const float mine = m;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1)
@@ -282,38 +284,37 @@ __global__ __launch_bounds__(kScThreads) void k_score(ScArgs a) {
   }
   if constexpr (TOP) {
     const int blocks = place(whole, 0) < n ? whole + 1 : whole;
-    // the thread's keys of a block whose values reach a bound
+    // the thread's keys of a block whose values reach a bound: which ones they are first, and then the few one by one
     auto block = [&](int b, unsigned bound, auto&& f) {
+      const float least = sc_value((Key)bound << 32);
       float x[U][P];
-      int from[U];
-      if (b < whole) {
+      if (b < whole)
         read(b, x);
-#pragma unroll
-        for (int u = 0; u < U; ++u) from[u] = place(b, u);
-      } else {
-        read_rest(b, x, from);
-      }
+      else
+        read_rest(b, x);
+      unsigned long long there = 0;
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int j = 0; j < P; ++j) {
-          const int e = from[u] + j;
-          if (sc_order(x[u][j]) >= bound && e >= place(b, u) && e < n) f(sc_key(x[u][j], (unsigned)(v0 + e)));
+          const int e = from(b, u) + j;
+          // what is not less: also NaN, and any value where the bound is none
+          if (!(x[u][j] < least) && e >= place(b, u) && e < n) there |= 1ull << (u * P + j);
         }
+      for (; there; there &= there - 1) {
+        const int i = __ffsll((unsigned long long)there) - 1, e = from(b, i / P) + i % P;
+        f(sc_key(to_f(z[e]), (unsigned)(v0 + e)));
+      }
     };
-    unsigned own = blocks ? sc_order(mine) : 0;
-    if (odd) {  // the maximum leaves NaN out
-      own = 0;
-      for (int b = 0; b < blocks; ++b) block(b, 0, [&](Key k) { own = max(own, sc_order(k)); });
-    }
     const float l = __builtin_amdgcn_logf(s);
+    // a NaN, or +inf, in the row: the maxima leave NaN out
+    const bool odd = s != s;
     sc_select(
-        own, a.K,
+        blocks ? sc_order(mine) : 0, !odd, a.K,
         [&](unsigned bound, auto&& f) {
-          if (odd || sc_order(other) >= bound)
-            for (int b = 0; b < blocks; ++b) block(b, bound, f);
-          else
-            block(best, bound, f);
+          const bool all = odd || sc_order(other) >= bound;
+          const int b1 = all ? blocks : best + 1;
+          for (int b = all ? 0 : best; b < b1; ++b) block(b, bound, f);
         },
         [&](int k, Key key) {
           if (SPLIT)
@@ -342,7 +343,7 @@ __global__ __launch_bounds__(kScThreads) void k_score_join(ScArgs a) {
     for (int k = tid; k < n; k += kScThreads) own = max(own, sc_order(keys[k]));
     const float l = __builtin_amdgcn_logf(s);
     sc_select(
-        own, a.K,
+        own, true, a.K,
         [&](unsigned bound, auto&& f) {
           for (int k = tid; k < n; k += kScThreads)
             if (const Key x = keys[k]; x && sc_order(x) >= bound) f(x);
@@ -391,7 +392,7 @@ __global__ __launch_bounds__(kScThreads) void k_score_bwd(ScArgs a) {
 }
 
 static int sc_check(int dtype, int64_t rows, int64_t V, int K, float tau) {
-  if (!lm_dtype_ok(dtype) || !(tau > 0.0f) || !(tau < INFINITY)) return LSH_ERR_ARG;
+  if (!lm_dtype_ok(dtype) || !(tau > 0.0f) || !(tau < INFINITY) || !(kScLog2e / tau < INFINITY)) return LSH_ERR_ARG;
   if (rows < 0 || !lm_grid_ok(rows, kScThreads) || V < 1 || V > 0x7fffffff / 2 || K < 0 || K > LSH_SCORE_MAX_TOP ||
       K > V)
     return LSH_ERR_SHAPE;

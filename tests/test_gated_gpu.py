@@ -346,6 +346,53 @@ def test_offsets_beyond_32_bits(dev):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_batches_beyond_32_bits(dev, dtype):
+    """Batches of which a wave holds several, 2^32 bytes and more apart: no 32-bit offset reaches from one to
+    the next."""
+    T, B, D = 300, 2, 32
+    x, gate, h0, st, dh, dend = inputs(T, B, D, dtype, dev, starts=True, seed=16)
+    apart = 2 ** 32 // x.element_size() + 2 ** 20
+    far = torch.empty(apart + 2 ** 20, dtype=dtype, device=dev)
+    views = [far.as_strided((T, B, D), (D, apart, 1), i * T * D) for i in range(3)]
+    for v, t in zip(views, (x, gate, dh)):
+        v.copy_(t)
+    got = run(views[0], views[1], h0, st, "sigmoid", True, views[2], dend)
+    check(got, reference(x, gate, h0, st, "sigmoid", True, dh, dend))
+
+
+def test_one_tensor_as_value_and_gate(dev):
+    from lifscan import hip_gated as G
+    x, _, h0, _, dh, _ = inputs(200, 2, 24, torch.float32, dev, seed=17)
+    y = x.clone().requires_grad_(True)
+    (got,) = torch.autograd.grad(G.gated_scan(y, y, h0)[0], y, dh)
+    want = reference(x, x, h0, None, "sigmoid", True, dh)
+    close(got, (want["dx"][0] + want["dgate"][0], want["dx"][1] + want["dgate"][1] + F * (want["dx"][0].abs() + want["dgate"][0].abs())))
+    # a gradient for one of them alone
+    for i in range(3):
+        ins = [x.clone(), x.clone(), h0.clone()]
+        ins[i].requires_grad_(True)
+        (got,) = torch.autograd.grad(G.gated_scan(*ins)[0], ins[i], dh)
+        close(got, want[("dx", "dgate", "dh0")[i]])
+
+
+def test_calls_at_once_on_two_streams(dev):
+    from lifscan import hip_gated as G
+    a, b = (inputs(3000, 2, 96, torch.bfloat16, dev, starts=True, seed=s) for s in (18, 19))
+    want = [run(*t[:4], "sigmoid", True, *t[4:]) for t in (a, b)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [None, None]
+    for n in range(3):
+        for i, t in enumerate((a, b)):
+            with torch.cuda.stream(streams[i]):
+                got[i] = run(*t[:4], "sigmoid", True, *t[4:])
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        for k in w:
+            assert torch.equal(g[k], w[k])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
 def test_same_bits_on_every_run_and_stream(dev, dtype):
     args = inputs(1500, 2, 200, dtype, dev, starts=True, seed=13)
     x, gate, h0, st, dh, dend = args

@@ -85,6 +85,7 @@ def test_score_checks():
     f = lambda dtype=1, z=P, tok=P, lp=P, en=P, tl=P, ti=P, rows=4, V=100, K=5, tau=1.0, ws=None, nb=0: L.lsh_score_fwd(  # noqa: E731
         dtype, z, V, tok, lp, en, None, tl, ti, rows, V, K, tau, ws, nb, None)
     assert f(dtype=3) == ARG and f(tau=0.0) == ARG and f(tau=float("inf")) == ARG and f(tau=float("nan")) == ARG
+    assert f(tau=1e-39) == ARG  # its reciprocal is no fp32 number
     assert f(z=None) == ARG and f(tok=None) == ARG and f(lp=None) == ARG and f(en=None) == ARG and f(tl=None) == ARG and f(ti=None) == ARG
     assert f(V=0) == SHAPE and f(K=65) == SHAPE and f(K=-1) == SHAPE and f(V=4, K=5) == SHAPE and f(rows=-1) == SHAPE
     assert f(rows=2 ** 24) == SHAPE and f(rows=0) == 0

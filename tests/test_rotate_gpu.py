@@ -282,6 +282,21 @@ def test_empty(dev):
     pos = torch.zeros(3, dtype=torch.int64, device=dev)
     a, b = LA.norm_rotate(q, k, pos, f)
     assert a.shape == q.shape and torch.equal(b, k)
+    # no queries, or neither: the others' gradients, and zeros for the weights
+    q.requires_grad_(True), k.requires_grad_(True)
+    g = torch.randn_like(k)
+    v = torch.ones(8, device=dev, requires_grad=True)
+    a, b = LA.norm_rotate(q, k, pos, f, v, w)
+    dq, dk, dv, dw = torch.autograd.grad((a, b), (q, k, v, w), (torch.zeros_like(a), g))
+    assert dq.shape == q.shape and not bool(dv.any())
+    want = reference(k, w, pos, f, 1e-6, "halves", g)
+    close(dk, want["dx"]), close(dw, want["dw"], 64 + 6)
+    a, b = LA.norm_rotate(q, q, pos, f, v, w)
+    dv, dw = torch.autograd.grad(a.sum() + b.sum(), (v, w))
+    assert not bool(dv.any()) and not bool(dw.any())
+    # frequencies of none are no rotation
+    a, b = LA.norm_rotate(k, k, pos, f[:0])
+    assert torch.equal(a, k) and torch.equal(b, k)
 
 
 def test_offsets_beyond_32_bits(dev):

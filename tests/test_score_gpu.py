@@ -289,6 +289,34 @@ def test_offsets_beyond_32_bits(dev):
     assert all(torch.equal(x, y) for x, y in zip(a, b)) and torch.equal(da, db)
 
 
+def test_rows_that_are_one_row(dev):
+    """Expanded logits: read through a row stride of 0, and their gradient is summed."""
+    from lifscan import hip_lm as LM
+    z, tok, gl, gh = inputs(7, 700, torch.float32, dev, seed=14)
+    y = z[:1].clone().requires_grad_(True)
+    out = LM.token_logprobs(y.expand(7, 700), tok, top=3)
+    (dz,) = torch.autograd.grad(out[:2], y, (gl, gh))
+    want = reference(z[:1].expand(7, 700), tok, 1.0, 3, gl, gh)
+    check(out, None, want, 700, 3)
+    err = (dz.double().cpu() - want["dz"].sum(0)).abs()
+    assert bool((err <= (64 + 700 / 64 + 7) * F * want["size"].sum(0) + 2.0 ** -126).all())
+
+
+def test_calls_at_once_on_two_streams(dev):
+    a, b = (inputs(5, 50000, torch.bfloat16, dev, seed=s) for s in (15, 16))
+    want = [run(t[0], t[1], 1.0, 20, *t[2:]) for t in (a, b)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [None, None]
+    for n in range(3):
+        for i, t in enumerate((a, b)):
+            with torch.cuda.stream(streams[i]):
+                got[i] = run(t[0], t[1], 1.0, 20, *t[2:])
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        assert all(torch.equal(x, y) for x, y in zip(g[0], w[0])) and torch.equal(g[1], w[1])
+
+
 def test_empty(dev):
     from lifscan import hip_lm as LM
     z = torch.zeros(0, 7, device=dev, requires_grad=True)
@@ -351,7 +379,7 @@ def test_refusals(dev):
            lambda: LM.token_logprobs(z, tok[:3]), lambda: LM.token_logprobs(z, tok[:, None]), lambda: LM.token_logprobs(z, tok.float()),
            lambda: LM.token_logprobs(z.double(), tok), lambda: LM.token_logprobs(z, tok, temperature=0.0),
            lambda: LM.token_logprobs(z, tok, temperature=float("inf")), lambda: LM.token_logprobs(z, tok, temperature=float("nan")),
-           lambda: LM.token_logprobs(z, tok, top=-1), lambda: LM.token_logprobs(z, tok, top=65),
+           lambda: LM.token_logprobs(z, tok, temperature=1e-39), lambda: LM.token_logprobs(z, tok, top=-1), lambda: LM.token_logprobs(z, tok, top=65),
            lambda: LM.token_logprobs(z[:, :20], tok, top=21), lambda: LM.token_logprobs(z[:, :0], tok),
            lambda: LM.token_logprobs(torch._neg_view(z), tok)]
     for f in bad:
