@@ -114,16 +114,25 @@ struct RtLane {
 #pragma unroll
     for (int e = 0; e < E; ++e) x[e][0] = *(const Vec<T, V>*)(p + lo[e]), x[e][1] = *(const Vec<T, V>*)(p + hi[e]);
   }
-  // as fp32, zeros where there are no columns
+  // as fp32; where there are no columns, some others of the head
   template <class T>
-  __device__ __forceinline__ void get(const Vec<T, V> (&x)[E][2], float (&f)[E][2 * V]) const {
+  static __device__ __forceinline__ void get(const Vec<T, V> (&x)[E][2], float (&f)[E][2 * V]) {
 #pragma unroll
     for (int e = 0; e < E; ++e)
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        f[e][j] = there[e] ? to_f(x[e][0].v[j]) : 0.0f;
-        f[e][V + j] = there[e] ? to_f(x[e][1].v[j]) : 0.0f;
-      }
+      for (int j = 0; j < V; ++j) f[e][j] = to_f(x[e][0].v[j]), f[e][V + j] = to_f(x[e][1].v[j]);
+  }
+  // the sum over a head of the products a*b
+  __device__ __forceinline__ float dot(const float (&a)[E][2 * V], const float (&b)[E][2 * V]) const {
+    float sum = 0.0f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      float s = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 2 * V; ++j) s = __builtin_fmaf(a[e][j], b[e][j], s);
+      sum += there[e] ? s : 0.0f;
+    }
+    return rt_sum<G>(sum);
   }
   template <class T>
   __device__ __forceinline__ void put(T* p, const float (&f)[E][2 * V]) const {
@@ -143,15 +152,20 @@ struct RtLane {
   }
 };
 
+// 8192 tokens of 16 + 4 heads of 128, bf16: forward 22 us for 84 MB (3.8 TB/s), gradients 31 us for 126 MB (4.1 TB/s)
+// and 4 for the weights' sums.  What bounds them: a wave's loads, its sums over lanes and its stores follow one
+// another, and registers leave 8 waves a SIMD forwards and 5 backwards to cover that.  (Copies of the work for heads of
+// q alone, of k alone and of either save the choice of weights, an instruction in ten, and cost the fifth wave: 34.)
 template <class T, int V, int G, int E, bool NEXT, bool BWD>
-__global__ __launch_bounds__(kRtWaves * 64) void k_rotate(RtArgs a) {
+__global__ __launch_bounds__(kRtWaves * 64, 5) void k_rotate(RtArgs a) {
   using Lane = RtLane<V, G, E, NEXT>;
+  using Row = float[E][2 * V];
   __shared__ float s_sum[BWD ? kRtWaves : 1][BWD ? 2 * 2 * V * E * G : 1];
   const Lane at(a);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), sub = (threadIdx.x & 63) / G;
   const bool norm = a.wq != nullptr;
   const float per = 1.0f / a.D;
-  float wq[E][2 * V], wk[E][2 * V], sq[E][2 * V] = {}, sk[E][2 * V] = {};
+  Row wq, wk, sq = {}, sk = {};
   if (norm) at.weights(a.wq, wq), at.weights(a.wk, wk);
   for (int64_t item = (int64_t)blockIdx.x * kRtWaves + wave; item < a.items; item += (int64_t)gridDim.x * kRtWaves) {
     const int64_t token = item / a.per_token, t = token / a.B, b = token - t * a.B;
@@ -170,25 +184,30 @@ __global__ __launch_bounds__(kRtWaves * 64) void k_rotate(RtArgs a) {
       const int head = live ? h + sub : head1 - 1;
       const bool is_q = head < a.H;
       const int own = is_q ? head : head - a.H;  // the head's number among those of q, or k
-      const int64_t from = is_q ? t * a.q_st + b * a.q_sb + own * a.q_sh : t * a.k_st + b * a.k_sb + own * a.k_sh;
-      const T* x = (const T*)(is_q ? a.q : a.k) + from;
       T* out = (T*)(is_q ? a.qo : a.ko) + (token * (is_q ? a.H : a.heads - a.H) + own) * a.D;
-      Vec<T, V> rx[E][2];
-      float f[E][2 * V], y[E][2 * V];
-      if (!BWD || norm) at.load(x, rx), at.get(rx, f);
-      float r = 1.0f;
+      Vec<T, V> rx[E][2], rg[E][2];
+      if (!BWD || norm)
+        at.load((const T*)(is_q ? a.q : a.k) +
+                    (is_q ? t * a.q_st + b * a.q_sb + own * a.q_sh : t * a.k_st + b * a.k_sb + own * a.k_sh),
+                rx);
+      if (BWD)
+        at.load((const T*)(is_q ? a.gq : a.gk) +
+                    (is_q ? t * a.gq_st + b * a.gq_sb + own * a.gq_sh : t * a.gk_st + b * a.gk_sb + own * a.gk_sh),
+                rg);
+      Row w, f, y;
+      if (norm)
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+#pragma unroll
+          for (int j = 0; j < 2 * V; ++j) w[e][j] = is_q ? wq[e][j] : wk[e][j];
       if constexpr (!BWD) {
+        at.get(rx, f);
         if (norm) {
-          float sum = 0.0f;
+          const float r = rt_rsqrt(at.dot(f, f) * per + a.eps);
 #pragma unroll
           for (int e = 0; e < E; ++e)
 #pragma unroll
-            for (int j = 0; j < 2 * V; ++j) sum = __builtin_fmaf(f[e][j], f[e][j], sum);
-          r = rt_rsqrt(rt_sum<G>(sum) * per + a.eps);
-#pragma unroll
-          for (int e = 0; e < E; ++e)
-#pragma unroll
-            for (int j = 0; j < 2 * V; ++j) f[e][j] *= r * (is_q ? wq[e][j] : wk[e][j]);
+            for (int j = 0; j < 2 * V; ++j) f[e][j] *= r * w[e][j];
         }
 #pragma unroll
         for (int e = 0; e < E; ++e)
@@ -199,10 +218,6 @@ __global__ __launch_bounds__(kRtWaves * 64) void k_rotate(RtArgs a) {
             y[e][Lane::second(j)] = __builtin_fmaf(u, s[e][j], v * c[e][j]);
           }
       } else {
-        const int64_t g_at =
-            is_q ? t * a.gq_st + b * a.gq_sb + own * a.gq_sh : t * a.gk_st + b * a.gk_sb + own * a.gk_sh;
-        Vec<T, V> rg[E][2];
-        at.load((const T*)(is_q ? a.gq : a.gk) + g_at, rg);
         at.get(rg, y);
 #pragma unroll
         for (int e = 0; e < E; ++e)
@@ -213,25 +228,23 @@ __global__ __launch_bounds__(kRtWaves * 64) void k_rotate(RtArgs a) {
             y[e][Lane::second(j)] = __builtin_fmaf(v, c[e][j], -(u * s[e][j]));
           }
         if (norm) {
-          float sum = 0.0f, dot = 0.0f;
+          at.get(rx, f);
+          const float r = rt_rsqrt(at.dot(f, f) * per + a.eps);
+          const bool to_q = live && is_q, to_k = live && !is_q;
 #pragma unroll
           for (int e = 0; e < E; ++e)
 #pragma unroll
             for (int j = 0; j < 2 * V; ++j) {
-              sum = __builtin_fmaf(f[e][j], f[e][j], sum);
-              dot = __builtin_fmaf(y[e][j] * (is_q ? wq[e][j] : wk[e][j]), f[e][j], dot);
+              const float x = y[e][j] * f[e][j];  // chosen and not multiplied by 0: a NaN stays in its own sum
+              sq[e][j] = to_q ? __builtin_fmaf(x, r, sq[e][j]) : sq[e][j];
+              sk[e][j] = to_k ? __builtin_fmaf(x, r, sk[e][j]) : sk[e][j];
+              y[e][j] *= w[e][j];
             }
-          r = rt_rsqrt(rt_sum<G>(sum) * per + a.eps);
-          const float back = r * r * (rt_sum<G>(dot) * per);
+          const float back = r * r * (at.dot(y, f) * per);
 #pragma unroll
           for (int e = 0; e < E; ++e)
 #pragma unroll
-            for (int j = 0; j < 2 * V; ++j) {
-              const float w = is_q ? wq[e][j] : wk[e][j], add = live ? y[e][j] * (f[e][j] * r) : 0.0f;
-              sq[e][j] += is_q ? add : 0.0f;
-              sk[e][j] += is_q ? 0.0f : add;
-              y[e][j] = r * __builtin_fmaf(-f[e][j], back, y[e][j] * w);
-            }
+            for (int j = 0; j < 2 * V; ++j) y[e][j] = r * __builtin_fmaf(-f[e][j], back, y[e][j]);
         }
       }
       if (live) at.put(out, y);
