@@ -8,11 +8,11 @@
 //   dx_t = w_t*E_t,  dgate_t = E_t*(h_{t-1} - [w = 1 - a]*x_t)*da/dgate
 //
 // A step is an affine map, and so is a run of steps: (P, H) with h_end = P*h_begin + H, and backwards (P, Q) with
-// F_begin = P*F_end + Q and the same P.  A lane has V neighbouring channels, a wave 8 or 16 rows of them in registers,
+// F_begin = P*F_end + Q and the same P.  A lane has V neighbouring channels, a wave 8 rows of them in registers,
 // and a workgroup's waves hold consecutive rows: the waves' maps meet in LDS, each wave composes those before its own,
 // and then writes its rows from the state before them.  Where there are too few channels for the chip the rows are cut
 // into segments, whose maps an extra pass over the operands forms.  The gradients take h_{t-1} from the state before
-// every kGsRows rows, which the forward keeps in fp32, and form it again: h itself may have 16 bits.
+// every kGsSave rows, which the forward keeps in fp32, and form it again: h itself may have 16 bits.
 //
 // A start is a factor -0 (decays are never negative): a marked product stays marked and drops what it is
 // applied to, also an infinity or a NaN.
@@ -25,8 +25,9 @@ namespace lsh {
 
 // Waves of a workgroup, what the rows of a segment are a multiple of, and the rows between saved states.
 constexpr int kGsW = 8, kGsRows = 128, kGsSave = 64;
-// Rows that a wave holds: forwards, backwards, and for a segment's map with so many bytes a lane and row
-constexpr int kGsFwd = 16, kGsBwd = 8;
+// Rows that a wave holds: forwards, backwards, and for a segment's map with so many bytes a lane and row.  (16 rows
+// forwards have not the registers for two workgroups a CU in every type: fp16 4096 x 4 x 2048 57 us, so 40; bf16 41, so 39.)
+constexpr int kGsFwd = 8, kGsBwd = 8;
 template <int BYTES>
 constexpr int kGsSum = BYTES == 8 ? 8 : 16;
 
@@ -97,7 +98,7 @@ __device__ __forceinline__ float gs_product(float first, float then) {
 // Bytes of a lane in a row: 8, 4, or one element of either size.  The first two have a row's lanes within 4 GB of each
 // other, so that an address is a scalar and an offset; the last reads a channel wherever it lies.  Wider is faster for
 // the maps (4096 x 4 x 2048 bf16: 36 us with 8 bytes, 41 with 4, 54 with 2), but the passes themselves have not the
-// registers for 8 (forward 61 us with 8 rows a wave of 8 bytes, 41 with 16 rows of 4, 55 with 2 bytes).
+// registers for 8 (forward 61 us with 8 rows a wave of 8 bytes, 39 with 8 rows of 4, 55 with 16 rows of 2).
 template <class T, int BYTES>
 constexpr int kGsV = BYTES > (int)sizeof(T) ? BYTES / (int)sizeof(T) : 1;
 template <int BYTES>
@@ -562,7 +563,8 @@ static int gs_check(const lsh_gated* a) {
 }
 
 // Segments: as many as give the chip 512 workgroups (two a CU), of whole rounds; one where the channels alone give
-// 384.  Returns the rows of a segment.
+// 384.  Returns the rows of a segment.  (4096 x 4 x 2048 bf16 with 256 workgroups: forward 43 us, gradients 91, so 39 and
+// 75; with 768 the maps take 45, so 36.)
 static int64_t gs_len(int64_t T, int64_t groups, int* S) {
   const int64_t rounds = (T + kGsRows - 1) / kGsRows;
   int64_t s = groups >= 384 ? 1 : (512 + groups - 1) / groups;
