@@ -21,7 +21,7 @@
 
 namespace lsh {
 
-constexpr int kScThreads = 256, kScUnroll = 4, kScParts = 64, kScList = 1024;
+constexpr int kScThreads = 256, kScUnroll = 4, kScParts = 64;
 constexpr float kScLog2e = 1.4426950408889634f, kScLn2 = 0.6931471805599453f;
 
 struct ScArgs {
@@ -82,25 +82,25 @@ __device__ __forceinline__ ScPiece<T> sc_load(const T* p) {
 // The K largest of keys that the threads of a workgroup hold between them, in order, to out (0: none).  own: the value of
 // a thread's largest, as sc_order (0: it has none); not known: the values of own are not to be relied on.  scan(bound, f)
 // calls f with each key of the thread whose value reaches bound (and others only where bound is none, or a NaN).  One
-// call a kernel: its LDS is not shared.
-template <class Scan, class Out>
+// call a kernel: its LDS is not shared.  NT threads, at least K.
+template <int NT, class Scan, class Out>
 __device__ __forceinline__ void sc_select(unsigned own, bool known, int K, Scan&& scan, Out&& out) {
-  __shared__ unsigned s_value[kScThreads], s_bound;
-  __shared__ Key s_list[kScList], s_key;
+  constexpr int LIST = 4 * NT;  // holds a key of each thread, too
+  __shared__ unsigned s_value[NT], s_bound;
+  __shared__ Key s_list[LIST], s_key;
   __shared__ int s_count;
-  static_assert(kScList >= kScThreads, "the list holds a key of each thread");
   const int tid = threadIdx.x;
   s_value[tid] = own;
   __syncthreads();
   if (tid < 64) {  // the K-th largest, bit by bit
-    unsigned v[kScThreads / 64], bound = 0;
+    unsigned v[NT / 64], bound = 0;
 #pragma unroll
-    for (int i = 0; i < kScThreads / 64; ++i) v[i] = s_value[tid + 64 * i];
+    for (int i = 0; i < NT / 64; ++i) v[i] = s_value[tid + 64 * i];
     for (unsigned bit = known ? 0x80000000u : 0; bit; bit >>= 1) {
       const unsigned t = bound | bit;
       int reach = 0;
 #pragma unroll
-      for (int i = 0; i < kScThreads / 64; ++i) reach += __popcll(__ballot(v[i] >= t));
+      for (int i = 0; i < NT / 64; ++i) reach += __popcll(__ballot(v[i] >= t));
       if (reach >= K) bound = t;
       if (reach == K) break;
     }
@@ -122,7 +122,7 @@ __device__ __forceinline__ void sc_select(unsigned own, bool known, int K, Scan&
         if (what == kList || what == kBounded) {
           if (x < least) return;
           const int at = atomicAdd(&s_count, 1);
-          if (at < kScList) s_list[at] = x;
+          if (at < LIST) s_list[at] = x;
         } else if (x < last) {
           best = max(best, x);
         }
@@ -130,14 +130,14 @@ __device__ __forceinline__ void sc_select(unsigned own, bool known, int K, Scan&
     __syncthreads();
     if (what == kList || what == kBounded) {
       const int n = s_count;
-      if (n <= kScList) {
-        for (int i = tid; i < n; i += kScThreads) {
+      if (n <= LIST) {
+        for (int i = tid; i < n; i += NT) {
           const Key x = s_list[i];
           int rank = 0;
           for (int j = 0; j < n; ++j) rank += s_list[j] > x;
           if (rank < K) out(rank, x);
         }
-        for (int i = n + tid; i < K; i += kScThreads) out(i, (Key)0);
+        for (int i = n + tid; i < K; i += NT) out(i, (Key)0);
         return;
       }
       what = what == kList ? kLargest : kNext;
@@ -146,7 +146,7 @@ __device__ __forceinline__ void sc_select(unsigned own, bool known, int K, Scan&
       if (tid == 0) s_count = 0, s_key = 0;
       __syncthreads();
       int above = 0;
-      for (int i = 0; i < kScThreads; ++i) above += s_list[i] > best;
+      for (int i = 0; i < NT; ++i) above += s_list[i] > best;
       if (above == K - 1 && best) s_key = best;
       __syncthreads();
       least = s_key;
@@ -154,7 +154,7 @@ __device__ __forceinline__ void sc_select(unsigned own, bool known, int K, Scan&
     } else {
       s_list[tid] = best;
       __syncthreads();
-      for (int o = kScThreads / 2; o > 0; o >>= 1) {
+      for (int o = NT / 2; o > 0; o >>= 1) {
         if (tid < o) s_list[tid] = max(s_list[tid], s_list[tid + o]);
         __syncthreads();
       }
@@ -186,17 +186,17 @@ __device__ __forceinline__ void sc_put(const ScArgs& a, int64_t row, int k, Key 
 
 // 8 waves a SIMD: while some workgroups select, others stream (2048 x 32000 bf16 with 5 alternatives: 37 us, with the 5
 // waves that the compiler would leave 39, without alternatives 28).
-template <class T, bool SPLIT, bool TOP>
-__global__ __launch_bounds__(kScThreads, 8) void k_score(ScArgs a) {
-  constexpr int P = kWide<T>, U = kScUnroll, STEP = U * kScThreads * P;
-  __shared__ float s_stat[kScThreads / 64][3];
+template <class T, bool SPLIT, bool TOP, int NT>
+__global__ __launch_bounds__(NT, 8) void k_score(ScArgs a) {
+  constexpr int P = kWide<T>, U = kScUnroll, STEP = U * NT * P;
+  __shared__ float s_stat[NT / 64][3];
   const int64_t row = SPLIT ? blockIdx.x / a.splits : blockIdx.x, part = SPLIT ? blockIdx.x % a.splits : 0;
   const int64_t v0 = part * a.len;
   const T* z = (const T*)a.z + row * a.stride + v0;
   const int n = (int)max((int64_t)0, min(a.len, a.V - v0));
   const int tid = threadIdx.x;
   // the first element of piece u of a thread in block b
-  auto place = [&](int b, int u) { return b * STEP + (u * kScThreads + tid) * P; };
+  auto place = [&](int b, int u) { return b * STEP + (u * NT + tid) * P; };
   float m = -INFINITY, s = 0.0f, t = 0.0f;
   int best = 0;             // the block of the largest
   float other = -INFINITY;  // the largest of the other blocks
@@ -273,7 +273,7 @@ __global__ __launch_bounds__(kScThreads, 8) void k_score(ScArgs a) {
   __syncthreads();
   m = s_stat[0][0], s = s_stat[0][1], t = s_stat[0][2];
 #pragma unroll
-  for (int w = 1; w < kScThreads / 64; ++w) sc_join(m, s, t, s_stat[w][0], s_stat[w][1], s_stat[w][2], a.c);
+  for (int w = 1; w < NT / 64; ++w) sc_join(m, s, t, s_stat[w][0], s_stat[w][1], s_stat[w][2], a.c);
   if (tid == 0) {
     if (SPLIT) {
       float* to = a.part + (row * a.splits + part) * 3;
@@ -309,7 +309,7 @@ __global__ __launch_bounds__(kScThreads, 8) void k_score(ScArgs a) {
     const float l = __builtin_amdgcn_logf(s);
     // a NaN, or +inf, in the row: the maxima leave NaN out
     const bool odd = s != s;
-    sc_select(
+    sc_select<NT>(
         blocks ? sc_order(mine) : 0, !odd, a.K,
         [&](unsigned bound, auto&& f) {
           const bool all = odd || sc_order(other) >= bound;
@@ -342,7 +342,7 @@ __global__ __launch_bounds__(kScThreads) void k_score_join(ScArgs a) {
     unsigned own = 0;
     for (int k = tid; k < n; k += kScThreads) own = max(own, sc_order(keys[k]));
     const float l = __builtin_amdgcn_logf(s);
-    sc_select(
+    sc_select<kScThreads>(
         own, true, a.K,
         [&](unsigned bound, auto&& f) {
           for (int k = tid; k < n; k += kScThreads)
@@ -445,10 +445,14 @@ extern "C" int lsh_score_fwd(int dtype, const void* logits, int64_t stride, cons
     auto go = [&](auto top) {
       constexpr bool TOP = decltype(top)::value;
       if (a.splits > 1) {
-        k_score<T, true, TOP><<<dim3((unsigned)(rows * a.splits)), kScThreads, 0, st>>>(a);
+        k_score<T, true, TOP, kScThreads><<<dim3((unsigned)(rows * a.splits)), kScThreads, 0, st>>>(a);
         k_score_join<T, TOP><<<dim3((unsigned)rows), TOP ? kScThreads : 64, 0, st>>>(a);
+      } else if (V <= 64 * kScUnroll * kWide<T> && K <= 32) {
+        // one block of one wave, which waits for no others (8192 x 300 bf16 with 20 alternatives: 22 us, with four waves
+        // 41); of more than half of its threads' largest the least is no bound to speak of
+        k_score<T, false, TOP, 64><<<dim3((unsigned)rows), 64, 0, st>>>(a);
       } else {
-        k_score<T, false, TOP><<<dim3((unsigned)rows), kScThreads, 0, st>>>(a);
+        k_score<T, false, TOP, kScThreads><<<dim3((unsigned)rows), kScThreads, 0, st>>>(a);
       }
     };
     if (K > 0)
