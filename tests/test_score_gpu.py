@@ -201,6 +201,31 @@ def test_values_that_are_not_finite(dev, V):
     check([o[4:5] for o in got], dz[4:5], ref, V, K)
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("V", [40, 9001])
+def test_masks_of_the_lowest_value(dev, dtype, V):
+    """Logits at the lowest value of their type are values: far below the others they have probability 0, and a
+    row of nothing else is uniform.  Such a difference times 1/tau is no fp32 number: it is not to become NaN."""
+    low = torch.finfo(dtype).min
+    z, tok, gl, gh = inputs(4, V, dtype, dev, seed=17)
+    tok = torch.tensor([3, 3, 5, 7], device=dev)
+    z[0, 6:] = low
+    z[1, :] = low
+    z[2, 5] = low
+    z[3, 7] = torch.finfo(dtype).max
+    out, dz = run(z, tok, 0.7, 5, gl, gh)
+    if dtype == torch.float16:
+        check(out, dz, reference(z, tok, 0.7, 5, gl, gh), V, 5)
+    else:  # 3.4e38 / 0.7 is beyond fp32, the type of the results: rounded, it is infinite
+        assert float(out[0][2]) == -math.inf
+    assert bool(dz.isfinite().all()) and not bool(torch.stack(out[:2]).isnan().any()) and not bool(out[2].isnan().any())
+    assert float((out[0][1] + math.log(V)).abs()) < 1e-5 and float((out[1][1] - math.log(V)).abs()) < 1e-5
+    assert out[3][1].tolist() == [0, 1, 2, 3, 4] and int(out[3][3, 0]) == 7 and float(out[1][3]) < 1e-5
+    want = reference(z[:1, :6], tok[:1], 0.7, 5, gl[:1], gh[:1])
+    check([o[:1] for o in out], dz[:1, :6], want, V, 5)
+    assert not bool(dz[0, 6:].any())
+
+
 def test_tokens_outside_the_vocabulary(dev):
     from lifscan import hip_lm as LM
     z, _, gl, gh = inputs(6, 77, torch.float32, dev, seed=4)
