@@ -803,7 +803,8 @@ struct NormRotate : public torch::autograd::Function<NormRotate> {
     ctx->saved_data["k"] = k.sizes().vec();
     ctx->saved_data["p"] = r.positions.defined() ? r.positions.sizes().vec() : std::vector<int64_t>{};
     ctx->saved_data["n"] = std::vector<int64_t>{neighbours, norm, r.freq.defined(), r.freq.defined() ? r.freq.size(0) : 0,
-                                                (int64_t)q.scalar_type()};
+                                                (int64_t)q.scalar_type(), norm && r.wq.requires_grad(),
+                                                norm && r.wk.requires_grad()};
     ctx->set_materialize_grads(false);
     return rotate_forward(r);
   }
@@ -846,7 +847,8 @@ struct NormRotate : public torch::autograd::Function<NormRotate> {
       strides(gk, st + 3);
     }
     Tensor dwq, dwk;
-    if (n[1]) dwq = torch::empty({D}, r.wq.options()), dwk = torch::empty({D}, r.wk.options());
+    if (n[5]) dwq = torch::empty({D}, r.wq.options());
+    if (n[6]) dwk = torch::empty({D}, r.wk.options());
     const size_t nb = g.lsh_rotate_bwd_workspace(&r.a);
     const Tensor ws = workspace(nb, like);
     check(g.lsh_rotate_bwd(&r.a, raw(gq), st[0], st[1], st[2], raw(gk), st[3], st[4], st[5], raw(dq), raw(dk), fp(dwq),

@@ -221,6 +221,28 @@ def test_one_output_alone(dev, which, norm):
         assert got["dw" + other] is None or not bool(got["dw" + other].any())
 
 
+def test_weights_that_ask_for_no_gradient(dev):
+    from lifscan import hip_linattn as LA
+    q, k, gq, gk, wq, wk, pos = inputs((30, 2), 4, 2, 64, torch.float32, dev)
+    f = freqs(64, dev)
+    want = run(q, k, wq, wk, pos, f, "halves", gq, gk)
+    for which in ("", "q", "k"):
+        a, b, u, v = (t.clone() for t in (q, k, wq, wk))
+        a.requires_grad_(True), b.requires_grad_(True)
+        ins, names = [a, b], ["dq", "dk"]
+        if which:
+            ins.append((u if which == "q" else v).requires_grad_(True))
+            names.append("dw" + which)
+        y, z = LA.norm_rotate(a, b, pos, f, u, v)
+        for got, n in zip(torch.autograd.grad((y, z), ins, (gq, gk)), names):
+            assert torch.equal(got, want[n])
+        if not which:  # the weights' alone
+            u.requires_grad_(True), v.requires_grad_(True)
+            y, z = LA.norm_rotate(q, k, pos, f, u, v)
+            for got, n in zip(torch.autograd.grad((y, z), (u, v), (gq, gk)), ("dwq", "dwk")):
+                assert torch.equal(got, want[n])
+
+
 def test_heads_of_zeros_and_large_eps(dev):
     q, k, gq, gk, wq, wk, pos = inputs((6, 2), 3, 1, 64, torch.float32, dev)
     q[2, 1] = 0.0
