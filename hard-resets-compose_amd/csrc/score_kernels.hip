@@ -167,20 +167,23 @@ __device__ __forceinline__ void sc_select(unsigned own, bool known, int K, Scan&
 }
 
 // What a row's statistics give: by one thread
-__device__ __forceinline__ float sc_logp(float z, float m, float l, float c) {
-  return l == -INFINITY ? -INFINITY : kScLn2 * ((z - m) * c - l);
+// In natural logarithms, and z and m apart where their difference is no fp32 number: a logit at the lowest value of its
+// type has a finite log p wherever fp32 has one.
+__device__ __forceinline__ float sc_logp(float z, float m, float l, float tau) {
+  const float d = z - m;
+  return l == -INFINITY ? -INFINITY : (d > -INFINITY ? d / tau : z / tau - m / tau) - kScLn2 * l;
 }
 template <class T>
 __device__ __forceinline__ void sc_finish(const ScArgs& a, int64_t row, float m, float s, float t) {
   const float l = __builtin_amdgcn_logf(s), H = s == 0.0f ? 0.0f : kScLn2 * (l - t / s);
   const int64_t y = a.token[row];
   const bool there = y >= 0 && y < a.V;
-  a.logp[row] = there ? sc_logp(to_f(((const T*)a.z)[row * a.stride + y]), m, l, a.c) : 0.0f;
+  a.logp[row] = there ? sc_logp(to_f(((const T*)a.z)[row * a.stride + y]), m, l, a.tau) : 0.0f;
   a.entropy[row] = H;
   if (a.stats) a.stats[row] = m, a.stats[a.rows + row] = l, a.stats[2 * a.rows + row] = H;
 }
 __device__ __forceinline__ void sc_put(const ScArgs& a, int64_t row, int k, Key key, float m, float l) {
-  a.top_logp[row * a.K + k] = sc_logp(sc_value(key), m, l, a.c);
+  a.top_logp[row * a.K + k] = sc_logp(sc_value(key), m, l, a.tau);
   a.top_id[row * a.K + k] = sc_id(key);
 }
 

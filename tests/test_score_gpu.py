@@ -226,6 +226,26 @@ def test_masks_of_the_lowest_value(dev, dtype, V):
     assert not bool(dz[0, 6:].any())
 
 
+@pytest.mark.parametrize("tau", [1.0, 2.0])
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("rows,V", [(3, 40), (3, 9001), (3, 70001), (1104, 9001)])
+def test_log_probabilities_of_the_lowest_value(dev, dtype, rows, V, tau):
+    """They are fp32 numbers, also where the logit's distance from the largest in other units, or before it is divided, is
+    none."""
+    z, _, gl, gh = inputs(3, V, dtype, dev, seed=19)
+    low, high = torch.finfo(dtype).min, torch.finfo(dtype).max
+    z[:, 5:] = low
+    z[1, 2] = -low if tau > 1 else 8.0
+    z[2, :] = low
+    z[2, V - 1] = high / 2 if tau > 1 else 3.0
+    tok = torch.tensor([6, V - 1, 0], device=dev)
+    out, dz = run(z.repeat(rows // 3, 1), tok.repeat(rows // 3), tau, 20, gl.repeat(rows // 3), gh.repeat(rows // 3))
+    want = reference(z, tok, tau, 20, gl, gh)
+    assert bool(want["logp"].float().isfinite().all()) and bool((want["logp"] < -1e4).all())
+    check([o[:3] for o in out], dz[:3], want, V, 20)
+    assert all(torch.equal(o, o[:3].repeat((rows // 3,) + (1,) * (o.dim() - 1))) for o in out)
+
+
 def test_tokens_outside_the_vocabulary(dev):
     from lifscan import hip_lm as LM
     z, _, gl, gh = inputs(6, 77, torch.float32, dev, seed=4)
