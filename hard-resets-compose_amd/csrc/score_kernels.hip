@@ -80,15 +80,15 @@ __device__ __forceinline__ ScPiece<T> sc_load(const T* p) {
 }
 
 // The K largest of keys that the threads of a workgroup hold between them, in order, to out (0: none).  own: the value of
-// a thread's largest, as sc_order (0: it has none); not known: the values of own are not to be relied on.  scan(bound, f)
-// calls f with each key of the thread whose value reaches bound (and others only where bound is none, or a NaN).  One
-// call a kernel: its LDS is not shared.  NT threads, at least K.
+// a thread's largest, as sc_order (0: it has none); not known: the values of own are not to be relied on.
+// scan(least, first, f) calls f with each key of the thread that is not less (and with some that are); first: its largest
+// is enough, which has the value of least.  One call a kernel: its LDS is not shared.  NT threads, at least K.
 template <int NT, class Scan, class Out>
 __device__ __forceinline__ void sc_select(unsigned own, bool known, int K, Scan&& scan, Out&& out) {
   constexpr int LIST = 4 * NT;  // holds a key of each thread, too
   __shared__ unsigned s_value[NT], s_bound;
   __shared__ Key s_list[LIST], s_key;
-  __shared__ int s_count;
+  __shared__ int s_count, s_reach;
   const int tid = threadIdx.x;
   s_value[tid] = own;
   __syncthreads();
@@ -96,29 +96,31 @@ __device__ __forceinline__ void sc_select(unsigned own, bool known, int K, Scan&
     unsigned v[NT / 64], bound = 0;
 #pragma unroll
     for (int i = 0; i < NT / 64; ++i) v[i] = s_value[tid + 64 * i];
-    for (unsigned bit = known ? 0x80000000u : 0; bit; bit >>= 1) {
+    int n = NT;  // threads that reach the bound
+    for (unsigned bit = known ? 0x80000000u : 0; bit && n != K; bit >>= 1) {
       const unsigned t = bound | bit;
       int reach = 0;
 #pragma unroll
       for (int i = 0; i < NT / 64; ++i) reach += __popcll(__ballot(v[i] >= t));
-      if (reach >= K) bound = t;
-      if (reach == K) break;
+      if (reach >= K) bound = t, n = reach;
     }
-    if (tid == 0) s_bound = bound, s_count = 0;
+    if (tid == 0) s_bound = bound, s_count = 0, s_reach = n;
   }
   __syncthreads();
   const unsigned bound = s_bound;
-  const bool mine = own && own >= bound;
-  // The list of all keys that reach the bound.  Where it does not hold them (long runs of equal values, as where most of
-  // a row is masked): the K-th largest of the threads' largest keys, and the list of all that reach that.  Where it does
-  // not hold those either (a few threads hold most): the keys one after the other.  One place in the code looks
-  // through a thread's keys for all of these: copies of it cost registers, and so waves.
-  enum { kList, kLargest, kBounded, kNext } what = known ? kList : kLargest;
-  Key least = 0, last = ~(Key)0;
+  bool mine = own && own >= bound;
+  // The list of all keys that reach the bound.  Where many threads reach it, or the list does not hold them (long runs of
+  // equal values, as where most of a row is masked): the K-th largest of the threads' largest keys, and the list of all
+  // that reach that (2048 x 32000 bf16 with 20 alternatives, all but about ten masked: 83 us, by a list of all first 299).
+  // Where it does not hold those either (a few threads hold most): the keys one after the other.  One place in the code
+  // looks through a thread's keys for all of these: copies of it cost registers, and so waves.
+  enum { kList, kLargest, kBounded, kNext } what = known && s_reach <= 2 * K + 32 ? kList : kLargest;
+  Key least = (Key)bound << 32, last = ~(Key)0;
   for (int k = 0;;) {
     Key best = 0;
-    if (mine)
-      scan(bound, [&](Key x) {
+    if (mine) {
+      const bool first = known && what == kLargest;
+      scan(first ? (Key)own << 32 : least, first, [&](Key x) {
         if (what == kList || what == kBounded) {
           if (x < least) return;
           const int at = atomicAdd(&s_count, 1);
@@ -127,6 +129,7 @@ __device__ __forceinline__ void sc_select(unsigned own, bool known, int K, Scan&
           best = max(best, x);
         }
       });
+    }
     __syncthreads();
     if (what == kList || what == kBounded) {
       const int n = s_count;
@@ -150,6 +153,7 @@ __device__ __forceinline__ void sc_select(unsigned own, bool known, int K, Scan&
       if (above == K - 1 && best) s_key = best;
       __syncthreads();
       least = s_key;
+      mine = best && best >= least;
       what = kBounded;
     } else {
       s_list[tid] = best;
@@ -187,7 +191,7 @@ __device__ __forceinline__ void sc_put(const ScArgs& a, int64_t row, int k, Key 
   a.top_id[row * a.K + k] = sc_id(key);
 }
 
-// 8 waves a SIMD: while some workgroups select, others stream (2048 x 32000 bf16 with 5 alternatives: 37 us, with the 5
+// 8 waves a SIMD: while some workgroups select, others stream (2048 x 32000 bf16 with 5 alternatives: 38 us, with the 5
 // waves that the compiler would leave 39, without alternatives 28).
 template <class T, bool SPLIT, bool TOP, int NT>
 __global__ __launch_bounds__(NT, 8) void k_score(ScArgs a) {
@@ -288,7 +292,7 @@ __global__ __launch_bounds__(NT, 8) void k_score(ScArgs a) {
   if constexpr (TOP) {
     const int blocks = place(whole, 0) < n ? whole + 1 : whole;
     // the thread's keys of a block whose values reach a bound: which ones they are first, and then the few one by one
-    auto block = [&](int b, unsigned bound, auto&& f) {
+    auto block = [&](int b, unsigned bound, bool first, auto&& f) {
       const float least = sc_value((Key)bound << 32);
       float x[U][P];
       if (b < whole)
@@ -304,6 +308,7 @@ __global__ __launch_bounds__(NT, 8) void k_score(ScArgs a) {
           // what is not less: also NaN, and any value where the bound is none
           if (!(x[u][j] < least) && e >= place(b, u) && e < n) there |= 1ull << (u * P + j);
         }
+      if (first) there &= -there;  // of equal values the lowest id, which is the thread's largest key
       for (; there; there &= there - 1) {
         const int i = __ffsll((unsigned long long)there) - 1, e = from(b, i / P) + i % P;
         f(sc_key(to_f(z[e]), (unsigned)(v0 + e)));
@@ -314,10 +319,12 @@ __global__ __launch_bounds__(NT, 8) void k_score(ScArgs a) {
     const bool odd = s != s;
     sc_select<NT>(
         blocks ? sc_order(mine) : 0, !odd, a.K,
-        [&](unsigned bound, auto&& f) {
-          const bool all = odd || sc_order(other) >= bound;
+        [&](Key least, bool first, auto&& f) {
+          const unsigned bound = least >> 32;
+          const bool all = odd || (!first && sc_order(other) >= bound);
           const int b1 = all ? blocks : best + 1;
-          for (int b = all ? 0 : best; b < b1; ++b) block(b, bound, f);
+          for (int b = all ? 0 : best; b < b1; ++b)  // behind the id of least: what is larger
+            block(b, bound + (!odd && v0 + (int64_t)b * STEP > (int64_t)sc_id(least)), first, f);
         },
         [&](int k, Key key) {
           if (SPLIT)
@@ -347,9 +354,9 @@ __global__ __launch_bounds__(kScThreads) void k_score_join(ScArgs a) {
     const float l = __builtin_amdgcn_logf(s);
     sc_select<kScThreads>(
         own, true, a.K,
-        [&](unsigned bound, auto&& f) {
+        [&](Key least, bool, auto&& f) {
           for (int k = tid; k < n; k += kScThreads)
-            if (const Key x = keys[k]; x && sc_order(x) >= bound) f(x);
+            if (const Key x = keys[k]; x && x >= least) f(x);
         },
         [&](int k, Key key) { sc_put(a, row, k, key, m, l); });
   }

@@ -161,6 +161,31 @@ def test_alternatives_in_any_order(dev, dtype, V, rows):
             assert bool((out[1] == 0).all()) and bool((out[0] == -math.inf).all()) and not bool(dz.any())
 
 
+@pytest.mark.parametrize("K", [1, 5, 20])
+@pytest.mark.parametrize("rows,V", [(8, 1001), (1104, 300), (1104, 20011), (8, 70001)])
+def test_few_alternatives_of_long_runs(dev, rows, V, K):
+    """More threads reach the bound than alternatives are asked for: equal values behind, between and before larger ones."""
+    from lifscan import hip_lm as LM
+    g = torch.Generator().manual_seed(V + K)
+    i = torch.arange(V)
+    for dtype in (torch.float32, torch.float16):
+        for low in (-math.inf, torch.finfo(dtype).min, 0.0, -0.0, 2.5):
+            print(f"alternatives of runs {rows}x{V} top {K} {dtype}: {low}", flush=True)
+            z = torch.full((8, V), low)
+            z[1, torch.randperm(V, generator=g)[:K // 2]] = 3.0  # fewer larger ones than alternatives
+            z[2, V // 2:] = 4.0
+            z[3, :V // 3] = 4.0
+            z[4] = torch.where(i % 3 == 1, 3.0, z[4])
+            z[5] = torch.where(i >= V - 2, 5.0, torch.where(i % 7 == 3, 3.0, z[5]))
+            z[6] = torch.where(i % 777 == 5, 3.0 + (i % 5), z[6])
+            z[7] = torch.where((i // 64) % 9 == 8, 3.0, -7.0)
+            z = z.to(dtype)
+            want = reference(z, torch.zeros(8, dtype=torch.int64), 1.0, K)
+            out = LM.token_logprobs(z.to(dev).repeat(rows // 8, 1), torch.zeros(rows, dtype=torch.int64, device=dev), top=K)
+            check([o[:8] for o in out], None, want, V, K)
+            assert torch.equal(out[3], out[3][:8].repeat(rows // 8, 1))
+
+
 @pytest.mark.parametrize("V", [500, 9000, 70000])
 def test_many_large_values_in_few_threads(dev, V):
     """More values reach the bound than the list holds: 60 pieces' threads hold the largest of every block."""
