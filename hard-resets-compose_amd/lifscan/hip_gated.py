@@ -33,7 +33,7 @@ def gated_scan(x, gate, h0=None, starts=None, decay="sigmoid", mix=True):
     (a = exp(gate); a gate above 0 counts as 0 and gets no gradient).  mix: inputs weighed by 1 - a, or as
     they are.  h0: the fp32 state before the first row, or None (zeros).  starts: bool [T, B], where a sequence
     starts anew: the state before that row, h0 among them, is dropped, whatever it holds.  Sums are fp32
-    throughout; h is rounded to the type of x once.
+    throughout; h is rounded to the type of x once.  A decay below the smallest normal fp32 number is 0.
 
     A value that is not finite reaches its own row and, until a start, the later rows of its channel, and no
     others.  What it reaches is not finite, but may be NaN where the recurrence has an infinity."""
