@@ -63,7 +63,7 @@ def token_logprobs(logits, tokens, temperature=1.0, top=0):
     logits [*rows, V], read through its row stride; tokens [*rows], int64 or int32.  A token outside the
     vocabulary is none: logp 0 without a gradient.  Alternatives come in order, equal logits by their id, NaN
     first; top up to 64 and V.  The logits get a gradient from logp and from the entropy, not from the
-    alternatives.  A logit of -inf has probability 0 (as one
-    below fp32's smallest normal number has); a row of nothing else has logp -inf, entropy 0 and no
-    gradient, and a row with NaN or +inf has NaN."""
+    alternatives.  A logit of -inf has probability 0, as has one whose probability is below the smallest normal
+    fp32 number; a row of nothing else has logp -inf, entropy 0 and no gradient, and a row with NaN or +inf has
+    NaN."""
     return tuple(_n.lm_ops().token_logprobs(logits, tokens, temperature, top))
