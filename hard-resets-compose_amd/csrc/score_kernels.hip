@@ -172,10 +172,11 @@ __device__ __forceinline__ void sc_select(unsigned own, bool known, int K, Scan&
 
 // What a row's statistics give: by one thread
 // In natural logarithms, and z and m apart where their difference is no fp32 number: a logit at the lowest value of its
-// type has a finite log p wherever fp32 has one.
+// type has a finite log p wherever fp32 has one.  With a finite z that needs a positive m, and below it z is -inf, as
+// log p then is: m/tau, which may be -inf as well (the lowest value over 0.7), is not taken from it.
 __device__ __forceinline__ float sc_logp(float z, float m, float l, float tau) {
   const float d = z - m;
-  return l == -INFINITY ? -INFINITY : (d > -INFINITY ? d / tau : z / tau - m / tau) - kScLn2 * l;
+  return l == -INFINITY ? -INFINITY : (d > -INFINITY ? d / tau : z / tau - fmaxf(m, 0.0f) / tau) - kScLn2 * l;
 }
 template <class T>
 __device__ __forceinline__ void sc_finish(const ScArgs& a, int64_t row, float m, float s, float t) {

@@ -271,6 +271,34 @@ def test_log_probabilities_of_the_lowest_value(dev, dtype, rows, V, tau):
     assert all(torch.equal(o, o[:3].repeat((rows // 3,) + (1,) * (o.dim() - 1))) for o in out)
 
 
+@pytest.mark.parametrize("tau", [0.7, 1.0])
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("rows,V", [(6, 40), (6, 9001), (6, 70001), (1104, 9001)])
+def test_masks_of_both_kinds(dev, dtype, rows, V, tau):
+    """-inf beside the lowest value of the type and nothing larger: log p is -inf there and uniform over the others, also
+    where the lowest value over tau is no fp32 number.  A row with NaN or +inf has NaN."""
+    low = torch.finfo(dtype).min
+    z, _, gl, gh = inputs(6, V, dtype, dev, seed=23)
+    i = torch.arange(V, device=dev)
+    z[0] = torch.where(i < 6, low, -math.inf)
+    z[1] = torch.where(i == V - 1, -math.inf, low)
+    z[2] = torch.where(i % 3 == 1, low, -math.inf)
+    z[3] = torch.where(i == V // 2, low, -math.inf)
+    z[4] = torch.where(i == 9, math.nan, z[0].float()).to(dtype)
+    z[5] = torch.where(i == 9, math.inf, z[0].float()).to(dtype)
+    tok = torch.tensor([7, V - 1, 1, 2, 7, 7], device=dev)
+    n = rows // 6
+    out, dz = run(z.repeat(n, 1), tok.repeat(n), tau, 20, gl.repeat(n), gh.repeat(n))
+    want = reference(z[:4], tok[:4], tau, 20, gl[:4], gh[:4])
+    assert want["logp"].isinf().tolist() == [True, True, False, True] and int(want["top"].isinf().sum()) == 14 + 19 + (7 if V == 40 else 0)
+    check([o[:4] for o in out], dz[:4], want, V, 20)
+    for o in out[:3]:
+        assert bool(o[4:6].isnan().all())
+    for o in out:
+        assert bool(((o == o[:6].repeat((n,) + (1,) * (o.dim() - 1))) | o.isnan()).all())
+
+
+
 def test_tokens_outside_the_vocabulary(dev):
     from lifscan import hip_lm as LM
     z, _, gl, gh = inputs(6, 77, torch.float32, dev, seed=4)
