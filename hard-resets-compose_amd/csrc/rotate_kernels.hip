@@ -107,6 +107,9 @@ struct RtLane {
         lo[e] = half + p, hi[e] = half + p + (a.D / 2 - half);
     }
   }
+  // Whether pair j of piece e turns.  The others are left alone: times a sine of 0 an infinity or a NaN in one column
+  // would reach the other.
+  __device__ __forceinline__ bool turns(const RtArgs& a, int e, int j) const { return pair[e] + j < a.rot / 2; }
   static __device__ __forceinline__ constexpr int first(int j) { return NEXT ? 2 * j : j; }
   static __device__ __forceinline__ constexpr int second(int j) { return NEXT ? 2 * j + 1 : V + j; }
   template <class T>
@@ -177,7 +180,7 @@ __global__ __launch_bounds__(kRtWaves * 64, 5) void k_rotate(RtArgs a) {
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         c[e][j] = 1.0f, s[e][j] = 0.0f;
-        if (at.pair[e] + j < a.rot / 2) rt_angle(position, a.freq[at.pair[e] + j], c[e][j], s[e][j]);
+        if (at.turns(a, e, j)) rt_angle(position, a.freq[at.pair[e] + j], c[e][j], s[e][j]);
       }
     for (int h = head0; h < head1; h += 64 / G) {
       const bool live = h + sub < head1;
@@ -214,8 +217,8 @@ __global__ __launch_bounds__(kRtWaves * 64, 5) void k_rotate(RtArgs a) {
 #pragma unroll
           for (int j = 0; j < V; ++j) {
             const float u = f[e][Lane::first(j)], v = f[e][Lane::second(j)];
-            y[e][Lane::first(j)] = __builtin_fmaf(u, c[e][j], -(v * s[e][j]));
-            y[e][Lane::second(j)] = __builtin_fmaf(u, s[e][j], v * c[e][j]);
+            y[e][Lane::first(j)] = at.turns(a, e, j) ? __builtin_fmaf(u, c[e][j], -(v * s[e][j])) : u;
+            y[e][Lane::second(j)] = at.turns(a, e, j) ? __builtin_fmaf(u, s[e][j], v * c[e][j]) : v;
           }
       } else {
         at.get(rg, y);
@@ -224,8 +227,8 @@ __global__ __launch_bounds__(kRtWaves * 64, 5) void k_rotate(RtArgs a) {
 #pragma unroll
           for (int j = 0; j < V; ++j) {
             const float u = y[e][Lane::first(j)], v = y[e][Lane::second(j)];
-            y[e][Lane::first(j)] = __builtin_fmaf(u, c[e][j], v * s[e][j]);
-            y[e][Lane::second(j)] = __builtin_fmaf(v, c[e][j], -(u * s[e][j]));
+            y[e][Lane::first(j)] = at.turns(a, e, j) ? __builtin_fmaf(u, c[e][j], v * s[e][j]) : u;
+            y[e][Lane::second(j)] = at.turns(a, e, j) ? __builtin_fmaf(v, c[e][j], -(u * s[e][j])) : v;
           }
         if (norm) {
           at.get(rx, f);

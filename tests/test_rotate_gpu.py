@@ -267,6 +267,36 @@ def test_values_that_are_not_finite_stay_in_their_head(dev):
     assert torch.equal(got["k"], want["k"]) and torch.equal(got["dwk"], want["dwk"])
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("pairs", ["halves", "neighbours"])
+@pytest.mark.parametrize("D,rot", [(64, 0), (64, 24), (66, 2), (80, 36), (128, 64), (250, 122), (256, 8)])
+def test_columns_that_pass_are_left_alone(dev, dtype, pairs, D, rot):
+    """Whatever the columns behind the rotated ones hold: without a norm they come out as they went in, in both
+    directions, and nothing of them reaches another column; with one, no other column's weight gets a gradient of it."""
+    q, k, gq, gk, wq, wk, pos = inputs((7, 2), 3, 2, D, dtype, dev)
+    f = freqs(rot, dev)
+    odd = torch.tensor([float("inf"), float("nan"), -0.0, float("-inf")], device=dev).to(dtype)
+    x, y = k.clone(), gk.clone()
+    for t in (x, y):
+        t[..., rot::3] = odd[torch.arange(t[..., rot::3].numel(), device=dev) % 4].view_as(t[..., rot::3])
+
+    def same(a, b):
+        assert bool(((a == b) & (torch.signbit(a) == torch.signbit(b)) | a.isnan() & b.isnan()).all())
+
+    got = run(q, x, None, None, pos, f, pairs, gq, y)
+    want = run(q, k, None, None, pos, f, pairs, gq, gk)
+    for name, t in (("k", x), ("dk", y)):
+        same(got[name][..., rot:], t[..., rot:])
+        assert torch.equal(got[name][..., :rot], want[name][..., :rot])
+    got = run(q, k, wq, wk, pos, f, pairs, gq, y)
+    want = run(q, k, wq, wk, pos, f, pairs, gq, gk)
+    others = torch.ones(D, dtype=torch.bool, device=dev)
+    others[rot::3] = False
+    assert torch.equal(got["dwk"][others], want["dwk"][others]) and torch.equal(got["dwq"], want["dwq"])
+    assert not bool(got["dwk"][~y.isfinite().flatten(0, 2).all(0)].isfinite().any())
+
+
+
 def test_gradients_against_differences(dev):
     """Central differences of the 64-bit sum of fp32 outputs: with steps of 2^-6 the third derivative leaves
     some 2^-12 of the terms' sum, and the outputs' roundings 2^-24 of it over the step."""
