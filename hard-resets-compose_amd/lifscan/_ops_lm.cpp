@@ -133,6 +133,20 @@ Tensor unpacked(const Tensor& t, torch::IntArrayRef sizes, torch::ScalarType typ
   return t;
 }
 
+// Operands of a step, which updates the state in place: what shares memory with the state would be read by some
+// workgroups while others write it, so it is copied first, as it was before the call.  By the ranges of their addresses:
+// a state is contiguous, so what lies between a view's elements counts as the view's.
+bool meets(const Tensor& t, const Tensor& state) {
+  if (t.numel() == 0 || state.numel() == 0) return false;
+  int64_t last = 0;
+  for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+  const uintptr_t a = (uintptr_t)t.data_ptr(), b = (uintptr_t)state.data_ptr();
+  return a < b + state.nbytes() && b < a + (last + 1) * t.element_size();
+}
+Tensor apart(const Tensor& t, const Tensor& state) {
+  return meets(t, state) ? t.clone(at::MemoryFormat::Contiguous) : t;
+}
+
 // ------------------------------------------------------------------------------- linear attention
 // An operand whose last axis is contiguous.
 Tensor rows_of(const Tensor& t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
@@ -742,9 +756,11 @@ Tensor gated_scan_step(const Tensor& x, const Tensor& gate, const Tensor& state,
   TORCH_CHECK_VALUE(!grad_wanted({x, gate, state}),
                     "gated_scan_step has no gradients (x, gate or the state asks for one): call it under torch.no_grad, "
                     "or gated_scan");
-  const Gates r = gates(x, gate, Tensor(), decay, mix, 2);
+  Gates r = gates(x, gate, Tensor(), decay, mix, 2);
   r.check_state(state, "state");
   TORCH_CHECK_VALUE(state.is_contiguous(), "state must be contiguous: it is updated in place");
+  if (meets(r.x, state) || meets(r.gate, state))
+    r = gates(apart(r.x, state), apart(r.gate, state), Tensor(), decay, mix, 2);
   const c10::DeviceGuard guard(r.x.device());
   const Tensor h = torch::empty({r.a.B, r.a.D}, r.x.options());
   check(g.lsh_gated_step(&r.a, fp(state), raw(h), stream_of(r.x)), "lsh_gated_step");

@@ -41,6 +41,6 @@ def gated_scan(x, gate, h0=None, starts=None, decay="sigmoid", mix=True):
 
 
 def gated_scan_step(x, gate, state, decay="sigmoid", mix=True):
-    """One token: x, gate [B, D] -> h [B, D]; `state` [B, D] (fp32, contiguous) is updated in place.  No
-    gradients: train with gated_scan."""
+    """One token: x, gate [B, D] -> h [B, D]; `state` [B, D] (fp32, contiguous) is updated in place.  x and gate
+    that share memory with it are taken as they were before.  No gradients: train with gated_scan."""
     return _n.lm_ops().gated_scan_step(x, gate, state, _decay(decay), bool(mix))

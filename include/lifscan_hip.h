@@ -632,7 +632,7 @@ int lsh_gated_bwd(const lsh_gated* a, const float* saved, const void* dh, int64_
                   const float* dh_end, void* dx, void* dgate, float* dh0, void* ws, size_t ws_bytes,
                   void* stream);
 /* One token (T = 1; row strides, starts and h0 are not read): `state` [B, D] fp32 is updated in place, h is
- * [B, D]. */
+ * [B, D].  x and gate must not share memory with state. */
 int lsh_gated_step(const lsh_gated* a, float* state, void* h, void* stream);
 
 /* Norms of queries and keys for each head and their rotation by position, over [T, B, heads, D]:

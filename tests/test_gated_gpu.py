@@ -313,6 +313,59 @@ def test_steps_read_views_and_continue_a_prompt(dev):
     assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("graph", [False, True])
+@pytest.mark.parametrize("B,D", [(1, 1000), (64, 1000), (37, 61)])
+def test_steps_whose_operands_share_memory_with_the_state(dev, B, D, graph):
+    """Values and gates are those from before the call, whichever part of the state, or more, they are views of."""
+    from lifscan import hip_gated as G
+    g = torch.Generator().manual_seed(B)
+    start = torch.randn(B * D + 2 * D + 5, generator=g).to(dev)
+    other = torch.randn(B, D, generator=g).to(dev)
+    forms = {
+        "one row": lambda s: s[D:2 * D].view(1, D).expand(B, D), "itself": lambda s: s[D:D + B * D].view(B, D),
+        "one value": lambda s: s[D + 3:D + 4].view(1, 1).expand(B, D), "a shift behind": lambda s: s[D + 5:D + 5 + B * D].view(B, D),
+        "a row before": lambda s: s[:B * D].view(B, D), "halves": lambda s: s.view(torch.bfloat16)[2 * D:2 * D + B * D].view(B, D),
+        "its end": lambda s: s[B * D + D - 1:B * D + 2 * D - 1].view(1, D).expand(B, D),
+        "columns": lambda s: s[D:D + B * D].view(D, B).t(), "every other": lambda s: s[D:D + B].view(B, 1).expand(B, D),
+    }
+    for name, of in forms.items():
+        for which in ("x", "gate", "both"):
+            buf, want = start.clone(), start.clone()
+            held = of(want).clone()
+            rest = other.to(held.dtype)
+            at = lambda b: b[D:D + B * D].view(B, D)  # noqa: E731
+            views = lambda v: (v if which != "gate" else rest, v if which != "x" else rest)  # noqa: E731
+            h_want = G.gated_scan_step(*views(held), at(want))
+            if graph:
+                captured, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+                torch.cuda.synchronize()
+                with torch.cuda.graph(captured, stream=side):
+                    h = G.gated_scan_step(*views(of(buf)), at(buf))
+                for _ in range(2):
+                    buf.copy_(start)
+                    captured.replay()
+                torch.cuda.synchronize()
+            else:
+                h = G.gated_scan_step(*views(of(buf)), at(buf))
+            # as bits: halves of fp32 numbers may be NaN
+            bits = torch.int16 if h.dtype == torch.bfloat16 else torch.int32
+            assert torch.equal(h.view(bits), h_want.view(bits)) and torch.equal(buf.view(torch.int32), want.view(torch.int32)), \
+                (name, which)
+
+
+def test_steps_whose_operands_lie_beside_the_state_are_not_copied(dev):
+    from lifscan import hip_gated as G
+    B, D = 5, 64
+    buf = torch.randn(3 * B * D, device=dev)
+    x, state, gate = (t.view(B, D) for t in buf.split(B * D))
+    G.gated_scan_step(x, gate, state)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    h = G.gated_scan_step(x, gate, state)
+    assert torch.cuda.max_memory_allocated() - before <= max(512, -(-h.nbytes // 512) * 512)
+
+
 def test_no_rows_no_batch(dev):
     from lifscan import hip_gated as G
     x = torch.zeros(0, 3, 8, device=dev, requires_grad=True)
