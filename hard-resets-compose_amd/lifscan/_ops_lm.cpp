@@ -138,8 +138,9 @@ Tensor unpacked(const Tensor& t, torch::IntArrayRef sizes, torch::ScalarType typ
 // a state is contiguous, so what lies between a view's elements counts as the view's.
 bool meets(const Tensor& t, const Tensor& state) {
   if (t.numel() == 0 || state.numel() == 0) return false;
+  const auto sizes = t.sizes(), strides = t.strides();
   int64_t last = 0;
-  for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+  for (size_t i = 0; i < sizes.size(); ++i) last += (sizes[i] - 1) * strides[i];
   const uintptr_t a = (uintptr_t)t.data_ptr(), b = (uintptr_t)state.data_ptr();
   return a < b + state.nbytes() && b < a + (last + 1) * t.element_size();
 }
@@ -311,6 +312,8 @@ Tensor lin_attn_step(const Tensor& q, const Tensor& k, const Tensor& v, const Te
   Attn r = attn(q, k, v, beta, scale, 3);
   r.check_state(state, "state");
   TORCH_CHECK_VALUE(state.is_contiguous(), "state must be contiguous: it is updated in place");
+  if (meets(r.q, state) || meets(r.k, state) || meets(r.v, state) || meets(r.beta, state))
+    r = attn(apart(r.q, state), apart(r.k, state), apart(r.v, state), apart(r.beta, state), scale, 3);
   const c10::DeviceGuard guard(r.q.device());
   const Tensor o = torch::empty({r.a.B, r.a.H, r.a.Dv}, r.q.options());
   r.a.o = o.data_ptr();

@@ -49,7 +49,8 @@ def lin_attn(q, k, v, beta, s0=None, scale=1.0):
 
 def lin_attn_step(q, k, v, beta, state, scale=1.0):
     """One token: q [B, Hq, Dk], k [B, Hk, Dk], v [B, Hv, Dv] -> o [B, H, Dv]; `state` [B, H, Dk, Dv]
-    (fp32, contiguous) is updated in place.  No gradients: train with lin_attn."""
+    (fp32, contiguous) is updated in place.  Operands that share memory with it are taken as they were before.  No
+    gradients: train with lin_attn."""
     return _n.lm_ops().lin_attn_step(q, k, v, _decays(beta, q, k, v), state, scale)
 
 

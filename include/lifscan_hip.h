@@ -549,7 +549,7 @@ int lsh_linattn_bwd(const lsh_linattn* a, const void* starts, const void* d_o, i
                     int64_t do_sb, int64_t do_sh, const float* ds_end, void* dq, void* dk, void* dv,
                     float* ds0, void* ws, size_t ws_bytes, void* stream);
 /* One token (T = 1; the row strides are not read): `state` [B, H, Dk, Dv] is updated in place, o is
- * [B, H, Dv].  s0 and s_end are not read. */
+ * [B, H, Dv].  s0 and s_end are not read; q, k, v and beta must not share memory with state. */
 int lsh_linattn_step(const lsh_linattn* a, float* state, void* stream);
 
 /* The norm after a block with its gate and residual scale, and the norm before the next block, over

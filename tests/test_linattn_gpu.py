@@ -281,6 +281,30 @@ def test_prompt_then_tokens(dev):
     assert bool(((state - s).abs().cpu().double() <= tol * s_most).all())
 
 
+def test_steps_whose_operands_share_memory_with_the_state(dev):
+    """Queries, keys, values and decays are those from before the call, whichever part of the state they are views of."""
+    from lifscan import hip_linattn as LA
+    B, H, Dk, Dv = 3, 4, 64, 64
+    q, k, v, beta, start, _, _ = _inputs(torch.float32, 1, B, (H, H, H), H, Dk, Dv, dev, seed=41)
+    forms = {
+        "rows": lambda s: s[:, :, 5], "columns": lambda s: s[..., 7], "one row": lambda s: s[1, 2, 3].expand(B, H, 64),
+        "one head": lambda s: s[:, :1, 63], "one value": lambda s: s[2, 3, 63, 63].expand(B, H, 64),
+        "a shift": lambda s: s.view(-1)[3:3 + B * H * 64].view(B, H, 64),
+    }
+    for name, of in forms.items():
+        for which in range(4):
+            def step(s, views):
+                ops = [q[0], k[0], v[0]]
+                if which == 3:
+                    return LA.lin_attn_step(*ops, views[0, :1, 0].expand(H) if name == "one head" else views[0, :, 0], s, scale=0.3)
+                ops[which] = views
+                return LA.lin_attn_step(*ops, beta, s, scale=0.3)
+            a, b = start.abs(), start.abs()  # decays are not negative
+            o = step(a, of(a).clone())
+            o1 = step(b, of(b))
+            assert torch.equal(o, o1) and torch.equal(a, b), (name, which)
+
+
 def test_no_tokens_and_no_batch(dev):
     from lifscan import hip_linattn as LA
     q, k, v, beta, s0, _, _ = _inputs(torch.float32, 0, 2, (2, 2, 2), 2, 8, 8, dev)
