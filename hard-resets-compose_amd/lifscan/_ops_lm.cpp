@@ -747,7 +747,8 @@ std::tuple<Tensor, Tensor> gated_scan(const Tensor& x, const Tensor& gate, const
     h0 = train ? h0.contiguous() : h0.detach().contiguous();
   }
   if (train) {
-    const auto out = Gated::apply(x, gate, maybe(h0), starts_in, decay, mix);
+    // what was laid out anew, with its gradient: once a call
+    const auto out = Gated::apply(r.x, r.gate, maybe(h0), maybe(r.starts), decay, mix);
     return {out[0], out[1]};
   }
   const GatedOut out = gated_forward(r, h0, false);

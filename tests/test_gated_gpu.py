@@ -173,6 +173,33 @@ def test_layouts(dev, dtype, layout):
     check({"h": h, "end": end, **dict(zip(("dx", "dgate", "dh0"), grads))}, want)
 
 
+def test_training_copies_an_operand_once(dev):
+    """Operands whose last axis is not contiguous, and strided starts, are laid out once a call, and their gradients
+    reach the tensors that were given."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Copies(TorchDispatchMode):
+        n = 0
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            self.n += func.overloadpacket in (torch.ops.aten.clone, torch.ops.aten.copy_)
+            return func(*args, **(kwargs or {}))
+
+    from lifscan import hip_gated as G
+    x, gate, h0, starts, dh, dend = inputs(40, 3, 32, torch.float32, dev, starts=True, seed=31)
+    want = run(x, gate, h0, starts, "sigmoid", True, dh, dend)
+    a, b = (t.transpose(0, 2).contiguous().transpose(0, 2).requires_grad_(True) for t in (x, gate))
+    late = starts.t().contiguous().t()
+    for train in (True, False):
+        with torch.set_grad_enabled(train), Copies() as seen:
+            h, end = G.gated_scan(a, b, h0, starts=late)
+        assert seen.n == 3, (train, seen.n)
+        assert torch.equal(h, want["h"]) and torch.equal(end, want["end"])
+        if train:
+            for got, name in zip(torch.autograd.grad((h, end), (a, b), (dh, dend)), ("dx", "dgate")):
+                assert torch.equal(got, want[name])
+
+
 def test_starts_of_either_type_and_any_stride(dev):
     from lifscan import hip_gated as G
     x, gate, h0, st, *_ = inputs(40, 3, 16, torch.float32, dev, starts=True, seed=5)
