@@ -291,7 +291,8 @@ std::tuple<Tensor, Tensor> lin_attn(const Tensor& q, const Tensor& k, const Tens
       r.check_state(s0, "s0");
       s0 = s0.contiguous();
     }
-    const auto out = LinAttn::apply(q, k, v, beta, maybe(s0), scale);
+    // what was laid out anew, with its gradient: once a call
+    const auto out = LinAttn::apply(r.q, r.k, r.v, r.beta, maybe(s0), scale);
     return {out[0], out[1]};
   }
   Attn r = attn(q.detach(), k.detach(), v.detach(), beta, scale, 4);

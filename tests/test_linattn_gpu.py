@@ -208,6 +208,34 @@ def test_layouts(dev, dtype, layout):
     assert torch.equal(o, want[0]) and torch.equal(s_end, want[1])
 
 
+def test_training_copies_an_operand_once(dev):
+    """Operands whose last axis is not contiguous are laid out once a call, and their gradients reach the tensors that
+    were given."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Copies(TorchDispatchMode):
+        n = 0
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            self.n += func.overloadpacket in (torch.ops.aten.clone, torch.ops.aten.copy_)
+            return func(*args, **(kwargs or {}))
+
+    from lifscan import hip_linattn as LA
+    q, k, v, beta, s0, do, ds = _inputs(torch.float32, 40, 3, (4, 2, 4), 4, 32, 16, dev, seed=37)
+    ins = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    o, s = LA.lin_attn(*ins, beta, s0=s0, scale=0.2)
+    want = torch.autograd.grad((o, s), ins, (do, ds))
+    late = [t.transpose(0, 3).contiguous().transpose(0, 3).requires_grad_(True) for t in (q, k, v)]
+    for train in (True, False):
+        with torch.set_grad_enabled(train), Copies() as seen:
+            o1, s1 = LA.lin_attn(*late, beta, s0=s0, scale=0.2)
+        assert seen.n == 3, (train, seen.n)
+        assert torch.equal(o1, o) and torch.equal(s1, s)
+        if train:
+            for a, b in zip(torch.autograd.grad((o1, s1), late, (do, ds)), want):
+                assert torch.equal(a, b)
+
+
 def test_offsets_beyond_32_bits(dev):
     """Rows more than 2^31 elements apart."""
     from lifscan import hip_linattn as LA
