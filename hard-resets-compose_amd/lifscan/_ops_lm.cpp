@@ -895,8 +895,9 @@ std::tuple<Tensor, Tensor> norm_rotate(const Tensor& q, const Tensor& k, const M
   TORCH_CHECK_VALUE(wq_in.has_value() == wk_in.has_value(), "q_weight and k_weight come together");
   TORCH_CHECK_VALUE(eps >= 0, "eps=", eps, " must not be negative");
   Heads r;
+  TORCH_CHECK_VALUE(freq_in.has_value() == positions_in.has_value(), "positions and inv_freq come together: a rotation "
+                    "needs both, and heads that are only normed neither");
   if (freq_in.has_value()) {
-    TORCH_CHECK_VALUE(positions_in.has_value(), "a rotation needs positions");
     const Tensor &f = *freq_in, &p = *positions_in;
     TORCH_CHECK_VALUE(f.dim() == 1 && f.device() == q.device() && f.is_floating_point() && f.size(0) <= D / 2,
                       "inv_freq must be a float tensor of up to ", D / 2, " frequencies on ", q.device());

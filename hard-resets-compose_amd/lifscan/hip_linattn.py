@@ -63,8 +63,9 @@ def norm_rotate(q, k, positions=None, inv_freq=None, q_weight=None, k_weight=Non
     q [T, B, Hq, D], k [T, B, Hk, D], or [B, heads, D] for one token each: float32, bfloat16 or float16, one
     type; even D from 2 to 256.  positions: int64 or int32, [T], [T, B], or [B] for one token each; any size,
     also negative: angles are formed in 64 bits.  inv_freq: up to D/2 frequencies on the device (float64 keeps
-    them as they are); the first 2*len columns rotate, the others pass; None: no rotation.  pairs: "halves"
-    (column p with p + len) or "neighbours" (2p with 2p + 1).  q_weight, k_weight: [D] each; both None: no norm.
+    them as they are); the first 2*len columns rotate, the others pass, whatever they hold.  They come together;
+    without them: no rotation.  pairs: "halves" (column p with p + len) or "neighbours" (2p with 2p + 1).
+    q_weight, k_weight: [D] each; both None: no norm.
     Gradients for q, k and the weights."""
     if pairs not in ("halves", "neighbours"):
         raise ValueError(f"pairs {pairs!r}: 'halves' or 'neighbours'")

@@ -451,6 +451,18 @@ def test_refusals(dev):
         torch.autograd.grad(a.sum(), y, create_graph=True)
 
 
+def test_positions_and_frequencies_come_together(dev):
+    from lifscan import hip_linattn as LA
+    q, k, _, _, wq, wk, pos = inputs((4, 2), 2, 1, 16, torch.float32, dev)
+    f = freqs(16, dev)
+    for args in ((pos, None), (None, f), (pos, None, wq, wk), (pos.int(), None)):
+        with pytest.raises(ValueError, match="inv_freq|positions"):
+            LA.norm_rotate(q, k, *args)
+    for a, b in zip(LA.norm_rotate(q, k), (q, k)):
+        assert torch.equal(a, b)
+
+
+
 def test_forward_mode_and_traces_are_refused(dev):
     import torch.autograd.forward_ad as fw
     from lifscan import hip_linattn as LA
