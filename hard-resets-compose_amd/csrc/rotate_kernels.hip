@@ -278,25 +278,43 @@ __global__ __launch_bounds__(kRtWaves * 64, 5) void k_rotate(RtArgs a) {
   }
 }
 
-// The workgroups' sums of dw, kRtRuns runs of workgroups at once and then in run order.
+// The workgroups' sums of dw: kRtRuns runs of workgroups at once, each as 8 sums, and pairs of those and of the runs.  One
+// after the other the up to 40 of a run and then the runs drift: equal terms are off by up to 14 * 2^-24 of their sum.
 constexpr int kRtCols = 32, kRtRuns = 32;
 __global__ __launch_bounds__(kRtCols* kRtRuns) void k_rotate_sums(const float* __restrict__ part, int P, int D,
                                                                   float* dwq, float* dwk) {
   __shared__ float s_run[kRtRuns][kRtCols];
   const int c = threadIdx.x % kRtCols, run = threadIdx.x / kRtCols, i = blockIdx.x * kRtCols + c;
   const int per = (P + kRtRuns - 1) / kRtRuns, p1 = min(P, (run + 1) * per);
-  float s = 0.0f;
-  if (i < 2 * D)
-#pragma unroll 8
-    for (int p = run * per; p < p1; ++p) s += part[(size_t)p * 2 * D + i];
-  s_run[run][c] = s;
+  float s[8] = {};
+  if (i < 2 * D) {
+    const size_t row = 2 * D;
+    const float* at = part + run * per * row + i;
+    int p = run * per;
+#pragma unroll 2
+    for (; p + 8 <= p1; p += 8, at += 8 * row)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s[j] += at[j * row];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (p + j < p1) s[j] += at[j * row];
+  }
+#pragma unroll
+  for (int n = 4; n > 0; n /= 2)
+#pragma unroll
+    for (int j = 0; j < n; ++j) s[j] += s[j + n];
+  s_run[run][c] = s[0];
   __syncthreads();
   if (run != 0 || i >= 2 * D) return;
-  s = 0.0f;
+  float r[kRtRuns];
 #pragma unroll
-  for (int r = 0; r < kRtRuns; ++r) s += s_run[r][c];
+  for (int j = 0; j < kRtRuns; ++j) r[j] = s_run[j][c];
+#pragma unroll
+  for (int n = kRtRuns / 2; n > 0; n /= 2)
+#pragma unroll
+    for (int j = 0; j < n; ++j) r[j] += r[j + n];
   float* out = i < D ? dwq : dwk;
-  if (out) out[i % D] = s;
+  if (out) out[i % D] = r[0];
 }
 
 // reads: whether q and k are read (the gradients of a rotation alone do without)

@@ -297,6 +297,22 @@ def test_columns_that_pass_are_left_alone(dev, dtype, pairs, D, rot):
 
 
 
+def test_the_weights_sums_do_not_drift(dev):
+    """1280 workgroups' equal sums of 4 equal terms.  Doubled they stay exact, so what rounds is 2 of the 3 additions in a
+    workgroup and as many as are made one after the other behind it: with 5 in a row and pairs from there on, 3.  Each is
+    off by F of what it has summed, and each term by 2 F (a root of 1 ulp, a product): 7 F in all; 40 in a row and 32 in
+    a row are off by up to 14 F."""
+    T, D = 5120, 256
+    g = torch.Generator().manual_seed(5)
+    grads = [(1 + torch.rand(D, generator=g)).to(dev).expand(T, 1, 1, D) for _ in range(2)]
+    x, w = torch.ones(T, 1, 1, D, device=dev), torch.ones(D, device=dev)
+    got = run(x, x, w, w, None, None, "halves", *grads, eps=0.0)
+    for name, t in zip(("dwq", "dwk"), grads):
+        want = T * t[0, 0, 0].double()
+        assert float(((got[name].double() - want).abs() / want).max()) <= 7 * F
+
+
+
 def test_gradients_against_differences(dev):
     """Central differences of the 64-bit sum of fp32 outputs: with steps of 2^-6 the third derivative leaves
     some 2^-12 of the terms' sum, and the outputs' roundings 2^-24 of it over the step."""
