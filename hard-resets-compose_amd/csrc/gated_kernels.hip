@@ -49,7 +49,9 @@ struct GsArgs {
 };
 
 // e^x for x <= 0: the hardware's power of two with what the product x*log2(e) loses put back.  16-bit gates go without
-// (6 instructions of 30 an element): it is |x|*2^-24 of a weight, of which 2^-8 or 2^-11 is seen.
+// (6 instructions of 30 an element): it is |x|*2^-24 of a decay.  What is rounded to 16 bits does not show it, and the
+// states and dh0, which are fp32, hardly (1024 rows of 4096 channels, of the states' norm: sigmoid bf16 0.97e-7, with it
+// 0.94e-7, fp16 1.00e-7 and 0.95e-7; log decays 0.78e-7 and 0.80e-7 either way; dh0 over 64 rows 2.0e-7 to 2.2e-7 either way).
 template <bool FINE>
 __device__ __forceinline__ float gs_exp(float x) {
   constexpr float kHi = 1.44269502f, kLo = 1.92596299e-8f;  // log2(e)

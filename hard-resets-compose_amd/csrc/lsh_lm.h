@@ -1,6 +1,6 @@
 // Device and host helpers shared by the language-model operators (linattn_kernels.hip,
-// blocknorm_kernels.hip, embed_kernels.hip, distill_kernels.hip): element types, wide accesses and
-// workgroup reductions.  Tensors are fp32, bf16 or fp16; every kernel computes in fp32 and rounds
+// blocknorm_kernels.hip, embed_kernels.hip, distill_kernels.hip, gated_kernels.hip, rotate_kernels.hip,
+// score_kernels.hip): element types, wide accesses and workgroup reductions.  Tensors are fp32, bf16 or fp16; every kernel computes in fp32 and rounds
 // to the tensor's type where it stores, to nearest even.
 #pragma once
 #include "lsh_abi.h"
